@@ -282,6 +282,110 @@ BFFT_EXPORT bfft_status bfft_stream_execute(bfft_stream_plan_t plan, const void*
                                             void* stream);
 BFFT_EXPORT bfft_status bfft_stream_plan_destroy(bfft_stream_plan_t plan);
 
+/* ------------------------------------------------------------------------
+ * Positions and the paged 8-bit cache of attention layers -- no counterpart in
+ * the reference.  A rotation multiplies each pair (a, b) of a head by a unit
+ * root of its token's position, c + is from a table made in float64 and rounded
+ * once like the twiddle tables: a' = a c - b s, b' = a s + b c.  All descriptor
+ * fields are 64 bits wide; strides count elements; the innermost (element)
+ * stride is 1.  Sequence tables live on the device and are read there: nothing
+ * here looks at them on the host, and page numbers outside the cache, positions
+ * outside the table and rows outside the tensors are never dereferenced. */
+enum { BFFT_F32 = 0, BFFT_F16 = 1, BFFT_BF16 = 2 };
+enum { BFFT_PAIRS_HALF = 0,       /* pairs (j, j + rotated / 2)                 */
+       BFFT_PAIRS_INTERLEAVED = 1 /* pairs (2 j, 2 j + 1)                       */ };
+enum { BFFT_CODE_INT8 = 0,        /* symmetric, +-127                           */
+       BFFT_CODE_E4M3 = 1         /* 8-bit floats, +-448                        */ };
+
+typedef struct bfft_rotate_desc {
+    int64_t batch, tokens, heads, dim; /* x, y: (batch, tokens, heads, dim)     */
+    int64_t rotated;                   /* even; the elements behind pass through */
+    int64_t x_batch, x_token, x_head, y_batch, y_token, y_head; /* strides       */
+    int64_t pos_batch, pos_token;      /* strides of positions (0 broadcasts)   */
+    int64_t table_rows;                /* table: (table_rows, rotated / 2, 2) float32 */
+    int64_t type, layout, transform_direction; /* INVERSE conjugates the roots  */
+    int64_t pos64;                     /* positions are int64 (else int32)      */
+    int64_t device;
+} bfft_rotate_desc;
+
+/* y = x rotated by position; y may be x.  A position outside the table makes
+ * that token's rotated part NaN.  The inverse direction is the adjoint: it maps
+ * the gradient of y to the gradient of x. */
+BFFT_EXPORT bfft_status bfft_rotate_positions(const bfft_rotate_desc* desc, const void* x, const void* positions,
+                                              const void* table, void* y, void* stream);
+
+/* Pages of `page` tokens, one block of codes per page and kv head, one float32
+ * scale per block for keys and one for values: token value = code * scale.  A
+ * block that ever held a NaN or an infinity reads as NaN. */
+typedef struct bfft_cache_desc {
+    void *k, *v;             /* [pages][kv_heads][page][dim] 8-bit codes, 16-byte aligned */
+    void *k_scale, *v_scale; /* [pages][kv_heads] float32                       */
+    int64_t pages, kv_heads;
+    int64_t page;            /* 16, 32, 64 or 128                               */
+    int64_t dim;             /* a multiple of 16, 16..256                       */
+    int64_t code;            /* BFFT_CODE_*                                     */
+} bfft_cache_desc;
+
+/* Ragged rows: sequence s owns rows [starts[s], starts[s + 1]) of the call's
+ * `tokens` rows, and its token i lies in page block_table[s][i / page]. */
+typedef struct bfft_sequence_desc {
+    const void* block_table; /* [seqs][max_pages] int32                         */
+    int64_t table_stride;
+    const void* lens;        /* [seqs] int32, see each call                     */
+    const void* starts;      /* [seqs + 1] int32                                */
+    int64_t seqs, max_pages, tokens;
+} bfft_sequence_desc;
+
+typedef struct bfft_append_desc {
+    const void *k, *v, *q;   /* (tokens, heads, dim); q may be null             */
+    void* q_out;             /* rotated q, (tokens, q_heads, dim)               */
+    const void* positions;   /* (tokens,), null: the place in the sequence      */
+    const void* table;       /* as in bfft_rotate_positions, null: no rotation  */
+    int64_t k_token, k_head, v_token, v_head, q_token, q_head, o_token, o_head;
+    int64_t table_rows, rotated, q_heads, type, layout, pos64, device;
+} bfft_append_desc;
+
+/* Appends each sequence's rows behind the lens[s] tokens that it holds: rotates
+ * q and k, quantises k and v, one launch.  A block's scale is the largest
+ * magnitude that it has held over 127 (448); where new rows make it grow, the
+ * block's earlier codes are rounded again to the new scale.  A sequence's first
+ * token of a page starts the block anew.  Sequences must not share a page that
+ * is written. */
+BFFT_EXPORT bfft_status bfft_cache_append(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
+                                          const bfft_append_desc* desc, void* stream);
+
+/* The values that the cache stands for: row starts[s] + i of k and v
+ * ((tokens, kv_heads, dim) of `type`, 16-byte aligned) is token lens[s] + i of
+ * sequence s.  A token without a valid page reads as NaN. */
+BFFT_EXPORT bfft_status bfft_cache_read(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs, int64_t type,
+                                        void* k, void* v, int64_t device, void* stream);
+
+typedef struct bfft_attention_desc {
+    const void* q;           /* (tokens, q_heads, dim), float16 or bfloat16     */
+    void* out;               /* (tokens, q_heads, dim) of q's type              */
+    void* lse;               /* (tokens, q_heads) float32, or null              */
+    int64_t q_token, q_head, o_token, o_head;
+    int64_t q_heads;         /* a multiple of kv_heads                          */
+    int64_t type;
+    int64_t causal;          /* row i of n sees tokens <= lens[s] - n + i       */
+    int64_t window;          /* > 0: and only the last `window` of them         */
+    double softmax_scale;
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t device;
+} bfft_attention_desc;
+
+/* out = softmax(softmax_scale q k^T) v over the lens[s] tokens of each row's
+ * sequence, lse the natural logarithm of the row's sum of exponentials.  A row
+ * that sees no token gets out = 0 and lse = -inf.  A token without a valid page
+ * is not seen.  The workspace (bfft_cache_attention_workspace bytes for the same
+ * descriptors, 16-byte aligned) holds the parts of rows whose tokens are shared
+ * out over several blocks. */
+BFFT_EXPORT bfft_status bfft_cache_attention_workspace(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
+                                                       const bfft_attention_desc* desc, size_t* bytes);
+BFFT_EXPORT bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
+                                             const bfft_attention_desc* desc, void* stream);
+
 /* Status bits the kernels set on `device` when a bounded wait expired
  * (bit 0: a TMA pass gave up waiting for a tile copy and returned early, so
  * its output is incomplete).  Synchronises the device; clear != 0 resets the

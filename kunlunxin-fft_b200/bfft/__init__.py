@@ -47,6 +47,13 @@ _LAZY = {
     "validate_input": "validate",
     "plan_hybrid": "adapter_hybrid",
     "run_hybrid": "adapter_hybrid",
+    "PagedCache": "cache",
+    "append_rotated": "cache",
+    "cache_attention": "cache",
+    "paged_cache": "cache",
+    "read_cache": "cache",
+    "rotary_table": "cache",
+    "rotate_positions": "cache",
 }
 
 __all__ = sorted([

@@ -27,7 +27,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libbfft.so")
 META_PATH = os.path.join(LIB_DIR, "build_meta.json")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
-NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-shared",
+NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--threads", "0", "-Xcompiler", "-fPIC", "-shared",
               "-Xcompiler", "-fvisibility=hidden", "-Xcompiler", "-Wall"]
 
 

@@ -34,7 +34,9 @@ EXPORTS = ("bfft_api_version", "bfft_last_error", "bfft_plan_create", "bfft_plan
            "bfft_dist_phase", "bfft_dist_plan_launches", "bfft_dist_plan_destroy", "bfft_device_status",
            "bfft_probe_bounded_waits",
            "bfft_stream_plan_create", "bfft_stream_plan_info", "bfft_stream_execute", "bfft_stream_plan_destroy",
-           "bfft_dist_p2p_prepare", "bfft_dist_p2p_attach", "bfft_dist_p2p_attach_pointers", "bfft_dist_p2p_phase")
+           "bfft_dist_p2p_prepare", "bfft_dist_p2p_attach", "bfft_dist_p2p_attach_pointers", "bfft_dist_p2p_phase",
+           "bfft_rotate_positions", "bfft_cache_append", "bfft_cache_read", "bfft_cache_attention_workspace",
+           "bfft_cache_attention")
 
 
 class PlanDesc(ctypes.Structure):
@@ -103,6 +105,12 @@ def load() -> ctypes.CDLL:
         L.bfft_dist_p2p_attach.argtypes = [vp, ctypes.c_char_p]
         L.bfft_dist_p2p_attach_pointers.argtypes = [vp, ctypes.POINTER(vp)]
         L.bfft_dist_p2p_phase.argtypes = [vp, i32, vp, vp, vp, sz, vp]
+        desc = ctypes.c_char_p  # descriptors of the position and cache calls: packed bytes (see cache.py)
+        L.bfft_rotate_positions.argtypes = [desc, vp, vp, vp, vp, vp]
+        L.bfft_cache_append.argtypes = [desc, desc, desc, vp]
+        L.bfft_cache_read.argtypes = [desc, desc, i64, vp, vp, i64, vp]
+        L.bfft_cache_attention_workspace.argtypes = [desc, desc, desc, ctypes.POINTER(sz)]
+        L.bfft_cache_attention.argtypes = [desc, desc, desc, vp]
         for name in EXPORTS:
             fn = getattr(L, name)
             if name not in ("bfft_api_version", "bfft_last_error", "bfft_launch_counter"):

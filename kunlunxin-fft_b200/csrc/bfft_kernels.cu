@@ -1003,6 +1003,22 @@ cudaError_t run_wait_probe(cudaStream_t s) {
     return cudaGetLastError();
 }
 
+cudaError_t device_status_word(unsigned int** word) {
+    static std::atomic<unsigned int*> words[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    void* p = words[dev].load(std::memory_order_acquire);
+    if (!p) {
+        e = cudaGetSymbolAddress(&p, g_kernel_status);
+        if (e != cudaSuccess) return e;
+        words[dev].store(static_cast<unsigned int*>(p), std::memory_order_release);
+    }
+    *word = static_cast<unsigned int*>(p);
+    return cudaSuccess;
+}
+
 cudaError_t read_device_status(unsigned* status, bool clear) {
     cudaError_t e = cudaMemcpyFromSymbol(status, g_kernel_status, sizeof(unsigned));
     if (e == cudaSuccess && clear) {

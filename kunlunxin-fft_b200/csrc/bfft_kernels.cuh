@@ -90,6 +90,9 @@ cudaError_t launch_fused_fft(int log2n, const float2* in, float2* out, void* wor
 // Status word the kernels set when a bounded wait expires (bit 0: an
 // mbarrier wait of the TMA pass); read synchronously, optionally cleared.
 cudaError_t read_device_status(unsigned* status, bool clear);
+// Device address of that word on the current device (kernels of the other
+// translation units record their expired waits in the same word).
+cudaError_t device_status_word(unsigned int** word);
 // One kernel whose two bounded waits (mbarrier, dependency counter) expire.
 cudaError_t run_wait_probe(cudaStream_t s);
 

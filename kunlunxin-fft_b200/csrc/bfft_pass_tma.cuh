@@ -25,130 +25,16 @@
 // more (bounded) for its copy in flight and returns.
 #pragma once
 
-#include <cuda.h>
-#include <cudaTypedefs.h>
+#include "bfft_async.cuh"
 
 namespace bfft {
 
 __device__ unsigned int g_kernel_status;  // bit 0: a bounded mbarrier wait expired
 
-constexpr uint64_t kWaitLimitNs = 1000000000ull;  // 1 s
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-// `p` (a pointer into dynamic shared memory) rounded up to an A-byte boundary
-// by pointer arithmetic, so the result keeps its shared-memory provenance and
-// the compiler emits shared-memory loads and stores (LDS / STS) through it.
-// (Rounding through an integer cast loses that: every access through the
-// result became a generic load or store, tracked by the long scoreboard.)
-template <int A>
-__device__ __forceinline__ unsigned char* align_smem(unsigned char* p) {
-    return p + ((A - (smem_u32(p) & (A - 1))) & (A - 1));
-}
-__device__ __forceinline__ uint64_t global_timer_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-__device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint64_t* b, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n"
-        " .reg .pred p;\n"
-        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(b)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// try_wait with a suspend-time hint: the thread may sleep until the phase
-// completes or about `hint_ns` pass, instead of spinning on the barrier (a
-// spinning producer warp takes issue slots from the computing warps).
-__device__ __forceinline__ bool mbar_try_wait_sleep(uint64_t* b, uint32_t parity, uint32_t hint_ns) {
-    uint32_t ok;
-    asm volatile(
-        "{\n"
-        " .reg .pred p;\n"
-        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
-        " selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(b)), "r"(parity), "r"(hint_ns)
-        : "memory");
-    return ok != 0;
-}
 // Wait for phase `parity` of `b` to complete; false (and status bit 0) when
 // it has not completed within kWaitLimitNs.
 __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* b, uint32_t parity) {
-    if (mbar_try_wait(b, parity)) return true;
-    const uint64_t t0 = global_timer_ns();
-    for (;;) {
-        if (mbar_try_wait_sleep(b, parity, 20000u)) return true;
-        if (global_timer_ns() - t0 > kWaitLimitNs) {
-            atomicOr(&g_kernel_status, 1u);
-            return false;
-        }
-    }
-}
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2,
-                                            uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
-        : "memory");
-}
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int c0, int c1, int c2, const void* src) {
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
-                     reinterpret_cast<uint64_t>(map)),
-                 "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(src))
-                 : "memory");
-}
-__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<uint64_t>(dst)),
-                 "r"(smem_u32(src)), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                     smem_u32(dst)),
-                 "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void bulk_wait_read() {
-    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void bulk_wait() {
-    asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory");
-}
-// Programmatic dependent launch: launch_dependents lets the next kernel on
-// the stream (if launched as a programmatic dependent) be scheduled once
-// every CTA of this grid has issued it or exited -- its CTAs then take the
-// SMs this grid's finished CTAs free and fill their tables; griddep_wait
-// blocks until the previous kernel has completed and its writes are visible
-// (at once for an ordinary launch).
-__device__ __forceinline__ void griddep_launch_dependents() {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-// Generic-proxy writes to shared memory become visible to the async proxy
-// (the TMA store engine) after this fence and a barrier.
-__device__ __forceinline__ void fence_proxy_async_smem() {
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    return mbar_wait_limited(b, parity, &g_kernel_status);
 }
 
 __host__ __device__ constexpr uint32_t rev4(int m) {

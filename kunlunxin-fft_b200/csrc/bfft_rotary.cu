@@ -1,0 +1,702 @@
+// bfft_rotary.cu -- rotation by position, appending rotated keys (and values) to
+// a paged 8-bit cache, and reading such a cache back.
+//
+// A rotation multiplies the pair (a, b) = a + ib of a head by a unit root of its
+// position p, m e^{i p w_j} = c + is from a table made in float64 and rounded
+// once (the form of the transforms' twiddle tables):
+//     a' = a c - b s,   b' = a s + b c.
+// The inverse direction conjugates the root; it is the adjoint, so it is also the
+// gradient's rotation.
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <mutex>
+#include <string>
+
+#include "../../include/bfft.h"
+#include "bfft_cache.cuh"
+#include "bfft_kernels.cuh"
+
+using namespace bfft;
+
+namespace bfft {
+
+// A head's row is cut into units of 2 P elements, two packs of P each: P pairs
+// that rotate (interleaved: neighbours; half: element j and j + rotated / 2), or
+// 2 P elements behind the rotated part, which pass through.
+struct RowShape {
+    int rotated;
+    int units;       // of a row
+    int rot_units;   // of them, rotating
+};
+
+template <int P, int LAYOUT>
+__device__ __forceinline__ void unit_offsets(const RowShape& r, int u, int& o0, int& o1) {
+    if (u >= r.rot_units) {
+        o0 = r.rotated + (u - r.rot_units) * 2 * P;
+        o1 = o0 + P;
+    } else if (LAYOUT == BFFT_PAIRS_HALF) {
+        o0 = u * P;
+        o1 = r.rotated / 2 + u * P;
+    } else {
+        o0 = u * 2 * P;
+        o1 = o0 + P;
+    }
+}
+
+template <typename T, int P>
+__device__ __forceinline__ void load_unit(const T* __restrict__ row, int o0, int o1, float (&e)[2 * P]) {
+    const Pack<T, P> a = *reinterpret_cast<const Pack<T, P>*>(row + o0);
+    const Pack<T, P> b = *reinterpret_cast<const Pack<T, P>*>(row + o1);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        e[i] = to_f32(a.v[i]);
+        e[P + i] = to_f32(b.v[i]);
+    }
+}
+
+template <typename T, int P>
+__device__ __forceinline__ void store_unit(T* __restrict__ row, int o0, int o1, const float (&e)[2 * P]) {
+    Pack<T, P> a, b;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        a.v[i] = from_f32<T>(e[i]);
+        b.v[i] = from_f32<T>(e[P + i]);
+    }
+    *reinterpret_cast<Pack<T, P>*>(row + o0) = a;
+    *reinterpret_cast<Pack<T, P>*>(row + o1) = b;
+}
+
+// Roots of unit u at position p; NaN where the table has no row p.
+template <int P>
+__device__ __forceinline__ void load_roots(const float2* __restrict__ table, int64_t rows, int pairs, int64_t p, int u,
+                                           float (&c)[P], float (&s)[P]) {
+    if (p >= 0 && p < rows) {
+        const float2* t = table + p * pairs + u * P;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const float2 w = t[i];
+            c[i] = w.x;
+            s[i] = w.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i) c[i] = s[i] = __int_as_float(0x7fffffff);
+    }
+}
+
+// STEPS: every product and sum rounded by itself (no contraction), so that the
+// 8-bit codes made from the result are those of the formula evaluated step by
+// step in 32 bits; a contracted product moves one in some 10^5 to its neighbour.
+template <int P, int LAYOUT, bool STEPS>
+__device__ __forceinline__ void rotate_unit(float (&e)[2 * P], const float (&c)[P], const float (&s)[P]) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int ia = LAYOUT == BFFT_PAIRS_HALF ? i : 2 * i, ib = LAYOUT == BFFT_PAIRS_HALF ? P + i : 2 * i + 1;
+        const float a = e[ia], b = e[ib];
+        if constexpr (STEPS) {
+            e[ia] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+            e[ib] = __fadd_rn(__fmul_rn(a, s[i]), __fmul_rn(b, c[i]));
+        } else {
+            e[ia] = a * c[i] - b * s[i];
+            e[ib] = a * s[i] + b * c[i];
+        }
+    }
+}
+
+// ---------------------------------------------------------------- rotation
+struct RotateArgs {
+    const void* x;
+    void* y;
+    const void* positions;
+    const float2* table;
+    int64_t tokens, rows;  // rows = batch * tokens
+    int64_t xb, xt, xh, yb, yt, yh, pb, pt;
+    int64_t table_rows;
+    RowShape shape;
+    int heads, groups;     // a thread takes heads g, g + groups, ...
+    int pos64;
+    float sign;            // of the sine: -1 conjugates
+};
+
+template <typename T, int P, int LAYOUT>
+__global__ void __launch_bounds__(256) k_rotate(RotateArgs a) {
+    const int u = threadIdx.x;
+    const int64_t slot = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    const int64_t row = slot / a.groups;
+    if (row >= a.rows) return;
+    const int g = (int)(slot - row * a.groups);
+    const int64_t b = row / a.tokens, t = row - b * a.tokens;
+    const T* x = static_cast<const T*>(a.x) + b * a.xb + t * a.xt;
+    T* y = static_cast<T*>(a.y) + b * a.yb + t * a.yt;
+    int o0, o1;
+    unit_offsets<P, LAYOUT>(a.shape, u, o0, o1);
+    const bool turns = u < a.shape.rot_units;
+    float c[P], s[P];
+    if (turns) {
+        const int64_t at = b * a.pb + t * a.pt;
+        const int64_t p = a.pos64 ? static_cast<const int64_t*>(a.positions)[at]
+                                  : (int64_t) static_cast<const int32_t*>(a.positions)[at];
+        load_roots<P>(a.table, a.table_rows, a.shape.rotated / 2, p, u, c, s);
+#pragma unroll
+        for (int i = 0; i < P; ++i) s[i] *= a.sign;
+    }
+    for (int h = g; h < a.heads; h += a.groups) {
+        float e[2 * P];
+        load_unit<T, P>(x + h * a.xh, o0, o1, e);
+        if (turns) rotate_unit<P, LAYOUT, false>(e, c, s);
+        store_unit<T, P>(y + h * a.yh, o0, o1, e);
+    }
+}
+
+// ---------------------------------------------------------------- append
+struct AppendArgs {
+    CacheView cache;
+    SequenceView seq;        // lens: tokens held before the call
+    const void *k, *v, *q;
+    void* q_out;
+    int64_t kt, kh, vt, vh, qt, qh, ot, oh;
+    const void* positions;   // null: the place in the cache
+    const float2* table;     // null: no rotation
+    int64_t table_rows;
+    RowShape k_shape, v_shape;
+    int q_heads, pos64;
+    int by_token;            // 1: a slot is a token, 0: a run of up to a page (see run_of_slot)
+    int64_t slots;           // runs at most
+};
+
+// The run of new tokens that slot i stands for: tokens [first, first + n) of
+// sequence s that go to one page, at place `at` of the sequence.  The runs of
+// sequence s take the slots from starts[s] / page + 2 s on (a sequence of n
+// tokens has at most n / page + 2 runs), so every slot finds its run by itself.
+// By token: a slot is a token, and the first of each run stands for it.
+struct Run {
+    int s;
+    int64_t first, n, at;
+};
+__device__ __forceinline__ bool run_of_slot(const AppendArgs& a, int64_t i, Run& r) {
+    const SequenceView& q = a.seq;
+    const int lg = a.cache.page_log2;
+    const int64_t page = (int64_t)1 << lg;
+    int s;
+    if (a.by_token) {
+        s = find_sequence(q.starts, q.seqs, i);
+    } else {
+        const int lane = threadIdx.x & 31;
+        int lo = 0, n = q.seqs;
+        while (n > 1) {
+            const int step = (n + 31) >> 5;
+            const int j = lane * step;
+            const bool le = j < n && ((int64_t)q.starts[lo + j] >> lg) + 2 * (int64_t)(lo + j) <= i;
+            const int c = __popc(__ballot_sync(0xffffffffu, le));
+            const int skip = (c > 0 ? c - 1 : 0) * step;
+            lo += skip;
+            n = n - skip < step ? n - skip : step;
+        }
+        s = lo;
+    }
+    const int64_t t0 = q.starts[s];
+    int64_t t1 = q.starts[s + 1];
+    if (t1 > q.tokens) t1 = q.tokens;
+    const int64_t held = q.lens[s];
+    if (t0 < 0 || t0 >= t1 || held < 0) return false;
+    int64_t at;  // place of the run's first token
+    if (a.by_token) {
+        if (i < t0 || i >= t1) return false;
+        at = held + (i - t0);
+        if (i != t0 && (at & (page - 1))) return false;
+    } else {
+        const int64_t j = i - ((t0 >> lg) + 2 * (int64_t)s);
+        if (j < 0) return false;
+        at = j == 0 ? held : (((held >> lg) + j) << lg);
+        if (at - held >= t1 - t0) return false;
+    }
+    r.s = s;
+    r.at = at;
+    r.first = t0 + (at - held);
+    const int64_t room = page - (at & (page - 1)), left = t1 - r.first;
+    r.n = room < left ? room : left;
+    return true;
+}
+
+__device__ __forceinline__ int64_t token_position(const AppendArgs& a, int64_t token, int64_t place) {
+    if (!a.positions) return place;
+    return a.pos64 ? static_cast<const int64_t*>(a.positions)[token]
+                   : (int64_t) static_cast<const int32_t*>(a.positions)[token];
+}
+
+constexpr int kAppendThreads = 128;
+
+// One run's rows of one kv head, of the keys (ROTATE) or the values: the largest
+// magnitude, the block's new scale, then the codes -- those that the page
+// already held first, where the scale grew.  max is taken on the bits of |x|, so
+// that infinities and NaN survive it: they make the scale NaN or infinite and
+// the block reads as NaN.
+template <typename T, int P, int LAYOUT, int CODE, bool ROTATE>
+__device__ __forceinline__ void append_rows(const AppendArgs& a, const Run& r, int64_t page_id, int head,
+                                            uint32_t* shared_max) {
+    const RowShape& shape = ROTATE ? a.k_shape : a.v_shape;
+    const T* x = static_cast<const T*>(ROTATE ? a.k : a.v) + head * (ROTATE ? a.kh : a.vh);
+    const int64_t xt = ROTATE ? a.kt : a.vt;
+    const int tid = threadIdx.x, dim = a.cache.dim;
+    const int64_t block = page_id * a.cache.kv_heads + head;
+    uint8_t* codes = (ROTATE ? a.cache.k : a.cache.v) + ((block << a.cache.page_log2) * dim);
+    float* scale = (ROTATE ? a.cache.k_scale : a.cache.v_scale) + block;
+    const int old = (int)(r.at & (((int64_t)1 << a.cache.page_log2) - 1));
+    const int total = (int)r.n * shape.units;
+
+    auto value = [&](int i, float (&e)[2 * P], int& o0, int& o1, int& row) {
+        row = i / shape.units;
+        const int u = i - row * shape.units;
+        unit_offsets<P, LAYOUT>(shape, u, o0, o1);
+        load_unit<T, P>(x + (r.first + row) * xt, o0, o1, e);
+        if (ROTATE && u < shape.rot_units) {
+            float c[P], s[P];
+            load_roots<P>(a.table, a.table_rows, shape.rotated / 2, token_position(a, r.first + row, r.at + row), u, c,
+                          s);
+            rotate_unit<P, LAYOUT, true>(e, c, s);
+        }
+    };
+
+    uint32_t big = 0;
+    for (int i = tid; i < total; i += kAppendThreads) {
+        float e[2 * P];
+        int o0, o1, row;
+        value(i, e, o0, o1, row);
+#pragma unroll
+        for (int j = 0; j < 2 * P; ++j) big = max(big, __float_as_uint(e[j]) & 0x7fffffffu);
+    }
+    big = __reduce_max_sync(0xffffffffu, big);
+    if ((tid & 31) == 0) shared_max[tid >> 5] = big;
+    const float before = old > 0 ? *scale : 0.f;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) big = max(big, shared_max[w]);
+    // a block under 2^-126 * most is zero: no denormal scales
+    float now = __uint_as_float(big) / CodeRange<CODE>::most;
+    if (now < 1.17549435e-38f) now = 0.f;
+    now = __uint_as_float(max(__float_as_uint(now), __float_as_uint(before) & 0x7fffffffu));
+    const float inv = now == 0.f ? 0.f : 1.f / now;
+    if (old > 0 && now != before) {
+        // codes times the ratio of the scales, in 64 bits: in 32 the three roundings of
+        // a code of 127 (127 * 3 * 2^-24) could pass a value over the middle of two codes
+        const double shrink = (double)before / (double)now;
+        for (int i = tid; i < old * dim / 16; i += kAppendThreads) {
+            Pack<uint8_t, 16> c = reinterpret_cast<const Pack<uint8_t, 16>*>(codes)[i];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) c.v[j] = to_code<CODE>((double)code_value<CODE>(c.v[j]) * shrink);
+            reinterpret_cast<Pack<uint8_t, 16>*>(codes)[i] = c;
+        }
+    }
+    if (tid == 0) *scale = now;
+    for (int i = tid; i < total; i += kAppendThreads) {
+        float e[2 * P];
+        int o0, o1, row;
+        value(i, e, o0, o1, row);
+        Pack<uint8_t, P> c0, c1;
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            c0.v[j] = to_code<CODE>(e[j] * inv);
+            c1.v[j] = to_code<CODE>(e[P + j] * inv);
+        }
+        uint8_t* to = codes + (old + row) * dim;
+        *reinterpret_cast<Pack<uint8_t, P>*>(to + o0) = c0;
+        *reinterpret_cast<Pack<uint8_t, P>*>(to + o1) = c1;
+    }
+}
+
+// Blocks [0, slots * kv_heads * 2): a run's keys or values of one head.  The
+// blocks behind them rotate the queries, one token each.
+template <typename T, int P, int LAYOUT, int CODE>
+__global__ void __launch_bounds__(kAppendThreads) k_append(AppendArgs a) {
+    __shared__ uint32_t shared_max[kAppendThreads / 32];
+    const int64_t per_slot = 2 * a.cache.kv_heads;
+    const int64_t runs = a.slots * per_slot;
+    int64_t i = blockIdx.x;
+    if (i < runs) {
+        const int64_t slot = i / per_slot;
+        const int which = (int)(i - slot * per_slot);
+        Run r;
+        if (!run_of_slot(a, slot, r)) return;
+        const int64_t page_id = page_of(a.seq, a.cache, r.s, r.at);
+        if (page_id < 0) return;
+        if (which < a.cache.kv_heads)
+            append_rows<T, P, LAYOUT, CODE, true>(a, r, page_id, which, shared_max);
+        else
+            append_rows<T, P, LAYOUT, CODE, false>(a, r, page_id, which - a.cache.kv_heads, shared_max);
+        return;
+    }
+    const int64_t token = i - runs;
+    const int s = find_sequence(a.seq.starts, a.seq.seqs, token);
+    const int64_t p = token_position(a, token, (int64_t)a.seq.lens[s] + (token - a.seq.starts[s]));
+    const T* x = static_cast<const T*>(a.q) + token * a.qt;
+    T* y = static_cast<T*>(a.q_out) + token * a.ot;
+    const RowShape& shape = a.k_shape;
+    for (int j = threadIdx.x; j < a.q_heads * shape.units; j += kAppendThreads) {
+        const int h = j / shape.units, u = j - h * shape.units;
+        int o0, o1;
+        unit_offsets<P, LAYOUT>(shape, u, o0, o1);
+        float e[2 * P];
+        load_unit<T, P>(x + h * a.qh, o0, o1, e);
+        if (u < shape.rot_units) {
+            float c[P], sn[P];
+            load_roots<P>(a.table, a.table_rows, shape.rotated / 2, p, u, c, sn);
+            rotate_unit<P, LAYOUT, false>(e, c, sn);
+        }
+        store_unit<T, P>(y + h * a.oh, o0, o1, e);
+    }
+}
+
+// ---------------------------------------------------------------- read
+struct ReadArgs {
+    CacheView cache;
+    SequenceView seq;  // lens: the first token that is read of each sequence
+    void *k, *v;       // [tokens][kv_heads][dim]
+};
+
+// A warp per token: its keys and values of all heads, 16 codes a lane and step.
+// Tokens without a valid page read as NaN.
+template <typename T, int CODE>
+__global__ void __launch_bounds__(256) k_read(ReadArgs a) {
+    const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (t >= a.seq.tokens) return;
+    const int lane = threadIdx.x & 31, dim = a.cache.dim, heads = a.cache.kv_heads;
+    const int s = find_sequence(a.seq.starts, a.seq.seqs, t);
+    const int64_t at = (int64_t)a.seq.lens[s] + (t - a.seq.starts[s]);
+    const int64_t page_id = t < a.seq.starts[s] ? -1 : page_of(a.seq, a.cache, s, at);
+    const int slot = (int)(at & (((int64_t)1 << a.cache.page_log2) - 1));
+    const int chunks = dim / 16, half = heads * chunks;
+    for (int i = lane; i < 2 * half; i += 32) {
+        const bool is_v = i >= half;
+        const int j = is_v ? i - half : i;
+        const int h = j / chunks, c = j - h * chunks;
+        float scale = __int_as_float(0x7fffffff);
+        Pack<uint8_t, 16> codes = {};
+        if (page_id >= 0) {
+            const int64_t block = page_id * heads + h;
+            scale = (is_v ? a.cache.v_scale : a.cache.k_scale)[block];
+            codes = *reinterpret_cast<const Pack<uint8_t, 16>*>((is_v ? a.cache.v : a.cache.k) +
+                                                                ((block << a.cache.page_log2) + slot) * dim + c * 16);
+        }
+        constexpr int P = 16 / sizeof(T);
+        T* to = static_cast<T*>(is_v ? a.v : a.k) + (t * heads + h) * dim + c * 16;
+#pragma unroll
+        for (int w = 0; w < 16 / P; ++w) {
+            Pack<T, P> o;
+#pragma unroll
+            for (int b = 0; b < P; ++b) o.v[b] = from_f32<T>(code_value<CODE>(codes.v[w * P + b]) * scale);
+            reinterpret_cast<Pack<T, P>*>(to)[w] = o;
+        }
+    }
+}
+
+}  // namespace bfft
+
+// ---------------------------------------------------------------- host side
+namespace {
+
+bfft_status fail(bfft_status st, const char* fmt, ...) {
+    char buf[384];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    set_last_error(buf);  // reported by bfft_last_error()
+    return st;
+}
+
+bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
+
+int type_bytes(int64_t type) { return type == BFFT_F32 ? 4 : 2; }
+
+// Largest pack of P elements (P * bytes <= 16) that divides every pointer's and
+// stride's alignment and cuts the rotated and the passing part into whole units.
+int pick_pack(int bytes, int layout, int64_t dim, int64_t rotated, const void* const* ptrs, int nptrs,
+              const int64_t* strides, int nstrides) {
+    for (int p = 16 / bytes; p > 1; p /= 2) {
+        const int64_t rot = layout == BFFT_PAIRS_HALF ? rotated / 2 : rotated;
+        bool ok = rot % (layout == BFFT_PAIRS_HALF ? p : 2 * p) == 0 && (dim - rotated) % (2 * p) == 0;
+        for (int i = 0; ok && i < nptrs; ++i) ok = aligned(ptrs[i], p * bytes);
+        for (int i = 0; ok && i < nstrides; ++i) ok = strides[i] % p == 0;
+        if (ok) return p;
+    }
+    return 1;
+}
+
+RowShape row_shape(int64_t dim, int64_t rotated, int p) {
+    RowShape r;
+    r.rotated = (int)rotated;
+    r.units = (int)(dim / (2 * p));
+    r.rot_units = (int)(rotated / (2 * p));
+    return r;
+}
+
+template <typename T, int P>
+void rotate_layout(int layout, const RotateArgs& a, dim3 grid, dim3 block, cudaStream_t s) {
+    if (layout == BFFT_PAIRS_HALF)
+        k_rotate<T, P, BFFT_PAIRS_HALF><<<grid, block, 0, s>>>(a);
+    else
+        k_rotate<T, P, BFFT_PAIRS_INTERLEAVED><<<grid, block, 0, s>>>(a);
+}
+template <typename T>
+void rotate_pack(int p, int layout, const RotateArgs& a, dim3 grid, dim3 block, cudaStream_t s) {
+    if constexpr (sizeof(T) == 2)
+        if (p == 8) return rotate_layout<T, 8>(layout, a, grid, block, s);
+    if (p == 4) return rotate_layout<T, 4>(layout, a, grid, block, s);
+    if (p == 2) return rotate_layout<T, 2>(layout, a, grid, block, s);
+    rotate_layout<T, 1>(layout, a, grid, block, s);
+}
+
+template <typename T, int P, int LAYOUT>
+void append_code(int code, const AppendArgs& a, dim3 grid, cudaStream_t s) {
+    if (code == BFFT_CODE_INT8)
+        k_append<T, P, LAYOUT, kCodeInt8><<<grid, kAppendThreads, 0, s>>>(a);
+    else
+        k_append<T, P, LAYOUT, kCodeE4m3><<<grid, kAppendThreads, 0, s>>>(a);
+}
+template <typename T, int P>
+void append_layout(int layout, int code, const AppendArgs& a, dim3 grid, cudaStream_t s) {
+    if (layout == BFFT_PAIRS_HALF)
+        append_code<T, P, BFFT_PAIRS_HALF>(code, a, grid, s);
+    else
+        append_code<T, P, BFFT_PAIRS_INTERLEAVED>(code, a, grid, s);
+}
+template <typename T>
+void append_pack(int p, int layout, int code, const AppendArgs& a, dim3 grid, cudaStream_t s) {
+    if constexpr (sizeof(T) == 2)
+        if (p == 8) return append_layout<T, 8>(layout, code, a, grid, s);
+    if (p == 4) return append_layout<T, 4>(layout, code, a, grid, s);
+    if (p == 2) return append_layout<T, 2>(layout, code, a, grid, s);
+    append_layout<T, 1>(layout, code, a, grid, s);
+}
+
+template <typename T>
+void read_code(int code, const ReadArgs& a, dim3 grid, cudaStream_t s) {
+    if (code == BFFT_CODE_INT8)
+        k_read<T, kCodeInt8><<<grid, 256, 0, s>>>(a);
+    else
+        k_read<T, kCodeE4m3><<<grid, 256, 0, s>>>(a);
+}
+
+struct Device {
+    int prev = -1;
+    bool ok = true;
+    explicit Device(int64_t dev) {
+        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+        if (prev != dev) ok = cudaSetDevice((int)dev) == cudaSuccess;
+        changed = ok && prev != dev;
+    }
+    ~Device() {
+        if (changed && prev >= 0) cudaSetDevice(prev);
+    }
+    bool changed = false;
+};
+
+}  // namespace
+
+namespace bfft {
+
+bfft_status check_cache(const bfft_cache_desc* c) {
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(BFFT_ERR_VALUE, "null cache pointer");
+    if (!aligned(c->k, 16) || !aligned(c->v, 16)) return fail(BFFT_ERR_VALUE, "cache codes must be 16-byte aligned");
+    if (!aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
+        return fail(BFFT_ERR_VALUE, "cache scales must be 4-byte aligned");
+    if (c->code != BFFT_CODE_INT8 && c->code != BFFT_CODE_E4M3)
+        return fail(BFFT_ERR_VALUE, "bad code %lld", (long long)c->code);
+    if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128)
+        return fail(BFFT_ERR_SHAPE, "page must be 16, 32, 64 or 128 tokens, got %lld", (long long)c->page);
+    if (c->dim < 16 || c->dim > 256 || c->dim % 16)
+        return fail(BFFT_ERR_SHAPE, "head dimension must be a multiple of 16 in [16, 256], got %lld",
+                    (long long)c->dim);
+    if (c->kv_heads < 1 || c->kv_heads > 65535 || c->pages < 1 || c->pages > 0x7fffffffLL)
+        return fail(BFFT_ERR_SHAPE, "bad cache of %lld pages, %lld heads", (long long)c->pages,
+                    (long long)c->kv_heads);
+    return BFFT_OK;
+}
+
+bfft_status check_sequences(const bfft_sequence_desc* q) {
+    if (!q->block_table || !q->lens || !q->starts) return fail(BFFT_ERR_VALUE, "null sequence pointer");
+    if (!aligned(q->block_table, 4) || !aligned(q->lens, 4) || !aligned(q->starts, 4))
+        return fail(BFFT_ERR_VALUE, "sequence tables must be 4-byte aligned");
+    if (q->seqs < 1 || q->seqs > 0x7ffffffeLL || q->max_pages < 1 || q->max_pages > 0x7fffffffLL)
+        return fail(BFFT_ERR_SHAPE, "bad table of %lld sequences, %lld pages each", (long long)q->seqs,
+                    (long long)q->max_pages);
+    if (q->tokens < 0 || q->tokens > 0x7fffffffLL) return fail(BFFT_ERR_SHAPE, "bad row count %lld", (long long)q->tokens);
+    return BFFT_OK;
+}
+
+CacheView cache_view(const bfft_cache_desc* c) {
+    CacheView v;
+    v.k = static_cast<uint8_t*>(c->k);
+    v.v = static_cast<uint8_t*>(c->v);
+    v.k_scale = static_cast<float*>(c->k_scale);
+    v.v_scale = static_cast<float*>(c->v_scale);
+    v.pages = c->pages;
+    v.kv_heads = (int)c->kv_heads;
+    v.dim = (int)c->dim;
+    v.page_log2 = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
+    return v;
+}
+
+SequenceView sequence_view(const bfft_sequence_desc* q) {
+    SequenceView v;
+    v.block_table = static_cast<const int32_t*>(q->block_table);
+    v.table_stride = q->table_stride;
+    v.lens = static_cast<const int32_t*>(q->lens);
+    v.starts = static_cast<const int32_t*>(q->starts);
+    v.seqs = (int)q->seqs;
+    v.max_pages = (int)q->max_pages;
+    v.tokens = q->tokens;
+    return v;
+}
+
+}  // namespace bfft
+
+extern "C" bfft_status bfft_rotate_positions(const bfft_rotate_desc* d, const void* x, const void* positions,
+                                             const void* table, void* y, void* stream) {
+    if (!d || !x || !positions || !table || !y) return fail(BFFT_ERR_VALUE, "null pointer");
+    if (d->type < BFFT_F32 || d->type > BFFT_BF16) return fail(BFFT_ERR_VALUE, "bad type %lld", (long long)d->type);
+    if (d->layout != BFFT_PAIRS_HALF && d->layout != BFFT_PAIRS_INTERLEAVED)
+        return fail(BFFT_ERR_VALUE, "bad layout %lld", (long long)d->layout);
+    if (d->transform_direction != BFFT_FORWARD && d->transform_direction != BFFT_INVERSE)
+        return fail(BFFT_ERR_VALUE, "bad transform_direction %lld", (long long)d->transform_direction);
+    if (d->batch < 0 || d->tokens < 0 || d->heads < 0 || d->batch > 0x7fffffffLL || d->tokens > 0x7fffffffLL ||
+        d->heads > 0x7fffffffLL)
+        return fail(BFFT_ERR_SHAPE, "bad shape %lld x %lld x %lld", (long long)d->batch, (long long)d->tokens,
+                    (long long)d->heads);
+    if (d->dim < 2 || d->dim > 512 || d->dim % 2)
+        return fail(BFFT_ERR_SHAPE, "head dimension must be even and in [2, 512], got %lld", (long long)d->dim);
+    if (d->rotated < 2 || d->rotated > d->dim || d->rotated % 2)
+        return fail(BFFT_ERR_SHAPE, "rotated part must be even and in [2, %lld], got %lld", (long long)d->dim,
+                    (long long)d->rotated);
+    const int bytes = type_bytes(d->type);
+    if (!aligned(x, bytes) || !aligned(y, bytes) || !aligned(table, 8) || !aligned(positions, d->pos64 ? 8 : 4))
+        return fail(BFFT_ERR_VALUE, "misaligned pointer");
+    if (d->batch == 0 || d->tokens == 0 || d->heads == 0) return BFFT_OK;
+    const void* ptrs[2] = {x, y};
+    const int64_t strides[6] = {d->x_batch, d->x_token, d->x_head, d->y_batch, d->y_token, d->y_head};
+    const int p = pick_pack(bytes, (int)d->layout, d->dim, d->rotated, ptrs, 2, strides, 6);
+    RotateArgs a;
+    a.x = x;
+    a.y = y;
+    a.positions = positions;
+    a.table = static_cast<const float2*>(table);
+    a.tokens = d->tokens;
+    a.rows = d->batch * d->tokens;
+    a.xb = d->x_batch, a.xt = d->x_token, a.xh = d->x_head;
+    a.yb = d->y_batch, a.yt = d->y_token, a.yh = d->y_head;
+    a.pb = d->pos_batch, a.pt = d->pos_token;
+    a.table_rows = d->table_rows;
+    a.shape = row_shape(d->dim, d->rotated, p);
+    a.heads = (int)d->heads;
+    a.groups = a.heads;
+    a.pos64 = d->pos64 != 0;
+    a.sign = d->transform_direction == BFFT_INVERSE ? -1.f : 1.f;
+    dim3 block((unsigned)a.shape.units, 1);
+    while (block.x * block.y * 2 <= 256) block.y *= 2;
+    const int64_t blocks = (a.rows * a.groups + block.y - 1) / block.y;
+    if (blocks > 0x7fffffffLL) return fail(BFFT_ERR_SHAPE, "too many rows: %lld", (long long)a.rows);
+    Device g(d->device);
+    if (!g.ok) return fail(BFFT_ERR_CUDA, "cannot select device %lld", (long long)d->device);
+    const dim3 grid((unsigned)blocks);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    count_launches(1);
+    if (d->type == BFFT_F32)
+        rotate_pack<float>(p, (int)d->layout, a, grid, block, s);
+    else if (d->type == BFFT_F16)
+        rotate_pack<__half>(p, (int)d->layout, a, grid, block, s);
+    else
+        rotate_pack<__nv_bfloat16>(p, (int)d->layout, a, grid, block, s);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? BFFT_OK : fail(BFFT_ERR_CUDA, "rotate_positions: %s", cudaGetErrorString(e));
+}
+
+extern "C" bfft_status bfft_cache_append(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
+                                         const bfft_append_desc* d, void* stream) {
+    if (!cache || !seqs || !d || !d->k || !d->v) return fail(BFFT_ERR_VALUE, "null pointer");
+    bfft_status st = check_cache(cache);
+    if (st == BFFT_OK) st = check_sequences(seqs);
+    if (st != BFFT_OK) return st;
+    if (d->type < BFFT_F32 || d->type > BFFT_BF16) return fail(BFFT_ERR_VALUE, "bad type %lld", (long long)d->type);
+    if (d->layout != BFFT_PAIRS_HALF && d->layout != BFFT_PAIRS_INTERLEAVED)
+        return fail(BFFT_ERR_VALUE, "bad layout %lld", (long long)d->layout);
+    const int64_t rotated = d->table ? d->rotated : 0;
+    if (rotated < 0 || rotated > cache->dim || rotated % 2 || (d->table && rotated < 2))
+        return fail(BFFT_ERR_SHAPE, "rotated part must be even and in [2, %lld], got %lld", (long long)cache->dim,
+                    (long long)d->rotated);
+    if ((d->q == nullptr) != (d->q_out == nullptr)) return fail(BFFT_ERR_VALUE, "q and q_out go together");
+    if (d->q && d->q_heads < 1) return fail(BFFT_ERR_SHAPE, "bad query head count %lld", (long long)d->q_heads);
+    const int bytes = type_bytes(d->type);
+    if (!aligned(d->k, bytes) || !aligned(d->v, bytes) || !aligned(d->q, bytes) || !aligned(d->q_out, bytes) ||
+        !aligned(d->table, 8) || !aligned(d->positions, d->pos64 ? 8 : 4))
+        return fail(BFFT_ERR_VALUE, "misaligned pointer");
+    if (seqs->tokens == 0) return BFFT_OK;
+    const void* ptrs[4] = {d->k, d->v, d->q, d->q_out};
+    const int64_t strides[8] = {d->k_token, d->k_head, d->v_token, d->v_head,
+                                d->q ? d->q_token : 0, d->q ? d->q_head : 0, d->q ? d->o_token : 0,
+                                d->q ? d->o_head : 0};
+    const int p = pick_pack(bytes, (int)d->layout, cache->dim, rotated, ptrs, 4, strides, 8);
+    AppendArgs a;
+    a.cache = cache_view(cache);
+    a.seq = sequence_view(seqs);
+    a.k = d->k, a.v = d->v, a.q = d->q, a.q_out = d->q_out;
+    a.kt = d->k_token, a.kh = d->k_head, a.vt = d->v_token, a.vh = d->v_head;
+    a.qt = d->q_token, a.qh = d->q_head, a.ot = d->o_token, a.oh = d->o_head;
+    a.positions = d->positions;
+    a.pos64 = d->pos64 != 0;
+    a.table = static_cast<const float2*>(d->table);
+    a.table_rows = d->table_rows;
+    a.k_shape = row_shape(cache->dim, rotated, p);
+    a.v_shape = row_shape(cache->dim, 0, p);
+    a.q_heads = (int)d->q_heads;
+    const int64_t runs = seqs->tokens / cache->page + 2 * seqs->seqs;
+    a.by_token = seqs->tokens <= runs;
+    a.slots = a.by_token ? seqs->tokens : runs;
+    const int64_t blocks = a.slots * 2 * cache->kv_heads + (d->q ? seqs->tokens : 0);
+    if (blocks > 0x7fffffffLL) return fail(BFFT_ERR_SHAPE, "too many rows: %lld", (long long)seqs->tokens);
+    Device g(d->device);
+    if (!g.ok) return fail(BFFT_ERR_CUDA, "cannot select device %lld", (long long)d->device);
+    const dim3 grid((unsigned)blocks);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int layout = (int)d->layout, code = (int)cache->code;
+    count_launches(1);
+    if (d->type == BFFT_F32)
+        append_pack<float>(p, layout, code, a, grid, s);
+    else if (d->type == BFFT_F16)
+        append_pack<__half>(p, layout, code, a, grid, s);
+    else
+        append_pack<__nv_bfloat16>(p, layout, code, a, grid, s);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? BFFT_OK : fail(BFFT_ERR_CUDA, "cache_append: %s", cudaGetErrorString(e));
+}
+
+extern "C" bfft_status bfft_cache_read(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs, int64_t type,
+                                       void* k, void* v, int64_t device, void* stream) {
+    if (!cache || !seqs || !k || !v) return fail(BFFT_ERR_VALUE, "null pointer");
+    bfft_status st = check_cache(cache);
+    if (st == BFFT_OK) st = check_sequences(seqs);
+    if (st != BFFT_OK) return st;
+    if (type < BFFT_F32 || type > BFFT_BF16) return fail(BFFT_ERR_VALUE, "bad type %lld", (long long)type);
+    if (!aligned(k, 16) || !aligned(v, 16)) return fail(BFFT_ERR_VALUE, "outputs must be 16-byte aligned");
+    if (seqs->tokens == 0) return BFFT_OK;
+    ReadArgs a;
+    a.cache = cache_view(cache);
+    a.seq = sequence_view(seqs);
+    a.k = k;
+    a.v = v;
+    Device g(device);
+    if (!g.ok) return fail(BFFT_ERR_CUDA, "cannot select device %lld", (long long)device);
+    const dim3 grid((unsigned)((seqs->tokens + 7) / 8));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    count_launches(1);
+    if (type == BFFT_F32)
+        read_code<float>((int)cache->code, a, grid, s);
+    else if (type == BFFT_F16)
+        read_code<__half>((int)cache->code, a, grid, s);
+    else
+        read_code<__nv_bfloat16>((int)cache->code, a, grid, s);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? BFFT_OK : fail(BFFT_ERR_CUDA, "cache_read: %s", cudaGetErrorString(e));
+}
