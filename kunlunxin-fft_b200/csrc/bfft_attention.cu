@@ -5,12 +5,14 @@
 // in 32 bits while the tokens pass once.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <string>
 
 #include "../../include/bfft.h"
+#include "bfft_async.cuh"
 #include "bfft_cache.cuh"
 #include "bfft_kernels.cuh"
 
@@ -30,56 +32,9 @@ struct AttentionArgs {
     float scale_log2;    // softmax_scale * log2(e)
 };
 
-// A warp per (row, query head), a token at a time, lanes over the dimensions.
-template <typename T, int CODE>
-__global__ void __launch_bounds__(256) k_attention_rows(AttentionArgs a) {
-    const int lane = threadIdx.x & 31, dim = a.cache.dim;
-    const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t row = i / a.q_heads;
-    if (row >= a.seq.tokens) return;
-    const int head = (int)(i - row * a.q_heads), kv = head / a.group;
-    const int s = find_sequence(a.seq.starts, a.seq.seqs, row);
-    const int64_t t0 = a.seq.starts[s], t1 = a.seq.starts[s + 1], len = a.seq.lens[s];
-    const int64_t pos = len - (t1 - row);
-    int64_t hi = a.causal ? pos + 1 : len, lo = 0;
-    if (a.window > 0 && pos - a.window + 1 > lo) lo = pos - a.window + 1;
-    if (row < t0 || row >= t1) hi = 0;
-    float q[8], o[8];
-    const T* x = static_cast<const T*>(a.q) + row * a.qt + head * a.qh;
-#pragma unroll
-    for (int d = 0; d < 8; ++d) {
-        q[d] = d * 32 + lane < dim ? to_f32(x[d * 32 + lane]) : 0.f;
-        o[d] = 0.f;
-    }
-    float m = -INFINITY, sum = 0.f;
-    for (int64_t j = lo; j < hi; ++j) {
-        const int64_t page = page_of(a.seq, a.cache, s, j);
-        if (page < 0) continue;
-        const int64_t block = page * a.cache.kv_heads + kv;
-        const int64_t at = ((block << a.cache.page_log2) + (j & (((int64_t)1 << a.cache.page_log2) - 1))) * dim;
-        float dot = 0.f;
-#pragma unroll
-        for (int d = 0; d < 8; ++d)
-            if (d * 32 + lane < dim) dot += q[d] * code_value<CODE>(a.cache.k[at + d * 32 + lane]);
-#pragma unroll
-        for (int w = 16; w; w >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, w);
-        const float z = dot * a.cache.k_scale[block] * a.scale_log2;
-        const float top = fmaxf(m, z), down = exp2f(m - top), p = exp2f(z - top), pv = p * a.cache.v_scale[block];
-        m = top;
-        sum = sum * down + p;
-#pragma unroll
-        for (int d = 0; d < 8; ++d)
-            if (d * 32 + lane < dim) o[d] = o[d] * down + pv * code_value<CODE>(a.cache.v[at + d * 32 + lane]);
-    }
-    T* y = static_cast<T*>(a.out) + row * a.ot + head * a.oh;
-    const bool none = sum == 0.f;  // no token seen (a NaN sum is not none)
-#pragma unroll
-    for (int d = 0; d < 8; ++d)
-        if (d * 32 + lane < dim) y[d * 32 + lane] = from_f32<T>(none ? 0.f : o[d] / sum);
-    if (a.lse && lane == 0) a.lse[row * a.q_heads + head] = none ? -INFINITY : (m + log2f(sum)) * 0.69314718f;
-}
-
 }  // namespace bfft
+
+#include "bfft_attention_split.cuh"
 
 namespace {
 
@@ -124,12 +79,143 @@ struct Device {
     }
 };
 
+using EncodeTiledFn = PFN_cuTensorMapEncodeTiled_v12000;
+
+EncodeTiledFn encoder() {
+    static EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(p);
+    }();
+    return fn;
+}
+
+// The codes as [pages][kv_heads * page * dim / 128][128 bytes], boxes of 16 tokens,
+// 128-byte swizzle (heads of 64, 128 or 256 elements: whole lines).
+bool encode_codes(CUtensorMap* m, const void* codes, const bfft_cache_desc* c) {
+    EncodeTiledFn enc = encoder();
+    if (!enc) return false;
+    const cuuint64_t lines = (cuuint64_t)(c->kv_heads * c->page * c->dim / 128);
+    cuuint64_t dims[3] = {128, lines, (cuuint64_t)c->pages};
+    cuuint64_t strides[2] = {128, 128 * lines};
+    cuuint32_t box[3] = {128, (cuuint32_t)(c->dim / 8), 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(codes), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count() {
+    static std::atomic<int> counts[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    int n = counts[dev].load(std::memory_order_relaxed);
+    if (!n) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
+        counts[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// How a call is cut: row tiles and chunks of the token axis.
+struct SplitPlan {
+    int nt, tile_tokens, token_tiles, by_token, chunk, chunks;
+    int64_t slots, ctas;
+    size_t bytes;
+};
+
+SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d, int sms) {
+    SplitPlan p;
+    const int64_t group = d->q_heads / c->kv_heads;
+    const int64_t each = q->tokens / q->seqs + (q->tokens % q->seqs != 0);  // rows of a sequence, about
+    p.nt = each * group > 8 && c->dim <= 128 ? 2 : 1;
+    const int64_t rows = 8 * p.nt;
+    p.tile_tokens = group <= rows ? (int)(rows / group) : 1;
+    p.token_tiles = group <= rows ? 1 : (int)((group + rows - 1) / rows);
+    const int64_t runs = q->tokens / p.tile_tokens + q->seqs;
+    p.by_token = q->tokens <= runs;
+    p.slots = p.by_token ? q->tokens : runs;
+    // tokens that a row tile sees at most
+    int64_t cover = q->max_pages * c->page;
+    if (d->causal && d->window > 0) {
+        const int64_t w = d->window + p.tile_tokens + 14;
+        if (w < cover) cover = w;
+    }
+    const int64_t tiles = (q->tokens + p.tile_tokens - 1) / p.tile_tokens;
+    const int64_t units = tiles * p.token_tiles * c->kv_heads, resident = 3 * (int64_t)sms;
+    int64_t chunks = units >= 2 * resident ? (cover + 2047) / 2048 : (2 * resident + units - 1) / units;
+    int64_t chunk = (cover + chunks - 1) / chunks;
+    if (chunk < 256) chunk = 256;
+    if (chunk > 4096) chunk = 4096;
+    chunk = (chunk + 127) / 128 * 128;
+    p.chunk = (int)chunk;
+    const int64_t n = (cover + chunk - 1) / chunk;
+    p.chunks = (int)n;
+    p.ctas = p.slots * p.token_tiles * c->kv_heads * n;
+    p.bytes = n > 1 ? (size_t)(q->tokens * d->q_heads * n) * (size_t)(c->dim + 2) * 4 : 0;
+    return p;
+}
+
+template <int DP, bool EXACT, int NT, typename T, int CODE>
+cudaError_t launch_split(const SplitArgs& a, const SplitPlan& p, const CUtensorMap& km, const CUtensorMap& vm,
+                         cudaStream_t s) {
+    static std::atomic<bool> ready[64];
+    using G = SplitGeo<DP, EXACT, NT>;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    auto* kernel = k_attention_split<DP, EXACT, NT, T, CODE>;
+    if (!ready[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem(DP));
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                     (int)cudaSharedmemCarveoutMaxShared);
+        if (e != cudaSuccess) return e;
+        ready[dev].store(true, std::memory_order_release);
+    }
+    kernel<<<(unsigned)p.ctas, kSplitThreads, G::smem(a.a.cache.dim), s>>>(a, km, vm);
+    return cudaGetLastError();
+}
+
+template <typename T, int CODE>
+cudaError_t split_shape(const SplitArgs& a, const SplitPlan& p, const CUtensorMap& km, const CUtensorMap& vm,
+                        cudaStream_t s) {
+    const int dim = a.a.cache.dim;
+    if (dim == 64)
+        return p.nt == 1 ? launch_split<64, true, 1, T, CODE>(a, p, km, vm, s)
+                         : launch_split<64, true, 2, T, CODE>(a, p, km, vm, s);
+    if (dim == 128)
+        return p.nt == 1 ? launch_split<128, true, 1, T, CODE>(a, p, km, vm, s)
+                         : launch_split<128, true, 2, T, CODE>(a, p, km, vm, s);
+    if (dim == 256) return launch_split<256, true, 1, T, CODE>(a, p, km, vm, s);
+    if (dim < 128)
+        return p.nt == 1 ? launch_split<128, false, 1, T, CODE>(a, p, km, vm, s)
+                         : launch_split<128, false, 2, T, CODE>(a, p, km, vm, s);
+    return launch_split<256, false, 1, T, CODE>(a, p, km, vm, s);
+}
+
 template <typename T>
-void rows_code(int64_t code, const AttentionArgs& a, unsigned grid, cudaStream_t s) {
-    if (code == BFFT_CODE_INT8)
-        k_attention_rows<T, kCodeInt8><<<grid, 256, 0, s>>>(a);
-    else
-        k_attention_rows<T, kCodeE4m3><<<grid, 256, 0, s>>>(a);
+cudaError_t run_split(const SplitArgs& a, const SplitPlan& p, const bfft_cache_desc* c, cudaStream_t s) {
+    CUtensorMap km{}, vm{};
+    if (c->dim == 64 || c->dim == 128 || c->dim == 256)
+        if (!encode_codes(&km, c->k, c) || !encode_codes(&vm, c->v, c)) return cudaErrorNotSupported;
+    cudaError_t e = c->code == BFFT_CODE_INT8 ? split_shape<T, kCodeInt8>(a, p, km, vm, s)
+                                              : split_shape<T, kCodeE4m3>(a, p, km, vm, s);
+    if (e != cudaSuccess || p.chunks == 1) return e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3((unsigned)(a.a.seq.tokens * a.a.q_heads));
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_attention_join<T>, a);
 }
 
 }  // namespace
@@ -139,7 +225,7 @@ extern "C" bfft_status bfft_cache_attention_workspace(const bfft_cache_desc* cac
     if (!bytes) return fail(BFFT_ERR_VALUE, "null pointer");
     const bfft_status st = check(cache, seqs, d);
     if (st != BFFT_OK) return st;
-    *bytes = 0;
+    *bytes = seqs->tokens ? plan_split(cache, seqs, d, sm_count()).bytes : 0;
     return BFFT_OK;
 }
 
@@ -160,16 +246,30 @@ extern "C" bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const 
     a.causal = d->causal != 0;
     a.window = (int)d->window;
     a.scale_log2 = (float)(d->softmax_scale * 1.4426950408889634);
-    const int64_t blocks = (seqs->tokens * d->q_heads + 7) / 8;
-    if (blocks > 0x7fffffffLL) return fail(BFFT_ERR_SHAPE, "too many rows: %lld", (long long)seqs->tokens);
     Device g(d->device);
     if (!g.ok) return fail(BFFT_ERR_CUDA, "cannot select device %lld", (long long)d->device);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    count_launches(1);
-    if (d->type == BFFT_F16)
-        rows_code<__half>(cache->code, a, (unsigned)blocks, s);
-    else
-        rows_code<__nv_bfloat16>(cache->code, a, (unsigned)blocks, s);
-    const cudaError_t e = cudaGetLastError();
+    const SplitPlan p = plan_split(cache, seqs, d, sm_count());
+    if (p.ctas > 0x7fffffffLL || seqs->tokens * d->q_heads > 0x7fffffffLL)
+        return fail(BFFT_ERR_SHAPE, "too many rows: %lld", (long long)seqs->tokens);
+    if (p.bytes && (!d->workspace || d->workspace_bytes < (int64_t)p.bytes))
+        return fail(BFFT_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)d->workspace_bytes,
+                    (long long)p.bytes);
+    if (p.bytes && !aligned(d->workspace, 16)) return fail(BFFT_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+    SplitArgs sa;
+    sa.a = a;
+    sa.parts = static_cast<float*>(d->workspace);
+    sa.stats = sa.parts + seqs->tokens * d->q_heads * p.chunks * cache->dim;
+    sa.chunk = p.chunk;
+    sa.chunks = p.chunks;
+    sa.tile_tokens = p.tile_tokens;
+    sa.token_tiles = p.token_tiles;
+    sa.by_token = p.by_token;
+    sa.slots = p.slots;
+    cudaError_t e = device_status_word(&sa.status);
+    if (e == cudaSuccess) {
+        count_launches(p.chunks > 1 ? 2 : 1);
+        e = d->type == BFFT_F16 ? run_split<__half>(sa, p, cache, s) : run_split<__nv_bfloat16>(sa, p, cache, s);
+    }
     return e == cudaSuccess ? BFFT_OK : fail(BFFT_ERR_CUDA, "cache_attention: %s", cudaGetErrorString(e));
 }

@@ -1,0 +1,700 @@
+// bfft_attention_split.cuh -- attention of few query rows over a long axis of
+// 8-bit tokens (single tokens, drafted tokens).  Included by bfft_attention.cu.
+//
+// Bound by the cache's bytes: with G query heads to a kv head a code (one byte)
+// meets G products, far under the tensor rate, so the design is about keeping
+// loads in flight and spending few instructions on a code:
+//
+// * The token axis is cut into chunks, one CTA per (row tile, kv head, chunk);
+//   its four warps take 32-token tiles in turn, each with a ring of its own that
+//   the copy engine fills (128-byte swizzled boxes for heads of 64, 128 and 256;
+//   plain bulk copies for other widths), so no barrier joins the warps until the
+//   chunk's end.  Parts of several chunks are joined by k_attention_join.
+// * Products on m16n8k16 matrix instructions with tokens as rows and query heads
+//   as columns, S^T = K Q^T and O^T = V^T P^T: eight heads fill a tile (rows of
+//   queries would fill half of a 16-row one).  The order of the 16 products of an
+//   instruction is free, so a lane takes 16 adjacent codes of a token (K) or of
+//   each of four tokens (V) with one 16-byte load and widens them in registers;
+//   both 8-bit types are exact in float16.
+// * A block's key scale multiplies the scores.  Its value scale is folded into
+//   the exponent: p' = 2^(z + log2 vs - m) with m the running maximum of z + log2
+//   vs, so P' (float16) times codes is the weighted value, and the sum takes
+//   p' / vs.  The largest p' is set to 2^14, near float16's top, so that weighted
+//   values keep their bits down to 2^-28 of the largest; m is renewed when one
+//   passes 2^15.5 (a vote instead of a reduction on most tiles).
+#pragma once
+
+namespace bfft {
+
+// Value scale of a zero block: its codes must not count, its weights must.
+constexpr float kZeroLog2 = -64.f;
+constexpr float kTop = 14.f, kRenew = 15.5f;  // log2 of p' at the maximum, and where the maximum is renewed
+
+struct SplitArgs {
+    AttentionArgs a;
+    float* parts;        // [tokens][q_heads][chunks][dim], then m and l as [..][chunks][2]
+    float* stats;
+    int chunk;           // tokens of a chunk, a multiple of 32 * kSplitWarps
+    int chunks;
+    int tile_tokens;     // query tokens of a row tile (group <= rows of a tile), else 1
+    int token_tiles;     // row tiles of a query token (group > rows of a tile), else 1
+    int by_token;        // slots are tokens (else runs of tile_tokens, see slot_rows)
+    int64_t slots;
+    unsigned int* status;
+};
+
+constexpr int kSplitWarps = 4;
+constexpr int kSplitThreads = 32 * kSplitWarps;
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// Four codes of a word as two pairs of float16, exactly.  Int8: c + 128 in the
+// low byte of 1024 (float16 holds integers to 2048), minus 1152.
+template <int CODE>
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (CODE == kCodeInt8) {
+        w ^= 0x80808080u;
+        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+        const uint32_t l = __byte_perm(w, 0x64646464u, 0x4140), h = __byte_perm(w, 0x64646464u, 0x4342);
+        __half2 l2 = __hsub2(*reinterpret_cast<const __half2*>(&l), bias);
+        __half2 h2 = __hsub2(*reinterpret_cast<const __half2*>(&h), bias);
+        lo = *reinterpret_cast<uint32_t*>(&l2);
+        hi = *reinterpret_cast<uint32_t*>(&h2);
+    } else {
+        asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Power of two that brings a row's largest magnitude to [1, 2), and its inverse,
+// so that bfloat16 queries fit float16 (exactly, but for elements under 2^-14 of
+// the row's largest, which lose bits under 2^-24 of it).  1 where the row is zero
+// or not finite.
+template <typename T>
+__device__ __forceinline__ void row_power(float big, float& down, float& up) {
+    down = up = 1.f;
+    if constexpr (sizeof(T) == 2) {
+        const int e = (int)(__float_as_uint(big) >> 23) & 255;
+        if (e > 0 && e < 254) {
+            down = __uint_as_float((uint32_t)(254 - e) << 23);
+            up = __uint_as_float((uint32_t)e << 23);
+        }
+    }
+}
+template <>
+__device__ __forceinline__ void row_power<__half>(float, float& down, float& up) {
+    down = up = 1.f;
+}
+
+// The value scale's part in the exponent, its inverse in the sum, and whether the
+// block's values count (a zero scale) or spoil the rows that see it.
+struct BlockScale {
+    float key;
+    float log2_value;
+    float inv_value;
+    int kind;  // 0 ordinary, 1 zero values, 2 values that are not finite
+};
+__device__ __forceinline__ BlockScale block_scale(float ks, float vs) {
+    BlockScale b;
+    b.key = ks;
+    b.kind = vs == 0.f ? 1 : (vs > 0.f && vs < INFINITY) ? 0 : 2;
+    b.log2_value = b.kind == 0 ? log2f(vs) : kZeroLog2;
+    b.inv_value = b.kind == 0 ? 1.f / vs : 18446744073709551616.f;
+    return b;
+}
+
+// The query tokens [first, first + n) of sequence s that slot i stands for, the
+// first of them row `place` of the sequence's `rows`.
+struct SlotRows {
+    int s;
+    int64_t first, place, rows;
+    int n;
+};
+__device__ __forceinline__ bool slot_rows(const SequenceView& q, int64_t i, int tile, int by_token, SlotRows& r) {
+    int s;
+    if (by_token) {
+        s = find_sequence(q.starts, q.seqs, i);
+    } else {
+        const int lane = threadIdx.x & 31;
+        int lo = 0, n = q.seqs;
+        while (n > 1) {
+            const int step = (n + 31) >> 5, j = lane * step;
+            const bool le = j < n && (int64_t)(q.starts[lo + j] / tile) + (lo + j) <= i;
+            const int c = __popc(__ballot_sync(0xffffffffu, le));
+            const int skip = (c > 0 ? c - 1 : 0) * step;
+            lo += skip;
+            n = n - skip < step ? n - skip : step;
+        }
+        s = lo;
+    }
+    const int64_t t0 = q.starts[s];
+    int64_t t1 = q.starts[s + 1];
+    if (t1 > q.tokens) t1 = q.tokens;
+    if (t0 < 0 || t0 >= t1) return false;
+    int64_t place;
+    if (by_token) {
+        if (i < t0 || i >= t1) return false;
+        place = i - t0;
+        if (place % tile) return false;
+    } else {
+        const int64_t j = i - (t0 / tile + s);
+        if (j < 0) return false;
+        place = j * tile;
+        if (place >= t1 - t0) return false;
+    }
+    r.s = s;
+    r.rows = t1 - t0;
+    r.place = place;
+    r.first = t0 + place;
+    r.n = (int)(r.rows - place < tile ? r.rows - place : tile);
+    return true;
+}
+
+// Tokens [lo, hi) that the row at `pos` sees.
+__device__ __forceinline__ void seen_range(const AttentionArgs& a, int64_t pos, int64_t len, int64_t& lo, int64_t& hi) {
+    hi = a.causal ? pos + 1 : len;
+    if (hi > len) hi = len;
+    lo = 0;
+    if (a.window > 0 && pos - a.window + 1 > 0) lo = pos - a.window + 1;
+}
+
+template <int DP, bool EXACT, int NT>
+struct SplitGeo {
+    static constexpr int STAGES = 2;
+    static constexpr int ROWS = 8 * NT;
+    static constexpr int KS = DP / 16;         // products of 16 along a head
+    static constexpr int VW = DP / 32;         // words of a token's values in a lane
+    static constexpr int MAX_ENTRIES = 4096 / 16 + 1;
+    // a ring stage: keys of both 16-token halves, then values
+    __host__ __device__ static constexpr int half_bytes(int dim) { return 16 * dim; }
+    __host__ __device__ static constexpr int ring_bytes(int dim) {
+        return kSplitWarps * STAGES * 4 * half_bytes(dim);
+    }
+    __host__ __device__ static constexpr int merge_bytes(int dim) { return kSplitWarps * ROWS * (dim + 2) * 4; }
+    __host__ __device__ static constexpr int smem(int dim) {
+        const int r = ring_bytes(dim), m = merge_bytes(dim);
+        return 1024 + (r > m ? r : m) + MAX_ENTRIES * (int)(sizeof(BlockScale) + 4) + 64;
+    }
+};
+
+template <int DP, bool EXACT, int NT, typename T, int CODE>
+__global__ void __launch_bounds__(kSplitThreads)
+    k_attention_split(SplitArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    using G = SplitGeo<DP, EXACT, NT>;
+    extern __shared__ unsigned char smem_raw[];
+    const AttentionArgs& a = p.a;
+    const int dim = EXACT ? DP : a.cache.dim;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
+    unsigned char* ring = align_smem<1024>(smem_raw);
+    const int body = G::ring_bytes(dim) > G::merge_bytes(dim) ? G::ring_bytes(dim) : G::merge_bytes(dim);
+    BlockScale* scales = reinterpret_cast<BlockScale*>(ring + body);
+    int* page_ids = reinterpret_cast<int*>(scales + G::MAX_ENTRIES);
+    __shared__ uint64_t full[kSplitWarps * G::STAGES];
+
+    // which rows and tokens
+    int64_t i = blockIdx.x;
+    const int chunk = (int)(i % p.chunks);
+    i /= p.chunks;
+    const int kv = (int)(i % a.cache.kv_heads);
+    i /= a.cache.kv_heads;
+    const int part = (int)(i % p.token_tiles);
+    const int64_t slot = i / p.token_tiles;
+    if (tid == 0) {
+        for (int b = 0; b < kSplitWarps * G::STAGES; ++b) mbar_init(&full[b], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    SlotRows sr;
+    if (!slot_rows(a.seq, slot, p.tile_tokens, p.by_token, sr)) return;
+    const int head0 = part * G::ROWS;                       // of the group, where a token takes several tiles
+    const int per_token = p.token_tiles > 1 ? min(a.group - head0, G::ROWS) : a.group;
+    const int rows = sr.n * per_token;
+    int64_t len = a.seq.lens[sr.s];
+    const int64_t most = (int64_t)a.seq.max_pages << a.cache.page_log2;
+    if (len > most) len = most;
+    const int64_t pos0 = (int64_t)a.seq.lens[sr.s] - sr.rows + sr.place;
+    int64_t lo_min, hi_max, lo_max, hi_min;
+    seen_range(a, pos0, len, lo_min, hi_min);
+    seen_range(a, pos0 + sr.n - 1, len, lo_max, hi_max);
+    const int64_t base = (lo_min & ~(int64_t)15) + (int64_t)chunk * p.chunk;
+    int64_t end = base + p.chunk;
+    if (end > hi_max) end = hi_max;
+    // row r of the tile: query token r / per_token, head r % per_token
+    auto row_of = [&](int r, int64_t& token, int& head) {
+        const int t = r / per_token;
+        token = sr.first + t;
+        head = kv * a.group + head0 + (r - t * per_token);
+    };
+    if (base >= end) {  // nothing of the axis in this chunk
+        if (tid < rows) {
+            int64_t token;
+            int head;
+            row_of(tid, token, head);
+            if (p.chunks > 1) {
+                float* st = p.stats + ((token * a.q_heads + head) * p.chunks + chunk) * 2;
+                st[0] = -INFINITY;
+                st[1] = 0.f;
+            } else if (a.lse) {
+                a.lse[token * a.q_heads + head] = -INFINITY;
+            }
+        }
+        if (p.chunks == 1)
+            for (int e = tid; e < rows * dim; e += kSplitThreads) {
+                int64_t token;
+                int head;
+                row_of(e / dim, token, head);
+                static_cast<T*>(a.out)[token * a.ot + head * a.oh + e % dim] = from_f32<T>(0.f);
+            }
+        return;
+    }
+    const int lg = a.cache.page_log2;
+    const int64_t page0 = base >> lg;
+    const int entries = (int)(((end - 1) >> lg) - page0) + 1;
+    for (int e = tid; e < entries; e += kSplitThreads) {
+        const int64_t id = a.seq.block_table[sr.s * a.seq.table_stride + page0 + e];
+        page_ids[e] = id >= 0 && id < a.cache.pages ? (int)id : -1;
+    }
+    __syncthreads();
+
+    // ring: tile t of this warp covers tokens [base + 32 (t kSplitWarps + warp), + 32)
+    const int tiles = (int)((end - base + 31) >> 5);
+    unsigned char* mine = ring + warp * (G::STAGES * 4 * G::half_bytes(dim));
+    uint64_t* bars = full + warp * G::STAGES;
+    const int lines = EXACT ? DP / 8 : 1;  // 128-byte lines of 16 tokens
+    auto fetch = [&](int t, int stage) {   // lanes 0..3: keys of half 0, 1, values of half 0, 1
+        const int64_t tok = base + (int64_t)t * 32 + (lane & 1) * 16;
+        int id = -1;
+        if (lane < 4 && tok < end) id = page_ids[(tok >> lg) - page0];
+        const unsigned any = __ballot_sync(0xffffffffu, id >= 0);
+        if (lane == 0) mbar_arrive_expect_tx(&bars[stage], (uint32_t)(__popc(any) * G::half_bytes(dim)));
+        __syncwarp();
+        if (id >= 0) {
+            unsigned char* dst = mine + (stage * 4 + lane) * G::half_bytes(dim);
+            const int slot_in = (int)(tok & (((int64_t)1 << lg) - 1));
+            if constexpr (EXACT) {
+                tma_load_3d(dst, lane < 2 ? &kmap : &vmap, 0, ((kv << lg) + slot_in) / 16 * lines, id, &bars[stage]);
+            } else {
+                const uint8_t* src = (lane < 2 ? a.cache.k : a.cache.v) +
+                                     ((((int64_t)id * a.cache.kv_heads + kv) << lg) + slot_in) * dim;
+                bulk_load(dst, src, (uint32_t)G::half_bytes(dim), &bars[stage]);
+            }
+        }
+    };
+    int ahead = warp;  // next tile to fetch
+    for (int s = 0; s < G::STAGES && ahead < tiles; ++s, ahead += kSplitWarps) fetch(ahead, s);
+    for (int e = tid; e < entries; e += kSplitThreads) {
+        const int id = page_ids[e];
+        if (id >= 0) {
+            const int64_t b = (int64_t)id * a.cache.kv_heads + kv;
+            scales[e] = block_scale(a.cache.k_scale[b], a.cache.v_scale[b]);
+        }
+    }
+
+    // queries as B fragments: lane (g, q4) holds row g of each 8-row tile, dims 16 (4 i + q4) + 4 t ..
+    uint32_t qf[NT][G::KS][2];
+    float row_scale[NT][2];      // of rows 2 q4, 2 q4 + 1: softmax scale (log2) times the row's power
+    int64_t row_lo[NT][2], row_hi[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = nt * 8 + g;
+        float big = 0.f;
+        const T* x = nullptr;
+        if (r < rows) {
+            int64_t token;
+            int head;
+            row_of(r, token, head);
+            x = static_cast<const T*>(a.q) + token * a.qt + head * a.qh;
+        }
+        float e[G::KS][4];
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int d = 16 * (4 * (ks >> 2) + q4) + 4 * (ks & 3) + j;
+                e[ks][j] = x && (EXACT || d < dim) ? to_f32(x[d]) : 0.f;
+                big = fmaxf(big, fabsf(e[ks][j]));
+            }
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        float down, up;
+        row_power<T>(big, down, up);
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks) {
+            qf[nt][ks][0] = pack_f16(e[ks][0] * down, e[ks][1] * down);
+            qf[nt][ks][1] = pack_f16(e[ks][2] * down, e[ks][3] * down);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            row_scale[nt][j] = __shfl_sync(0xffffffffu, up, (2 * q4 + j) * 4) * a.scale_log2;
+            const int rr = nt * 8 + 2 * q4 + j;
+            seen_range(a, pos0 + (rr < rows ? rr / per_token : 0), len, row_lo[nt][j], row_hi[nt][j]);
+        }
+    }
+    __syncthreads();
+
+    float o[NT][2 * G::VW][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2 * G::VW; ++u)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[nt][u][c] = 0.f;
+    }
+
+    auto at = [&](int byte) { return EXACT ? byte ^ (((byte >> 7) & 7) << 4) : byte; };
+    // token of fragment row r < 8: even rows in place, odd ones four apart, so that
+    // the eight lanes of a 16-byte load phase meet eight different banks
+    auto row_token = [](int r) { return (r & 1) ? r ^ 4 : r; };
+    const int tk = row_token(g);
+
+    bool ok = true;
+    int it = 0;
+    for (int t = warp; t < tiles; t += kSplitWarps, ++it) {
+        const int stage = it % G::STAGES;
+        ok = mbar_wait_limited(&bars[stage], (uint32_t)((it / G::STAGES) & 1), p.status);
+        if (__any_sync(0xffffffffu, !ok)) {
+            ok = false;
+            break;
+        }
+        const int64_t tok0 = base + (int64_t)t * 32;
+        const unsigned char* buf = mine + stage * 4 * G::half_bytes(dim);
+        float z[2][NT][4];
+        BlockScale bs[2];
+        bool live[2];
+        float worst = -INFINITY;  // largest z - m of this lane
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t tok = tok0 + 16 * h;
+            const int e = (int)((tok >> lg) - page0);
+            live[h] = tok < end && page_ids[e < entries ? e : entries - 1] >= 0;
+            if (!live[h]) continue;
+            bs[h] = scales[e];
+            const unsigned char* kb = buf + h * G::half_bytes(dim);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) z[h][nt][0] = z[h][nt][1] = z[h][nt][2] = z[h][nt][3] = 0.f;
+#pragma unroll
+            for (int c = 0; c < (DP + 63) / 64; ++c) {
+                uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
+                const int col = 16 * (4 * c + q4);
+                if (EXACT || col < dim) {
+                    w0 = *reinterpret_cast<const uint4*>(kb + at(tk * dim + col));
+                    w1 = *reinterpret_cast<const uint4*>(kb + at((tk + 8) * dim + col));
+                }
+                const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    uint32_t a0, a1, a2, a3;
+                    widen<CODE>(u0[s], a0, a2);
+                    widen<CODE>(u1[s], a1, a3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma_f16(z[h][nt], a0, a1, a2, a3, qf[nt][c * 4 + s][0], qf[nt][c * 4 + s][1]);
+                }
+            }
+            const bool inside = tok >= lo_max && tok + 16 <= hi_min && tok + 16 <= end;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float v = z[h][nt][c] * (bs[h].key * row_scale[nt][c & 1]) + bs[h].log2_value;
+                    if (!inside) {
+                        const int64_t j = tok + tk + (c >> 1) * 8;
+                        if (j < row_lo[nt][c & 1] || j >= row_hi[nt][c & 1] || j >= end) v = -INFINITY;
+                    }
+                    z[h][nt][c] = v;
+                    worst = fmaxf(worst, v == -INFINITY ? v : v - m[nt][c & 1]);
+                }
+        }
+        if (__any_sync(0xffffffffu, worst > kRenew)) {  // a score far over a reference (or the first one): renew them
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (live[h]) top = fmaxf(top, fmaxf(z[h][nt][j], z[h][nt][2 + j]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float now = fmaxf(m[nt][j], top - kTop);
+                    const float f = now == -INFINITY ? 1.f : exp2_approx(m[nt][j] - now);
+                    m[nt][j] = now;
+                    l[nt][j] *= f;
+#pragma unroll
+                    for (int u = 0; u < 2 * G::VW; ++u) {
+                        o[nt][u][j] *= f;
+                        o[nt][u][2 + j] *= f;
+                    }
+                }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (!live[h]) continue;
+            const int64_t tok = tok0 + 16 * h;
+            uint32_t pf[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+                float e0 = exp2_approx(z[h][nt][0] - m0), e1 = exp2_approx(z[h][nt][1] - m1);
+                float e2 = exp2_approx(z[h][nt][2] - m0), e3 = exp2_approx(z[h][nt][3] - m1);
+                l[nt][0] += (e0 + e2) * bs[h].inv_value;
+                l[nt][1] += (e1 + e3) * bs[h].inv_value;
+                if (bs[h].kind) {
+                    if (bs[h].kind == 2) {  // values that are not finite spoil the rows that see one of them
+                        int seen0 = z[h][nt][0] != -INFINITY || z[h][nt][2] != -INFINITY;
+                        int seen1 = z[h][nt][1] != -INFINITY || z[h][nt][3] != -INFINITY;
+#pragma unroll
+                        for (int w = 4; w < 32; w <<= 1) {
+                            seen0 |= __shfl_xor_sync(0xffffffffu, seen0, w);
+                            seen1 |= __shfl_xor_sync(0xffffffffu, seen1, w);
+                        }
+#pragma unroll
+                        for (int u = 0; u < 2 * G::VW; ++u) {
+                            if (seen0) o[nt][u][0] = o[nt][u][2] = __int_as_float(0x7fffffff);
+                            if (seen1) o[nt][u][1] = o[nt][u][3] = __int_as_float(0x7fffffff);
+                        }
+                    }
+                    e0 = e1 = e2 = e3 = 0.f;
+                }
+                pf[nt][0] = movmatrix_trans(pack_f16(e0, e1));
+                pf[nt][1] = movmatrix_trans(pack_f16(e2, e3));
+            }
+            // values: tokens t0, t1, t0 + 8, t1 + 8 of this lane, dims 4 w .. 4 w + 3 of its columns
+            const unsigned char* vb = buf + (2 + h) * G::half_bytes(dim);
+            const int t0 = row_token(2 * q4), t1 = row_token(2 * q4 + 1);
+            const int toks[4] = {t0, t1, t0 + 8, t1 + 8};
+            uint32_t w[4][G::VW];
+            const bool whole = tok >= lo_min && tok + 16 <= end;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (DP == 64) {
+                    uint2 x = make_uint2(0, 0);
+                    if (EXACT || 8 * g < dim) x = *reinterpret_cast<const uint2*>(vb + at(toks[k] * dim + 8 * g));
+                    w[k][0] = x.x;
+                    w[k][1] = x.y;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < DP / 128; ++c) {
+                        uint4 x = make_uint4(0, 0, 0, 0);
+                        const int col = 16 * g + 128 * c;
+                        if (EXACT || col < dim) x = *reinterpret_cast<const uint4*>(vb + at(toks[k] * dim + col));
+                        w[k][4 * c] = x.x;
+                        w[k][4 * c + 1] = x.y;
+                        w[k][4 * c + 2] = x.z;
+                        w[k][4 * c + 3] = x.w;
+                    }
+                }
+                if (!whole) {  // codes of slots that no row sees may be anything: 0 times NaN is NaN
+                    const int64_t j = tok + toks[k];
+                    if (j < lo_min || j >= end)
+#pragma unroll
+                        for (int c = 0; c < G::VW; ++c) w[k][c] = 0;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < G::VW; ++c)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const uint32_t sel = s ? 0x7362 : 0x5140;
+                    uint32_t a0, a1, a2, a3;
+                    widen<CODE>(__byte_perm(w[0][c], w[1][c], sel), a0, a1);
+                    widen<CODE>(__byte_perm(w[2][c], w[3][c], sel), a2, a3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * c + s], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
+                }
+        }
+        __syncwarp();
+        if (ahead < tiles) {
+            fetch(ahead, stage);
+            ahead += kSplitWarps;
+        }
+    }
+    if (!ok)  // status bit 0 is set; wait (bounded) for the copies that are still under way
+        for (int t = warp + kSplitWarps * it; t < ahead; t += kSplitWarps, ++it)
+            mbar_wait_limited(&bars[it % G::STAGES], (uint32_t)((it / G::STAGES) & 1), p.status);
+
+    // join the warps: rows' m and l, then O, through the ring's memory
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 4);
+            l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 8);
+            l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
+        }
+    __syncthreads();
+    float* part_o = reinterpret_cast<float*>(ring);
+    float* part_ml = part_o + kSplitWarps * G::ROWS * dim;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int r = nt * 8 + 2 * q4 + j;
+            float* dst = part_o + (warp * G::ROWS + r) * dim;
+#pragma unroll
+            for (int c = 0; c < G::VW; ++c) {
+                const int d = DP == 64 ? 8 * g + 4 * c : 128 * (c >> 2) + 16 * g + 4 * (c & 3);
+                if (EXACT || d < dim)
+                    *reinterpret_cast<float4*>(dst + d) = make_float4(o[nt][2 * c][j], o[nt][2 * c][2 + j],
+                                                                      o[nt][2 * c + 1][j], o[nt][2 * c + 1][2 + j]);
+            }
+            if (g == 0) {
+                part_ml[(warp * G::ROWS + r) * 2] = m[nt][j];
+                part_ml[(warp * G::ROWS + r) * 2 + 1] = l[nt][j];
+            }
+        }
+    __syncthreads();
+    for (int e = tid; e < rows * (dim / 4); e += kSplitThreads) {
+        const int r = e / (dim / 4), d = (e - r * (dim / 4)) * 4;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kSplitWarps; ++w) top = fmaxf(top, part_ml[(w * G::ROWS + r) * 2]);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kSplitWarps; ++w) {
+            const float mw = part_ml[(w * G::ROWS + r) * 2];
+            const float f = mw == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : exp2_approx(mw - top);
+            const float4 x = *reinterpret_cast<const float4*>(part_o + (w * G::ROWS + r) * dim + d);
+            sum += part_ml[(w * G::ROWS + r) * 2 + 1] * f;
+            v.x += x.x * f;
+            v.y += x.y * f;
+            v.z += x.z * f;
+            v.w += x.w * f;
+        }
+        int64_t token;
+        int head;
+        row_of(r, token, head);
+        if (p.chunks > 1) {
+            const int64_t at_part = (token * a.q_heads + head) * p.chunks + chunk;
+            *reinterpret_cast<float4*>(p.parts + at_part * dim + d) = v;
+            if (d == 0) {
+                p.stats[at_part * 2] = top;
+                p.stats[at_part * 2 + 1] = sum;
+            }
+        } else {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            T* y = static_cast<T*>(a.out) + token * a.ot + head * a.oh + d;
+            y[0] = from_f32<T>(v.x * inv);
+            y[1] = from_f32<T>(v.y * inv);
+            y[2] = from_f32<T>(v.z * inv);
+            y[3] = from_f32<T>(v.w * inv);
+            if (d == 0 && a.lse)
+                a.lse[token * a.q_heads + head] =
+                    sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * 0.693147180559945309f;
+        }
+    }
+}
+
+// Joins the chunks of a (row, head): a CTA each, its warps over the chunks, lanes
+// over the dimensions.  A chunk in which the row saw nothing has l = 0 and no part.
+constexpr int kJoinRun = 512;
+
+template <typename T>
+__global__ void __launch_bounds__(128) k_attention_join(SplitArgs p) {
+    __shared__ float weight[kJoinRun];
+    __shared__ float red[8];
+    __shared__ float4 acc_s[3][64];
+    const AttentionArgs& a = p.a;
+    griddep_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dim = a.cache.dim;
+    const int64_t i = blockIdx.x;
+    const int64_t token = i / a.q_heads;
+    const int head = (int)(i - token * a.q_heads);
+    const float2* st = reinterpret_cast<const float2*>(p.stats) + i * p.chunks;
+    const float* parts = p.parts + i * p.chunks * dim;
+    float top = -INFINITY;
+    for (int c = tid; c < p.chunks; c += 128) top = fmaxf(top, st[c].x);
+#pragma unroll
+    for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    float sum = 0.f;
+    for (int c0 = 0; c0 < p.chunks; c0 += kJoinRun) {
+        const int n = min(kJoinRun, p.chunks - c0);
+        __syncthreads();
+        for (int c = tid; c < n; c += 128) {
+            const float2 v = st[c0 + c];
+            // a NaN sum without a maximum keeps its weight: the row is NaN
+            const float f = v.y == 0.f ? 0.f : v.x == -INFINITY ? 1.f : exp2_approx(v.x - top);
+            weight[c] = f;
+            sum += v.y * f;
+        }
+        __syncthreads();
+#pragma unroll 4
+        for (int c = warp; c < n; c += 4) {
+            const float f = weight[c];
+            const float4* o = reinterpret_cast<const float4*>(parts + (int64_t)(c0 + c) * dim);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (f != 0.f && (k * 32 + lane) * 4 < dim) {
+                    const float4 x = o[k * 32 + lane];
+                    acc[k].x += x.x * f;
+                    acc[k].y += x.y * f;
+                    acc[k].z += x.z * f;
+                    acc[k].w += x.w * f;
+                }
+        }
+    }
+#pragma unroll
+    for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    if (lane == 0) red[4 + warp] = sum;
+    if (warp)
+        for (int k = 0; k < 2; ++k) acc_s[warp - 1][k * 32 + lane] = acc[k];
+    __syncthreads();
+    if (warp) return;
+    sum = (red[4] + red[5]) + (red[6] + red[7]);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T* y = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int d = (k * 32 + lane) * 4;
+        if (d >= dim) continue;
+        float4 v = acc[k];
+#pragma unroll
+        for (int w = 0; w < 3; ++w) {
+            const float4 x = acc_s[w][k * 32 + lane];
+            v.x += x.x;
+            v.y += x.y;
+            v.z += x.z;
+            v.w += x.w;
+        }
+        y[d] = from_f32<T>(v.x * inv);
+        y[d + 1] = from_f32<T>(v.y * inv);
+        y[d + 2] = from_f32<T>(v.z * inv);
+        y[d + 3] = from_f32<T>(v.w * inv);
+    }
+    if (a.lse && lane == 0)
+        a.lse[i] = sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * 0.693147180559945309f;
+}
+
+}  // namespace bfft
