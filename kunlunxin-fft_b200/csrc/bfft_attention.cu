@@ -30,11 +30,13 @@ struct AttentionArgs {
     int q_heads, group;  // group = q_heads / kv_heads
     int causal, window;
     float scale_log2;    // softmax_scale * log2(e)
+    int q_packs, o_packs;  // rows of q / out start on 16 bytes
 };
 
 }  // namespace bfft
 
 #include "bfft_attention_split.cuh"
+#include "bfft_attention_tiles.cuh"
 
 namespace {
 
@@ -120,6 +122,24 @@ int sm_count() {
     return n;
 }
 
+// Tokens that a row tile of `tile` query tokens sees at most.
+int64_t seen_cover(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d, int tile,
+                   int align) {
+    int64_t cover = q->max_pages * c->page;
+    if (d->causal && d->window > 0) {
+        const int64_t w = d->window + tile - 1 + align - 1;
+        if (w < cover) cover = w;
+    }
+    return cover;
+}
+
+// Chunks and slots of the kernel for many rows.
+struct TilePlan {
+    int tile_tokens, by_token, chunk, chunks;
+    int64_t slots, ctas;
+    size_t bytes;
+};
+
 // How a call is cut: row tiles and chunks of the token axis.
 struct SplitPlan {
     int nt, tile_tokens, token_tiles, by_token, chunk, chunks;
@@ -138,12 +158,7 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
     const int64_t runs = q->tokens / p.tile_tokens + q->seqs;
     p.by_token = q->tokens <= runs;
     p.slots = p.by_token ? q->tokens : runs;
-    // tokens that a row tile sees at most
-    int64_t cover = q->max_pages * c->page;
-    if (d->causal && d->window > 0) {
-        const int64_t w = d->window + p.tile_tokens + 14;
-        if (w < cover) cover = w;
-    }
+    const int64_t cover = seen_cover(c, q, d, p.tile_tokens, 16);
     const int64_t tiles = (q->tokens + p.tile_tokens - 1) / p.tile_tokens;
     const int64_t units = tiles * p.token_tiles * c->kv_heads, resident = 3 * (int64_t)sms;
     int64_t chunks = units >= 2 * resident ? (cover + 2047) / 2048 : (2 * resident + units - 1) / units;
@@ -157,6 +172,88 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
     p.ctas = p.slots * p.token_tiles * c->kv_heads * n;
     p.bytes = n > 1 ? (size_t)(q->tokens * d->q_heads * n) * (size_t)(c->dim + 2) * 4 : 0;
     return p;
+}
+
+// Whether a call is one for the tensor-core tiles: with 48 rows or more to a kv
+// head (16 rows of 32 heads over 16384 tokens: 44 us, split kernel 73; 8 rows: 58
+// by either) and enough work to pay for a CTA's start and its 128-row halves, some
+// 3 million (query head, token) pairs of 128 dimensions: 40 rows of 32 heads over
+// 900 tokens 30 us by the split kernel and 42 by this, 128 rows 58 and 48.
+bool use_tiles(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d) {
+    const int64_t group = d->q_heads / c->kv_heads, each = q->tokens / q->seqs;
+    if (c->dim > 128 || group > 128 || each * group < 48) return false;
+    const double pairs = (double)q->tokens * (double)d->q_heads * (double)seen_cover(c, q, d, 1, 1);
+    return pairs * (double)c->dim >= 3.0e6 * 128;
+}
+
+TilePlan plan_tiles(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d, int sms) {
+    TilePlan p;
+    const int64_t group = d->q_heads / c->kv_heads;
+    p.tile_tokens = (int)(256 / group);
+    const int64_t runs = q->tokens / p.tile_tokens + q->seqs;
+    p.by_token = q->tokens <= runs;
+    p.slots = p.by_token ? q->tokens : runs;
+    const int64_t cover = seen_cover(c, q, d, p.tile_tokens, 128);
+    const int64_t units = (q->tokens + p.tile_tokens - 1) / p.tile_tokens * c->kv_heads;
+    int64_t chunks = units >= sms ? 1 : sms / units;
+    int64_t chunk = (cover + chunks - 1) / chunks;
+    if (chunk < 512) chunk = 512;
+    chunk = (chunk + 127) / 128 * 128;
+    if (chunk > 0x7fffff80LL) chunk = 0x7fffff80LL;
+    p.chunk = (int)chunk;
+    p.chunks = (int)((cover + chunk - 1) / chunk);
+    p.ctas = p.slots * c->kv_heads * p.chunks;
+    p.bytes = p.chunks > 1 ? (size_t)(q->tokens * d->q_heads * p.chunks) * (size_t)(c->dim + 2) * 4 : 0;
+    return p;
+}
+
+template <int DP, typename T, int CODE>
+cudaError_t launch_tiles(const TileArgs& a, const TilePlan& p, cudaStream_t s) {
+    static std::atomic<bool> ready[64];
+    using G = TileGeo<DP>;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    auto* kernel = k_attention_tiles<DP, T, CODE>;
+    if (!ready[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
+        if (e != cudaSuccess) return e;
+        ready[dev].store(true, std::memory_order_release);
+    }
+    kernel<<<(unsigned)p.ctas, G::THREADS, G::SMEM, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t run_join(const SplitArgs& a, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3((unsigned)(a.a.seq.tokens * a.a.q_heads));
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_attention_join<T>, a);
+}
+
+template <typename T>
+cudaError_t run_tiles(const TileArgs& a, const TilePlan& p, const bfft_cache_desc* c, cudaStream_t s) {
+    cudaError_t e;
+    if (c->dim <= 64)
+        e = c->code == BFFT_CODE_INT8 ? launch_tiles<64, T, kCodeInt8>(a, p, s) : launch_tiles<64, T, kCodeE4m3>(a, p, s);
+    else
+        e = c->code == BFFT_CODE_INT8 ? launch_tiles<128, T, kCodeInt8>(a, p, s)
+                                      : launch_tiles<128, T, kCodeE4m3>(a, p, s);
+    if (e != cudaSuccess || p.chunks == 1) return e;
+    SplitArgs j{};
+    j.a = a.a;
+    j.parts = a.parts;
+    j.stats = a.stats;
+    j.chunks = a.chunks;
+    return run_join<T>(j, s);
 }
 
 template <int DP, bool EXACT, int NT, typename T, int CODE>
@@ -206,16 +303,7 @@ cudaError_t run_split(const SplitArgs& a, const SplitPlan& p, const bfft_cache_d
     cudaError_t e = c->code == BFFT_CODE_INT8 ? split_shape<T, kCodeInt8>(a, p, km, vm, s)
                                               : split_shape<T, kCodeE4m3>(a, p, km, vm, s);
     if (e != cudaSuccess || p.chunks == 1) return e;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3((unsigned)(a.a.seq.tokens * a.a.q_heads));
-    cfg.blockDim = dim3(128);
-    cfg.stream = s;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_attention_join<T>, a);
+    return run_join<T>(a, s);
 }
 
 }  // namespace
@@ -225,7 +313,11 @@ extern "C" bfft_status bfft_cache_attention_workspace(const bfft_cache_desc* cac
     if (!bytes) return fail(BFFT_ERR_VALUE, "null pointer");
     const bfft_status st = check(cache, seqs, d);
     if (st != BFFT_OK) return st;
-    *bytes = seqs->tokens ? plan_split(cache, seqs, d, sm_count()).bytes : 0;
+    if (!seqs->tokens)
+        *bytes = 0;
+    else
+        *bytes = use_tiles(cache, seqs, d) ? plan_tiles(cache, seqs, d, sm_count()).bytes
+                                           : plan_split(cache, seqs, d, sm_count()).bytes;
     return BFFT_OK;
 }
 
@@ -249,27 +341,35 @@ extern "C" bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const 
     Device g(d->device);
     if (!g.ok) return fail(BFFT_ERR_CUDA, "cannot select device %lld", (long long)d->device);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const SplitPlan p = plan_split(cache, seqs, d, sm_count());
-    if (p.ctas > 0x7fffffffLL || seqs->tokens * d->q_heads > 0x7fffffffLL)
+    a.q_packs = aligned(d->q, 16) && d->q_token % 8 == 0 && d->q_head % 8 == 0;
+    a.o_packs = aligned(d->out, 16) && d->o_token % 8 == 0 && d->o_head % 8 == 0;
+    unsigned int* status;
+    cudaError_t e = device_status_word(&status);
+    if (e != cudaSuccess) return fail(BFFT_ERR_CUDA, "cache_attention: %s", cudaGetErrorString(e));
+    const bool tiles = use_tiles(cache, seqs, d);
+    TilePlan tp{};
+    SplitPlan sp{};
+    if (tiles)
+        tp = plan_tiles(cache, seqs, d, sm_count());
+    else
+        sp = plan_split(cache, seqs, d, sm_count());
+    const int chunks = tiles ? tp.chunks : sp.chunks;
+    const size_t bytes = tiles ? tp.bytes : sp.bytes;
+    if ((tiles ? tp.ctas : sp.ctas) > 0x7fffffffLL || seqs->tokens * d->q_heads > 0x7fffffffLL)
         return fail(BFFT_ERR_SHAPE, "too many rows: %lld", (long long)seqs->tokens);
-    if (p.bytes && (!d->workspace || d->workspace_bytes < (int64_t)p.bytes))
+    if (bytes && (!d->workspace || d->workspace_bytes < (int64_t)bytes))
         return fail(BFFT_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)d->workspace_bytes,
-                    (long long)p.bytes);
-    if (p.bytes && !aligned(d->workspace, 16)) return fail(BFFT_ERR_WORKSPACE, "workspace must be 16-byte aligned");
-    SplitArgs sa;
-    sa.a = a;
-    sa.parts = static_cast<float*>(d->workspace);
-    sa.stats = sa.parts + seqs->tokens * d->q_heads * p.chunks * cache->dim;
-    sa.chunk = p.chunk;
-    sa.chunks = p.chunks;
-    sa.tile_tokens = p.tile_tokens;
-    sa.token_tiles = p.token_tiles;
-    sa.by_token = p.by_token;
-    sa.slots = p.slots;
-    cudaError_t e = device_status_word(&sa.status);
-    if (e == cudaSuccess) {
-        count_launches(p.chunks > 1 ? 2 : 1);
-        e = d->type == BFFT_F16 ? run_split<__half>(sa, p, cache, s) : run_split<__nv_bfloat16>(sa, p, cache, s);
+                    (long long)bytes);
+    if (bytes && !aligned(d->workspace, 16)) return fail(BFFT_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+    float* parts = static_cast<float*>(d->workspace);
+    float* stats = parts ? parts + seqs->tokens * d->q_heads * chunks * cache->dim : nullptr;
+    count_launches(chunks > 1 ? 2 : 1);
+    if (tiles) {
+        TileArgs ta{a, parts, stats, tp.chunk, tp.chunks, tp.tile_tokens, tp.by_token, tp.slots, status};
+        e = d->type == BFFT_F16 ? run_tiles<__half>(ta, tp, cache, s) : run_tiles<__nv_bfloat16>(ta, tp, cache, s);
+    } else {
+        SplitArgs sa{a, parts, stats, sp.chunk, sp.chunks, sp.tile_tokens, sp.token_tiles, sp.by_token, sp.slots, status};
+        e = d->type == BFFT_F16 ? run_split<__half>(sa, sp, cache, s) : run_split<__nv_bfloat16>(sa, sp, cache, s);
     }
     return e == cudaSuccess ? BFFT_OK : fail(BFFT_ERR_CUDA, "cache_attention: %s", cudaGetErrorString(e));
 }
