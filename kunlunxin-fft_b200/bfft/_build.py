@@ -4,7 +4,9 @@
 ``-gencode arch=compute_100a,code=sm_100a`` and records the compiler version
 in ``bfft/_lib/build_meta.json`` (part of the environment fingerprint).  The
 library is linked against the static CUDA runtime and carries no torch
-dependency; the Python layer loads it with ctypes.
+dependency; the Python layer loads it with ctypes.  ``csrc/bfft_torch.cpp``
+(host code only) becomes the extension module ``bfft/_lib/bfft_torch.so``, which
+takes torch tensors to the library's position and cache calls.
 """
 from __future__ import annotations
 
@@ -24,6 +26,8 @@ CSRC = os.path.join(ROOT, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB_DIR = os.path.join(PKG_DIR, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libbfft.so")
+TORCH_SRC = os.path.join(CSRC, "bfft_torch.cpp")
+TORCH_LIB_PATH = os.path.join(LIB_DIR, "bfft_torch.so")
 META_PATH = os.path.join(LIB_DIR, "build_meta.json")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -43,7 +47,7 @@ def sources() -> list[str]:
 
 
 def _deps() -> list[str]:
-    return sources() + sorted(glob.glob(os.path.join(CSRC, "*.cuh"))) + \
+    return sources() + [TORCH_SRC] + sorted(glob.glob(os.path.join(CSRC, "*.cuh"))) + \
         sorted(glob.glob(os.path.join(INCLUDE, "*.h")))
 
 
@@ -66,11 +70,35 @@ def build_meta() -> dict | None:
 
 def up_to_date() -> bool:
     meta = build_meta()
-    return os.path.exists(LIB_PATH) and meta is not None and meta.get("source_hash") == source_hash()
+    return os.path.exists(LIB_PATH) and os.path.exists(TORCH_LIB_PATH) and meta is not None and meta.get("source_hash") == source_hash()
+
+
+def build_torch_module(verbose: bool = True) -> str:
+    """Compile the torch binding against the installed torch's headers, with the
+    host compiler that nvcc uses: its C++ runtime has to be torch's own."""
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    include = os.path.join(root, "include")
+    tmp = TORCH_LIB_PATH + ".tmp"
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE,
+           "-I", sysconfig.get_paths()["include"], "-isystem", include,
+           "-isystem", os.path.join(include, "torch", "csrc", "api", "include"),
+           "-isystem", os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include"),
+           "-o", tmp, TORCH_SRC, "-L", os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+           "-lc10_cuda"]
+    if verbose:
+        print("[bfft] " + " ".join(cmd), file=sys.stderr, flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, TORCH_LIB_PATH)
+    return TORCH_LIB_PATH
 
 
 def build(force: bool = False, verbose: bool = True) -> str:
-    """Compile libbfft.so if its sources changed; returns the library path."""
+    """Compile libbfft.so and the torch binding if their sources changed; returns the library path."""
     if not force and up_to_date():
         return LIB_PATH
     nvcc = nvcc_path()
@@ -81,6 +109,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
         print("[bfft] " + " ".join(cmd), file=sys.stderr, flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB_PATH)
+    build_torch_module(verbose)
     ver = subprocess.run([nvcc, "--version"], capture_output=True, text=True).stdout
     m = re.search(r"release ([0-9.]+), V([0-9.]+)", ver)
     meta = {"nvcc": m.group(2) if m else ver.strip().splitlines()[-1],

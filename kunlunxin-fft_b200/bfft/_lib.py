@@ -105,7 +105,7 @@ def load() -> ctypes.CDLL:
         L.bfft_dist_p2p_attach.argtypes = [vp, ctypes.c_char_p]
         L.bfft_dist_p2p_attach_pointers.argtypes = [vp, ctypes.POINTER(vp)]
         L.bfft_dist_p2p_phase.argtypes = [vp, i32, vp, vp, vp, sz, vp]
-        desc = ctypes.c_char_p  # descriptors of the position and cache calls: packed bytes (see cache.py)
+        desc = ctypes.c_char_p  # descriptors of the position and cache calls: packed bytes
         L.bfft_rotate_positions.argtypes = [desc, vp, vp, vp, vp, vp]
         L.bfft_cache_append.argtypes = [desc, desc, desc, vp]
         L.bfft_cache_read.argtypes = [desc, desc, i64, vp, vp, i64, vp]

@@ -8,7 +8,13 @@ import torch
 
 import bfft
 from bfft import _build, _lib
-from bfft import cache as C
+
+# struct bfft_rotate_desc, bfft_cache_desc, ... of include/bfft.h: every field is 8 bytes wide
+pack_rotate = struct.Struct("19q").pack
+pack_cache = struct.Struct("4Q5q").pack
+pack_sequences = struct.Struct("Qq2Q3q").pack
+pack_append = struct.Struct("6Q15q").pack
+pack_attention = struct.Struct("3Q8qdQ2q").pack
 
 
 @pytest.fixture(scope="module")
@@ -90,23 +96,23 @@ A = 1 << 20  # a 16-byte aligned address: nothing dereferences it before a launc
 
 
 def cache_desc(k=A, v=A, ks=A, vs=A, pages=4, heads=2, page=16, dim=32, code=0):
-    return C._CACHE(k, v, ks, vs, pages, heads, page, dim, code)
+    return pack_cache(k, v, ks, vs, pages, heads, page, dim, code)
 
 
 def seq_desc(table=A, lens=A, starts=A, seqs=1, pages=4, tokens=3):
-    return C._SEQUENCES(table, pages, lens, starts, seqs, pages, tokens)
+    return pack_sequences(table, pages, lens, starts, seqs, pages, tokens)
 
 
 def attention_desc(q=A, out=A, heads=4, kind=2, window=0, scale=1.0, ws=0, size=0):
-    return C._ATTENTION(q, out, 0, 128, 32, 128, 32, heads, kind, 1, window, scale, ws, size, 0)
+    return pack_attention(q, out, 0, 128, 32, 128, 32, heads, kind, 1, window, scale, ws, size, 0)
 
 
 def append_desc(k=A, v=A, q=0, out=0, table=A, rotated=32, kind=2, layout=0, q_heads=0):
-    return C._APPEND(k, v, q, out, 0, table, 64, 32, 64, 32, 0, 0, 0, 0, 100, rotated, q_heads, kind, layout, 0, 0)
+    return pack_append(k, v, q, out, 0, table, 64, 32, 64, 32, 0, 0, 0, 0, 100, rotated, q_heads, kind, layout, 0, 0)
 
 
 def rotate_desc(tokens=3, dim=32, rotated=32, kind=2, layout=0, direction=0):
-    return C._ROTATE(1, tokens, 2, dim, rotated, 0, 64, 32, 0, 64, 32, 0, 1, 100, kind, layout, direction, 0, 0)
+    return pack_rotate(1, tokens, 2, dim, rotated, 0, 64, 32, 0, 64, 32, 0, 1, 100, kind, layout, direction, 0, 0)
 
 
 def test_descriptors_match_the_header():
