@@ -43,28 +43,57 @@ struct alignas(sizeof(T) * P) Pack {
 // c * s.  Int8 codes are symmetric (+-127); e4m3 codes use +-448.
 enum : int { kCodeInt8 = 0, kCodeE4m3 = 1 };
 
+__device__ __forceinline__ float finite(float v) { return fmaxf(v, -3.0e38f); }  // NaN becomes a number
+
 template <int CODE>
 struct CodeRange {
     static constexpr float most = CODE == kCodeInt8 ? 127.f : 448.f;
 };
 
-// Nearest code of v (ties to even), saturating.
-template <int CODE>
-__device__ __forceinline__ uint8_t to_code(float v) {
+// Codes of P values within the block's range (|v| <= most but for the last bit of
+// a product; ties to even).  Int8: v + 1.5 * 2^23 leaves the integer in the low
+// byte.  NaN gives any code but e4m3's NaN: its block reads as NaN through the scale,
+// and a NaN code would reach rows that do not see its token.
+template <int CODE, int P>
+__device__ __forceinline__ Pack<uint8_t, P> to_codes(const float* v) {
+    Pack<uint8_t, P> c;
     if constexpr (CODE == kCodeInt8) {
-        const int q = __float2int_rn(v);  // NaN -> 0: its block reads as NaN through the scale
-        return static_cast<uint8_t>(static_cast<int8_t>(q < -127 ? -127 : (q > 127 ? 127 : q)));
+        uint32_t w[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) w[i] = __float_as_uint(__fadd_rn(v[i], 12582912.f));
+        if constexpr (P % 4 == 0) {
+            uint32_t* q = reinterpret_cast<uint32_t*>(&c);
+#pragma unroll
+            for (int i = 0; i < P; i += 4)
+                q[i / 4] = __byte_perm(__byte_perm(w[i], w[i + 1], 0x0040), __byte_perm(w[i + 2], w[i + 3], 0x0040), 0x5410);
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i) c.v[i] = static_cast<uint8_t>(w[i]);
+        }
+    } else if constexpr (P % 4 == 0) {
+        uint32_t* q = reinterpret_cast<uint32_t*>(&c);
+#pragma unroll
+        for (int i = 0; i < P; i += 4) {
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(finite(v[i]), finite(v[i + 1])), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(finite(v[i + 2]), finite(v[i + 3])), __NV_SATFINITE, __NV_E4M3);
+            q[i / 4] = lo | (hi << 16);
+        }
     } else {
-        return static_cast<uint8_t>(__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3));
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+            c.v[i] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(finite(v[i]), __NV_SATFINITE, __NV_E4M3));
     }
+    return c;
 }
+
+// Nearest code of v (ties to even), saturating.
 template <int CODE>
 __device__ __forceinline__ uint8_t to_code(double v) {
     if constexpr (CODE == kCodeInt8) {
-        const int q = __double2int_rn(v);
+        const int q = __double2int_rn(v);  // NaN gives some code: its block reads as NaN through the scale
         return static_cast<uint8_t>(static_cast<int8_t>(q < -127 ? -127 : (q > 127 ? 127 : q)));
     } else {
-        return static_cast<uint8_t>(__nv_cvt_double_to_fp8(v, __NV_SATFINITE, __NV_E4M3));
+        return static_cast<uint8_t>(__nv_cvt_double_to_fp8(v == v ? v : 0.0, __NV_SATFINITE, __NV_E4M3));
     }
 }
 template <int CODE>

@@ -47,18 +47,28 @@ __device__ __forceinline__ void unit_offsets(const RowShape& r, int u, int& o0, 
 }
 
 template <typename T, int P>
-__device__ __forceinline__ void load_unit(const T* __restrict__ row, int o0, int o1, float (&e)[2 * P]) {
-    const Pack<T, P> a = *reinterpret_cast<const Pack<T, P>*>(row + o0);
-    const Pack<T, P> b = *reinterpret_cast<const Pack<T, P>*>(row + o1);
+struct Unit {
+    Pack<T, P> a, b;
+};
+
+template <typename T, int P>
+__device__ __forceinline__ Unit<T, P> load_unit(const T* row, int o0, int o1) {
+    Unit<T, P> u;
+    u.a = *reinterpret_cast<const Pack<T, P>*>(row + o0);
+    u.b = *reinterpret_cast<const Pack<T, P>*>(row + o1);
+    return u;
+}
+template <typename T, int P>
+__device__ __forceinline__ void widen_unit(const Unit<T, P>& u, float (&e)[2 * P]) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        e[i] = to_f32(a.v[i]);
-        e[P + i] = to_f32(b.v[i]);
+        e[i] = to_f32(u.a.v[i]);
+        e[P + i] = to_f32(u.b.v[i]);
     }
 }
 
 template <typename T, int P>
-__device__ __forceinline__ void store_unit(T* __restrict__ row, int o0, int o1, const float (&e)[2 * P]) {
+__device__ __forceinline__ void store_unit(T* row, int o0, int o1, const float (&e)[2 * P]) {
     Pack<T, P> a, b;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -75,11 +85,22 @@ __device__ __forceinline__ void load_roots(const float2* __restrict__ table, int
                                            float (&c)[P], float (&s)[P]) {
     if (p >= 0 && p < rows) {
         const float2* t = table + p * pairs + u * P;
+        if (P >= 2 && (reinterpret_cast<uintptr_t>(t) & 15) == 0) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const float2 w = t[i];
-            c[i] = w.x;
-            s[i] = w.y;
+            for (int i = 0; i < P; i += 2) {
+                const float4 w = *reinterpret_cast<const float4*>(t + i);
+                c[i] = w.x;
+                s[i] = w.y;
+                c[i + (P > 1)] = w.z;
+                s[i + (P > 1)] = w.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const float2 w = t[i];
+                c[i] = w.x;
+                s[i] = w.y;
+            }
         }
     } else {
 #pragma unroll
@@ -121,37 +142,69 @@ struct RotateArgs {
     float sign;            // of the sine: -1 conjugates
 };
 
+// Heads g, g + step, ... of one token, unit (o0, o1) of each: two heads' loads are
+// in flight before the first product, and the roots are loaded once for all heads.
+// `roots` is called after the first loads (what it waits for runs beside them).
+// y may be x: a thread writes only elements that it has read.
+constexpr int kHeadsAhead = 1;
+template <typename T, int P, int LAYOUT, typename Roots>
+__device__ __forceinline__ void rotate_heads(const T* x, T* y, int64_t xh, int64_t yh, int heads, int g, int step, int o0,
+                                             int o1, bool turns, float sign, Roots roots) {
+    float c[P], s[P];
+    bool have = false;
+    for (int h0 = g; h0 < heads; h0 += kHeadsAhead * step) {
+        Unit<T, P> w[kHeadsAhead];
+#pragma unroll
+        for (int k = 0; k < kHeadsAhead; ++k) {
+            const int h = h0 + k * step;
+            if (h < heads) w[k] = load_unit<T, P>(x + h * xh, o0, o1);
+        }
+        if (!have) {
+            if (turns) {
+                roots(c, s);
+#pragma unroll
+                for (int i = 0; i < P; ++i) s[i] *= sign;
+            }
+            have = true;
+        }
+#pragma unroll
+        for (int k = 0; k < kHeadsAhead; ++k) {
+            const int h = h0 + k * step;
+            if (h >= heads) break;
+            float e[2 * P];
+            widen_unit<T, P>(w[k], e);
+            if (turns) rotate_unit<P, LAYOUT, false>(e, c, s);
+            store_unit<T, P>(y + h * yh, o0, o1, e);
+        }
+    }
+}
+
 template <typename T, int P, int LAYOUT>
-__global__ void __launch_bounds__(256) k_rotate(RotateArgs a) {
+__global__ void __launch_bounds__(256, 3) k_rotate(RotateArgs a) {
     const int u = threadIdx.x;
     const int64_t slot = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const int64_t row = slot / a.groups;
     if (row >= a.rows) return;
     const int g = (int)(slot - row * a.groups);
     const int64_t b = row / a.tokens, t = row - b * a.tokens;
-    const T* x = static_cast<const T*>(a.x) + b * a.xb + t * a.xt;
-    T* y = static_cast<T*>(a.y) + b * a.yb + t * a.yt;
     int o0, o1;
     unit_offsets<P, LAYOUT>(a.shape, u, o0, o1);
-    const bool turns = u < a.shape.rot_units;
-    float c[P], s[P];
-    if (turns) {
-        const int64_t at = b * a.pb + t * a.pt;
-        const int64_t p = a.pos64 ? static_cast<const int64_t*>(a.positions)[at]
-                                  : (int64_t) static_cast<const int32_t*>(a.positions)[at];
-        load_roots<P>(a.table, a.table_rows, a.shape.rotated / 2, p, u, c, s);
-#pragma unroll
-        for (int i = 0; i < P; ++i) s[i] *= a.sign;
-    }
-    for (int h = g; h < a.heads; h += a.groups) {
-        float e[2 * P];
-        load_unit<T, P>(x + h * a.xh, o0, o1, e);
-        if (turns) rotate_unit<P, LAYOUT, false>(e, c, s);
-        store_unit<T, P>(y + h * a.yh, o0, o1, e);
-    }
+    rotate_heads<T, P, LAYOUT>(static_cast<const T*>(a.x) + b * a.xb + t * a.xt, static_cast<T*>(a.y) + b * a.yb + t * a.yt,
+                               a.xh, a.yh, a.heads, g, a.groups, o0, o1, u < a.shape.rot_units, a.sign,
+                               [&](float (&c)[P], float (&s)[P]) {
+                                   const int64_t at = b * a.pb + t * a.pt;
+                                   const int64_t p = a.pos64 ? static_cast<const int64_t*>(a.positions)[at]
+                                                             : (int64_t) static_cast<const int32_t*>(a.positions)[at];
+                                   load_roots<P>(a.table, a.table_rows, a.shape.rotated / 2, p, u, c, s);
+                               });
 }
 
 // ---------------------------------------------------------------- append
+// A call with long runs of new tokens (prompts) takes two launches, its queries'
+// rotation and a block for each run and head; one of short runs (single tokens)
+// takes one, a warp for each run and head and for each token's queries: there the
+// chain of dependent loads (sequence, page, scale) is the time, and warps hide it
+// (256 tokens of 32 + 8 + 8 heads of 128: 41 us with a block of 256 threads each).
 struct AppendArgs {
     CacheView cache;
     SequenceView seq;        // lens: tokens held before the call
@@ -227,126 +280,272 @@ __device__ __forceinline__ int64_t token_position(const AppendArgs& a, int64_t t
                    : (int64_t) static_cast<const int32_t*>(a.positions)[token];
 }
 
-constexpr int kAppendThreads = 128;
+constexpr int kAppendThreads = 256;  // of the kernel of short runs
+constexpr int kRunThreads = 256;     // of the kernel of long runs: two units of 64 rows of 128 elements each
 
-// One run's rows of one kv head, of the keys (ROTATE) or the values: the largest
-// magnitude, the block's new scale, then the codes -- those that the page
-// already held first, where the scale grew.  max is taken on the bits of |x|, so
-// that infinities and NaN survive it: they make the scale NaN or infinite and
-// the block reads as NaN.
-template <typename T, int P, int LAYOUT, int CODE, bool ROTATE>
+// max of |x| that keeps NaN
+__device__ __forceinline__ float max_abs(float m, float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+    return r;
+}
+
+// Unit i of a run: its row and its packs' places.
+struct Place {
+    int row, u, o0, o1;
+};
+template <int P, int LAYOUT>
+__device__ __forceinline__ Place place_of(const RowShape& shape, int i) {
+    Place p;
+    p.row = i / shape.units;
+    p.u = i - p.row * shape.units;
+    unit_offsets<P, LAYOUT>(shape, p.u, p.o0, p.o1);
+    return p;
+}
+
+// What a thread holds of a run, the same for all heads: the places of HELD units and
+// (keys) their roots.
+template <int P, int HELD>
+struct RunUnits {
+    Place at[HELD];
+    bool has[HELD], turns[HELD];
+    float c[HELD][P], s[HELD][P];
+};
+template <int P, int LAYOUT, bool ROTATE, int HELD>
+__device__ __forceinline__ void find_units(const AppendArgs& a, const Run& r, int tid, int threads, RunUnits<P, HELD>& m) {
+    const RowShape& shape = ROTATE ? a.k_shape : a.v_shape;
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+        const int i = tid + k * threads;
+        m.has[k] = i < (int)r.n * shape.units;
+        m.at[k] = place_of<P, LAYOUT>(shape, i);
+        m.turns[k] = ROTATE && m.has[k] && m.at[k].u < shape.rot_units;
+        if (m.turns[k])
+            load_roots<P>(a.table, a.table_rows, shape.rotated / 2,
+                          token_position(a, r.first + m.at[k].row, r.at + m.at[k].row), m.at[k].u, m.c[k], m.s[k]);
+    }
+}
+template <typename T, int P, bool ROTATE, int HELD>
+__device__ __forceinline__ void fetch_units(const AppendArgs& a, const Run& r, int head, const RunUnits<P, HELD>& m,
+                                            Unit<T, P> (&raw)[HELD]) {
+    const T* x = static_cast<const T*>(ROTATE ? a.k : a.v) + head * (ROTATE ? a.kh : a.vh);
+    const int64_t xt = ROTATE ? a.kt : a.vt;
+#pragma unroll
+    for (int k = 0; k < HELD; ++k)
+        if (m.has[k]) raw[k] = load_unit<T, P>(x + (r.first + m.at[k].row) * xt, m.at[k].o0, m.at[k].o1);
+}
+
+// One run's rows of one kv head, of the keys (ROTATE) or the values, by `threads`
+// threads: the largest magnitude, the block's new scale, then the codes -- those
+// that the page already held first, where the scale grew.  An infinity or a
+// NaN survives the maximum: it makes the scale NaN, so that the block reads as NaN.
+// The HELD units a thread of `raw` are rotated once and stay in registers; a longer
+// run's others are read for the maximum and again for the codes.
+template <typename T, int P, int LAYOUT, int CODE, bool ROTATE, int HELD, typename Most>
 __device__ __forceinline__ void append_rows(const AppendArgs& a, const Run& r, int64_t page_id, int head,
-                                            uint32_t* shared_max) {
+                                            const RunUnits<P, HELD>& m, const Unit<T, P> (&raw)[HELD], int tid, int threads,
+                                            Most most_of) {
     const RowShape& shape = ROTATE ? a.k_shape : a.v_shape;
     const T* x = static_cast<const T*>(ROTATE ? a.k : a.v) + head * (ROTATE ? a.kh : a.vh);
     const int64_t xt = ROTATE ? a.kt : a.vt;
-    const int tid = threadIdx.x, dim = a.cache.dim;
+    const int dim = a.cache.dim;
+    const int old = (int)(r.at & (((int64_t)1 << a.cache.page_log2) - 1));
+    const int total = (int)r.n * shape.units;
     const int64_t block = page_id * a.cache.kv_heads + head;
     uint8_t* codes = (ROTATE ? a.cache.k : a.cache.v) + ((block << a.cache.page_log2) * dim);
     float* scale = (ROTATE ? a.cache.k_scale : a.cache.v_scale) + block;
-    const int old = (int)(r.at & (((int64_t)1 << a.cache.page_log2) - 1));
-    const int total = (int)r.n * shape.units;
+    const float before = old > 0 ? *scale : 0.f;
 
-    auto value = [&](int i, float (&e)[2 * P], int& o0, int& o1, int& row) {
-        row = i / shape.units;
-        const int u = i - row * shape.units;
-        unit_offsets<P, LAYOUT>(shape, u, o0, o1);
-        load_unit<T, P>(x + (r.first + row) * xt, o0, o1, e);
-        if (ROTATE && u < shape.rot_units) {
+    auto value = [&](const Place& p, float (&e)[2 * P]) {
+        widen_unit<T, P>(load_unit<T, P>(x + (r.first + p.row) * xt, p.o0, p.o1), e);
+        if (ROTATE && p.u < shape.rot_units) {
             float c[P], s[P];
-            load_roots<P>(a.table, a.table_rows, shape.rotated / 2, token_position(a, r.first + row, r.at + row), u, c,
+            load_roots<P>(a.table, a.table_rows, shape.rotated / 2, token_position(a, r.first + p.row, r.at + p.row), p.u, c,
                           s);
             rotate_unit<P, LAYOUT, true>(e, c, s);
         }
     };
-
-    uint32_t big = 0;
-    for (int i = tid; i < total; i += kAppendThreads) {
+    float held[HELD][2 * P];
+    float most = 0.f;
+#pragma unroll
+    for (int k = 0; k < HELD; ++k)
+        if (m.has[k]) {
+            widen_unit<T, P>(raw[k], held[k]);
+            if (m.turns[k]) rotate_unit<P, LAYOUT, true>(held[k], m.c[k], m.s[k]);
+#pragma unroll
+            for (int j = 0; j < 2 * P; ++j) most = max_abs(most, held[k][j]);
+        }
+#pragma unroll 1
+    for (int i = tid + HELD * threads; i < total; i += threads) {
         float e[2 * P];
-        int o0, o1, row;
-        value(i, e, o0, o1, row);
+        value(place_of<P, LAYOUT>(shape, i), e);
 #pragma unroll
-        for (int j = 0; j < 2 * P; ++j) big = max(big, __float_as_uint(e[j]) & 0x7fffffffu);
+        for (int j = 0; j < 2 * P; ++j) most = max_abs(most, e[j]);
     }
-    big = __reduce_max_sync(0xffffffffu, big);
-    if ((tid & 31) == 0) shared_max[tid >> 5] = big;
-    const float before = old > 0 ? *scale : 0.f;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; ++w) big = max(big, shared_max[w]);
+    // the order of magnitudes' bits puts NaN over infinity over numbers; also orders the reads of the scale before
+    // its write
+    const uint32_t big = most_of(__float_as_uint(most) & 0x7fffffffu);
     // a block under 2^-126 * most is zero: no denormal scales
     float now = __uint_as_float(big) / CodeRange<CODE>::most;
     if (now < 1.17549435e-38f) now = 0.f;
+    if (big >= 0x7f800000u) now = __int_as_float(0x7fffffff);
     now = __uint_as_float(max(__float_as_uint(now), __float_as_uint(before) & 0x7fffffffu));
     const float inv = now == 0.f ? 0.f : 1.f / now;
     if (old > 0 && now != before) {
         // codes times the ratio of the scales, in 64 bits: in 32 the three roundings of
         // a code of 127 (127 * 3 * 2^-24) could pass a value over the middle of two codes
         const double shrink = (double)before / (double)now;
-        for (int i = tid; i < old * dim / 16; i += kAppendThreads) {
+#pragma unroll 1
+        for (int i = tid; i < old * dim / 16; i += threads) {
             Pack<uint8_t, 16> c = reinterpret_cast<const Pack<uint8_t, 16>*>(codes)[i];
-#pragma unroll
+#pragma unroll 4
             for (int j = 0; j < 16; ++j) c.v[j] = to_code<CODE>((double)code_value<CODE>(c.v[j]) * shrink);
             reinterpret_cast<Pack<uint8_t, 16>*>(codes)[i] = c;
         }
     }
     if (tid == 0) *scale = now;
-    for (int i = tid; i < total; i += kAppendThreads) {
-        float e[2 * P];
-        int o0, o1, row;
-        value(i, e, o0, o1, row);
-        Pack<uint8_t, P> c0, c1;
+    auto write = [&](const Place& p, float (&e)[2 * P]) {
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-            c0.v[j] = to_code<CODE>(e[j] * inv);
-            c1.v[j] = to_code<CODE>(e[P + j] * inv);
-        }
-        uint8_t* to = codes + (old + row) * dim;
-        *reinterpret_cast<Pack<uint8_t, P>*>(to + o0) = c0;
-        *reinterpret_cast<Pack<uint8_t, P>*>(to + o1) = c1;
+        for (int j = 0; j < 2 * P; ++j) e[j] = __fmul_rn(e[j], inv);
+        uint8_t* to = codes + (old + p.row) * dim;
+        *reinterpret_cast<Pack<uint8_t, P>*>(to + p.o0) = to_codes<CODE, P>(e);
+        *reinterpret_cast<Pack<uint8_t, P>*>(to + p.o1) = to_codes<CODE, P>(e + P);
+    };
+#pragma unroll
+    for (int k = 0; k < HELD; ++k)
+        if (m.has[k]) write(m.at[k], held[k]);
+#pragma unroll 1
+    for (int i = tid + HELD * threads; i < total; i += threads) {
+        const Place p = place_of<P, LAYOUT>(shape, i);
+        float e[2 * P];
+        value(p, e);
+        write(p, e);
     }
 }
 
-// Blocks [0, slots * kv_heads * 2): a run's keys or values of one head.  The
-// blocks behind them rotate the queries, one token each.
+// A block for each run and group of kv heads, of keys or values: the run, its page
+// and its roots are found once for the group's heads, and a head's rows load while
+// the head before is coded.
+template <typename T, int P, int LAYOUT, int CODE, bool ROTATE, int HELD>
+__device__ __forceinline__ void append_heads(const AppendArgs& a, const Run& r, int first, int last,
+                                             uint32_t (*shared_max)[kRunThreads / 32]) {
+    RunUnits<P, HELD> m;
+    Unit<T, P> raw[HELD], next[HELD];
+    find_units<P, LAYOUT, ROTATE, HELD>(a, r, threadIdx.x, kRunThreads, m);
+    fetch_units<T, P, ROTATE, HELD>(a, r, first, m, next);
+    const int64_t page_id = page_of(a.seq, a.cache, r.s, r.at);
+    if (page_id < 0) return;
+    for (int head = first; head < last; ++head) {
+#pragma unroll
+        for (int k = 0; k < HELD; ++k) raw[k] = next[k];
+        if (head + 1 < last) fetch_units<T, P, ROTATE, HELD>(a, r, head + 1, m, next);
+        auto most_of = [&](uint32_t big) {
+            big = __reduce_max_sync(0xffffffffu, big);
+            if ((threadIdx.x & 31) == 0) shared_max[head & 1][threadIdx.x >> 5] = big;
+            __syncthreads();
+            return __reduce_max_sync(0xffffffffu, shared_max[head & 1][threadIdx.x & (kRunThreads / 32 - 1)]);
+        };
+        append_rows<T, P, LAYOUT, CODE, ROTATE, HELD>(a, r, page_id, head, m, raw, threadIdx.x, kRunThreads, most_of);
+    }
+}
+
 template <typename T, int P, int LAYOUT, int CODE>
-__global__ void __launch_bounds__(kAppendThreads) k_append(AppendArgs a) {
-    __shared__ uint32_t shared_max[kAppendThreads / 32];
-    const int64_t per_slot = 2 * a.cache.kv_heads;
-    const int64_t runs = a.slots * per_slot;
-    int64_t i = blockIdx.x;
+__global__ void __launch_bounds__(kRunThreads, 2) k_append_runs(AppendArgs a, int heads_per_block) {
+    __shared__ uint32_t shared_max[2][kRunThreads / 32];
+    const int heads = a.cache.kv_heads, parts = (heads + heads_per_block - 1) / heads_per_block;
+    const int64_t slot = blockIdx.x / (2 * parts);
+    const int which = (int)(blockIdx.x - slot * 2 * parts);
+    Run r;
+    if (!run_of_slot(a, slot, r)) return;
+    const bool keys = which < parts;
+    const int first = (keys ? which : which - parts) * heads_per_block;
+    const int last = first + heads_per_block < heads ? first + heads_per_block : heads;
+    constexpr int HELD = P >= 4 ? 2 : 4;
+    if (keys)
+        append_heads<T, P, LAYOUT, CODE, true, HELD>(a, r, first, last, shared_max);
+    else
+        append_heads<T, P, LAYOUT, CODE, false, HELD>(a, r, first, last, shared_max);
+}
+
+// A warp's run of one kv head.
+template <typename T, int P, int LAYOUT, int CODE, bool ROTATE>
+__device__ __forceinline__ void append_warp(const AppendArgs& a, const Run& r, int head, int lane) {
+    RunUnits<P, 1> m;
+    Unit<T, P> raw[1];
+    find_units<P, LAYOUT, ROTATE, 1>(a, r, lane, 32, m);
+    fetch_units<T, P, ROTATE, 1>(a, r, head, m, raw);
+    const int64_t page_id = page_of(a.seq, a.cache, r.s, r.at);
+    if (page_id < 0) return;
+    append_rows<T, P, LAYOUT, CODE, ROTATE, 1>(a, r, page_id, head, m, raw, lane, 32,
+                                               [](uint32_t big) { return __reduce_max_sync(0xffffffffu, big); });
+}
+
+// Position of a new token.
+__device__ __forceinline__ int64_t new_position(const AppendArgs& a, int64_t token, int s) {
+    return token_position(a, token, (int64_t)a.seq.lens[s] + (token - a.seq.starts[s]));
+}
+
+// Warps [0, slots * kv_heads * 2): a run's keys or values of one head.  The warps
+// behind them rotate the queries, one token each.
+template <typename T, int P, int LAYOUT, int CODE>
+__global__ void __launch_bounds__(kAppendThreads, 3) k_append(AppendArgs a) {
+    const int lane = threadIdx.x & 31;
+    const int64_t per_slot = 2 * a.cache.kv_heads, runs = a.slots * per_slot;
+    const int64_t i = (int64_t)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
     if (i < runs) {
         const int64_t slot = i / per_slot;
         const int which = (int)(i - slot * per_slot);
         Run r;
         if (!run_of_slot(a, slot, r)) return;
-        const int64_t page_id = page_of(a.seq, a.cache, r.s, r.at);
-        if (page_id < 0) return;
         if (which < a.cache.kv_heads)
-            append_rows<T, P, LAYOUT, CODE, true>(a, r, page_id, which, shared_max);
+            append_warp<T, P, LAYOUT, CODE, true>(a, r, which, lane);
         else
-            append_rows<T, P, LAYOUT, CODE, false>(a, r, page_id, which - a.cache.kv_heads, shared_max);
+            append_warp<T, P, LAYOUT, CODE, false>(a, r, which - a.cache.kv_heads, lane);
         return;
     }
     const int64_t token = i - runs;
+    if (!a.q || token >= a.seq.tokens) return;
     const int s = find_sequence(a.seq.starts, a.seq.seqs, token);
-    const int64_t p = token_position(a, token, (int64_t)a.seq.lens[s] + (token - a.seq.starts[s]));
-    const T* x = static_cast<const T*>(a.q) + token * a.qt;
-    T* y = static_cast<T*>(a.q_out) + token * a.ot;
     const RowShape& shape = a.k_shape;
-    for (int j = threadIdx.x; j < a.q_heads * shape.units; j += kAppendThreads) {
-        const int h = j / shape.units, u = j - h * shape.units;
+    const int64_t p = new_position(a, token, s);
+    // the lanes over the units of one or several heads
+    const int across = shape.units < 32 ? shape.units : 32, heads = 32 / across;
+    for (int u = lane % across; u < shape.units && lane < across * heads; u += across) {
         int o0, o1;
         unit_offsets<P, LAYOUT>(shape, u, o0, o1);
-        float e[2 * P];
-        load_unit<T, P>(x + h * a.qh, o0, o1, e);
-        if (u < shape.rot_units) {
-            float c[P], sn[P];
-            load_roots<P>(a.table, a.table_rows, shape.rotated / 2, p, u, c, sn);
-            rotate_unit<P, LAYOUT, false>(e, c, sn);
-        }
-        store_unit<T, P>(y + h * a.oh, o0, o1, e);
+        rotate_heads<T, P, LAYOUT>(static_cast<const T*>(a.q) + token * a.qt, static_cast<T*>(a.q_out) + token * a.ot, a.qh,
+                                   a.oh, a.q_heads, lane / across, heads, o0, o1, u < shape.rot_units, 1.f,
+                                   [&](float (&c)[P], float (&sn)[P]) {
+                                       load_roots<P>(a.table, a.table_rows, shape.rotated / 2, p, u, c, sn);
+                                   });
     }
+}
+
+// The queries of long runs: as k_rotate, the position from the token's sequence.
+template <typename T, int P, int LAYOUT>
+__global__ void __launch_bounds__(256, 3) k_rotate_new(AppendArgs a, int groups, int rows_per_block) {
+    __shared__ int64_t position[256];
+    const int units = a.k_shape.units;
+    const int64_t token0 = (int64_t)blockIdx.x * rows_per_block;
+    // a warp for each of the block's tokens in turn finds its position
+    for (int r = threadIdx.x >> 5; r < rows_per_block; r += 8) {
+        const int64_t token = token0 + r;
+        if (token >= a.seq.tokens) break;
+        const int s = find_sequence(a.seq.starts, a.seq.seqs, token);
+        if ((threadIdx.x & 31) == 0) position[r] = new_position(a, token, s);
+    }
+    __syncthreads();
+    const int per = units * groups, r = threadIdx.x / per, at = threadIdx.x - r * per;
+    const int64_t token = token0 + r;
+    if (r >= rows_per_block || token >= a.seq.tokens) return;
+    const int g = at / units, u = at - g * units;
+    int o0, o1;
+    unit_offsets<P, LAYOUT>(a.k_shape, u, o0, o1);
+    rotate_heads<T, P, LAYOUT>(static_cast<const T*>(a.q) + token * a.qt, static_cast<T*>(a.q_out) + token * a.ot, a.qh, a.oh,
+                               a.q_heads, g, groups, o0, o1, u < a.k_shape.rot_units, 1.f,
+                               [&](float (&c)[P], float (&sn)[P]) {
+                                   load_roots<P>(a.table, a.table_rows, a.k_shape.rotated / 2, position[r], u, c, sn);
+                               });
 }
 
 // ---------------------------------------------------------------- read
@@ -368,6 +567,7 @@ __global__ void __launch_bounds__(256) k_read(ReadArgs a) {
     const int64_t page_id = t < a.seq.starts[s] ? -1 : page_of(a.seq, a.cache, s, at);
     const int slot = (int)(at & (((int64_t)1 << a.cache.page_log2) - 1));
     const int chunks = dim / 16, half = heads * chunks;
+#pragma unroll 4
     for (int i = lane; i < 2 * half; i += 32) {
         const bool is_v = i >= half;
         const int j = is_v ? i - half : i;
@@ -449,27 +649,44 @@ void rotate_pack(int p, int layout, const RotateArgs& a, dim3 grid, dim3 block, 
     rotate_layout<T, 1>(layout, a, grid, block, s);
 }
 
+// Launches of one append; `runs`: by runs (see AppendArgs).
+struct AppendPlan {
+    bool runs;
+    unsigned blocks;              // of the kernel of keys and values (and queries, where not by runs)
+    int heads_per_block;          // kv heads, by runs
+    int groups, rows_per_block;   // of the queries' rotation by runs
+    unsigned q_blocks;
+};
+
 template <typename T, int P, int LAYOUT>
-void append_code(int code, const AppendArgs& a, dim3 grid, cudaStream_t s) {
+void append_code(int code, const AppendArgs& a, const AppendPlan& p, cudaStream_t s) {
+    if (!p.runs) {
+        if (code == BFFT_CODE_INT8)
+            k_append<T, P, LAYOUT, kCodeInt8><<<p.blocks, kAppendThreads, 0, s>>>(a);
+        else
+            k_append<T, P, LAYOUT, kCodeE4m3><<<p.blocks, kAppendThreads, 0, s>>>(a);
+        return;
+    }
+    if (p.q_blocks) k_rotate_new<T, P, LAYOUT><<<p.q_blocks, 256, 0, s>>>(a, p.groups, p.rows_per_block);
     if (code == BFFT_CODE_INT8)
-        k_append<T, P, LAYOUT, kCodeInt8><<<grid, kAppendThreads, 0, s>>>(a);
+        k_append_runs<T, P, LAYOUT, kCodeInt8><<<p.blocks, kRunThreads, 0, s>>>(a, p.heads_per_block);
     else
-        k_append<T, P, LAYOUT, kCodeE4m3><<<grid, kAppendThreads, 0, s>>>(a);
+        k_append_runs<T, P, LAYOUT, kCodeE4m3><<<p.blocks, kRunThreads, 0, s>>>(a, p.heads_per_block);
 }
 template <typename T, int P>
-void append_layout(int layout, int code, const AppendArgs& a, dim3 grid, cudaStream_t s) {
+void append_layout(int layout, int code, const AppendArgs& a, const AppendPlan& p, cudaStream_t s) {
     if (layout == BFFT_PAIRS_HALF)
-        append_code<T, P, BFFT_PAIRS_HALF>(code, a, grid, s);
+        append_code<T, P, BFFT_PAIRS_HALF>(code, a, p, s);
     else
-        append_code<T, P, BFFT_PAIRS_INTERLEAVED>(code, a, grid, s);
+        append_code<T, P, BFFT_PAIRS_INTERLEAVED>(code, a, p, s);
 }
 template <typename T>
-void append_pack(int p, int layout, int code, const AppendArgs& a, dim3 grid, cudaStream_t s) {
+void append_pack(int pack, int layout, int code, const AppendArgs& a, const AppendPlan& p, cudaStream_t s) {
     if constexpr (sizeof(T) == 2)
-        if (p == 8) return append_layout<T, 8>(layout, code, a, grid, s);
-    if (p == 4) return append_layout<T, 4>(layout, code, a, grid, s);
-    if (p == 2) return append_layout<T, 2>(layout, code, a, grid, s);
-    append_layout<T, 1>(layout, code, a, grid, s);
+        if (pack == 8) return append_layout<T, 8>(layout, code, a, p, s);
+    if (pack == 4) return append_layout<T, 4>(layout, code, a, p, s);
+    if (pack == 2) return append_layout<T, 2>(layout, code, a, p, s);
+    append_layout<T, 1>(layout, code, a, p, s);
 }
 
 template <typename T>
@@ -591,7 +808,11 @@ extern "C" bfft_status bfft_rotate_positions(const bfft_rotate_desc* d, const vo
     a.table_rows = d->table_rows;
     a.shape = row_shape(d->dim, d->rotated, p);
     a.heads = (int)d->heads;
-    a.groups = a.heads;
+    // a thread takes eight heads of its token (the roots are loaded once for them),
+    // fewer where that leaves the GPU without 1024 threads to an SM
+    int per = 8;
+    while (per > 1 && a.rows * ((a.heads + per - 1) / per) * a.shape.units < (int64_t)148 * 1024) per /= 2;
+    a.groups = (a.heads + per - 1) / per;
     a.pos64 = d->pos64 != 0;
     a.sign = d->transform_direction == BFFT_INVERSE ? -1.f : 1.f;
     dim3 block((unsigned)a.shape.units, 1);
@@ -654,20 +875,39 @@ extern "C" bfft_status bfft_cache_append(const bfft_cache_desc* cache, const bff
     const int64_t runs = seqs->tokens / cache->page + 2 * seqs->seqs;
     a.by_token = seqs->tokens <= runs;
     a.slots = a.by_token ? seqs->tokens : runs;
-    const int64_t blocks = a.slots * 2 * cache->kv_heads + (d->q ? seqs->tokens : 0);
+    AppendPlan plan{};
+    plan.runs = !a.by_token && seqs->tokens >= 16 * seqs->seqs;
+    int64_t blocks = a.slots * 2 * cache->kv_heads, q_blocks = 0;
+    if (plan.runs) {
+        // four kv heads a block, fewer where that leaves less than four blocks to an SM
+        plan.heads_per_block = 4;
+        while (plan.heads_per_block > 1 &&
+               a.slots * 2 * ((cache->kv_heads + plan.heads_per_block - 1) / plan.heads_per_block) < 4 * 148)
+            plan.heads_per_block /= 2;
+        blocks = a.slots * 2 * ((cache->kv_heads + plan.heads_per_block - 1) / plan.heads_per_block);
+        // threads over the units of a group of heads, eight heads a thread at most
+        const int units = a.k_shape.units;
+        plan.groups = (int)((d->q_heads + 7) / 8);
+        while (plan.groups > 1 && units * plan.groups > 256) plan.groups = (plan.groups + 1) / 2;
+        plan.rows_per_block = 256 / (units * (plan.groups > 0 ? plan.groups : 1));
+        if (d->q) q_blocks = (seqs->tokens + plan.rows_per_block - 1) / plan.rows_per_block;
+    } else {
+        blocks = (blocks + (d->q ? seqs->tokens : 0) + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
+    }
     if (blocks > 0x7fffffffLL) return fail(BFFT_ERR_SHAPE, "too many rows: %lld", (long long)seqs->tokens);
+    plan.blocks = (unsigned)blocks;
+    plan.q_blocks = (unsigned)q_blocks;
     Device g(d->device);
     if (!g.ok) return fail(BFFT_ERR_CUDA, "cannot select device %lld", (long long)d->device);
-    const dim3 grid((unsigned)blocks);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int layout = (int)d->layout, code = (int)cache->code;
-    count_launches(1);
+    count_launches(q_blocks ? 2 : 1);
     if (d->type == BFFT_F32)
-        append_pack<float>(p, layout, code, a, grid, s);
+        append_pack<float>(p, layout, code, a, plan, s);
     else if (d->type == BFFT_F16)
-        append_pack<__half>(p, layout, code, a, grid, s);
+        append_pack<__half>(p, layout, code, a, plan, s);
     else
-        append_pack<__nv_bfloat16>(p, layout, code, a, grid, s);
+        append_pack<__nv_bfloat16>(p, layout, code, a, plan, s);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? BFFT_OK : fail(BFFT_ERR_CUDA, "cache_append: %s", cudaGetErrorString(e));
 }
