@@ -161,11 +161,18 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
     const int64_t cover = seen_cover(c, q, d, p.tile_tokens, 16);
     const int64_t tiles = (q->tokens + p.tile_tokens - 1) / p.tile_tokens;
     const int64_t units = tiles * p.token_tiles * c->kv_heads, resident = 3 * (int64_t)sms;
-    int64_t chunks = units >= 2 * resident ? (cover + 2047) / 2048 : (2 * resident + units - 1) / units;
+    // Where rows are many, chunks of 2048 tokens (512..4096 measure alike for 64 ragged
+    // sequences).  Where they are few the axis is shared out over one wave of CTAs: a
+    // second wave's start costs more than it hides (one sequence of 131001 tokens: 71.6
+    // us, two waves 75.8, three 84.0) unless many sequences of different lengths leave
+    // the first one ragged (16 of 2000..8000: 63.5 us in one, 59.4 in two, 69.6 in three).
+    const int64_t waves = q->seqs > 8 ? 2 : 1;
+    int64_t chunks = units >= 2 * resident ? (cover + 2047) / 2048 : waves * resident / units;
+    if (chunks < 1) chunks = 1;
     int64_t chunk = (cover + chunks - 1) / chunks;
+    chunk = (chunk + 31) / 32 * 32;
     if (chunk < 256) chunk = 256;
     if (chunk > 4096) chunk = 4096;
-    chunk = (chunk + 127) / 128 * 128;
     p.chunk = (int)chunk;
     const int64_t n = (cover + chunk - 1) / chunk;
     p.chunks = (int)n;
@@ -230,13 +237,14 @@ cudaError_t run_join(const SplitArgs& a, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     cfg.gridDim = dim3((unsigned)(a.a.seq.tokens * a.a.q_heads));
-    cfg.blockDim = dim3(128);
+    const bool many = a.chunks > 16;
+    cfg.blockDim = dim3(many ? 512 : 128);
     cfg.stream = s;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_attention_join<T>, a);
+    return many ? cudaLaunchKernelEx(&cfg, k_attention_join<T, 16>, a) : cudaLaunchKernelEx(&cfg, k_attention_join<T, 4>, a);
 }
 
 template <typename T>

@@ -34,7 +34,7 @@ struct SplitArgs {
     AttentionArgs a;
     float* parts;        // [tokens][q_heads][chunks][dim], then m and l as [..][chunks][2]
     float* stats;
-    int chunk;           // tokens of a chunk, a multiple of 32 * kSplitWarps
+    int chunk;           // tokens of a chunk, a multiple of 32
     int chunks;
     int tile_tokens;     // query tokens of a row tile (group <= rows of a tile), else 1
     int token_tiles;     // row tiles of a query token (group > rows of a tile), else 1
@@ -541,6 +541,7 @@ __global__ void __launch_bounds__(kSplitThreads)
         for (int t = warp + kSplitWarps * it; t < ahead; t += kSplitWarps, ++it)
             mbar_wait_limited(&bars[it % G::STAGES], (uint32_t)((it / G::STAGES) & 1), p.status);
 
+    griddep_launch_dependents();  // the joining kernel's CTAs may take their places and wait for this grid
     // join the warps: rows' m and l, then O, through the ring's memory
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -615,13 +616,15 @@ __global__ void __launch_bounds__(kSplitThreads)
 
 // Joins the chunks of a (row, head): a CTA each, its warps over the chunks, lanes
 // over the dimensions.  A chunk in which the row saw nothing has l = 0 and no part.
+// Bound by the latency of the parts' loads: 16 warps where there are many chunks (64
+// rows of 103 chunks: 18.9 us with four).
 constexpr int kJoinRun = 512;
 
-template <typename T>
-__global__ void __launch_bounds__(128) k_attention_join(SplitArgs p) {
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) k_attention_join(SplitArgs p) {
     __shared__ float weight[kJoinRun];
-    __shared__ float red[8];
-    __shared__ float4 acc_s[3][64];
+    __shared__ float red[2][WARPS];
+    __shared__ float4 acc_s[WARPS][64];
     const AttentionArgs& a = p.a;
     griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dim = a.cache.dim;
@@ -631,18 +634,19 @@ __global__ void __launch_bounds__(128) k_attention_join(SplitArgs p) {
     const float2* st = reinterpret_cast<const float2*>(p.stats) + i * p.chunks;
     const float* parts = p.parts + i * p.chunks * dim;
     float top = -INFINITY;
-    for (int c = tid; c < p.chunks; c += 128) top = fmaxf(top, st[c].x);
+    for (int c = tid; c < p.chunks; c += WARPS * 32) top = fmaxf(top, st[c].x);
 #pragma unroll
     for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-    if (lane == 0) red[warp] = top;
+    if (lane == 0) red[0][warp] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, red[0][w]);
     float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
     float sum = 0.f;
     for (int c0 = 0; c0 < p.chunks; c0 += kJoinRun) {
         const int n = min(kJoinRun, p.chunks - c0);
         __syncthreads();
-        for (int c = tid; c < n; c += 128) {
+        for (int c = tid; c < n; c += WARPS * 32) {
             const float2 v = st[c0 + c];
             // a NaN sum without a maximum keeps its weight: the row is NaN
             const float f = v.y == 0.f ? 0.f : v.x == -INFINITY ? 1.f : exp2_approx(v.x - top);
@@ -650,8 +654,8 @@ __global__ void __launch_bounds__(128) k_attention_join(SplitArgs p) {
             sum += v.y * f;
         }
         __syncthreads();
-#pragma unroll 4
-        for (int c = warp; c < n; c += 4) {
+#pragma unroll 8
+        for (int c = warp; c < n; c += WARPS) {
             const float f = weight[c];
             const float4* o = reinterpret_cast<const float4*>(parts + (int64_t)(c0 + c) * dim);
 #pragma unroll
@@ -667,33 +671,22 @@ __global__ void __launch_bounds__(128) k_attention_join(SplitArgs p) {
     }
 #pragma unroll
     for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-    if (lane == 0) red[4 + warp] = sum;
-    if (warp)
-        for (int k = 0; k < 2; ++k) acc_s[warp - 1][k * 32 + lane] = acc[k];
+    if (lane == 0) red[1][warp] = sum;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) acc_s[warp][k * 32 + lane] = acc[k];
     __syncthreads();
-    if (warp) return;
-    sum = (red[4] + red[5]) + (red[6] + red[7]);
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) sum += red[1][w];
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T* y = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
+    for (int d = tid; d < dim; d += WARPS * 32) {
+        float v = 0.f;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int d = (k * 32 + lane) * 4;
-        if (d >= dim) continue;
-        float4 v = acc[k];
-#pragma unroll
-        for (int w = 0; w < 3; ++w) {
-            const float4 x = acc_s[w][k * 32 + lane];
-            v.x += x.x;
-            v.y += x.y;
-            v.z += x.z;
-            v.w += x.w;
-        }
-        y[d] = from_f32<T>(v.x * inv);
-        y[d + 1] = from_f32<T>(v.y * inv);
-        y[d + 2] = from_f32<T>(v.z * inv);
-        y[d + 3] = from_f32<T>(v.w * inv);
+        for (int w = 0; w < WARPS; ++w) v += reinterpret_cast<const float*>(acc_s[w])[d];
+        y[d] = from_f32<T>(v * inv);
     }
-    if (a.lse && lane == 0)
+    if (a.lse && tid == 0)
         a.lse[i] = sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * 0.693147180559945309f;
 }
 
