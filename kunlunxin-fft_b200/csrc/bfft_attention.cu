@@ -9,7 +9,6 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
-#include <string>
 
 #include "../../include/bfft.h"
 #include "bfft_async.cuh"
@@ -142,7 +141,7 @@ struct TilePlan {
 
 // How a call is cut: row tiles and chunks of the token axis.
 struct SplitPlan {
-    int nt, tile_tokens, token_tiles, by_token, chunk, chunks;
+    int nt, tile_tokens, token_tiles, by_token, chunk, chunks, cluster;
     int64_t slots, ctas;
     size_t bytes;
 };
@@ -173,11 +172,22 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
     chunk = (chunk + 31) / 32 * 32;
     if (chunk < 256) chunk = 256;
     if (chunk > 4096) chunk = 4096;
+    // Few rows over a short axis: eight chunks at most, one cluster that joins them
+    // itself (8 row tiles over 704 tokens 10.1 us a call, two launches 14.7; over 2000
+    // tokens 12.3 by either, over 4000 15.4 and 12.7; 64 row tiles 28.7 and 22.6: a
+    // cluster's CTAs keep their places until the last is done)
+    const bool brief = units <= 32 && cover <= 2048;
+    if (brief) {
+        chunk = (cover + 7) / 8;
+        chunk = (chunk + 31) / 32 * 32;
+        if (chunk < 128) chunk = 128;
+    }
     p.chunk = (int)chunk;
     const int64_t n = (cover + chunk - 1) / chunk;
     p.chunks = (int)n;
+    p.cluster = brief && n > 1;
     p.ctas = p.slots * p.token_tiles * c->kv_heads * n;
-    p.bytes = n > 1 ? (size_t)(q->tokens * d->q_heads * n) * (size_t)(c->dim + 2) * 4 : 0;
+    p.bytes = n > 1 && !p.cluster ? (size_t)(q->tokens * d->q_heads * n) * (size_t)(c->dim + 2) * 4 : 0;
     return p;
 }
 
@@ -282,8 +292,18 @@ cudaError_t launch_split(const SplitArgs& a, const SplitPlan& p, const CUtensorM
         if (e != cudaSuccess) return e;
         ready[dev].store(true, std::memory_order_release);
     }
-    kernel<<<(unsigned)p.ctas, kSplitThreads, G::smem(a.a.cache.dim), s>>>(a, km, vm);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3((unsigned)p.ctas);
+    cfg.blockDim = dim3(kSplitThreads);
+    cfg.dynamicSmemBytes = G::smem(a.a.cache.dim);
+    cfg.stream = s;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.chunks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.cluster ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, a, km, vm);
 }
 
 template <typename T, int CODE>
@@ -310,7 +330,7 @@ cudaError_t run_split(const SplitArgs& a, const SplitPlan& p, const bfft_cache_d
         if (!encode_codes(&km, c->k, c) || !encode_codes(&vm, c->v, c)) return cudaErrorNotSupported;
     cudaError_t e = c->code == BFFT_CODE_INT8 ? split_shape<T, kCodeInt8>(a, p, km, vm, s)
                                               : split_shape<T, kCodeE4m3>(a, p, km, vm, s);
-    if (e != cudaSuccess || p.chunks == 1) return e;
+    if (e != cudaSuccess || p.chunks == 1 || p.cluster) return e;
     return run_join<T>(a, s);
 }
 
@@ -371,12 +391,12 @@ extern "C" bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const 
     if (bytes && !aligned(d->workspace, 16)) return fail(BFFT_ERR_WORKSPACE, "workspace must be 16-byte aligned");
     float* parts = static_cast<float*>(d->workspace);
     float* stats = parts ? parts + seqs->tokens * d->q_heads * chunks * cache->dim : nullptr;
-    count_launches(chunks > 1 ? 2 : 1);
+    count_launches(chunks > 1 && !sp.cluster ? 2 : 1);
     if (tiles) {
         TileArgs ta{a, parts, stats, tp.chunk, tp.chunks, tp.tile_tokens, tp.by_token, tp.slots, status};
         e = d->type == BFFT_F16 ? run_tiles<__half>(ta, tp, cache, s) : run_tiles<__nv_bfloat16>(ta, tp, cache, s);
     } else {
-        SplitArgs sa{a, parts, stats, sp.chunk, sp.chunks, sp.tile_tokens, sp.token_tiles, sp.by_token, sp.slots, status};
+        SplitArgs sa{a, parts, stats, sp.chunk, sp.chunks, sp.tile_tokens, sp.token_tiles, sp.by_token, sp.slots, sp.cluster, status};
         e = d->type == BFFT_F16 ? run_split<__half>(sa, sp, cache, s) : run_split<__nv_bfloat16>(sa, sp, cache, s);
     }
     return e == cudaSuccess ? BFFT_OK : fail(BFFT_ERR_CUDA, "cache_attention: %s", cudaGetErrorString(e));

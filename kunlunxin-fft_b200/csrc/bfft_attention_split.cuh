@@ -9,7 +9,8 @@
 //   its four warps take 32-token tiles in turn, each with a ring of its own that
 //   the copy engine fills (128-byte swizzled boxes for heads of 64, 128 and 256;
 //   plain bulk copies for other widths), so no barrier joins the warps until the
-//   chunk's end.  Parts of several chunks are joined by k_attention_join.
+//   chunk's end.  Up to eight chunks are a thread-block cluster and joined through
+//   distributed shared memory; the parts of more by k_attention_join.
 // * Products on m16n8k16 matrix instructions with tokens as rows and query heads
 //   as columns, S^T = K Q^T and O^T = V^T P^T: eight heads fill a tile (rows of
 //   queries would fill half of a 16-row one).  The order of the 16 products of an
@@ -40,6 +41,7 @@ struct SplitArgs {
     int token_tiles;     // row tiles of a query token (group > rows of a tile), else 1
     int by_token;        // slots are tokens (else runs of tile_tokens, see slot_rows)
     int64_t slots;
+    int cluster;         // the chunks of a row tile are one thread-block cluster, which joins them
     unsigned int* status;
 };
 
@@ -59,6 +61,29 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
+}
+
+// Shared memory at `local`'s place in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_address(const void* local, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -195,7 +220,8 @@ struct SplitGeo {
     __host__ __device__ static constexpr int ring_bytes(int dim) {
         return kSplitWarps * STAGES * 4 * half_bytes(dim);
     }
-    __host__ __device__ static constexpr int merge_bytes(int dim) { return kSplitWarps * ROWS * (dim + 2) * 4; }
+    // the warps' parts, and the CTA's for the cluster
+    __host__ __device__ static constexpr int merge_bytes(int dim) { return (kSplitWarps + 1) * ROWS * (dim + 2) * 4; }
     __host__ __device__ static constexpr int smem(int dim) {
         const int r = ring_bytes(dim), m = merge_bytes(dim);
         return 1024 + (r > m ? r : m) + MAX_ENTRIES * (int)(sizeof(BlockScale) + 4) + 64;
@@ -249,12 +275,19 @@ __global__ void __launch_bounds__(kSplitThreads)
         token = sr.first + t;
         head = kv * a.group + head0 + (r - t * per_token);
     };
+    float* part_o = reinterpret_cast<float*>(ring);  // of the warps, at the end; then of the CTA
+    float* part_ml = part_o + kSplitWarps * G::ROWS * dim;
+    float* cta_o = part_ml + kSplitWarps * G::ROWS * 2;
+    float* cta_ml = cta_o + G::ROWS * dim;
     if (base >= end) {  // nothing of the axis in this chunk
         if (tid < rows) {
             int64_t token;
             int head;
             row_of(tid, token, head);
-            if (p.chunks > 1) {
+            if (p.cluster) {
+                cta_ml[tid * 2] = -INFINITY;
+                cta_ml[tid * 2 + 1] = 0.f;
+            } else if (p.chunks > 1) {
                 float* st = p.stats + ((token * a.q_heads + head) * p.chunks + chunk) * 2;
                 st[0] = -INFINITY;
                 st[1] = 0.f;
@@ -269,8 +302,8 @@ __global__ void __launch_bounds__(kSplitThreads)
                 row_of(e / dim, token, head);
                 static_cast<T*>(a.out)[token * a.ot + head * a.oh + e % dim] = from_f32<T>(0.f);
             }
-        return;
-    }
+        if (!p.cluster) return;
+    } else {
     const int lg = a.cache.page_log2;
     const int64_t page0 = base >> lg;
     const int entries = (int)(((end - 1) >> lg) - page0) + 1;
@@ -552,8 +585,6 @@ __global__ void __launch_bounds__(kSplitThreads)
             l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
         }
     __syncthreads();
-    float* part_o = reinterpret_cast<float*>(ring);
-    float* part_ml = part_o + kSplitWarps * G::ROWS * dim;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -593,7 +624,13 @@ __global__ void __launch_bounds__(kSplitThreads)
         int64_t token;
         int head;
         row_of(r, token, head);
-        if (p.chunks > 1) {
+        if (p.cluster) {
+            *reinterpret_cast<float4*>(cta_o + r * dim + d) = v;
+            if (d == 0) {
+                cta_ml[r * 2] = top;
+                cta_ml[r * 2 + 1] = sum;
+            }
+        } else if (p.chunks > 1) {
             const int64_t at_part = (token * a.q_heads + head) * p.chunks + chunk;
             *reinterpret_cast<float4*>(p.parts + at_part * dim + d) = v;
             if (d == 0) {
@@ -612,6 +649,47 @@ __global__ void __launch_bounds__(kSplitThreads)
                     sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * 0.693147180559945309f;
         }
     }
+    }
+    if (!p.cluster) return;
+    // the chunks' parts, each CTA a share of the tile's elements
+    __syncthreads();
+    cluster_sync();
+    for (int e = tid + chunk * kSplitThreads; e < rows * (dim / 4); e += p.chunks * kSplitThreads) {
+        const int r = e / (dim / 4), d = (e - r * (dim / 4)) * 4;
+        float top = -INFINITY, sum = 0.f;
+        float2 ml[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            ml[c] = c < p.chunks ? cluster_load2(cluster_address(cta_ml + r * 2, c)) : make_float2(-INFINITY, 0.f);
+            top = fmaxf(top, ml[c].x);
+        }
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (ml[c].y == 0.f) continue;  // nothing seen there, and no part
+            const float f = ml[c].x == -INFINITY ? 1.f : exp2_approx(ml[c].x - top);
+            const float4 x = cluster_load4(cluster_address(cta_o + r * dim + d, c));
+            sum += ml[c].y * f;
+            v.x += x.x * f;
+            v.y += x.y * f;
+            v.z += x.z * f;
+            v.w += x.w * f;
+        }
+        int64_t token;
+        int head;
+        row_of(r, token, head);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        T* y = static_cast<T*>(a.out) + token * a.ot + head * a.oh + d;
+        y[0] = from_f32<T>(v.x * inv);
+        y[1] = from_f32<T>(v.y * inv);
+        y[2] = from_f32<T>(v.z * inv);
+        y[3] = from_f32<T>(v.w * inv);
+        if (d == 0 && a.lse)
+            a.lse[token * a.q_heads + head] =
+                sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * 0.693147180559945309f;
+    }
+    __syncthreads();
+    cluster_sync();  // no CTA leaves while another reads its part
 }
 
 // Joins the chunks of a (row, head): a CTA each, its warps over the chunks, lanes

@@ -200,11 +200,14 @@ __global__ void __launch_bounds__(256, 3) k_rotate(RotateArgs a) {
 }
 
 // ---------------------------------------------------------------- append
-// A call with long runs of new tokens (prompts) takes two launches, its queries'
-// rotation and a block for each run and head; one of short runs (single tokens)
-// takes one, a warp for each run and head and for each token's queries: there the
-// chain of dependent loads (sequence, page, scale) is the time, and warps hide it
-// (256 tokens of 32 + 8 + 8 heads of 128: 41 us with a block of 256 threads each).
+// One launch has a warp for each run and head and for each token's queries: the
+// chain of dependent loads (sequence, page, scale) is the time, and many warps hide
+// it (256 tokens of 32 + 8 + 8 heads of 128: 41 us with a block of 256 threads
+// each).  A few long runs (a prompt) leave too few warps: they take two launches,
+// the queries' rotation and a block for each run and group of heads.  Append and
+// read back, 32 + 8 + 8 heads: 1024 tokens of one sequence 21.5 us by blocks, 30.8
+// by warps; 64 sequences of 16 tokens 30.8 and 20.5; 16.9k tokens of 16 sequences
+// 134 and 125.
 struct AppendArgs {
     CacheView cache;
     SequenceView seq;        // lens: tokens held before the call
@@ -281,7 +284,7 @@ __device__ __forceinline__ int64_t token_position(const AppendArgs& a, int64_t t
 }
 
 constexpr int kAppendThreads = 256;  // of the kernel of short runs
-constexpr int kRunThreads = 256;     // of the kernel of long runs: two units of 64 rows of 128 elements each
+constexpr int kRunThreads = 256;     // of the kernel of long runs: two units each of 64 rows of 128 elements
 
 // max of |x| that keeps NaN
 __device__ __forceinline__ float max_abs(float m, float x) {
@@ -423,9 +426,8 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, const Run& r, i
     }
 }
 
-// A block for each run and group of kv heads, of keys or values: the run, its page
-// and its roots are found once for the group's heads, and a head's rows load while
-// the head before is coded.
+// The run, its page and its roots are found once for the block's heads, and a
+// head's rows load while the head before is coded.
 template <typename T, int P, int LAYOUT, int CODE, bool ROTATE, int HELD>
 __device__ __forceinline__ void append_heads(const AppendArgs& a, const Run& r, int first, int last,
                                              uint32_t (*shared_max)[kRunThreads / 32]) {
@@ -876,7 +878,7 @@ extern "C" bfft_status bfft_cache_append(const bfft_cache_desc* cache, const bff
     a.by_token = seqs->tokens <= runs;
     a.slots = a.by_token ? seqs->tokens : runs;
     AppendPlan plan{};
-    plan.runs = !a.by_token && seqs->tokens >= 16 * seqs->seqs;
+    plan.runs = !a.by_token && seqs->tokens >= 48 * seqs->seqs && a.slots * 2 * cache->kv_heads < 4096;
     int64_t blocks = a.slots * 2 * cache->kv_heads, q_blocks = 0;
     if (plan.runs) {
         // four kv heads a block, fewer where that leaves less than four blocks to an SM

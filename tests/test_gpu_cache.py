@@ -625,3 +625,15 @@ def test_refusals_come_before_any_launch():
 
 def test_no_bounded_wait_expired_here():
     assert _lib.device_status(0) == 0
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_decode_example(code):
+    from bfft import decode_example
+
+    got = decode_example.run(prompt=150, steps=5, code=code)
+    # a value is off by up to scale / 2 (2^-7.6 of the block's largest, some 3.5 deviations) or 2^-4 of itself, in the
+    # mean 1 / sqrt 3 of it; keys the same, and rounding again as blocks fill
+    assert got["value_rel_error"] < (0.02 if code == "int8" else 0.045)
+    assert got["attention_rel_error"] < (0.03 if code == "int8" else 0.06)
+    assert got["gradient_is_adjoint"]
