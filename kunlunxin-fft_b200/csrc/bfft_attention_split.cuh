@@ -27,6 +27,7 @@
 
 namespace bfft {
 
+constexpr int kDeadBlock = 3;  // BlockScale::kind of tokens that nothing sees
 // Value scale of a zero block: its codes must not count, its weights must.
 constexpr float kZeroLog2 = -64.f;
 constexpr float kTop = 14.f, kRenew = 15.5f;  // log2 of p' at the maximum, and where the maximum is renewed
@@ -142,7 +143,7 @@ struct BlockScale {
     float key;
     float log2_value;
     float inv_value;
-    int kind;  // 0 ordinary, 1 zero values, 2 values that are not finite
+    int kind;  // 0 ordinary, 1 zero values, 2 values that are not finite, kDeadBlock
 };
 __device__ __forceinline__ BlockScale block_scale(float ks, float vs) {
     BlockScale b;
@@ -229,7 +230,7 @@ struct SplitGeo {
 };
 
 template <int DP, bool EXACT, int NT, typename T, int CODE>
-__global__ void __launch_bounds__(kSplitThreads)
+__global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     k_attention_split(SplitArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using G = SplitGeo<DP, EXACT, NT>;
     extern __shared__ unsigned char smem_raw[];
@@ -304,9 +305,13 @@ __global__ void __launch_bounds__(kSplitThreads)
             }
         if (!p.cluster) return;
     } else {
+    // from here on tokens are counted from `base`, in 32 bits
     const int lg = a.cache.page_log2;
     const int64_t page0 = base >> lg;
-    const int entries = (int)(((end - 1) >> lg) - page0) + 1;
+    const int off = (int)(base & (((int64_t)1 << lg) - 1)), span = (int)(end - base);
+    const int entries = ((off + span - 1) >> lg) + 1;
+    auto rel = [&](int64_t t) { return (int)(t < base ? 0 : t - base > span ? span : t - base); };
+    const int lo_all = rel(lo_max), hi_all = rel(hi_min), lo_any = rel(lo_min);
     for (int e = tid; e < entries; e += kSplitThreads) {
         const int64_t id = a.seq.block_table[sr.s * a.seq.table_stride + page0 + e];
         page_ids[e] = id >= 0 && id < a.cache.pages ? (int)id : -1;
@@ -314,20 +319,20 @@ __global__ void __launch_bounds__(kSplitThreads)
     __syncthreads();
 
     // ring: tile t of this warp covers tokens [base + 32 (t kSplitWarps + warp), + 32)
-    const int tiles = (int)((end - base + 31) >> 5);
+    const int tiles = (span + 31) >> 5;
     unsigned char* mine = ring + warp * (G::STAGES * 4 * G::half_bytes(dim));
     uint64_t* bars = full + warp * G::STAGES;
     const int lines = EXACT ? DP / 8 : 1;  // 128-byte lines of 16 tokens
     auto fetch = [&](int t, int stage) {   // lanes 0..3: keys of half 0, 1, values of half 0, 1
-        const int64_t tok = base + (int64_t)t * 32 + (lane & 1) * 16;
+        const int tok = t * 32 + (lane & 1) * 16;
         int id = -1;
-        if (lane < 4 && tok < end) id = page_ids[(tok >> lg) - page0];
+        if (lane < 4 && tok < span) id = page_ids[(off + tok) >> lg];
         const unsigned any = __ballot_sync(0xffffffffu, id >= 0);
         if (lane == 0) mbar_arrive_expect_tx(&bars[stage], (uint32_t)(__popc(any) * G::half_bytes(dim)));
         __syncwarp();
         if (id >= 0) {
             unsigned char* dst = mine + (stage * 4 + lane) * G::half_bytes(dim);
-            const int slot_in = (int)(tok & (((int64_t)1 << lg) - 1));
+            const int slot_in = (off + tok) & ((1 << lg) - 1);
             if constexpr (EXACT) {
                 tma_load_3d(dst, lane < 2 ? &kmap : &vmap, 0, ((kv << lg) + slot_in) / 16 * lines, id, &bars[stage]);
             } else {
@@ -344,13 +349,15 @@ __global__ void __launch_bounds__(kSplitThreads)
         if (id >= 0) {
             const int64_t b = (int64_t)id * a.cache.kv_heads + kv;
             scales[e] = block_scale(a.cache.k_scale[b], a.cache.v_scale[b]);
+        } else {
+            scales[e].kind = kDeadBlock;
         }
     }
 
     // queries as B fragments: lane (g, q4) holds row g of each 8-row tile, dims 16 (4 i + q4) + 4 t ..
     uint32_t qf[NT][G::KS][2];
     float row_scale[NT][2];      // of rows 2 q4, 2 q4 + 1: softmax scale (log2) times the row's power
-    int64_t row_lo[NT][2], row_hi[NT][2];
+    int row_lo[NT][2], row_hi[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int r = nt * 8 + g;
@@ -384,7 +391,10 @@ __global__ void __launch_bounds__(kSplitThreads)
         for (int j = 0; j < 2; ++j) {
             row_scale[nt][j] = __shfl_sync(0xffffffffu, up, (2 * q4 + j) * 4) * a.scale_log2;
             const int rr = nt * 8 + 2 * q4 + j;
-            seen_range(a, pos0 + (rr < rows ? rr / per_token : 0), len, row_lo[nt][j], row_hi[nt][j]);
+            int64_t lo, hi;
+            seen_range(a, pos0 + (rr < rows ? rr / per_token : 0), len, lo, hi);
+            row_lo[nt][j] = rel(lo);
+            row_hi[nt][j] = rel(hi);
         }
     }
     __syncthreads();
@@ -416,7 +426,7 @@ __global__ void __launch_bounds__(kSplitThreads)
             ok = false;
             break;
         }
-        const int64_t tok0 = base + (int64_t)t * 32;
+        const int tok0 = t * 32;
         const unsigned char* buf = mine + stage * 4 * G::half_bytes(dim);
         float z[2][NT][4];
         BlockScale bs[2];
@@ -424,11 +434,11 @@ __global__ void __launch_bounds__(kSplitThreads)
         float worst = -INFINITY;  // largest z - m of this lane
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int64_t tok = tok0 + 16 * h;
-            const int e = (int)((tok >> lg) - page0);
-            live[h] = tok < end && page_ids[e < entries ? e : entries - 1] >= 0;
+            const int tok = tok0 + 16 * h;
+            const int e = (off + tok) >> lg;
+            bs[h] = scales[e < entries ? e : entries - 1];
+            live[h] = tok < span && bs[h].kind != kDeadBlock;
             if (!live[h]) continue;
-            bs[h] = scales[e];
             const unsigned char* kb = buf + h * G::half_bytes(dim);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) z[h][nt][0] = z[h][nt][1] = z[h][nt][2] = z[h][nt][3] = 0.f;
@@ -451,15 +461,15 @@ __global__ void __launch_bounds__(kSplitThreads)
                         mma_f16(z[h][nt], a0, a1, a2, a3, qf[nt][c * 4 + s][0], qf[nt][c * 4 + s][1]);
                 }
             }
-            const bool inside = tok >= lo_max && tok + 16 <= hi_min && tok + 16 <= end;
+            const bool inside = tok >= lo_all && tok + 16 <= hi_all;  // hi_all is at most span
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float v = z[h][nt][c] * (bs[h].key * row_scale[nt][c & 1]) + bs[h].log2_value;
                     if (!inside) {
-                        const int64_t j = tok + tk + (c >> 1) * 8;
-                        if (j < row_lo[nt][c & 1] || j >= row_hi[nt][c & 1] || j >= end) v = -INFINITY;
+                        const int j = tok + tk + (c >> 1) * 8;
+                        if (j < row_lo[nt][c & 1] || j >= row_hi[nt][c & 1]) v = -INFINITY;
                     }
                     z[h][nt][c] = v;
                     worst = fmaxf(worst, v == -INFINITY ? v : v - m[nt][c & 1]);
@@ -491,7 +501,7 @@ __global__ void __launch_bounds__(kSplitThreads)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if (!live[h]) continue;
-            const int64_t tok = tok0 + 16 * h;
+            const int tok = tok0 + 16 * h;
             uint32_t pf[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -525,7 +535,7 @@ __global__ void __launch_bounds__(kSplitThreads)
             const int t0 = row_token(2 * q4), t1 = row_token(2 * q4 + 1);
             const int toks[4] = {t0, t1, t0 + 8, t1 + 8};
             uint32_t w[4][G::VW];
-            const bool whole = tok >= lo_min && tok + 16 <= end;
+            const bool whole = tok >= lo_any && tok + 16 <= span;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 if constexpr (DP == 64) {
@@ -546,8 +556,8 @@ __global__ void __launch_bounds__(kSplitThreads)
                     }
                 }
                 if (!whole) {  // codes of slots that no row sees may be anything: 0 times NaN is NaN
-                    const int64_t j = tok + toks[k];
-                    if (j < lo_min || j >= end)
+                    const int j = tok + toks[k];
+                    if (j < lo_any || j >= span)
 #pragma unroll
                         for (int c = 0; c < G::VW; ++c) w[k][c] = 0;
                 }

@@ -59,7 +59,6 @@ struct TileGeo {
     static constexpr uint32_t S0 = 0, O0 = 256;   // columns: S_h at 128 h, O_h at 256 + 128 h
 };
 
-constexpr int kDeadBlock = 3;  // BlockScale::kind of tokens that nothing sees
 // As kTop and kRenew: a renewal costs a row's O one trip through registers, so the
 // maximum leaves room for scores 32 times larger.
 constexpr float kTileTop = 10.f, kTileRenew = 15.5f;
