@@ -23,6 +23,11 @@
 //   p' / vs.  The largest p' is set to 2^14, near float16's top, so that weighted
 //   values keep their bits down to 2^-28 of the largest; m is renewed when one
 //   passes 2^15.5 (a vote instead of a reduction on most tiles).
+//
+// 64 sequences of 1024..32768 tokens, one row of 32 heads each (8 kv heads, 128
+// dimensions): int8 418 us, 5430 GB/s, 0.83 of the measured HBM rate; e4m3, whose
+// codes take 2 instructions for 4 to widen instead of 5, 385 us and 0.90.  One
+// sequence of 131001 e4m3 tokens, 64 heads: 53 us and 7 for joining.
 #pragma once
 
 namespace bfft {

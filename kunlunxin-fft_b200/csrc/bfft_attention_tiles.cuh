@@ -18,6 +18,16 @@
 //
 // Key and value scales enter in the exponent as in the split kernel:
 // p' = 2^(s * ks + log2 vs - m), sum of p' / vs.
+//
+// 2 x 2048 prompt rows of 32 heads (8 kv heads, 128 dimensions) over 8192 and 16384
+// int8 tokens: 856 us, 884 TFLOP/s, 0.54 of the measured bf16 rate.  Bound by the
+// chain of a half's tile, not by one pipe: 4900 clocks a tile for 2048 of tensor
+// work.  Leaving a stage out (in a copy) gives, of 880 us: no widening 782, no
+// exponentials 872, no maximum 862, half of the value products 832.  The special
+// function pipe is 43 % busy, so exponentials by polynomials did not help; tiles of
+// 64 tokens with two score buffers a half were slower (an M128 N64 product takes as
+// long as N128 when the widening shares its shared memory); waits that poll without
+// reading the clock, 975 us.
 #pragma once
 
 namespace bfft {
@@ -69,31 +79,29 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    uint64_t d = 0;
-    d |= (uint64_t)((addr >> 4) & 0x3fff);
-    d |= (uint64_t)((lbo >> 4) & 0x3fff) << 16;
-    d |= (uint64_t)((sbo >> 4) & 0x3fff) << 32;
-    d |= (uint64_t)1 << 46;  // descriptor version of sm_100
-    d |= (uint64_t)2 << 61;  // 128-byte swizzle
-    return d;
-}
+// Descriptor of an operand with 128-byte swizzle: the low word holds the address (in
+// 16 bytes) and the leading offset, the high word, the same for every step, the stride
+// of eight rows, the version and the layout.  A step along the operand adds to the
+// low word: one thread issues the products (2 x 2048 prompt rows 881 us with 64-bit
+// descriptors built anew for each, 856 so).
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 // float16 operands, float32 accumulator, M = 128
 __host__ __device__ constexpr uint32_t tile_idesc(int n, bool b_n_major) {
     return (1u << 4) | (b_n_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh)
         : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
@@ -622,21 +630,25 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
     } else if (warp == 13 && lane == 0) {
         // ------------------------------------------------------------ products
         constexpr uint32_t qk = tile_idesc(G::N, false), pv = tile_idesc(DP, true);
+        const uint32_t q_low = desc_low(smem_u32(q_s), 16), k_low = desc_low(smem_u32(t_s), 16),
+                       v_low = desc_low(smem_u32(t_s), G::PANEL);
         auto scores = [&](int h, int j) {
-            const uint32_t qa = smem_u32(q_s + h * G::Q_HALF), ka = smem_u32(t_s + (2 * j % G::T_RING) * G::T_BUF);
+            const int buf = 2 * j % G::T_RING;
+            const uint32_t qa = q_low + (h ? G::Q_HALF >> 4 : 0), ka = k_low + buf * (G::T_BUF >> 4);
+            const uint32_t d = tmem + G::S0 + h * 128;
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
-                mma_ss(tmem + G::S0 + h * 128, tile_desc(qa + (k >> 2) * G::Q_PANEL + (k & 3) * 32, 16, 1024),
-                       tile_desc(ka + (k >> 2) * G::PANEL + (k & 3) * 32, 16, 1024), qk, k > 0);
+                mma_ss(d, qa + (((k >> 2) * G::Q_PANEL + (k & 3) * 32) >> 4),
+                       ka + (((k >> 2) * G::PANEL + (k & 3) * 32) >> 4), qk, k > 0);
             mma_commit(&s_full[h]);
-            if (h == halves - 1) mma_commit(&t_empty[2 * j % G::T_RING]);
+            if (h == halves - 1) mma_commit(&t_empty[buf]);
         };
         auto values = [&](int h, int j, int from) {  // over the first or the last 64 tokens
-            const uint32_t va = smem_u32(t_s + ((2 * j + 1) % G::T_RING) * G::T_BUF);
+            const uint32_t va = v_low + ((2 * j + 1) % G::T_RING) * (G::T_BUF >> 4) + from * (2048 >> 4);
+            const uint32_t d = tmem + G::O0 + h * 128, pa = tmem + G::S0 + h * 128 + from * 8;
+            const uint32_t more = j > 0 || from > 0;
 #pragma unroll
-            for (int k = from; k < from + 4; ++k)
-                mma_ts(tmem + G::O0 + h * 128, tmem + G::S0 + h * 128 + k * 8, tile_desc(va + k * 2048, G::PANEL, 1024), pv,
-                       j > 0 || k > 0);
+            for (int k = 0; k < 4; ++k) mma_ts(d, pa + k * 8, va + k * (2048 >> 4), pv, k > 0 ? 1u : more);
         };
         auto ready = [&](int n) { return wait(&t_full[n % G::T_RING], (uint32_t)((n / G::T_RING) & 1)); };
         bool ok = wait(q_full, 0) && ready(0);

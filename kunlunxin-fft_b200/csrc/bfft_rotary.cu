@@ -142,10 +142,12 @@ struct RotateArgs {
     float sign;            // of the sine: -1 conjugates
 };
 
-// Heads g, g + step, ... of one token, unit (o0, o1) of each: two heads' loads are
-// in flight before the first product, and the roots are loaded once for all heads.
+// Heads g, g + step, ... of one token, unit (o0, o1) of each: the first head's loads
+// are in flight beside the roots', which are loaded once for all heads.
 // `roots` is called after the first loads (what it waits for runs beside them).
-// y may be x: a thread writes only elements that it has read.
+// y may be x: a thread writes only elements that it has read.  Bound by HBM: 16384
+// tokens of 32 bf16 heads of 128 in 51 us, 5.4 TB/s, 0.82 of the measured rate (float32
+// 0.93); two heads ahead took registers for nothing (57 us), four 70.
 constexpr int kHeadsAhead = 1;
 template <typename T, int P, int LAYOUT, typename Roots>
 __device__ __forceinline__ void rotate_heads(const T* x, T* y, int64_t xh, int64_t yh, int heads, int g, int step, int o0,
@@ -557,7 +559,8 @@ struct ReadArgs {
     void *k, *v;       // [tokens][kv_heads][dim]
 };
 
-// A warp per token: its keys and values of all heads, 16 codes a lane and step.
+// A warp per token: its keys and values of all heads, 16 codes a lane and step
+// (17.9k tokens of 8 + 8 heads of 128: 25 us, 4.4 TB/s).
 // Tokens without a valid page read as NaN.
 template <typename T, int CODE>
 __global__ void __launch_bounds__(256) k_read(ReadArgs a) {
