@@ -109,10 +109,10 @@ bool encode_codes(CUtensorMap* m, const void* codes, const bfft_cache_desc* c) {
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int sm_count() {
+int sm_count(int64_t device) {
     static std::atomic<int> counts[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (device < 0 || device >= 64) return 148;
+    const int dev = (int)device;
     int n = counts[dev].load(std::memory_order_relaxed);
     if (!n) {
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
@@ -344,8 +344,8 @@ extern "C" bfft_status bfft_cache_attention_workspace(const bfft_cache_desc* cac
     if (!seqs->tokens)
         *bytes = 0;
     else
-        *bytes = use_tiles(cache, seqs, d) ? plan_tiles(cache, seqs, d, sm_count()).bytes
-                                           : plan_split(cache, seqs, d, sm_count()).bytes;
+        *bytes = use_tiles(cache, seqs, d) ? plan_tiles(cache, seqs, d, sm_count(d->device)).bytes
+                                           : plan_split(cache, seqs, d, sm_count(d->device)).bytes;
     return BFFT_OK;
 }
 
@@ -378,9 +378,9 @@ extern "C" bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const 
     TilePlan tp{};
     SplitPlan sp{};
     if (tiles)
-        tp = plan_tiles(cache, seqs, d, sm_count());
+        tp = plan_tiles(cache, seqs, d, sm_count(d->device));
     else
-        sp = plan_split(cache, seqs, d, sm_count());
+        sp = plan_split(cache, seqs, d, sm_count(d->device));
     const int chunks = tiles ? tp.chunks : sp.chunks;
     const size_t bytes = tiles ? tp.bytes : sp.bytes;
     if ((tiles ? tp.ctas : sp.ctas) > 0x7fffffffLL || seqs->tokens * d->q_heads > 0x7fffffffLL)

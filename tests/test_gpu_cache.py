@@ -637,3 +637,90 @@ def test_decode_example(code):
     assert got["value_rel_error"] < (0.02 if code == "int8" else 0.045)
     assert got["attention_rel_error"] < (0.03 if code == "int8" else 0.06)
     assert got["gradient_is_adjoint"]
+
+
+# ------------------------------------------------------------------------------- many rows, long axes
+
+def long_pages(seed, *, code="int8", page=64, dim=128, lens=(4100, 333), heads=2):
+    return Pages(seed, list(lens), [0] * len(lens), code=code, page=page, heads=heads, dim=dim)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("page, dim, group", [
+    (16, 48, 4), (32, 80, 4), (128, 112, 4), (16, 64, 4), (64, 96, 7), (128, 128, 4), (32, 16, 32),
+])
+@pytest.mark.parametrize("causal, window", [(True, 0), (True, 517), (False, 0)])
+def test_attention_many_rows(code, page, dim, group, causal, window):
+    p = long_pages(dim + page, code=code, page=page, dim=dim)
+    q = normal(p.g, 333, 2 * group, dim, dtype=BF16) * 1.5
+    check_attention(p, q, [4100, 333], [300, 33], causal=causal, window=window)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("page", [16, 64])
+def test_attention_many_rows_ignore_what_none_sees(code, page):
+    p = long_pages(5, code=code, page=page)
+    q = normal(p.g, 400, 8, 128, dtype=F16)
+    lens, new = [4100, 333], [300, 100]
+    p.cache.v_scale[p.ids[0][40]] = 0.0                      # a block of zero values counts in the sum
+    want = check_attention(p, q, lens, new, window=1000)
+    for codes, scale in zip(p.cache[:2], p.cache[2:]):
+        for s, n in enumerate(lens):
+            codes.view(torch.uint8)[p.ids[s][n // page], :, n % page:] = 0x7f
+        used = torch.zeros(scale.shape[0], dtype=torch.bool, device="cuda")
+        for s, n in enumerate(lens):
+            for i in range(max(0, n - new[s] + 1 - 1000) // page, (n - 1) // page + 1):
+                used[p.ids[s][i]] = True
+        scale[~used] = math.nan
+    got = bfft.cache_attention(q, p.cache, p.table, ints(lens), ints([0, 300, 400]), window=1000, return_lse=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    again = bfft.cache_attention(q, p.cache, p.table, ints(lens), ints([0, 300, 400]), window=1000, return_lse=True)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+def test_attention_many_rows_nan_and_missing_pages():
+    p = long_pages(6)
+    q = normal(p.g, 300, 8, 128, dtype=BF16)
+    starts, lens = ints([0, 300, 300]), ints([4100, 333])
+    clean = bfft.cache_attention(q, p.cache, p.table, lens, starts, return_lse=True)
+    last = 4100 - 20                                          # seen by the last 20 rows only
+    p.cache.v_scale[p.ids[0][last // 64], 1] = math.nan
+    out, lse = bfft.cache_attention(q, p.cache, p.table, lens, starts, return_lse=True)
+    first = 300 - (4100 - last // 64 * 64)                    # the first row that sees the block
+    assert out[first:, 4:].isnan().all() and out[:first].isfinite().all() and out[:, :4].isfinite().all()
+    assert torch.equal(out[:, :4], clean[0][:, :4]) and lse.isfinite().all()
+    p.cache.v_scale[p.ids[0][last // 64], 1] = 0.02
+    p.cache.k_scale[p.ids[0][3], 0] = math.nan
+    out, lse = bfft.cache_attention(q, p.cache, p.table, lens, starts, return_lse=True)
+    assert out[:, :4].isnan().all() and lse[:, :4].isnan().all() and out[:, 4:].isfinite().all()
+    table = p.table.clone()
+    table[0, 3] = p.cache.k.shape[0]                          # no such page: as if its tokens were not there
+    got = bfft.cache_attention(q, p.cache, table, lens, starts, causal=False)
+    k, v = (p.values(w, 0, 0, 4100)[0][:, 0] for w in (0, 1))
+    keep = torch.ones(4100, dtype=torch.bool, device="cuda")
+    keep[192:256] = False
+    z = torch.einsum("qhd,kd->qhk", q[:, :4].double(), k[keep]) * 128 ** -0.5
+    assert (got[:, :4].double() - torch.softmax(z, -1) @ v[keep]).abs().max() < 2.0 ** -7 * float(v.abs().max())
+
+
+def test_attention_many_rows_strides_and_sizes():
+    p = long_pages(7)
+    wide = normal(p.g, 333, 9, 130, dtype=BF16)
+    odd = wide[:, 1:, 1:129]                                  # rows on odd elements
+    want, _ = check_attention(p, odd, [4100, 333], [300, 33])
+    buffer = torch.zeros(8, 333, 136, dtype=BF16, device="cuda")
+    out = buffer[:, :, 8:].transpose(0, 1)
+    assert bfft.cache_attention(odd.contiguous(), p.cache, p.table, ints([4100, 333]), ints([0, 300, 333]), out=out) is not None
+    assert torch.equal(out, want) and (buffer[:, :, :8] == 0).all()
+    big = odd * 2.0 ** 50                                     # outside float16
+    p.cache.k_scale.mul_(2.0 ** -30)
+    check_attention(p, big, [4100, 333], [300, 33], scale=2.0 ** -20)
+
+
+@pytest.mark.parametrize("dim", [144, 176, 240])
+def test_attention_wide_heads(dim):
+    lens, new = [700, 33, 0], [1, 20, 2]
+    p = Pages(dim, lens, [0] * 3, code="int8", page=32, heads=2, dim=dim)
+    q = normal(p.g, 23, 6, dim, dtype=BF16)
+    check_attention(p, q, lens, new)
+    check_attention(p, q, lens, new, causal=False, window=50)
