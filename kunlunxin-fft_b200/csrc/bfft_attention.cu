@@ -173,7 +173,7 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
     if (chunk < 256) chunk = 256;
     if (chunk > 4096) chunk = 4096;
     // Few rows over a short axis: eight chunks at most, one cluster that joins them
-    // itself (8 row tiles over 704 tokens 10.1 us a call, two launches 14.7; over 2000
+    // itself (8 row tiles over 704 tokens 10.1 us a call, by two launches 14.7; over 2000
     // tokens 12.3 by either, over 4000 15.4 and 12.7; 64 row tiles 28.7 and 22.6: a
     // cluster's CTAs keep their places until the last is done)
     const bool brief = units <= 32 && cover <= 2048;
@@ -238,23 +238,14 @@ cudaError_t launch_tiles(const TileArgs& a, const TilePlan& p, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         ready[dev].store(true, std::memory_order_release);
     }
-    kernel<<<(unsigned)p.ctas, G::THREADS, G::SMEM, s>>>(a);
-    return cudaGetLastError();
+    return launch_dependent(kernel, (unsigned)p.ctas, G::THREADS, G::SMEM, s, a);
 }
 
 template <typename T>
 cudaError_t run_join(const SplitArgs& a, cudaStream_t s) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3((unsigned)(a.a.seq.tokens * a.a.q_heads));
-    const bool many = a.chunks > 16;
-    cfg.blockDim = dim3(many ? 512 : 128);
-    cfg.stream = s;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return many ? cudaLaunchKernelEx(&cfg, k_attention_join<T, 16>, a) : cudaLaunchKernelEx(&cfg, k_attention_join<T, 4>, a);
+    const unsigned rows = (unsigned)(a.a.seq.tokens * a.a.q_heads);
+    return a.chunks > 16 ? launch_dependent(k_attention_join<T, 16>, rows, 512, 0, s, a)
+                         : launch_dependent(k_attention_join<T, 4>, rows, 128, 0, s, a);
 }
 
 template <typename T>
@@ -293,16 +284,18 @@ cudaError_t launch_split(const SplitArgs& a, const SplitPlan& p, const CUtensorM
         ready[dev].store(true, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3((unsigned)p.ctas);
     cfg.blockDim = dim3(kSplitThreads);
     cfg.dynamicSmemBytes = G::smem(a.a.cache.dim);
     cfg.stream = s;
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)p.chunks;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // as launch_dependent
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.chunks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = p.cluster ? 1 : 0;
+    cfg.numAttrs = p.cluster ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, a, km, vm);
 }
 

@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     using G = SplitGeo<DP, EXACT, NT>;
     extern __shared__ unsigned char smem_raw[];
     const AttentionArgs& a = p.a;
+    griddep_wait();
     const int dim = EXACT ? DP : a.cache.dim;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
     unsigned char* ring = align_smem<1024>(smem_raw);

@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
     using G = TileGeo<DP>;
     extern __shared__ unsigned char smem_raw[];
     const AttentionArgs& a = p.a;
+    griddep_wait();
     const int dim = a.cache.dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lg = a.cache.page_log2;
 
     // which rows and tokens

@@ -146,7 +146,7 @@ struct RotateArgs {
 // are in flight beside the roots', which are loaded once for all heads.
 // `roots` is called after the first loads (what it waits for runs beside them).
 // y may be x: a thread writes only elements that it has read.  Bound by HBM: 16384
-// tokens of 32 bf16 heads of 128 in 51 us, 5.4 TB/s, 0.82 of the measured rate (float32
+// tokens of 32 bf16 heads of 128 in 49 us, 5.7 TB/s, 0.87 of the measured rate (float32
 // 0.93); two heads ahead took registers for nothing (57 us), four 70.
 constexpr int kHeadsAhead = 1;
 template <typename T, int P, int LAYOUT, typename Roots>
@@ -183,6 +183,8 @@ __device__ __forceinline__ void rotate_heads(const T* x, T* y, int64_t xh, int64
 
 template <typename T, int P, int LAYOUT>
 __global__ void __launch_bounds__(256, 3) k_rotate(RotateArgs a) {
+    griddep_wait();
+    griddep_launch_dependents();
     const int u = threadIdx.x;
     const int64_t slot = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const int64_t row = slot / a.groups;
@@ -455,6 +457,8 @@ __device__ __forceinline__ void append_heads(const AppendArgs& a, const Run& r, 
 
 template <typename T, int P, int LAYOUT, int CODE>
 __global__ void __launch_bounds__(kRunThreads, 2) k_append_runs(AppendArgs a, int heads_per_block) {
+    griddep_wait();
+    griddep_launch_dependents();
     __shared__ uint32_t shared_max[2][kRunThreads / 32];
     const int heads = a.cache.kv_heads, parts = (heads + heads_per_block - 1) / heads_per_block;
     const int64_t slot = blockIdx.x / (2 * parts);
@@ -493,6 +497,8 @@ __device__ __forceinline__ int64_t new_position(const AppendArgs& a, int64_t tok
 // behind them rotate the queries, one token each.
 template <typename T, int P, int LAYOUT, int CODE>
 __global__ void __launch_bounds__(kAppendThreads, 3) k_append(AppendArgs a) {
+    griddep_wait();
+    griddep_launch_dependents();
     const int lane = threadIdx.x & 31;
     const int64_t per_slot = 2 * a.cache.kv_heads, runs = a.slots * per_slot;
     const int64_t i = (int64_t)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
@@ -528,6 +534,8 @@ __global__ void __launch_bounds__(kAppendThreads, 3) k_append(AppendArgs a) {
 // The queries of long runs: as k_rotate, the position from the token's sequence.
 template <typename T, int P, int LAYOUT>
 __global__ void __launch_bounds__(256, 3) k_rotate_new(AppendArgs a, int groups, int rows_per_block) {
+    griddep_wait();
+    griddep_launch_dependents();
     __shared__ int64_t position[256];
     const int units = a.k_shape.units;
     const int64_t token0 = (int64_t)blockIdx.x * rows_per_block;
@@ -564,6 +572,8 @@ struct ReadArgs {
 // Tokens without a valid page read as NaN.
 template <typename T, int CODE>
 __global__ void __launch_bounds__(256) k_read(ReadArgs a) {
+    griddep_wait();
+    griddep_launch_dependents();
     const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (t >= a.seq.tokens) return;
     const int lane = threadIdx.x & 31, dim = a.cache.dim, heads = a.cache.kv_heads;
@@ -641,9 +651,9 @@ RowShape row_shape(int64_t dim, int64_t rotated, int p) {
 template <typename T, int P>
 void rotate_layout(int layout, const RotateArgs& a, dim3 grid, dim3 block, cudaStream_t s) {
     if (layout == BFFT_PAIRS_HALF)
-        k_rotate<T, P, BFFT_PAIRS_HALF><<<grid, block, 0, s>>>(a);
+        launch_dependent(k_rotate<T, P, BFFT_PAIRS_HALF>, grid.x, block, 0, s, a);
     else
-        k_rotate<T, P, BFFT_PAIRS_INTERLEAVED><<<grid, block, 0, s>>>(a);
+        launch_dependent(k_rotate<T, P, BFFT_PAIRS_INTERLEAVED>, grid.x, block, 0, s, a);
 }
 template <typename T>
 void rotate_pack(int p, int layout, const RotateArgs& a, dim3 grid, dim3 block, cudaStream_t s) {
@@ -667,16 +677,16 @@ template <typename T, int P, int LAYOUT>
 void append_code(int code, const AppendArgs& a, const AppendPlan& p, cudaStream_t s) {
     if (!p.runs) {
         if (code == BFFT_CODE_INT8)
-            k_append<T, P, LAYOUT, kCodeInt8><<<p.blocks, kAppendThreads, 0, s>>>(a);
+            launch_dependent(k_append<T, P, LAYOUT, kCodeInt8>, p.blocks, kAppendThreads, 0, s, a);
         else
-            k_append<T, P, LAYOUT, kCodeE4m3><<<p.blocks, kAppendThreads, 0, s>>>(a);
+            launch_dependent(k_append<T, P, LAYOUT, kCodeE4m3>, p.blocks, kAppendThreads, 0, s, a);
         return;
     }
-    if (p.q_blocks) k_rotate_new<T, P, LAYOUT><<<p.q_blocks, 256, 0, s>>>(a, p.groups, p.rows_per_block);
+    if (p.q_blocks) launch_dependent(k_rotate_new<T, P, LAYOUT>, p.q_blocks, 256, 0, s, a, p.groups, p.rows_per_block);
     if (code == BFFT_CODE_INT8)
-        k_append_runs<T, P, LAYOUT, kCodeInt8><<<p.blocks, kRunThreads, 0, s>>>(a, p.heads_per_block);
+        launch_dependent(k_append_runs<T, P, LAYOUT, kCodeInt8>, p.blocks, kRunThreads, 0, s, a, p.heads_per_block);
     else
-        k_append_runs<T, P, LAYOUT, kCodeE4m3><<<p.blocks, kRunThreads, 0, s>>>(a, p.heads_per_block);
+        launch_dependent(k_append_runs<T, P, LAYOUT, kCodeE4m3>, p.blocks, kRunThreads, 0, s, a, p.heads_per_block);
 }
 template <typename T, int P>
 void append_layout(int layout, int code, const AppendArgs& a, const AppendPlan& p, cudaStream_t s) {
@@ -697,9 +707,9 @@ void append_pack(int pack, int layout, int code, const AppendArgs& a, const Appe
 template <typename T>
 void read_code(int code, const ReadArgs& a, dim3 grid, cudaStream_t s) {
     if (code == BFFT_CODE_INT8)
-        k_read<T, kCodeInt8><<<grid, 256, 0, s>>>(a);
+        launch_dependent(k_read<T, kCodeInt8>, grid.x, 256, 0, s, a);
     else
-        k_read<T, kCodeE4m3><<<grid, 256, 0, s>>>(a);
+        launch_dependent(k_read<T, kCodeE4m3>, grid.x, 256, 0, s, a);
 }
 
 struct Device {
