@@ -22,7 +22,8 @@
 //   vs, so P' (float16) times codes is the weighted value, and the sum takes
 //   p' / vs.  The largest p' is set to 2^14, near float16's top, so that weighted
 //   values keep their bits down to 2^-28 of the largest; m is renewed when one
-//   passes 2^15.5 (a vote instead of a reduction on most tiles).
+//   passes 2^15.5 (a vote instead of a reduction on most tiles).  A CTA that meets
+//   a value scale under 2^-48 keeps its sum 2^36 times smaller (see SmallScales).
 //
 // 64 sequences of 1024..32768 tokens, one row of 32 heads each (8 kv heads, 128
 // dimensions): int8 418 us, 5430 GB/s, 0.83 of the measured HBM rate; e4m3, whose
@@ -35,6 +36,18 @@ namespace bfft {
 constexpr int kDeadBlock = 3;  // BlockScale::kind of tokens that nothing sees
 // Value scale of a zero block: its codes must not count, its weights must.
 constexpr float kZeroLog2 = -64.f;
+// The sum takes p' / vs: up to 2^15.5 a token over a value scale of 2^-126, the least
+// that is kept, and 2^20 tokens pass float32's 2^128 from 2^-91 on.  The joining
+// kernel and the output take a sum in any unit that O shares, so where a CTA's tokens
+// have a scale under 2^-48 its sum and, at the end, its O are held 2^36 times smaller
+// (at most 2^126; large scales stay clear of 2^-126 up to 2^80).  There a zero block
+// counts as 2^-126: as 2^-64 it would set the maximum by which the weights of such
+// small values are rounded.  Looking for it costs 0.1 us of a short decode (8.4).
+struct SmallScales {
+    static constexpr float under_log2 = -48.f, zero_log2 = -126.f, shift = 36.f;
+    static constexpr float factor = 1.f / 68719476736.f;                 // 2^-36
+    static constexpr float inv_zero = 1237940039285380274899124224.f;   // 2^126 2^-36
+};
 constexpr float kTop = 14.f, kRenew = 15.5f;  // log2 of p' at the maximum, and where the maximum is renewed
 
 struct SplitArgs {
@@ -143,7 +156,8 @@ __device__ __forceinline__ void row_power<__half>(float, float& down, float& up)
 }
 
 // The value scale's part in the exponent, its inverse in the sum, and whether the
-// block's values count (a zero scale) or spoil the rows that see it.
+// block's values count (a zero scale, or one under 2^-126: the append keeps none) or
+// spoil the rows that see it.
 struct BlockScale {
     float key;
     float log2_value;
@@ -153,10 +167,17 @@ struct BlockScale {
 __device__ __forceinline__ BlockScale block_scale(float ks, float vs) {
     BlockScale b;
     b.key = ks;
-    b.kind = vs == 0.f ? 1 : (vs > 0.f && vs < INFINITY) ? 0 : 2;
+    b.kind = vs >= 0.f && vs < 1.17549435e-38f ? 1 : (vs > 0.f && vs < INFINITY) ? 0 : 2;
     b.log2_value = b.kind == 0 ? log2f(vs) : kZeroLog2;
     b.inv_value = b.kind == 0 ? 1.f / vs : 18446744073709551616.f;
     return b;
+}
+__device__ __forceinline__ bool small_scale(const BlockScale& b) {
+    return b.kind == 0 && b.log2_value < SmallScales::under_log2;
+}
+__device__ __forceinline__ void to_small(BlockScale& b) {
+    b.inv_value = b.kind == 0 ? b.inv_value * SmallScales::factor : SmallScales::inv_zero;
+    if (b.kind != 0) b.log2_value = SmallScales::zero_log2;
 }
 
 // The query tokens [first, first + n) of sequence s that slot i stands for, the
@@ -350,11 +371,13 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     };
     int ahead = warp;  // next tile to fetch
     for (int s = 0; s < G::STAGES && ahead < tiles; ++s, ahead += kSplitWarps) fetch(ahead, s);
+    bool any_small = false;
     for (int e = tid; e < entries; e += kSplitThreads) {
         const int id = page_ids[e];
         if (id >= 0) {
             const int64_t b = (int64_t)id * a.cache.kv_heads + kv;
             scales[e] = block_scale(a.cache.k_scale[b], a.cache.v_scale[b]);
+            any_small |= small_scale(scales[e]);
         } else {
             scales[e].kind = kDeadBlock;
         }
@@ -403,7 +426,11 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
             row_hi[nt][j] = rel(hi);
         }
     }
-    __syncthreads();
+    const bool small = __syncthreads_or(any_small);  // a small value scale in the chunk
+    if (small) {
+        for (int e = tid; e < entries; e += kSplitThreads) to_small(scales[e]);
+        __syncthreads();
+    }
 
     float o[NT][2 * G::VW][4];
     float m[NT][2], l[NT][2];
@@ -636,6 +663,13 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
             v.y += x.y * f;
             v.z += x.z * f;
             v.w += x.w * f;
+        }
+        if (small) {
+            v.x *= SmallScales::factor;
+            v.y *= SmallScales::factor;
+            v.z *= SmallScales::factor;
+            v.w *= SmallScales::factor;
+            top += SmallScales::shift;
         }
         int64_t token;
         int head;

@@ -6,6 +6,8 @@
 //
 //   loader warp    bulk copies of the 8-bit blocks, one ring for keys and values
 //                  in the order of their use, and the tile's block scales
+//   2 warps        look for a small value scale among the chunk's while the first
+//                  tile loads
 //   4 warps        widen codes to float16 (exact) in the layout of the matrix
 //                  instructions: [token][64 dims] panels, 128-byte swizzle.  Keys
 //                  (K-major) and values (N-major) share it
@@ -17,7 +19,10 @@
 //                  score passes it by the room that float16 leaves
 //
 // Key and value scales enter in the exponent as in the split kernel:
-// p' = 2^(s * ks + log2 vs - m), sum of p' / vs.
+// p' = 2^(s * ks + log2 vs - m), sum of p' / vs; a chunk with a small value scale
+// (SmallScales) holds its sums 2^36 times smaller: the loader writes its scales so,
+// and the rows take it back at their end (a flag that the rows' loop looked at cost
+// 2 % of the two-prompt case).
 //
 // 2 x 2048 prompt rows of 32 heads (8 kv heads, 128 dimensions) over 8192 and 16384
 // int8 tokens: 856 us, 884 TFLOP/s, 0.54 of the measured bf16 rate.  Bound by the
@@ -63,7 +68,7 @@ struct TileGeo {
     static constexpr int BODY = 2 * Q_HALF + T_RING * T_BUF + RAW_RING * RAW_BUF;
     static constexpr int BARS = 2 * RAW_RING + 2 * T_RING + SLOTS + 2 + 2 * 2 + 1 + 2 + 1;
     // at least half of an SM's shared memory: a second CTA could not have its tensor memory
-    static constexpr int SMEM_NEED = 1024 + BODY + SLOTS * GROUPS * 16 + BARS * 8 + 8 + SLOTS * 4;
+    static constexpr int SMEM_NEED = 1024 + BODY + SLOTS * GROUPS * 16 + BARS * 8 + 8 + SLOTS * 4 + 4;
     static constexpr int SMEM = SMEM_NEED > 118 * 1024 ? SMEM_NEED : 118 * 1024;
     static constexpr uint32_t TMEM = 512;
     static constexpr uint32_t S0 = 0, O0 = 256;   // columns: S_h at 128 h, O_h at 256 + 128 h
@@ -243,6 +248,7 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
              *p_half = s_full + 2, *p_full = p_half + 2, *q_full = p_full + 2, *o_full = q_full + 1, *drained = o_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + G::BARS);
     int* tile_kind = reinterpret_cast<int*>(bars + G::BARS + 1);  // of a tile: 0 where all its blocks are ordinary
+    volatile int* small_s = tile_kind + G::SLOTS;                 // whether the chunk has a small value scale
     if (warp == 13) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                      "r"(G::TMEM)
@@ -267,6 +273,7 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
         }
         mbar_init(q_full, 256);
         mbar_init(drained, 1);
+        *small_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     tmem_fence_before();
@@ -459,6 +466,8 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
             if (ok) {
                 tmem_fence_after();
                 const float inv = l == 0.f ? 0.f : 1.f / l;
+                const bool small = *small_s;
+                if (small) m += SmallScales::shift;
                 const int64_t at = ((token * a.q_heads + head) * p.chunks + chunk);
                 T* y = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
 #pragma unroll
@@ -466,6 +475,10 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                     uint32_t o[32];
                     tmem_load(o_addr + c * 32, o);
                     if (!mine) continue;
+                    if (small) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * SmallScales::factor);
+                    }
 #pragma unroll
                     for (int k = 0; k < 32; k += 8) {
                         const int d = c * 32 + k;
@@ -598,17 +611,21 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
             if (!value) who = copies_of(j, id0, src);
             ok = !__any_sync(0xffffffffu, !wait(&raw_empty[rb], (uint32_t)(((n / G::RAW_RING) & 1) ^ 1)));
             if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&raw_full[rb], (uint32_t)(__popc(who) * unit * dim));
+            __syncwarp();
+            if ((who >> lane) & 1)
+                bulk_load(raw_s + rb * G::RAW_BUF + lane * unit * dim, (value ? a.cache.v : a.cache.k) + src,
+                          (uint32_t)(unit * dim), &raw_full[rb]);
             if (!value) {
-                const bool odd = lane < G::GROUPS && (id0 < 0 || !(ks0 >= 0.f) || !(vs0 > 0.f) || vs0 == INFINITY);
-                const bool any = __any_sync(0xffffffffu, odd);
-                if (lane < G::GROUPS) {
-                    BlockScale b = block_scale(ks0, vs0);
-                    if (id0 < 0) {
-                        b.kind = kDeadBlock;
-                        b.key = 0.f;
-                    }
-                    scale_s[(j % G::SLOTS) * G::GROUPS + lane] = b;
+                BlockScale b = block_scale(ks0, vs0);
+                const bool any = __any_sync(0xffffffffu, lane < G::GROUPS && (id0 < 0 || !(ks0 >= 0.f) || b.kind != 0));
+                if (id0 < 0) {
+                    b.kind = kDeadBlock;
+                    b.key = 0.f;
                 }
+                if (n == 0) asm volatile("barrier.cta.sync 1, 96;" ::: "memory");  // *small_s is known
+                if (*small_s) to_small(b);
+                if (lane < G::GROUPS) scale_s[(j % G::SLOTS) * G::GROUPS + lane] = b;
                 if (lane == 0) tile_kind[j % G::SLOTS] = any;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&scale_full[j % G::SLOTS]);
@@ -619,16 +636,22 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                 scale_at(id1, ks1, vs1);
                 id2 = page_at(group_tok(j + 3));
             }
-            if (lane == 0) mbar_arrive_expect_tx(&raw_full[rb], (uint32_t)(__popc(who) * unit * dim));
-            __syncwarp();
-            if ((who >> lane) & 1)
-                bulk_load(raw_s + rb * G::RAW_BUF + lane * unit * dim, (value ? a.cache.v : a.cache.k) + src,
-                          (uint32_t)(unit * dim), &raw_full[rb]);
         }
         if (!ok)  // an expired wait has set the status bit; wait (bounded) for the copies under way
             for (int b = n > G::RAW_RING ? n - G::RAW_RING : 0; b < n; ++b)
                 wait(&raw_full[b % G::RAW_RING], (uint32_t)((b / G::RAW_RING) & 1));
-    } else if (warp == 13 && lane == 0) {
+    } else if (warp >= 14) {
+        // ------------------------------------------------------------ value scales of the blocks that are seen
+        const int64_t seen = base > lo_min ? base : lo_min;
+        bool small = false;
+        for (int64_t b = (seen >> lg) + (tid - 448); b <= (end - 1) >> lg; b += 64) {
+            const int64_t id = a.seq.block_table[sr.s * a.seq.table_stride + b];
+            if (id >= 0 && id < a.cache.pages) small |= small_scale(block_scale(0.f, a.cache.v_scale[id * a.cache.kv_heads + kv]));
+        }
+        if (small) *small_s = 1;
+        __threadfence_block();
+        asm volatile("barrier.cta.arrive 1, 96;" ::: "memory");
+    } else if (lane == 0) {
         // ------------------------------------------------------------ products
         constexpr uint32_t qk = tile_idesc(G::N, false), pv = tile_idesc(DP, true);
         const uint32_t q_low = desc_low(smem_u32(q_s), 16), k_low = desc_low(smem_u32(t_s), 16),

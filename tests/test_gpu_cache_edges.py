@@ -1,0 +1,115 @@
+"""Position and cache calls at the edges of their ranges, against plain float64 forms.
+
+Tolerances are those of the other tests of these calls: 32-bit sums, float16 weights,
+one rounding of the output.
+"""
+import math
+
+import pytest
+import torch
+
+import bfft
+from test_gpu_cache import BF16, F16, HALF_UNIT, Pages, attention64, cumulative, ints, normal
+
+pytestmark = pytest.mark.gpu
+
+
+def takes_tiles(p, q, new, table, *, causal=True, window=0):
+    """The rule by which a call goes to the tensor-core tiles: rows of a sequence in the mean, and pairs in all."""
+    group, each = q.shape[1] // p.heads, q.shape[0] // len(new)
+    cover = table.shape[1] * p.page
+    if causal and window:
+        cover = min(cover, window)
+    return p.dim <= 128 and group <= 128 and each * group >= 48 and q.shape[0] * q.shape[1] * cover * p.dim >= 3e6 * 128
+
+
+def lost_under(p, q, lens, starts, top, *, scale, causal, window):
+    """What float16 weights lose of each output: a weight times its value scale is rounded to float16 with the row's
+    largest at 2^top or over, so to within half of 2^-24, which then meets the tokens' codes."""
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    group = q.shape[1] // p.heads
+    for s, n in enumerate(lens):
+        rows = slice(starts[s], starts[s + 1])
+        k, (v, vs) = p.values(0, s, 0, n)[0], p.values(1, s, 0, n)
+        codes = torch.where(vs[..., None] > 0, v / vs[..., None], 0.0).abs()
+        pos = torch.arange(n - (starts[s + 1] - starts[s]), n, device="cuda")[:, None]
+        key = torch.arange(n, device="cuda")
+        seen = (key <= pos if causal else key >= 0) & ((key > pos - window) if window else key >= 0)
+        for h in range(q.shape[1]):
+            j = h // group
+            z = (q[rows, h].double() @ k[:, j].T * scale).masked_fill(~seen, -math.inf)
+            largest = (torch.softmax(z, -1) * vs[:, j]).amax(-1, keepdim=True)
+            out[rows, h] = 2.0 ** -(25 + top) * largest * (seen.double() @ codes[:, j])
+    return out
+
+
+def check_relative(p, q, lens, new, *, tiles, scale=None, causal=True, window=0):
+    """Every row against its own size: nothing absolute but the last bit of bfloat16's (float16's) smallest values."""
+    assert takes_tiles(p, q, new, p.table, causal=causal, window=window) == tiles
+    starts = cumulative(new)
+    got, lse = bfft.cache_attention(q, p.cache, p.table, ints(lens), ints(starts), softmax_scale=scale, causal=causal,
+                                    window=window, return_lse=True)
+    factor = p.dim ** -0.5 if scale is None else scale
+    want, want_lse, size, slack = attention64(p, q, lens, starts, scale=factor, causal=causal, window=window)
+    assert lse.isfinite().all() and got.isfinite().all()
+    delta = 2.0 ** -21 * (1 + slack)
+    tol = HALF_UNIT[q.dtype] * want.abs() + (2.0 ** -10 + 2 * delta[..., None]) * size
+    tol = tol + lost_under(p, q, lens, starts, 10 if tiles else 14, scale=factor, causal=causal, window=window)
+    tol = tol + (2.0 ** -133 if q.dtype == BF16 else 2.0 ** -24)
+    assert ((got.double() - want).abs() <= tol).all()
+    assert ((lse.double() - want_lse).abs() <= delta + 2.0 ** -20 * (1 + want_lse.abs())).all()
+    return got, lse
+
+
+# ------------------------------------------------------------------------------- small value scales
+
+def small_pages(code, where, lens, *, page=32, dim=128):
+    """Pages whose values are ordinary, but for those of `where` in each sequence: about 1e-36."""
+    p = Pages(dim + len(lens), lens, [0] * len(lens), code=code, page=page, heads=2, dim=dim)
+    for ids in p.ids:
+        kept = [i for i in ids if i >= 0]
+        p.cache.v_scale[kept if where is None else [i for j, i in enumerate(kept) if j in where]] = 1e-36
+    return p
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lens, new, tiles", [
+    ([700], [1], False),             # one cluster
+    ([6000, 41], [1, 1], False),     # chunks and a joining kernel
+    ([900], [40], False),            # several rows, and rows that see one page only
+    ([4100], [4100], True),          # row tiles, no joining: the first rows see the first page only
+    ([4100, 333], [300, 33], True),  # row tiles, chunks joined
+])
+def test_attention_over_tiny_values(code, dtype, lens, new, tiles):
+    """The weights' sum holds 1 / value scale: it may not overflow however small the scales are."""
+    p = small_pages(code, None, lens)
+    q = normal(p.g, sum(new), 8, 128, dtype=dtype)
+    out, _ = check_relative(p, q, lens, new, tiles=tiles)
+    if dtype == BF16:
+        assert out.abs().amax() > 1e-36
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("where", [{0}, {3}, {0, 1, 2, 3, 4, 5, 6, 7}])
+@pytest.mark.parametrize("lens, new, tiles", [
+    ([700], [1], False), ([6000, 41], [1, 1], False), ([300], [300], False), ([4100], [4100], True),
+    ([4100, 333], [300, 33], True),
+])
+def test_attention_over_a_tiny_page_among_ordinary_ones(code, where, lens, new, tiles):
+    p = small_pages(code, where, lens)
+    q = normal(p.g, sum(new), 8, 128, dtype=BF16)
+    check_relative(p, q, lens, new, tiles=tiles)
+
+
+@pytest.mark.parametrize("rows, tiles", [(1, False), (300, True)])
+def test_attention_over_scales_without_a_normal_float(rows, tiles):
+    """A scale under 2^-126 stands for zeros, as the append has it: its block's tokens count in the sum only."""
+    p = small_pages("int8", None, [4100])
+    p.cache.v_scale[p.ids[0][1::2]] = 1e-39
+    q = normal(p.g, rows, 8, 128, dtype=BF16)
+    got = bfft.cache_attention(q, p.cache, p.table, ints([4100]), ints([0, rows]), return_lse=True)
+    p.cache.v_scale[p.ids[0][1::2]] = 0.0
+    want = bfft.cache_attention(q, p.cache, p.table, ints([4100]), ints([0, rows]), return_lse=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[1].isfinite().all()
+    check_relative(p, q, [4100], [rows], tiles=tiles)
