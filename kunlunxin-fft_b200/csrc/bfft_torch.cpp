@@ -99,6 +99,12 @@ int64_t type_id(const Tensor& t, const char* name, bool halves = false) {
     type_error(name, " must be ", halves ? "" : "float32, ", "float16 or bfloat16, got ", at::toString(t.scalar_type()));
 }
 
+// The entry points write through pointers: an operator that saved the tensor for its
+// gradient learns of that by the version (tensors of inference mode have none).
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // (tokens, heads, dim) rows with adjacent elements
 void rows(const Tensor& t, const char* name, int64_t tokens, int64_t dim, int64_t device) {
     on_device(t, name, device);
@@ -128,6 +134,7 @@ int64_t positions_64(const Tensor& t, int64_t device) {
 struct Cache {
     bfft_cache_desc desc;
     int64_t device;
+    const Tensor* parts[4];  // k, v, k_scale, v_scale
 };
 Cache cache_of(PyObject* o) {
     if ((!PyTuple_Check(o) && !PyList_Check(o)) || PySequence_Fast_GET_SIZE(o) != 4)
@@ -135,7 +142,7 @@ Cache cache_of(PyObject* o) {
     PyObject** items = PySequence_Fast_ITEMS(o);
     const Tensor &k = tensor(items[0], "cache k"), &v = tensor(items[1], "cache v"),
                  &ks = tensor(items[2], "cache k_scale"), &vs = tensor(items[3], "cache v_scale");
-    Cache c;
+    Cache c{{}, 0, {&k, &v, &ks, &vs}};
     if (k.scalar_type() == at::kChar)
         c.desc.code = BFFT_CODE_INT8;
     else if (k.scalar_type() == at::kFloat8_e4m3fn)
@@ -233,6 +240,7 @@ Tensor launch_rotate(const Tensor& x, const Tensor& positions, const Tensor& tab
     d.transform_direction = direction;
     d.pos64 = positions.scalar_type() == at::kLong;
     d.device = x.get_device();
+    if (out) written(y);
     check(g_entry.rotate(&d, x.data_ptr(), positions.data_ptr(), table.data_ptr(), y.data_ptr(), stream_of(d.device)),
           "rotate_positions");
     return y;
@@ -351,7 +359,10 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
         d.o_head = out.stride(1);
         if (!d.q_heads) d.q = d.q_out = nullptr;
     }
-    if (tokens) check(g_entry.append(&c.desc, &q, &d, stream_of(c.device)), "append_rotated");
+    if (tokens) {
+        for (const Tensor* t : c.parts) written(*t);
+        check(g_entry.append(&c.desc, &q, &d, stream_of(c.device)), "append_rotated");
+    }
     if (!out.defined()) Py_RETURN_NONE;
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
@@ -432,6 +443,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
             d.workspace = scratch.data_ptr();
             d.workspace_bytes = (int64_t)bytes;
         }
+        if (args[9] != Py_None) written(out);
         check(g_entry.attention(&c.desc, &s, &d, stream_of(c.device)), "cache_attention");
     }
     if (want_lse) return pair(out, lse);

@@ -113,3 +113,49 @@ def test_attention_over_scales_without_a_normal_float(rows, tiles):
     want = bfft.cache_attention(q, p.cache, p.table, ints([4100]), ints([0, rows]), return_lse=True)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[1].isfinite().all()
     check_relative(p, q, [4100], [rows], tiles=tiles)
+
+
+# ------------------------------------------------------------------------------- what autograd has to know
+
+def step_inputs(rows=2):
+    p = Pages(3, [20] * rows, [4] * rows, code="int8", page=16, heads=2, dim=32)
+    x = normal(p.g, rows, 2, 32, dtype=BF16)
+    return p, x, normal(p.g, rows, 4, 32, dtype=BF16), ints([20] * rows), ints(list(range(rows + 1))), bfft.rotary_table(64, 32)
+
+
+def test_in_place_rotation_is_seen_by_saved_tensors():
+    table = bfft.rotary_table(16, 32)
+    x, where = normal(torch.Generator("cuda").manual_seed(1), 4, 2, 32), ints([0, 1, 2, 3])
+    w = torch.ones_like(x).requires_grad_(True)
+    loss = (w * x).sum()                                     # saves x for w's gradient
+    bfft.rotate_positions(x, where, table, out=x)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+
+
+def test_writes_raise_the_versions():
+    p, x, q, held, starts, table = step_inputs()
+    out = torch.empty_like(q)
+    view = torch.empty(2, 4, 64, dtype=BF16, device="cuda")
+    before = [t._version for t in (*p.cache, out, view)]
+    bfft.append_rotated(p.cache, x, x, p.table, held, starts, table, q=q)
+    bfft.cache_attention(q, p.cache, p.table, ints([21, 21]), starts, out=out)
+    bfft.rotate_positions(q, held, table, out=view[..., 16:48])
+    after = [t._version for t in (*p.cache, out, view)]
+    assert all(a > b for a, b in zip(after, before))
+    reads = [t._version for t in (x, q, held, starts, table, *p.cache)]
+    bfft.rotate_positions(q, held, table)
+    bfft.cache_attention(q, p.cache, p.table, ints([21, 21]), starts)
+    bfft.read_cache(p.cache, p.table, held, starts, 2)
+    assert reads == [t._version for t in (x, q, held, starts, table, *p.cache)]
+
+
+def test_calls_in_and_on_tensors_of_inference_mode():
+    with torch.inference_mode():
+        p, x, q, held, starts, table = step_inputs()
+        bfft.append_rotated(p.cache, x, x, p.table, held, starts, table, q=q)
+        want = bfft.cache_attention(q, p.cache, p.table, ints([21, 21]), starts, out=torch.empty_like(q))
+    # tensors made in inference mode have no versions; they still can be written
+    bfft.append_rotated(p.cache, x, x, p.table, held, starts, table, q=q)
+    got = bfft.cache_attention(q, p.cache, p.table, ints([21, 21]), starts, out=torch.empty_like(q))
+    assert torch.equal(got, want)
