@@ -105,6 +105,12 @@ void written(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// As torch's own out arguments, an output cannot be a part of the graph.
+void writable(const Tensor& out) {
+    if (at::GradMode::is_enabled() && out.requires_grad())
+        value_error("out requires a gradient: detach it or call under torch.no_grad()");
+}
+
 // (tokens, heads, dim) rows with adjacent elements
 void rows(const Tensor& t, const char* name, int64_t tokens, int64_t dim, int64_t device) {
     on_device(t, name, device);
@@ -296,6 +302,7 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
         on_device(*out, "out", device);
         if (out->sizes() != x.sizes() || out->stride(-1) != 1)
             value_error("out must be ", shape_of(x), " with adjacent elements, got ", shape_of(*out));
+        writable(*out);
     }
     if (x.requires_grad() && at::GradMode::is_enabled()) {
         if (out) value_error("out cannot be given where x requires a gradient");
@@ -423,6 +430,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         of_type(out, "out", q.scalar_type());
         rows(out, "out", tokens, c.desc.dim, c.device);
         if (out.size(1) != d.q_heads) value_error("out must be ", shape_of(q), ", got ", shape_of(out));
+        writable(out);
     } else {
         out = at::empty(q.sizes(), q.options().requires_grad(false));
     }

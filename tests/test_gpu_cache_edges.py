@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import bfft
+from bfft import _lib
 from test_gpu_cache import BF16, F16, HALF_UNIT, Pages, attention64, cumulative, ints, normal
 
 pytestmark = pytest.mark.gpu
@@ -159,3 +160,20 @@ def test_calls_in_and_on_tensors_of_inference_mode():
     bfft.append_rotated(p.cache, x, x, p.table, held, starts, table, q=q)
     got = bfft.cache_attention(q, p.cache, p.table, ints([21, 21]), starts, out=torch.empty_like(q))
     assert torch.equal(got, want)
+
+
+def test_outputs_that_require_a_gradient_are_refused():
+    p, x, q, held, starts, table = step_inputs()
+    out = torch.empty_like(q).requires_grad_(True)
+    lens = ints([21, 21])
+    count = _lib.launch_counter()
+    with pytest.raises(ValueError, match="gradient"):
+        bfft.rotate_positions(q, held, table, out=out)
+    with pytest.raises(ValueError, match="gradient"):
+        bfft.cache_attention(q, p.cache, p.table, lens, starts, out=out)
+    assert _lib.launch_counter() == count
+    with torch.no_grad():                                    # as torch's own out arguments: only the graph forbids it
+        assert bfft.rotate_positions(q, held, table, out=out) is out
+        assert torch.equal(out, bfft.rotate_positions(q, held, table))
+        bfft.cache_attention(q, p.cache, p.table, lens, starts, out=out)
+        assert torch.equal(out, bfft.cache_attention(q, p.cache, p.table, lens, starts))
