@@ -21,8 +21,9 @@ device, and ``starts[-1]`` has to be the number of rows.
 
 Calls enqueue on the current stream of the tensors' device.  Bad arguments raise
 before any launch: TypeError for a non-tensor or a wrong dtype, ValueError for
-shapes, strides and devices.  The checks and the calls themselves are in
-``csrc/bfft_torch.cpp``.
+shapes, strides and devices.  Only ``x`` of ``rotate_positions`` has a gradient: where
+gradients are enabled, the other calls and arguments refuse tensors that require one
+(ValueError).  The checks and the calls themselves are in ``csrc/bfft_torch.cpp``.
 """
 from __future__ import annotations
 

@@ -105,6 +105,12 @@ void written(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// Only x of a rotation has a gradient: a result that silently lacks one is refused.
+void constant(const Tensor& t, const char* name) {
+    if (at::GradMode::is_enabled() && t.requires_grad())
+        value_error("this call has no gradient for ", name, ": detach it or call under torch.no_grad()");
+}
+
 // As torch's own out arguments, an output cannot be a part of the graph.
 void writable(const Tensor& out) {
     if (at::GradMode::is_enabled() && out.requires_grad())
@@ -169,6 +175,8 @@ Cache cache_of(PyObject* o) {
         value_error("cache scales must be (pages, kv_heads), got ", shape_of(ks), " and ", shape_of(vs));
     if (!k.is_contiguous() || !v.is_contiguous() || !ks.is_contiguous() || !vs.is_contiguous())
         value_error("cache tensors must be contiguous");
+    constant(ks, "cache k_scale");
+    constant(vs, "cache v_scale");
     c.desc.k = k.data_ptr();
     c.desc.v = v.data_ptr();
     c.desc.k_scale = ks.data_ptr();
@@ -289,6 +297,7 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (x.dim() != 3 && x.dim() != 4)
         value_error("x must be (tokens, heads, dim) or (batch, tokens, heads, dim), got ", shape_of(x));
     table_rotated(table, x.size(-1), device);
+    constant(table, "table");
     if (x.stride(-1) != 1) value_error("x must have adjacent elements in its last dimension");
     positions_64(positions, device);
     const int64_t tokens = x.size(-3);
@@ -329,10 +338,13 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     rows(v, "v", tokens, dim, c.device);
     if (k.size(1) != heads || v.size(1) != heads)
         value_error("k and v must have the cache's ", heads, " heads, got ", k.size(1), " and ", v.size(1));
+    constant(k, "k");
+    constant(v, "v");
     const bfft_sequence_desc q = sequences(args[3], args[4], args[5], "held", tokens, c.device);
     if (args[6] != Py_None) {
         const Tensor& table = tensor(args[6], "table");
         d.rotated = table_rotated(table, dim, c.device);
+        constant(table, "table");
         d.table = table.data_ptr();
         d.table_rows = table.size(0);
     }
@@ -356,6 +368,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const Tensor& query = tensor(args[9], "q");
         of_type(query, "q", k.scalar_type());
         rows(query, "q", tokens, dim, c.device);
+        constant(query, "q");
         out = at::empty(query.sizes(), query.options().requires_grad(false));
         d.q = query.data_ptr();
         d.q_out = out.data_ptr();
@@ -410,6 +423,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     bfft_attention_desc d{};
     d.type = type_id(q, "q", true);
     rows(q, "q", -1, c.desc.dim, c.device);
+    constant(q, "q");
     const int64_t tokens = q.size(0);
     d.q_heads = q.size(1);
     if (d.q_heads < 1 || d.q_heads % c.desc.kv_heads)

@@ -177,3 +177,36 @@ def test_outputs_that_require_a_gradient_are_refused():
         assert torch.equal(out, bfft.rotate_positions(q, held, table))
         bfft.cache_attention(q, p.cache, p.table, lens, starts, out=out)
         assert torch.equal(out, bfft.cache_attention(q, p.cache, p.table, lens, starts))
+
+
+def test_calls_without_a_gradient_refuse_inputs_that_require_one():
+    """None of these may return a result that silently has no gradient."""
+    p, x, q, held, starts, table = step_inputs()
+    lens, k_scale = ints([21, 21]), p.cache.k_scale.clone().requires_grad_(True)
+    learned = bfft.PagedCache(p.cache.k, p.cache.v, k_scale, p.cache.v_scale)
+
+    def leaf(t):
+        return t.clone().requires_grad_(True)
+
+    rot, app, att, read = bfft.rotate_positions, bfft.append_rotated, bfft.cache_attention, bfft.read_cache
+    calls = [
+        (rot, (q, held, leaf(table)), {}), (rot, (leaf(q), held, leaf(table)), {}),
+        (app, (p.cache, leaf(x), x, p.table, held, starts, table), {}),
+        (app, (p.cache, x, leaf(x), p.table, held, starts, table), {}),
+        (app, (p.cache, x, x, p.table, held, starts, leaf(table)), {}),
+        (app, (p.cache, x, x, p.table, held, starts, table), {"q": leaf(q)}),
+        (app, (learned, x, x, p.table, held, starts, table), {}),
+        (att, (leaf(q), p.cache, p.table, lens, starts), {}),
+        (att, (q, learned, p.table, lens, starts), {}),
+        (read, (learned, p.table, held, starts, 2), {}),
+    ]
+    before = [t.clone() for t in p.cache]
+    count = _lib.launch_counter()
+    for fn, args, kw in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            fn(*args, **kw)
+    assert _lib.launch_counter() == count
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, p.cache))
+    with torch.no_grad():
+        for fn, args, kw in calls:
+            fn(*args, **kw)
