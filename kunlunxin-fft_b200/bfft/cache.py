@@ -23,7 +23,7 @@ Calls enqueue on the current stream of the tensors' device.  Bad arguments raise
 before any launch: TypeError for a non-tensor or a wrong dtype, ValueError for
 shapes, strides and devices.  Only ``x`` of ``rotate_positions`` has a gradient: where
 gradients are enabled, the other calls and arguments refuse tensors that require one
-(ValueError).  The checks and the calls themselves are in ``csrc/bfft_torch.cpp``.
+(ValueError).  There is no forward-mode gradient.  The checks and the calls themselves are in ``csrc/bfft_torch.cpp``.
 """
 from __future__ import annotations
 

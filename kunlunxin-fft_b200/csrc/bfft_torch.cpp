@@ -105,14 +105,21 @@ void written(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// No call has a forward-mode gradient.
+void no_tangent(const Tensor& t, const char* name) {
+    if (t._fw_grad(0).defined()) value_error("this call has no forward-mode gradient for ", name);
+}
+
 // Only x of a rotation has a gradient: a result that silently lacks one is refused.
 void constant(const Tensor& t, const char* name) {
+    no_tangent(t, name);
     if (at::GradMode::is_enabled() && t.requires_grad())
         value_error("this call has no gradient for ", name, ": detach it or call under torch.no_grad()");
 }
 
 // As torch's own out arguments, an output cannot be a part of the graph.
 void writable(const Tensor& out) {
+    no_tangent(out, "out");
     if (at::GradMode::is_enabled() && out.requires_grad())
         value_error("out requires a gradient: detach it or call under torch.no_grad()");
 }
@@ -292,6 +299,7 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor &x = tensor(args[0], "x"), &positions = tensor(args[1], "positions"), &table = tensor(args[2], "table");
     const int64_t layout = integer(args[3], "layout", 0), direction = integer(args[4], "direction", 0);
     type_id(x, "x");
+    no_tangent(x, "x");
     on_device(x, "x", -1);
     const int64_t device = x.get_device();
     if (x.dim() != 3 && x.dim() != 4)

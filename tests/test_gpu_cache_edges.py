@@ -7,6 +7,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import bfft
 from bfft import _lib
@@ -210,3 +211,20 @@ def test_calls_without_a_gradient_refuse_inputs_that_require_one():
     with torch.no_grad():
         for fn, args, kw in calls:
             fn(*args, **kw)
+
+
+def test_forward_mode_tangents_are_refused():
+    p, x, q, held, starts, table = step_inputs()
+    lens = ints([21, 21])
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        dual_x = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: bfft.rotate_positions(dual, held, table),
+                     lambda: bfft.rotate_positions(q, held, forward_ad.make_dual(table, torch.ones_like(table))),
+                     lambda: bfft.append_rotated(p.cache, dual_x, x, p.table, held, starts, table),
+                     lambda: bfft.append_rotated(p.cache, x, x, p.table, held, starts, table, q=dual),
+                     lambda: bfft.cache_attention(dual, p.cache, p.table, lens, starts),
+                     lambda: bfft.rotate_positions(q, held, table, out=forward_ad.make_dual(q.clone(), torch.ones_like(q)))):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+        assert forward_ad.unpack_dual(bfft.rotate_positions(q, held, table)).tangent is None
