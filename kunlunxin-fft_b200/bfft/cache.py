@@ -23,7 +23,9 @@ Calls enqueue on the current stream of the tensors' device.  Bad arguments raise
 before any launch: TypeError for a non-tensor or a wrong dtype, ValueError for
 shapes, strides and devices.  Only ``x`` of ``rotate_positions`` has a gradient: where
 gradients are enabled, the other calls and arguments refuse tensors that require one
-(ValueError).  There is no forward-mode gradient.  The checks and the calls themselves are in ``csrc/bfft_torch.cpp``.
+(ValueError).  There is no forward-mode gradient.  An ``out`` may be the input itself,
+but not overlap it otherwise.  The checks and the calls themselves are in
+``csrc/bfft_torch.cpp``.
 """
 from __future__ import annotations
 

@@ -117,6 +117,61 @@ void constant(const Tensor& t, const char* name) {
         value_error("this call has no gradient for ", name, ": detach it or call under torch.no_grad()");
 }
 
+// The dimensions of more than one element, widest stride first, and the elements
+// from the first to the last one.
+struct Extent {
+    int64_t size[4], stride[4], span = 1;
+    int dims = 0;
+    bool apart = true;  // each stride passes what lies under it: no element twice
+};
+Extent extent_of(const Tensor& t) {
+    Extent e;
+    for (int64_t i = 0; i < t.dim(); ++i) {
+        if (t.size(i) == 1) continue;
+        int at = e.dims++;
+        for (; at > 0 && e.stride[at - 1] < t.stride(i); --at) {
+            e.size[at] = e.size[at - 1];
+            e.stride[at] = e.stride[at - 1];
+        }
+        e.size[at] = t.size(i);
+        e.stride[at] = t.stride(i);
+    }
+    for (int i = e.dims - 1; i >= 0; --i) {
+        e.apart = e.apart && e.stride[i] >= e.span;
+        e.span += (e.size[i] - 1) * e.stride[i];
+    }
+    return e;
+}
+// Whether an element of e lies `d` elements behind one of the same tensor: with strides
+// apart, a dimension's share of d is one of two multiples of its stride.
+bool meets(const Extent& e, int dim, int64_t d) {
+    if (d == 0) return true;
+    if (dim == e.dims) return false;
+    const int64_t s = e.stride[dim], low = d / s - (d % s < 0);
+    for (int64_t k = low; k <= low + 1; ++k)
+        if (k < e.size[dim] && -k < e.size[dim] && meets(e, dim + 1, d - k * s)) return true;
+    return false;
+}
+// An output whose rows overlap, or overlap those of its input (of the same shape and
+// type) other than as the same tensor, is a race.
+void apart(const Tensor& out, const Tensor& x, const char* name) {
+    if (!out.numel()) return;
+    const Extent o = extent_of(out), e = extent_of(x);
+    if (!o.apart) value_error("out has elements that overlap");
+    const auto bytes = static_cast<int64_t>(out.element_size());
+    const int64_t d = reinterpret_cast<intptr_t>(out.data_ptr()) - reinterpret_cast<intptr_t>(x.data_ptr());
+    if (d >= e.span * bytes || -d >= o.span * bytes) return;
+    bool same = true;
+    for (int64_t i = 0; i < out.dim(); ++i) same = same && (out.size(i) == 1 || out.stride(i) == x.stride(i));
+    if (same && d % bytes == 0 && (d == 0 || !meets(o, 0, d / bytes))) return;
+    value_error("out overlaps ", name, ": it has to be ", name, " itself or lie apart from it");
+}
+// Two contiguous tensors of a size.
+void apart_whole(const Tensor& a, const Tensor& b, const char* names) {
+    const intptr_t d = reinterpret_cast<intptr_t>(a.data_ptr()) - reinterpret_cast<intptr_t>(b.data_ptr());
+    if (d < (intptr_t)b.nbytes() && -d < (intptr_t)a.nbytes()) value_error(names, " overlap");
+}
+
 // As torch's own out arguments, an output cannot be a part of the graph.
 void writable(const Tensor& out) {
     no_tangent(out, "out");
@@ -320,6 +375,7 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (out->sizes() != x.sizes() || out->stride(-1) != 1)
             value_error("out must be ", shape_of(x), " with adjacent elements, got ", shape_of(*out));
         writable(*out);
+        apart(*out, x, "x");
     }
     if (x.requires_grad() && at::GradMode::is_enabled()) {
         if (out) value_error("out cannot be given where x requires a gradient");
@@ -336,6 +392,8 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK(n == 10, "append takes 10 arguments");
     const Cache c = cache_of(args[0]);
+    apart_whole(*c.parts[0], *c.parts[1], "cache k and v");
+    apart_whole(*c.parts[2], *c.parts[3], "cache k_scale and v_scale");
     const Tensor &k = tensor(args[1], "k"), &v = tensor(args[2], "v");
     const int64_t heads = c.desc.kv_heads, dim = c.desc.dim;
     bfft_append_desc d{};
@@ -453,6 +511,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         rows(out, "out", tokens, c.desc.dim, c.device);
         if (out.size(1) != d.q_heads) value_error("out must be ", shape_of(q), ", got ", shape_of(out));
         writable(out);
+        apart(out, q, "q");
     } else {
         out = at::empty(q.sizes(), q.options().requires_grad(false));
     }

@@ -228,3 +228,50 @@ def test_forward_mode_tangents_are_refused():
             with pytest.raises(ValueError, match="gradient"):
                 call()
         assert forward_ad.unpack_dual(bfft.rotate_positions(q, held, table)).tangent is None
+
+
+# ------------------------------------------------------------------------------- overlapping memory
+
+def test_outputs_that_overlap_are_refused():
+    p, x, q, held, starts, table = step_inputs()
+    lens, where = ints([21, 21]), held
+    wide = normal(p.g, 2, 9, 80, dtype=BF16)
+    src = wide[:, 1:5, 8:40]
+    flat = normal(p.g, 2000, dtype=BF16)
+    outs = [
+        wide[:, 2:6, 8:40],                                   # a head on
+        wide[:, 1:5, 9:41],                                   # an element on
+        wide[:, 0:8:2, 8:40],                                 # other strides over the same memory
+        wide.new_zeros(1, 4, 32).expand(2, 4, 32),            # rows written twice
+        torch.as_strided(flat, (2, 4, 32), (64, 16, 1)),      # heads that run into each other
+    ]
+    count = _lib.launch_counter()
+    for out in outs:
+        with pytest.raises(ValueError, match="overlap"):
+            bfft.rotate_positions(src, where, table, out=out)
+        with pytest.raises(ValueError, match="overlap"):
+            bfft.cache_attention(src, p.cache, p.table, lens, starts, out=out)
+    # keys and values in one place: fine to read, not to append to
+    one = bfft.PagedCache(p.cache.k, p.cache.k, p.cache.k_scale, p.cache.k_scale)
+    for bad in (one, bfft.PagedCache(p.cache.k, p.cache.v, p.cache.k_scale, p.cache.k_scale)):
+        with pytest.raises(ValueError, match="overlap"):
+            bfft.append_rotated(bad, x, x, p.table, held, starts, table)
+    assert _lib.launch_counter() == count
+    k, v = bfft.read_cache(one, p.table, ints([0, 0]), starts, 2)
+    assert torch.equal(k, v)
+
+
+def test_outputs_between_the_inputs_rows_are_taken():
+    p, x, q, held, starts, table = step_inputs()
+    lens = ints([21, 21])
+    wide = normal(p.g, 2, 9, 80, dtype=BF16)
+    for src, out in ((wide[:, 0:8:2, :32], wide[:, 1:9:2, :32]),          # heads in turn
+                     (wide[:, 1:5, :32], wide[:, 1:5, 32:64]),            # halves of the rows
+                     (wide[:1].expand(2, 9, 80)[:, 2:6, :32], wide.new_zeros(2, 4, 32)),
+                     (wide[:, 3:7, 8:40], wide[:, 3:7, 8:40])):           # in place
+        want = bfft.rotate_positions(src, held, table)
+        want_y = bfft.cache_attention(src, p.cache, p.table, lens, starts)
+        kept = src.clone()
+        assert torch.equal(bfft.cache_attention(src, p.cache, p.table, lens, starts, out=out), want_y)
+        src.copy_(kept) if src.data_ptr() == out.data_ptr() else None
+        assert torch.equal(bfft.rotate_positions(src, held, table, out=out), want)
