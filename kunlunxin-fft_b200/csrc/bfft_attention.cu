@@ -141,7 +141,7 @@ struct TilePlan {
 
 // How a call is cut: row tiles and chunks of the token axis.
 struct SplitPlan {
-    int nt, tile_tokens, token_tiles, by_token, chunk, chunks, cluster;
+    int nt, tile_tokens, token_tiles, by_token, chunk, chunks, cluster, entries;
     int64_t slots, ctas;
     size_t bytes;
 };
@@ -182,6 +182,19 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
         chunk = (chunk + 31) / 32 * 32;
         if (chunk < 128) chunk = 128;
     }
+    // The parts of many rows over a wide table (the plan knows the table's width, not the
+    // lengths) are kept to 256 MB by longer chunks, as far as shared memory holds their
+    // pages' scales (4.4 GB without: 512 sequences of 4 rows of 64 heads, 131072 tokens wide)
+    const int64_t part = q->tokens * d->q_heads * (c->dim + 2) * 4, budget = (int64_t)256 << 20;
+    if (!brief && (cover + chunk - 1) / chunk * part > budget) {
+        const int64_t n = part < budget ? budget / part : 1;
+        const int64_t room = (kSplitSmemMost - split_smem((int)c->dim, 8 * p.nt, 0)) / (int64_t)(sizeof(BlockScale) + 4);
+        int64_t most = (room - 2) * c->page;
+        if (most > 1 << 20) most = 1 << 20;
+        chunk = ((cover + n - 1) / n + 31) / 32 * 32;
+        if (chunk > most) chunk = most / 32 * 32;
+    }
+    p.entries = (int)(chunk / c->page + 2);
     p.chunk = (int)chunk;
     const int64_t n = (cover + chunk - 1) / chunk;
     p.chunks = (int)n;
@@ -276,7 +289,7 @@ cudaError_t launch_split(const SplitArgs& a, const SplitPlan& p, const CUtensorM
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     auto* kernel = k_attention_split<DP, EXACT, NT, T, CODE>;
     if (!ready[dev].load(std::memory_order_acquire)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem(DP));
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmemMost);
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                                      (int)cudaSharedmemCarveoutMaxShared);
@@ -287,7 +300,7 @@ cudaError_t launch_split(const SplitArgs& a, const SplitPlan& p, const CUtensorM
     cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3((unsigned)p.ctas);
     cfg.blockDim = dim3(kSplitThreads);
-    cfg.dynamicSmemBytes = G::smem(a.a.cache.dim);
+    cfg.dynamicSmemBytes = split_smem(a.a.cache.dim, G::ROWS, a.entries);
     cfg.stream = s;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // as launch_dependent
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -389,7 +402,7 @@ extern "C" bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const 
         TileArgs ta{a, parts, stats, tp.chunk, tp.chunks, tp.tile_tokens, tp.by_token, tp.slots, status};
         e = d->type == BFFT_F16 ? run_tiles<__half>(ta, tp, cache, s) : run_tiles<__nv_bfloat16>(ta, tp, cache, s);
     } else {
-        SplitArgs sa{a, parts, stats, sp.chunk, sp.chunks, sp.tile_tokens, sp.token_tiles, sp.by_token, sp.slots, sp.cluster, status};
+        SplitArgs sa{a, parts, stats, sp.chunk, sp.chunks, sp.tile_tokens, sp.token_tiles, sp.by_token, sp.slots, sp.cluster, sp.entries, status};
         e = d->type == BFFT_F16 ? run_split<__half>(sa, sp, cache, s) : run_split<__nv_bfloat16>(sa, sp, cache, s);
     }
     return e == cudaSuccess ? BFFT_OK : fail(BFFT_ERR_CUDA, "cache_attention: %s", cudaGetErrorString(e));

@@ -61,6 +61,7 @@ struct SplitArgs {
     int by_token;        // slots are tokens (else runs of tile_tokens, see slot_rows)
     int64_t slots;
     int cluster;         // the chunks of a row tile are one thread-block cluster, which joins them
+    int entries;         // pages that a chunk can touch
     unsigned int* status;
 };
 
@@ -235,24 +236,27 @@ __device__ __forceinline__ void seen_range(const AttentionArgs& a, int64_t pos, 
     if (a.window > 0 && pos - a.window + 1 > 0) lo = pos - a.window + 1;
 }
 
+// Shared memory: the warps' rings (a stage: keys of both 16-token halves, then values),
+// in whose place the warps' parts and the CTA's for the cluster come, and the scale and
+// number of each page.
+constexpr int kSplitStages = 2;
+constexpr int kSplitSmemMost = 226 * 1024;
+__host__ __device__ constexpr int split_half_bytes(int dim) { return 16 * dim; }
+__host__ __device__ constexpr int split_body_bytes(int dim, int rows) {
+    const int ring = kSplitWarps * kSplitStages * 4 * split_half_bytes(dim), merge = (kSplitWarps + 1) * rows * (dim + 2) * 4;
+    return ring > merge ? ring : merge;
+}
+__host__ __device__ constexpr int split_smem(int dim, int rows, int entries) {
+    return 1024 + split_body_bytes(dim, rows) + entries * (int)(sizeof(BlockScale) + 4) + 64;
+}
+
 template <int DP, bool EXACT, int NT>
 struct SplitGeo {
-    static constexpr int STAGES = 2;
+    static constexpr int STAGES = kSplitStages;
     static constexpr int ROWS = 8 * NT;
     static constexpr int KS = DP / 16;         // products of 16 along a head
     static constexpr int VW = DP / 32;         // words of a token's values in a lane
-    static constexpr int MAX_ENTRIES = 4096 / 16 + 1;
-    // a ring stage: keys of both 16-token halves, then values
-    __host__ __device__ static constexpr int half_bytes(int dim) { return 16 * dim; }
-    __host__ __device__ static constexpr int ring_bytes(int dim) {
-        return kSplitWarps * STAGES * 4 * half_bytes(dim);
-    }
-    // the warps' parts, and the CTA's for the cluster
-    __host__ __device__ static constexpr int merge_bytes(int dim) { return (kSplitWarps + 1) * ROWS * (dim + 2) * 4; }
-    __host__ __device__ static constexpr int smem(int dim) {
-        const int r = ring_bytes(dim), m = merge_bytes(dim);
-        return 1024 + (r > m ? r : m) + MAX_ENTRIES * (int)(sizeof(BlockScale) + 4) + 64;
-    }
+    __host__ __device__ static constexpr int half_bytes(int dim) { return split_half_bytes(dim); }
 };
 
 template <int DP, bool EXACT, int NT, typename T, int CODE>
@@ -265,9 +269,8 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     const int dim = EXACT ? DP : a.cache.dim;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
     unsigned char* ring = align_smem<1024>(smem_raw);
-    const int body = G::ring_bytes(dim) > G::merge_bytes(dim) ? G::ring_bytes(dim) : G::merge_bytes(dim);
-    BlockScale* scales = reinterpret_cast<BlockScale*>(ring + body);
-    int* page_ids = reinterpret_cast<int*>(scales + G::MAX_ENTRIES);
+    BlockScale* scales = reinterpret_cast<BlockScale*>(ring + split_body_bytes(dim, G::ROWS));
+    int* page_ids = reinterpret_cast<int*>(scales + p.entries);
     __shared__ uint64_t full[kSplitWarps * G::STAGES];
 
     // which rows and tokens

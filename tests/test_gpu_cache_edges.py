@@ -11,7 +11,7 @@ from torch.autograd import forward_ad
 
 import bfft
 from bfft import _lib
-from test_gpu_cache import BF16, F16, HALF_UNIT, Pages, attention64, cumulative, ints, normal
+from test_gpu_cache import BF16, F16, HALF_UNIT, Pages, attention64, check_attention, cumulative, ints, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -275,3 +275,24 @@ def test_outputs_between_the_inputs_rows_are_taken():
         assert torch.equal(bfft.cache_attention(src, p.cache, p.table, lens, starts, out=out), want_y)
         src.copy_(kept) if src.data_ptr() == out.data_ptr() else None
         assert torch.equal(bfft.rotate_positions(src, held, table, out=out), want)
+
+
+# ------------------------------------------------------------------------------- tables wider than the lengths
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_attention_of_many_rows_over_a_wide_table(page, code):
+    """Parts of 512 sequences over 131072 tokens would take more than the workspace's limit: chunks of over 8000 tokens."""
+    lens = [70001] + [5 + 31 * i % 300 for i in range(511)]
+    p = Pages(page, lens, [0] * 512, code=code, page=page, heads=2, dim=128)
+    table = torch.full((512, 131072 // page), -1, dtype=torch.int32, device="cuda")
+    table[:, :p.table.shape[1]] = p.table
+    q = normal(p.g, 2048, 16, 128, dtype=BF16) * 1.5
+    assert not takes_tiles(p, q, [4] * 512, table)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    bfft.cache_attention(q, p.cache, table, ints(lens), ints(cumulative([4] * 512)))
+    assert torch.cuda.max_memory_allocated() - held < (256 << 20) + 2 * q.numel() * 2
+    check_attention(p, q, lens, [4] * 512, table=table)
+    check_attention(p, q, lens, [4] * 512, table=table, causal=False, window=30000)
