@@ -113,7 +113,7 @@ void no_tangent(const Tensor& t, const char* name) {
 // Only x of a rotation has a gradient: a result that silently lacks one is refused.
 void constant(const Tensor& t, const char* name) {
     no_tangent(t, name);
-    if (at::GradMode::is_enabled() && t.requires_grad())
+    if (t.requires_grad() && at::GradMode::is_enabled())
         value_error("this call has no gradient for ", name, ": detach it or call under torch.no_grad()");
 }
 
@@ -175,7 +175,7 @@ void apart_whole(const Tensor& a, const Tensor& b, const char* names) {
 // As torch's own out arguments, an output cannot be a part of the graph.
 void writable(const Tensor& out) {
     no_tangent(out, "out");
-    if (at::GradMode::is_enabled() && out.requires_grad())
+    if (out.requires_grad() && at::GradMode::is_enabled())
         value_error("out requires a gradient: detach it or call under torch.no_grad()");
 }
 
