@@ -6,7 +6,10 @@ in ``bfft/_lib/build_meta.json`` (part of the environment fingerprint).  The
 library is linked against the static CUDA runtime and carries no torch
 dependency; the Python layer loads it with ctypes.  ``csrc/bfft_torch.cpp``
 (host code only) becomes the extension module ``bfft/_lib/bfft_torch.so``, which
-takes torch tensors to the library's position and cache calls.
+takes torch tensors to the library's position and cache calls.  It has a record of
+its own (``torch_meta.json``: its sources, and the torch and Python it was compiled
+for); where it cannot be compiled (no host compiler, no torch headers), the library
+is complete without it and only those calls are missing.
 """
 from __future__ import annotations
 
@@ -18,6 +21,7 @@ import re
 import shutil
 import subprocess
 import sys
+import warnings
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
@@ -29,6 +33,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libbfft.so")
 TORCH_SRC = os.path.join(CSRC, "bfft_torch.cpp")
 TORCH_LIB_PATH = os.path.join(LIB_DIR, "bfft_torch.so")
 META_PATH = os.path.join(LIB_DIR, "build_meta.json")
+TORCH_META_PATH = os.path.join(LIB_DIR, "torch_meta.json")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--threads", "0", "-Xcompiler", "-fPIC", "-shared",
@@ -47,39 +52,76 @@ def sources() -> list[str]:
 
 
 def _deps() -> list[str]:
-    return sources() + [TORCH_SRC] + sorted(glob.glob(os.path.join(CSRC, "*.cuh"))) + \
+    return sources() + sorted(glob.glob(os.path.join(CSRC, "*.cuh"))) + \
         sorted(glob.glob(os.path.join(INCLUDE, "*.h")))
 
 
-def source_hash() -> str:
+def _hash(paths: list[str]) -> str:
     h = hashlib.sha256()
-    for p in _deps():
+    for p in paths:
         with open(p, "rb") as f:
             h.update(os.path.basename(p).encode())
             h.update(f.read())
     return h.hexdigest()[:16]
 
 
-def build_meta() -> dict | None:
+def source_hash() -> str:
+    return _hash(_deps())
+
+
+def _read_meta(path: str) -> dict | None:
     try:
-        with open(META_PATH) as f:
+        with open(path) as f:
             return json.load(f)
     except (OSError, json.JSONDecodeError):
         return None
 
 
+def build_meta() -> dict | None:
+    return _read_meta(META_PATH)
+
+
 def up_to_date() -> bool:
     meta = build_meta()
-    return os.path.exists(LIB_PATH) and os.path.exists(TORCH_LIB_PATH) and meta is not None and meta.get("source_hash") == source_hash()
+    return os.path.exists(LIB_PATH) and meta is not None and meta.get("source_hash") == source_hash()
 
 
-def build_torch_module(verbose: bool = True) -> str:
-    """Compile the torch binding against the installed torch's headers, with the
-    host compiler that nvcc uses: its C++ runtime has to be torch's own."""
+def torch_target() -> dict:
+    """What a binding is compiled for: the running torch and Python."""
     import sysconfig
 
     import torch
 
+    return {"torch": torch.__version__, "cxx11_abi": bool(torch._C._GLIBCXX_USE_CXX11_ABI),
+            "python": sysconfig.get_config_var("SOABI")}
+
+
+def torch_module_fits() -> bool:
+    """Whether the built binding, if any, was compiled for the running torch and Python."""
+    meta = _read_meta(TORCH_META_PATH)
+    return os.path.exists(TORCH_LIB_PATH) and meta is not None and meta.get("target") == torch_target()
+
+
+def torch_module_up_to_date() -> bool:
+    return torch_module_fits() and _read_meta(TORCH_META_PATH)["source_hash"] == _torch_hash()
+
+
+def _torch_hash() -> str:
+    return _hash([TORCH_SRC, os.path.join(INCLUDE, "bfft.h")])
+
+
+def build_torch_module(verbose: bool = True) -> str:
+    """Compile the torch binding against the installed torch's headers, with the
+    host compiler that nvcc uses: its C++ runtime has to be torch's own.  Raises where
+    that fails; a binding of other sources or another torch is gone by then."""
+    import sysconfig
+
+    import torch
+
+    for path in (TORCH_META_PATH, TORCH_LIB_PATH):
+        if os.path.exists(path):
+            os.remove(path)
+    os.makedirs(LIB_DIR, exist_ok=True)
     root = os.path.dirname(torch.__file__)
     include = os.path.join(root, "include")
     tmp = TORCH_LIB_PATH + ".tmp"
@@ -94,13 +136,12 @@ def build_torch_module(verbose: bool = True) -> str:
         print("[bfft] " + " ".join(cmd), file=sys.stderr, flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, TORCH_LIB_PATH)
+    with open(TORCH_META_PATH, "w") as f:
+        json.dump({"target": torch_target(), "source_hash": _torch_hash()}, f, indent=1)
     return TORCH_LIB_PATH
 
 
-def build(force: bool = False, verbose: bool = True) -> str:
-    """Compile libbfft.so and the torch binding if their sources changed; returns the library path."""
-    if not force and up_to_date():
-        return LIB_PATH
+def _build_library(verbose: bool) -> None:
     nvcc = nvcc_path()
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = LIB_PATH + ".tmp"
@@ -109,13 +150,25 @@ def build(force: bool = False, verbose: bool = True) -> str:
         print("[bfft] " + " ".join(cmd), file=sys.stderr, flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB_PATH)
-    build_torch_module(verbose)
     ver = subprocess.run([nvcc, "--version"], capture_output=True, text=True).stdout
     m = re.search(r"release ([0-9.]+), V([0-9.]+)", ver)
     meta = {"nvcc": m.group(2) if m else ver.strip().splitlines()[-1],
             "arch": "sm_100a", "flags": ARCH_FLAGS + NVCC_FLAGS, "source_hash": source_hash()}
     with open(META_PATH, "w") as f:
         json.dump(meta, f, indent=1)
+
+
+def build(force: bool = False, verbose: bool = True) -> str:
+    """Compile libbfft.so and the torch binding if their sources (or the binding's torch)
+    changed; returns the library path.  A binding that cannot be compiled is a warning:
+    the position and cache calls then raise, and the transforms are there."""
+    if force or not up_to_date():
+        _build_library(verbose)
+    if force or not torch_module_up_to_date():
+        try:
+            build_torch_module(verbose)
+        except (OSError, RuntimeError, subprocess.CalledProcessError) as e:
+            warnings.warn(f"bfft_torch.so was not built, position and cache calls will raise: {e}", stacklevel=2)
     return LIB_PATH
 
 

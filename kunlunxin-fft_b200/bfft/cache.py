@@ -60,6 +60,8 @@ def _load():
             if not os.path.exists(path):
                 raise RuntimeError(f"bfft_torch.so not found at {path}; build it with bfft._build.build() "
                                    "-- there is no fallback")
+            if not _build.torch_module_fits():
+                raise RuntimeError(f"{path} was built for another torch or Python; build it again with bfft._build.build()")
             lib = _lib.load()
             loader = importlib.machinery.ExtensionFileLoader("bfft_torch", path)
             module = importlib.util.module_from_spec(importlib.util.spec_from_loader("bfft_torch", loader))
