@@ -7,8 +7,6 @@
 
 #include <atomic>
 #include <cmath>
-#include <cstdarg>
-#include <cstdio>
 
 #include "../../include/bfft.h"
 #include "bfft_async.cuh"
@@ -39,18 +37,6 @@ struct AttentionArgs {
 
 namespace {
 
-bfft_status fail(bfft_status st, const char* fmt, ...) {
-    char buf[384];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
-    va_end(ap);
-    set_last_error(buf);  // reported by bfft_last_error()
-    return st;
-}
-
-bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
-
 bfft_status check(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs, const bfft_attention_desc* d) {
     if (!cache || !seqs || !d || !d->q || !d->out) return fail(BFFT_ERR_VALUE, "null pointer");
     bfft_status st = check_cache(cache);
@@ -66,19 +52,6 @@ bfft_status check(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs, 
     if (!aligned(d->q, 2) || !aligned(d->out, 2) || !aligned(d->lse, 4)) return fail(BFFT_ERR_VALUE, "misaligned pointer");
     return BFFT_OK;
 }
-
-struct Device {
-    int prev = -1;
-    bool ok = true, changed = false;
-    explicit Device(int64_t dev) {
-        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev != dev) ok = cudaSetDevice((int)dev) == cudaSuccess;
-        changed = ok && prev != dev;
-    }
-    ~Device() {
-        if (changed && prev >= 0) cudaSetDevice(prev);
-    }
-};
 
 using EncodeTiledFn = PFN_cuTensorMapEncodeTiled_v12000;
 
@@ -115,7 +88,10 @@ int sm_count(int64_t device) {
     const int dev = (int)device;
     int n = counts[dev].load(std::memory_order_relaxed);
     if (!n) {
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            n = 148;
+        }
         counts[dev].store(n, std::memory_order_relaxed);
     }
     return n;
@@ -379,7 +355,7 @@ extern "C" bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const 
     a.o_packs = aligned(d->out, 16) && d->o_token % 8 == 0 && d->o_head % 8 == 0;
     unsigned int* status;
     cudaError_t e = device_status_word(&status);
-    if (e != cudaSuccess) return fail(BFFT_ERR_CUDA, "cache_attention: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) return launched(e, "cache_attention");
     const bool tiles = use_tiles(cache, seqs, d);
     TilePlan tp{};
     SplitPlan sp{};
@@ -405,5 +381,5 @@ extern "C" bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const 
         SplitArgs sa{a, parts, stats, sp.chunk, sp.chunks, sp.tile_tokens, sp.token_tiles, sp.by_token, sp.slots, sp.cluster, sp.entries, status};
         e = d->type == BFFT_F16 ? run_split<__half>(sa, sp, cache, s) : run_split<__nv_bfloat16>(sa, sp, cache, s);
     }
-    return e == cudaSuccess ? BFFT_OK : fail(BFFT_ERR_CUDA, "cache_attention: %s", cudaGetErrorString(e));
+    return launched(e, "cache_attention");
 }

@@ -176,7 +176,23 @@ inline cudaError_t launch_dependent(void (*kernel)(P...), unsigned grid, dim3 bl
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Host side (bfft_rotary.cu): the checks that every call on a cache makes.
+// Host side (bfft_rotary.cu).  An error's text goes to bfft_last_error(); the runtime's
+// own record of it is cleared, so that the next call on this thread does not report it.
+bfft_status fail(bfft_status st, const char* fmt, ...);
+bfft_status launched(cudaError_t e, const char* call);  // the status of a call's launches
+inline bool aligned(const void* p, int64_t bytes) {
+    return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0;
+}
+
+// The call's device, and the caller's again when the call returns.
+struct Device {
+    int prev = -1;
+    bool ok = true, changed = false;
+    explicit Device(int64_t dev);
+    ~Device();
+};
+
+// The checks that every call on a cache makes.
 bfft_status check_cache(const bfft_cache_desc* c);
 bfft_status check_sequences(const bfft_sequence_desc* q);
 CacheView cache_view(const bfft_cache_desc* c);

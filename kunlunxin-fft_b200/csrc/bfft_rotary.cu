@@ -612,18 +612,6 @@ __global__ void __launch_bounds__(256) k_read(ReadArgs a) {
 // ---------------------------------------------------------------- host side
 namespace {
 
-bfft_status fail(bfft_status st, const char* fmt, ...) {
-    char buf[384];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
-    va_end(ap);
-    set_last_error(buf);  // reported by bfft_last_error()
-    return st;
-}
-
-bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
-
 int type_bytes(int64_t type) { return type == BFFT_F32 ? 4 : 2; }
 
 // Largest pack of P elements (P * bytes <= 16) that divides every pointer's and
@@ -649,19 +637,17 @@ RowShape row_shape(int64_t dim, int64_t rotated, int p) {
 }
 
 template <typename T, int P>
-void rotate_layout(int layout, const RotateArgs& a, dim3 grid, dim3 block, cudaStream_t s) {
-    if (layout == BFFT_PAIRS_HALF)
-        launch_dependent(k_rotate<T, P, BFFT_PAIRS_HALF>, grid.x, block, 0, s, a);
-    else
-        launch_dependent(k_rotate<T, P, BFFT_PAIRS_INTERLEAVED>, grid.x, block, 0, s, a);
+cudaError_t rotate_layout(int layout, const RotateArgs& a, dim3 grid, dim3 block, cudaStream_t s) {
+    if (layout == BFFT_PAIRS_HALF) return launch_dependent(k_rotate<T, P, BFFT_PAIRS_HALF>, grid.x, block, 0, s, a);
+    return launch_dependent(k_rotate<T, P, BFFT_PAIRS_INTERLEAVED>, grid.x, block, 0, s, a);
 }
 template <typename T>
-void rotate_pack(int p, int layout, const RotateArgs& a, dim3 grid, dim3 block, cudaStream_t s) {
+cudaError_t rotate_pack(int p, int layout, const RotateArgs& a, dim3 grid, dim3 block, cudaStream_t s) {
     if constexpr (sizeof(T) == 2)
         if (p == 8) return rotate_layout<T, 8>(layout, a, grid, block, s);
     if (p == 4) return rotate_layout<T, 4>(layout, a, grid, block, s);
     if (p == 2) return rotate_layout<T, 2>(layout, a, grid, block, s);
-    rotate_layout<T, 1>(layout, a, grid, block, s);
+    return rotate_layout<T, 1>(layout, a, grid, block, s);
 }
 
 // Launches of one append; `runs`: by runs (see AppendArgs).
@@ -674,61 +660,70 @@ struct AppendPlan {
 };
 
 template <typename T, int P, int LAYOUT>
-void append_code(int code, const AppendArgs& a, const AppendPlan& p, cudaStream_t s) {
+cudaError_t append_code(int code, const AppendArgs& a, const AppendPlan& p, cudaStream_t s) {
     if (!p.runs) {
         if (code == BFFT_CODE_INT8)
-            launch_dependent(k_append<T, P, LAYOUT, kCodeInt8>, p.blocks, kAppendThreads, 0, s, a);
-        else
-            launch_dependent(k_append<T, P, LAYOUT, kCodeE4m3>, p.blocks, kAppendThreads, 0, s, a);
-        return;
+            return launch_dependent(k_append<T, P, LAYOUT, kCodeInt8>, p.blocks, kAppendThreads, 0, s, a);
+        return launch_dependent(k_append<T, P, LAYOUT, kCodeE4m3>, p.blocks, kAppendThreads, 0, s, a);
     }
-    if (p.q_blocks) launch_dependent(k_rotate_new<T, P, LAYOUT>, p.q_blocks, 256, 0, s, a, p.groups, p.rows_per_block);
+    if (p.q_blocks) {
+        const cudaError_t e =
+            launch_dependent(k_rotate_new<T, P, LAYOUT>, p.q_blocks, 256, 0, s, a, p.groups, p.rows_per_block);
+        if (e != cudaSuccess) return e;
+    }
     if (code == BFFT_CODE_INT8)
-        launch_dependent(k_append_runs<T, P, LAYOUT, kCodeInt8>, p.blocks, kRunThreads, 0, s, a, p.heads_per_block);
-    else
-        launch_dependent(k_append_runs<T, P, LAYOUT, kCodeE4m3>, p.blocks, kRunThreads, 0, s, a, p.heads_per_block);
+        return launch_dependent(k_append_runs<T, P, LAYOUT, kCodeInt8>, p.blocks, kRunThreads, 0, s, a, p.heads_per_block);
+    return launch_dependent(k_append_runs<T, P, LAYOUT, kCodeE4m3>, p.blocks, kRunThreads, 0, s, a, p.heads_per_block);
 }
 template <typename T, int P>
-void append_layout(int layout, int code, const AppendArgs& a, const AppendPlan& p, cudaStream_t s) {
-    if (layout == BFFT_PAIRS_HALF)
-        append_code<T, P, BFFT_PAIRS_HALF>(code, a, p, s);
-    else
-        append_code<T, P, BFFT_PAIRS_INTERLEAVED>(code, a, p, s);
+cudaError_t append_layout(int layout, int code, const AppendArgs& a, const AppendPlan& p, cudaStream_t s) {
+    if (layout == BFFT_PAIRS_HALF) return append_code<T, P, BFFT_PAIRS_HALF>(code, a, p, s);
+    return append_code<T, P, BFFT_PAIRS_INTERLEAVED>(code, a, p, s);
 }
 template <typename T>
-void append_pack(int pack, int layout, int code, const AppendArgs& a, const AppendPlan& p, cudaStream_t s) {
+cudaError_t append_pack(int pack, int layout, int code, const AppendArgs& a, const AppendPlan& p, cudaStream_t s) {
     if constexpr (sizeof(T) == 2)
         if (pack == 8) return append_layout<T, 8>(layout, code, a, p, s);
     if (pack == 4) return append_layout<T, 4>(layout, code, a, p, s);
     if (pack == 2) return append_layout<T, 2>(layout, code, a, p, s);
-    append_layout<T, 1>(layout, code, a, p, s);
+    return append_layout<T, 1>(layout, code, a, p, s);
 }
 
 template <typename T>
-void read_code(int code, const ReadArgs& a, dim3 grid, cudaStream_t s) {
-    if (code == BFFT_CODE_INT8)
-        launch_dependent(k_read<T, kCodeInt8>, grid.x, 256, 0, s, a);
-    else
-        launch_dependent(k_read<T, kCodeE4m3>, grid.x, 256, 0, s, a);
+cudaError_t read_code(int code, const ReadArgs& a, dim3 grid, cudaStream_t s) {
+    if (code == BFFT_CODE_INT8) return launch_dependent(k_read<T, kCodeInt8>, grid.x, 256, 0, s, a);
+    return launch_dependent(k_read<T, kCodeE4m3>, grid.x, 256, 0, s, a);
 }
-
-struct Device {
-    int prev = -1;
-    bool ok = true;
-    explicit Device(int64_t dev) {
-        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev != dev) ok = cudaSetDevice((int)dev) == cudaSuccess;
-        changed = ok && prev != dev;
-    }
-    ~Device() {
-        if (changed && prev >= 0) cudaSetDevice(prev);
-    }
-    bool changed = false;
-};
 
 }  // namespace
 
 namespace bfft {
+
+bfft_status fail(bfft_status st, const char* fmt, ...) {
+    char buf[384];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    set_last_error(buf);  // reported by bfft_last_error()
+    return st;
+}
+
+bfft_status launched(cudaError_t e, const char* call) {
+    if (e == cudaSuccess) return BFFT_OK;
+    cudaGetLastError();
+    return fail(BFFT_ERR_CUDA, "%s: %s", call, cudaGetErrorString(e));
+}
+
+Device::Device(int64_t dev) {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    if (prev != dev) ok = cudaSetDevice((int)dev) == cudaSuccess;
+    changed = ok && prev != dev;
+    if (!ok || prev < 0) cudaGetLastError();
+}
+Device::~Device() {
+    if (changed && prev >= 0) cudaSetDevice(prev);
+}
 
 bfft_status check_cache(const bfft_cache_desc* c) {
     if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(BFFT_ERR_VALUE, "null cache pointer");
@@ -839,14 +834,10 @@ extern "C" bfft_status bfft_rotate_positions(const bfft_rotate_desc* d, const vo
     const dim3 grid((unsigned)blocks);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     count_launches(1);
-    if (d->type == BFFT_F32)
-        rotate_pack<float>(p, (int)d->layout, a, grid, block, s);
-    else if (d->type == BFFT_F16)
-        rotate_pack<__half>(p, (int)d->layout, a, grid, block, s);
-    else
-        rotate_pack<__nv_bfloat16>(p, (int)d->layout, a, grid, block, s);
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? BFFT_OK : fail(BFFT_ERR_CUDA, "rotate_positions: %s", cudaGetErrorString(e));
+    return launched(d->type == BFFT_F32   ? rotate_pack<float>(p, (int)d->layout, a, grid, block, s)
+                    : d->type == BFFT_F16 ? rotate_pack<__half>(p, (int)d->layout, a, grid, block, s)
+                                       : rotate_pack<__nv_bfloat16>(p, (int)d->layout, a, grid, block, s),
+                    "rotate_positions");
 }
 
 extern "C" bfft_status bfft_cache_append(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
@@ -917,14 +908,10 @@ extern "C" bfft_status bfft_cache_append(const bfft_cache_desc* cache, const bff
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int layout = (int)d->layout, code = (int)cache->code;
     count_launches(q_blocks ? 2 : 1);
-    if (d->type == BFFT_F32)
-        append_pack<float>(p, layout, code, a, plan, s);
-    else if (d->type == BFFT_F16)
-        append_pack<__half>(p, layout, code, a, plan, s);
-    else
-        append_pack<__nv_bfloat16>(p, layout, code, a, plan, s);
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? BFFT_OK : fail(BFFT_ERR_CUDA, "cache_append: %s", cudaGetErrorString(e));
+    return launched(d->type == BFFT_F32   ? append_pack<float>(p, layout, code, a, plan, s)
+                    : d->type == BFFT_F16 ? append_pack<__half>(p, layout, code, a, plan, s)
+                                       : append_pack<__nv_bfloat16>(p, layout, code, a, plan, s),
+                    "cache_append");
 }
 
 extern "C" bfft_status bfft_cache_read(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs, int64_t type,
@@ -946,12 +933,8 @@ extern "C" bfft_status bfft_cache_read(const bfft_cache_desc* cache, const bfft_
     const dim3 grid((unsigned)((seqs->tokens + 7) / 8));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     count_launches(1);
-    if (type == BFFT_F32)
-        read_code<float>((int)cache->code, a, grid, s);
-    else if (type == BFFT_F16)
-        read_code<__half>((int)cache->code, a, grid, s);
-    else
-        read_code<__nv_bfloat16>((int)cache->code, a, grid, s);
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? BFFT_OK : fail(BFFT_ERR_CUDA, "cache_read: %s", cudaGetErrorString(e));
+    return launched(type == BFFT_F32   ? read_code<float>((int)cache->code, a, grid, s)
+                    : type == BFFT_F16 ? read_code<__half>((int)cache->code, a, grid, s)
+                                       : read_code<__nv_bfloat16>((int)cache->code, a, grid, s),
+                    "cache_read");
 }

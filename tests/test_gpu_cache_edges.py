@@ -11,6 +11,7 @@ from torch.autograd import forward_ad
 
 import bfft
 from bfft import _lib
+from test_cache_host import pack_append, pack_attention, pack_cache, pack_rotate, pack_sequences
 from test_gpu_cache import BF16, F16, HALF_UNIT, Pages, attention64, check_attention, cumulative, ints, normal
 
 pytestmark = pytest.mark.gpu
@@ -296,3 +297,43 @@ def test_attention_of_many_rows_over_a_wide_table(page, code):
     assert torch.cuda.max_memory_allocated() - held < (256 << 20) + 2 * q.numel() * 2
     check_attention(p, q, lens, [4] * 512, table=table)
     check_attention(p, q, lens, [4] * 512, table=table, causal=False, window=30000)
+
+
+# ------------------------------------------------------------------------------- the C entries' status
+
+def test_a_device_that_is_not_there_fails_its_own_call_only():
+    """The failed call's error does not stay behind for the next one to report."""
+    lib = _lib.load()
+    p, x, q, held, starts, table = step_inputs()
+    out, lens = torch.empty_like(q), ints([21, 21])
+    k, v = torch.empty_like(x), torch.empty_like(x)
+    stream = torch.cuda.current_stream().cuda_stream
+    cache = pack_cache(*(t.data_ptr() for t in p.cache), p.cache.k.shape[0], 2, 16, 32, 0)
+
+    def seqs(lens):
+        return pack_sequences(p.table.data_ptr(), p.table.stride(0), lens.data_ptr(), starts.data_ptr(), 2, p.table.shape[1], 2)
+
+    def rotate(device):
+        d = pack_rotate(1, 2, 4, 32, 32, 0, 128, 32, 0, 128, 32, 0, 1, 64, 2, 0, 0, 0, device)
+        return lib.bfft_rotate_positions(d, q.data_ptr(), held.data_ptr(), table.data_ptr(), out.data_ptr(), stream)
+
+    def append(device):
+        d = pack_append(x.data_ptr(), x.data_ptr(), 0, 0, 0, 0, 64, 32, 64, 32, 0, 0, 0, 0, 0, 0, 0, 2, 0, 0, device)
+        return lib.bfft_cache_append(cache, seqs(held), d, stream)
+
+    def read(device):
+        return lib.bfft_cache_read(cache, seqs(held), 2, k.data_ptr(), v.data_ptr(), device, stream)
+
+    def attend(device):
+        d = pack_attention(q.data_ptr(), out.data_ptr(), 0, 128, 32, 128, 32, 4, 2, 1, 0, 0.2, 0, 0, device)
+        return lib.bfft_cache_attention(cache, seqs(lens), d, stream)
+
+    calls = (rotate, append, read, attend)
+    for bad in calls:
+        for good in calls:
+            assert bad(99) == _lib.ERR_CUDA and "99" in _lib.last_error()
+            assert good(0) == _lib.OK, (bad.__name__, good.__name__, _lib.last_error())
+        assert bad(99) == _lib.ERR_CUDA
+        y, _ = bfft.run_fft(torch.ones(64, dtype=torch.complex64, device="cuda"), "dit", profile_hash=None)
+        assert abs(complex(y[0]) - 64) < 1e-3
+    torch.cuda.synchronize()
