@@ -389,8 +389,8 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, const Run& r, i
 #pragma unroll
         for (int j = 0; j < 2 * P; ++j) most = max_abs(most, e[j]);
     }
-    // the order of magnitudes' bits puts NaN over infinity over numbers; also orders the reads of the scale before
-    // its write
+    // the order of magnitudes' bits puts NaN over infinity over numbers; its barrier also orders the reads of the
+    // scale before its write
     const uint32_t big = most_of(__float_as_uint(most) & 0x7fffffffu);
     // a block under 2^-126 * most is zero: no denormal scales
     float now = __uint_as_float(big) / CodeRange<CODE>::most;
@@ -484,8 +484,11 @@ __device__ __forceinline__ void append_warp(const AppendArgs& a, const Run& r, i
     fetch_units<T, P, ROTATE, 1>(a, r, head, m, raw);
     const int64_t page_id = page_of(a.seq, a.cache, r.s, r.at);
     if (page_id < 0) return;
-    append_rows<T, P, LAYOUT, CODE, ROTATE, 1>(a, r, page_id, head, m, raw, lane, 32,
-                                               [](uint32_t big) { return __reduce_max_sync(0xffffffffu, big); });
+    append_rows<T, P, LAYOUT, CODE, ROTATE, 1>(a, r, page_id, head, m, raw, lane, 32, [](uint32_t big) {
+        big = __reduce_max_sync(0xffffffffu, big);
+        __syncwarp();  // the reduction alone does not order memory
+        return big;
+    });
 }
 
 // Position of a new token.
