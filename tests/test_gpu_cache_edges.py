@@ -26,9 +26,10 @@ def takes_tiles(p, q, new, table, *, causal=True, window=0):
     return p.dim <= 128 and group <= 128 and each * group >= 48 and q.shape[0] * q.shape[1] * cover * p.dim >= 3e6 * 128
 
 
-def lost_under(p, q, lens, starts, top, *, scale, causal, window):
+def lost_under(p, q, lens, starts, top, *, scale, causal, window, zero_as=0.0):
     """What float16 weights lose of each output: a weight times its value scale is rounded to float16 with the row's
-    largest at 2^top or over, so to within half of 2^-24, which then meets the tokens' codes."""
+    largest at 2^top or over, so to within half of 2^-24, which then meets the tokens' codes.  A zero value scale
+    takes part in that largest as `zero_as`."""
     out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
     group = q.shape[1] // p.heads
     for s, n in enumerate(lens):
@@ -41,12 +42,12 @@ def lost_under(p, q, lens, starts, top, *, scale, causal, window):
         for h in range(q.shape[1]):
             j = h // group
             z = (q[rows, h].double() @ k[:, j].T * scale).masked_fill(~seen, -math.inf)
-            largest = (torch.softmax(z, -1) * vs[:, j]).amax(-1, keepdim=True)
+            largest = (torch.softmax(z, -1) * torch.where(vs == 0, zero_as, vs)[:, j]).amax(-1, keepdim=True)
             out[rows, h] = 2.0 ** -(25 + top) * largest * (seen.double() @ codes[:, j])
     return out
 
 
-def check_relative(p, q, lens, new, *, tiles, scale=None, causal=True, window=0):
+def check_relative(p, q, lens, new, *, tiles, scale=None, causal=True, window=0, zero_as=0.0):
     """Every row against its own size: nothing absolute but the last bit of bfloat16's (float16's) smallest values."""
     assert takes_tiles(p, q, new, p.table, causal=causal, window=window) == tiles
     starts = cumulative(new)
@@ -57,7 +58,8 @@ def check_relative(p, q, lens, new, *, tiles, scale=None, causal=True, window=0)
     assert lse.isfinite().all() and got.isfinite().all()
     delta = 2.0 ** -21 * (1 + slack)
     tol = HALF_UNIT[q.dtype] * want.abs() + (2.0 ** -10 + 2 * delta[..., None]) * size
-    tol = tol + lost_under(p, q, lens, starts, 10 if tiles else 14, scale=factor, causal=causal, window=window)
+    tol = tol + lost_under(p, q, lens, starts, 10 if tiles else 14, scale=factor, causal=causal, window=window,
+                           zero_as=zero_as)
     tol = tol + (2.0 ** -133 if q.dtype == BF16 else 2.0 ** -24)
     assert ((got.double() - want).abs() <= tol).all()
     assert ((lse.double() - want_lse).abs() <= delta + 2.0 ** -20 * (1 + want_lse.abs())).all()
