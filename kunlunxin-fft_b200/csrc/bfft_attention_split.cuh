@@ -136,16 +136,17 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Power of two that brings a row's largest magnitude to [1, 2), and its inverse,
-// so that bfloat16 queries fit float16 (exactly, but for elements under 2^-14 of
-// the row's largest, which lose bits under 2^-24 of it).  1 where the row is zero
-// or not finite.
+// Power of two that brings a row's largest magnitude to [1, 2), in the last binades to
+// [1, 4) (the power is a normal float), and its inverse, so that bfloat16 queries fit
+// float16 (exactly, but for elements under 2^-14 of the row's largest, which lose bits
+// under 2^-24 of it).  1 where the row is zero or not finite.
 template <typename T>
 __device__ __forceinline__ void row_power(float big, float& down, float& up) {
     down = up = 1.f;
     if constexpr (sizeof(T) == 2) {
-        const int e = (int)(__float_as_uint(big) >> 23) & 255;
-        if (e > 0 && e < 254) {
+        int e = (int)(__float_as_uint(big) >> 23) & 255;
+        if (e > 0 && e < 255) {
+            e = e < 253 ? e : 253;
             down = __uint_as_float((uint32_t)(254 - e) << 23);
             up = __uint_as_float((uint32_t)e << 23);
         }

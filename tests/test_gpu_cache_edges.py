@@ -339,3 +339,17 @@ def test_a_device_that_is_not_there_fails_its_own_call_only():
         y, _ = bfft.run_fft(torch.ones(64, dtype=torch.complex64, device="cuda"), "dit", profile_hash=None)
         assert abs(complex(y[0]) - 64) < 1e-3
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------- queries near the largest float
+
+@pytest.mark.parametrize("new, tiles", [([1], False), ([40], False), ([300], True)])
+def test_attention_of_queries_near_the_largest_float(new, tiles):
+    """bfloat16 queries go through float16 by a power of two of their row, up to the type's last binade."""
+    p = Pages(33, [4100], [0], code="int8", page=64, heads=2, dim=128)
+    p.cache.k_scale.mul_(2.0 ** -120)
+    q = normal(p.g, new[0], 8, 128).clamp(-3.9, 3.9)
+    q[..., 5] = 3.9
+    q = (q * 2.0 ** 126).to(BF16)                            # 3.9 * 2^126 lies in [2^127, 2^128)
+    assert q.isfinite().all() and (q.abs().amax(-1) >= 2.0 ** 127).all()
+    check_relative(p, q, [4100], new, tiles=tiles, scale=2.0 ** -8)
