@@ -316,7 +316,9 @@ BFFT_EXPORT bfft_status bfft_rotate_positions(const bfft_rotate_desc* desc, cons
 
 /* Pages of `page` tokens, one block of codes per page and kv head, one float32
  * scale per block for keys and one for values: token value = code * scale.  A
- * block that ever held a NaN or an infinity reads as NaN. */
+ * block that ever held a NaN or an infinity reads as NaN.  Scales are not
+ * negative; attention takes a value scale under 2^-126 as zero (the append
+ * writes none). */
 typedef struct bfft_cache_desc {
     void *k, *v;             /* [pages][kv_heads][page][dim] 8-bit codes, 16-byte aligned */
     void *k_scale, *v_scale; /* [pages][kv_heads] float32                       */
@@ -346,7 +348,8 @@ typedef struct bfft_append_desc {
 } bfft_append_desc;
 
 /* Appends each sequence's rows behind the lens[s] tokens that it holds: rotates
- * q and k, quantises k and v, one launch.  A block's scale is the largest
+ * q and k, quantises k and v; one launch, two where runs are few and long.  A
+ * block's scale is the largest
  * magnitude that it has held over 127 (448); where new rows make it grow, the
  * block's earlier codes are rounded again to the new scale.  A sequence's first
  * token of a page starts the block anew.  Sequences must not share a page that
@@ -368,7 +371,7 @@ typedef struct bfft_attention_desc {
     int64_t q_heads;         /* a multiple of kv_heads                          */
     int64_t type;
     int64_t causal;          /* row i of n sees tokens <= lens[s] - n + i       */
-    int64_t window;          /* > 0: and only the last `window` of them         */
+    int64_t window;          /* > 0: and none before lens[s] - n + i + 1 - window */
     double softmax_scale;
     void* workspace;
     int64_t workspace_bytes;
@@ -380,7 +383,8 @@ typedef struct bfft_attention_desc {
  * that sees no token gets out = 0 and lse = -inf.  A token without a valid page
  * is not seen.  The workspace (bfft_cache_attention_workspace bytes for the same
  * descriptors, 16-byte aligned) holds the parts of rows whose tokens are shared
- * out over several blocks. */
+ * out over several blocks: at most 256 MB, or what one to a few parts of each row
+ * take where that is more.  out may be q, but not overlap it otherwise. */
 BFFT_EXPORT bfft_status bfft_cache_attention_workspace(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
                                                        const bfft_attention_desc* desc, size_t* bytes);
 BFFT_EXPORT bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,

@@ -1,15 +1,15 @@
 """Rotation by position, and attention over a paged 8-bit cache.
 
-No counterpart in the reference.  What an attention layer needs next to the
-transforms: its queries and keys are rotated by unit roots of their positions
-(the twiddle product, with a table made in float64), the keys and values of past
-tokens are kept in 8 bits, and new tokens attend to them.
+No counterpart in the reference, and no transform is part of it; what it shares with
+them is the product by unit roots from a table made in float64.  An attention layer's
+queries and keys are rotated by unit roots of their positions, the keys and values of
+past tokens are kept in 8 bits, and new tokens attend to them.
 
 * ``rotary_table`` / ``rotate_positions``: the rotation, forward and inverse;
   differentiable (the gradient is rotated by the conjugate roots).
 * ``paged_cache`` / ``append_rotated``: pages of 16..128 tokens hold int8 or e4m3
   codes with one scale per page and kv head; new tokens are rotated, quantised
-  and written by one launch.
+  and written by one launch (two where few sequences append long runs).
 * ``cache_attention``: causal, windowed or full attention of ragged rows (one
   token, a few drafted ones, or a prompt's chunk per sequence) over the cache.
 * ``read_cache``: the values that the cache stands for.
@@ -107,7 +107,9 @@ def rotary_table(positions: int, rotated: int, *, base: float = 10000.0, scaling
     base * factor^(rotated / (rotated - 2)), so that the slowest is divided by the
     factor and the fastest stays; "banded" divides those that make fewer than
     ``low_turns`` turns over the ``original`` context, keeps those that make more
-    than ``high_turns`` and blends between them by their turns."""
+    than ``high_turns`` and blends between them linearly in their turns (a blend that
+    is linear in the index j, as some models are trained with, gives other
+    frequencies: make that table yourself)."""
     if positions < 1 or rotated < 2 or rotated % 2:
         raise ValueError(f"need positions >= 1 and an even rotated part, got {positions} and {rotated}")
     if scaling not in SCALINGS:
@@ -169,7 +171,8 @@ def append_rotated(cache, k, v, block_table, held, starts, table=None, *, layout
     Two sequences must not append to one page.  Rows whose page is not in the table
     are dropped.
 
-    q: (tokens, q_heads, dim) of k's type; its rotated rows are returned (else None)."""
+    q: (tokens, q_heads, dim) of k's type; its rotated rows are returned (else None).
+    ``cache_attention`` takes them in float16 or bfloat16."""
     return (_native or _load()).append(cache, k, v, block_table, held, starts, table, _layout(layout), positions, q)
 
 
@@ -192,7 +195,12 @@ def cache_attention(q, cache, block_table, lens, starts, *, softmax_scale: float
     lens[s]: tokens that sequence s has in the cache, those of its new rows among
     them.  Row i of a sequence's n rows is its token lens[s] - n + i; causal rows
     see the tokens up to their own, and with ``window`` > 0 only the last ``window``
-    of those.  A row that sees no token gets zeros and a log-sum-exp of -inf.
+    of those (rows that are not causal: from there to the sequence's end).  A row that
+    sees no token gets zeros and a log-sum-exp of -inf.
+
+    The weights, times their block's value scale, are rounded to float16 before they
+    meet the codes, with a row's largest near float16's top: to 2^-11 down to 2^-24 of
+    the largest (few rows: 2^-28), to nothing under 2^-34 (2^-38).
 
     Returns out (tokens, q_heads, dim), with ``return_lse`` also the rows' log-sum-exp
     (tokens, q_heads) float32."""

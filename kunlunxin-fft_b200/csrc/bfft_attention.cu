@@ -137,10 +137,16 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
     const int64_t tiles = (q->tokens + p.tile_tokens - 1) / p.tile_tokens;
     const int64_t units = tiles * p.token_tiles * c->kv_heads, resident = 3 * (int64_t)sms;
     // Where rows are many, chunks of 2048 tokens (512..4096 measure alike for 64 ragged
-    // sequences).  Where they are few the axis is shared out over one wave of CTAs: a
-    // second wave's start costs more than it hides (one sequence of 131001 tokens: 71.6
-    // us, two waves 75.8, three 84.0) unless many sequences of different lengths leave
-    // the first one ragged (16 of 2000..8000: 63.5 us in one, 59.4 in two, 69.6 in three).
+    // sequences).  Where they are few the table's width is shared out over a number of
+    // CTAs that is counted as if three were resident on an SM (two are with 16 rows a
+    // tile, one with heads over 128) and as if row tiles were full (those of sequences of
+    // few rows are not: a tile's rows are one sequence's): "waves" times that many.  One
+    // sequence of 131001 tokens, whose tiles are full: 71.6 us with 1, 75.8 with 2, 84.0
+    // with 3, so 1, as a further wave's start costs more than it hides; 16 of 2000..8000
+    // tokens, whose 4-row tiles are half full: 63.5, 59.4 and 69.6, so 2 for many
+    // sequences.  The table's width is all that the host knows of the lengths: with a
+    // table of 131072 tokens one row over 700 takes 21.5 us (14.3 with a table of 700,
+    // timed with a cold L2), 8 over 4000 74.8 (37.9).
     const int64_t waves = q->seqs > 8 ? 2 : 1;
     int64_t chunks = units >= 2 * resident ? (cover + 2047) / 2048 : waves * resident / units;
     if (chunks < 1) chunks = 1;
@@ -184,7 +190,12 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
 // head (16 rows of 32 heads over 16384 tokens: 44 us, split kernel 73; 8 rows: 58
 // by either) and enough work to pay for a CTA's start and its 128-row halves, some
 // 3 million (query head, token) pairs of 128 dimensions: 40 rows of 32 heads over
-// 900 tokens 30 us by the split kernel and 42 by this, 128 rows 58 and 48.
+// 900 tokens 30 us by the split kernel and 42 by this, 128 rows 58 and 48.  The rows
+// are the mean of the call's sequences, so one kernel takes a prompt and single tokens
+// together: a prompt of 4096 rows with 255 single tokens of 4096, 32 heads, 1139 us
+// (apart 234 and 392), of 512 rows 661 (33 and 392).  Heads over 128 (S and O of two
+// halves are more than tensor memory) and groups over 128 stay with the split kernel:
+// 2 x 2048 rows of 16 heads of 256 over 8192 and 16384 tokens 10.6 ms, of 128 0.45.
 bool use_tiles(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d) {
     const int64_t group = d->q_heads / c->kv_heads, each = q->tokens / q->seqs;
     if (c->dim > 128 || group > 128 || each * group < 48) return false;

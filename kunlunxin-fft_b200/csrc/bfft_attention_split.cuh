@@ -26,9 +26,10 @@
 //   a value scale under 2^-48 keeps its sum 2^36 times smaller (see SmallScales).
 //
 // 64 sequences of 1024..32768 tokens, one row of 32 heads each (8 kv heads, 128
-// dimensions): int8 418 us, 5430 GB/s, 0.83 of the measured HBM rate; e4m3, whose
-// codes take 2 instructions for 4 to widen instead of 5, 385 us and 0.90.  One
-// sequence of 131001 e4m3 tokens, 64 heads: 53 us and 7 for joining.
+// dimensions): int8 417 us, 5440 GB/s, 0.83 of the measured HBM rate (417 to 455, 0.76,
+// on the GPUs that it was measured on; a GPU repeats itself within 1 %); e4m3, whose
+// codes take 2 instructions for 4 to widen instead of 5, 386 us and 0.90.  One
+// sequence of 131001 e4m3 tokens, 64 heads: 55 us, the joining kernel's among them.
 #pragma once
 
 namespace bfft {

@@ -25,11 +25,13 @@
 // 2 % of the two-prompt case).
 //
 // 2 x 2048 prompt rows of 32 heads (8 kv heads, 128 dimensions) over 8192 and 16384
-// int8 tokens: 856 us, 884 TFLOP/s, 0.54 of the measured bf16 rate.  Bound by the
-// chain of a half's tile, not by one pipe: 4900 clocks a tile for 2048 of tensor
-// work.  Leaving a stage out (in a copy) gives, of 880 us: no widening 782, no
+// int8 tokens: 860 us (854 to 882 by the GPU), 880 TFLOP/s, 0.54 of the measured bf16
+// rate.  Bound by the chain of a half's tile, not by one pipe: 4900 clocks a tile for
+// 2048 of tensor work; and by the schedule: 512 CTAs of 65 to 113 tiles in the order
+// of their slots end at 372 tile times where an even spread would be 318 (counted).
+// Leaving a stage out (in a copy) gives, of 880 us: no widening 782, no
 // exponentials 872, no maximum 862, half of the value products 832.  The special
-// function pipe is 43 % busy, so exponentials by polynomials did not help; tiles of
+// function pipe is 46 % busy, so exponentials by polynomials did not help; tiles of
 // 64 tokens with two score buffers a half were slower (an M128 N64 product takes as
 // long as N128 when the widening shares its shared memory); waits that poll without
 // reading the clock, 975 us.
@@ -88,7 +90,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // 16 bytes) and the leading offset, the high word, the same for every step, the stride
 // of eight rows, the version and the layout.  A step along the operand adds to the
 // low word: one thread issues the products (2 x 2048 prompt rows 881 us with 64-bit
-// descriptors built anew for each, 856 so).
+// descriptors built anew for each, 856 so on that GPU).
 __device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
 constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 // float16 operands, float32 accumulator, M = 128
