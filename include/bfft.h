@@ -383,8 +383,8 @@ typedef struct bfft_attention_desc {
  * that sees no token gets out = 0 and lse = -inf.  A token without a valid page
  * is not seen.  The workspace (bfft_cache_attention_workspace bytes for the same
  * descriptors, 16-byte aligned) holds the parts of rows whose tokens are shared
- * out over several blocks: at most 256 MB, or what one to a few parts of each row
- * take where that is more.  out may be q, but not overlap it otherwise. */
+ * out over several blocks: at most 256 MB, or one part of each row for each 65536
+ * tokens of the table's width where that is more.  out may be q, but not overlap it otherwise. */
 BFFT_EXPORT bfft_status bfft_cache_attention_workspace(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
                                                        const bfft_attention_desc* desc, size_t* bytes);
 BFFT_EXPORT bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
