@@ -314,6 +314,20 @@ typedef struct bfft_rotate_desc {
 BFFT_EXPORT bfft_status bfft_rotate_positions(const bfft_rotate_desc* desc, const void* x, const void* positions,
                                               const void* table, void* y, void* stream);
 
+/* Positions of several axes (time, height, width): pair j of the rotated part takes the
+ * row of the table that its axis's position names, c + is = table[p_axis(j)][j]. */
+typedef struct bfft_axes_desc {
+    const void* axis;        /* host memory: rotated / 2 bytes, each pair's axis */
+    int64_t axes;            /* 1..4                                            */
+    int64_t pos_axis;        /* stride of positions between axes                */
+} bfft_axes_desc;
+
+/* bfft_rotate_positions with positions (axes, batch, tokens): pos_batch and pos_token
+ * are the strides within an axis.  A position outside the table makes the pairs of its
+ * axis NaN. */
+BFFT_EXPORT bfft_status bfft_rotate_axes(const bfft_rotate_desc* desc, const bfft_axes_desc* axes, const void* x,
+                                         const void* positions, const void* table, void* y, void* stream);
+
 /* Pages of `page` tokens, one block of codes per page and kv head, one float32
  * scale per block for keys and one for values: token value = code * scale.  A
  * block that ever held a NaN or an infinity reads as NaN.  Scales are not
@@ -356,6 +370,11 @@ typedef struct bfft_append_desc {
  * is written. */
 BFFT_EXPORT bfft_status bfft_cache_append(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
                                           const bfft_append_desc* desc, void* stream);
+
+/* bfft_cache_append with positions (axes, tokens), adjacent within an axis; they and the
+ * table must be given. */
+BFFT_EXPORT bfft_status bfft_cache_append_axes(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
+                                               const bfft_append_desc* desc, const bfft_axes_desc* axes, void* stream);
 
 /* The values that the cache stands for: row starts[s] + i of k and v
  * ((tokens, kv_heads, dim) of `type`, 16-byte aligned) is token lens[s] + i of

@@ -30,6 +30,7 @@ but not overlap it otherwise.  The checks and the calls themselves are in
 from __future__ import annotations
 
 import ctypes
+import functools
 import importlib.machinery
 import importlib.util
 import math
@@ -45,6 +46,8 @@ TYPE_IDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 CODE_DTYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 LAYOUT_IDS = {"half": 0, "interleaved": 1}
 SCALINGS = ("none", "linear", "ntk", "banded")
+AXIS_ORDERS = ("blocks", "cyclic")
+SPECTRA = ("shared", "axial")
 PAGE_SIZES = (16, 32, 64, 128)
 
 _native = None
@@ -68,7 +71,8 @@ def _load():
             loader.exec_module(module)
             module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
                           for name in ("bfft_rotate_positions", "bfft_cache_append", "bfft_cache_read",
-                                       "bfft_cache_attention_workspace", "bfft_cache_attention", "bfft_last_error")))
+                                       "bfft_cache_attention_workspace", "bfft_cache_attention", "bfft_last_error",
+                                       "bfft_rotate_axes", "bfft_cache_append_axes")))
             _native = module
     return _native
 
@@ -96,9 +100,46 @@ def paged_cache(pages: int, kv_heads: int, page: int, dim: int, *, code: str = "
                       *(torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in "kv"))
 
 
+def _axes_map(axes, axis_order) -> tuple[int, ...]:
+    """The axis of each pair."""
+    axes = tuple(axes)
+    if axis_order not in AXIS_ORDERS:
+        raise ValueError(f"axis_order must be one of {AXIS_ORDERS}, got {axis_order!r}")
+    if not 1 <= len(axes) <= 4 or any(type(n) is not int or n < 0 for n in axes) or not 1 <= sum(axes) <= 256:
+        raise ValueError(f"axes must be the pairs of each of 1 to 4 axes, up to 256 together, got {axes}")
+    if axis_order == "blocks":
+        return tuple(a for a, n in enumerate(axes) for _ in range(n))
+    return tuple(a for i in range(max(axes)) for a, n in enumerate(axes) if i < n)
+
+
+@functools.lru_cache(maxsize=64)
+def _axes_bytes(axes, axis_order) -> bytes:
+    """The number of axes, then the axis of each pair (a function of the numbers alone: made once for a model)."""
+    return bytes((len(axes), *_axes_map(axes, axis_order)))
+
+
+def _axes(axes, axis_order):
+    if axes is None:
+        return None
+    return _axes_bytes(axes if type(axes) is tuple else tuple(axes), axis_order)
+
+
+def _frequencies(rotated, base, scaling, factor, original, low_turns, high_turns, device):
+    if scaling == "ntk" and rotated > 2:
+        base = base * factor ** (rotated / (rotated - 2))
+    w = base ** (-torch.arange(0, rotated, 2, dtype=torch.float64, device=device) / rotated)
+    if scaling == "linear":
+        w = w / factor
+    elif scaling == "banded":
+        keep = ((original * w / (2 * math.pi) - low_turns) / (high_turns - low_turns)).clamp(0.0, 1.0)
+        w = w * keep + w / factor * (1.0 - keep)
+    return w
+
+
 def rotary_table(positions: int, rotated: int, *, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
                  original: int | None = None, low_turns: float = 1.0, high_turns: float = 32.0,
-                 amplitude: float = 1.0, device="cuda") -> torch.Tensor:
+                 amplitude: float = 1.0, axes=None, axis_order: str = "blocks", spectrum: str = "shared",
+                 device="cuda") -> torch.Tensor:
     """(positions, rotated / 2, 2) float32: amplitude * (cos, sin) of p * w_j with
     w_j = base^(-2 j / rotated), made in float64 and rounded once.
 
@@ -109,23 +150,37 @@ def rotary_table(positions: int, rotated: int, *, base: float = 10000.0, scaling
     ``low_turns`` turns over the ``original`` context, keeps those that make more
     than ``high_turns`` and blends between them linearly in their turns (a blend that
     is linear in the index j, as some models are trained with, gives other
-    frequencies: make that table yourself)."""
+    frequencies: make that table yourself).
+
+    A table for positions of several axes (``axes`` and ``axis_order`` as in
+    ``rotate_positions``) has the same columns with ``spectrum`` "shared": the axes
+    take the frequencies where their pairs lie.  "axial" gives each axis a spectrum of
+    its own: pair i of an axis's n has base^(-i / n) (and the scaling of a rotated part
+    of 2 n elements)."""
     if positions < 1 or rotated < 2 or rotated % 2:
         raise ValueError(f"need positions >= 1 and an even rotated part, got {positions} and {rotated}")
     if scaling not in SCALINGS:
         raise ValueError(f"scaling must be one of {SCALINGS}, got {scaling!r}")
     if not factor >= 1.0 or not base > 0.0:
         raise ValueError(f"need factor >= 1 and base > 0, got {factor} and {base}")
-    if scaling == "ntk" and rotated > 2:
-        base = base * factor ** (rotated / (rotated - 2))
-    w = base ** (-torch.arange(0, rotated, 2, dtype=torch.float64, device=device) / rotated)
-    if scaling == "linear":
-        w = w / factor
-    elif scaling == "banded":
-        if original is None or original < 1 or not high_turns > low_turns:
-            raise ValueError("banded scaling needs the original context length and low_turns < high_turns")
-        keep = ((original * w / (2 * math.pi) - low_turns) / (high_turns - low_turns)).clamp(0.0, 1.0)
-        w = w * keep + w / factor * (1.0 - keep)
+    if scaling == "banded" and (original is None or original < 1 or not high_turns > low_turns):
+        raise ValueError("banded scaling needs the original context length and low_turns < high_turns")
+    if spectrum not in SPECTRA:
+        raise ValueError(f"spectrum must be one of {SPECTRA}, got {spectrum!r}")
+    how = (base, scaling, factor, original, low_turns, high_turns, device)
+    if axes is None:
+        if spectrum != "shared":
+            raise ValueError("an axial spectrum needs axes")
+        w = _frequencies(rotated, *how)
+    else:
+        axis_of = _axes_map(axes, axis_order)
+        if 2 * len(axis_of) != rotated:
+            raise ValueError(f"axes have {len(axis_of)} pairs, a rotated part of {rotated} has {rotated // 2}")
+        w = _frequencies(rotated, *how)
+        if spectrum == "axial":
+            of = torch.tensor(axis_of, device=device)
+            for a in set(axis_of):
+                w[of == a] = _frequencies(2 * axis_of.count(a), *how)
     angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * w
     return (torch.stack((angle.cos(), angle.sin()), -1) * amplitude).float()
 
@@ -139,7 +194,8 @@ def _layout(layout: str) -> int:
     return kind
 
 
-def rotate_positions(x, positions, table, *, layout: str = "half", transform_direction: str = "forward", out=None):
+def rotate_positions(x, positions, table, *, layout: str = "half", transform_direction: str = "forward", axes=None,
+                     axis_order: str = "blocks", out=None):
     """x with the first ``2 * table.shape[1]`` elements of each head rotated by its
     token's position; the other elements pass through.
 
@@ -149,17 +205,26 @@ def rotate_positions(x, positions, table, *, layout: str = "half", transform_dir
     outside the table makes its token's rotated part NaN.  layout "half" pairs
     elements j and j + rotated / 2, "interleaved" 2 j and 2 j + 1.
     transform_direction "inverse" rotates back (conjugate roots; with an amplitude m
-    in the table it is m^2 times the inverse, the adjoint).  ``out`` may be x."""
+    in the table it is m^2 times the inverse, the adjoint).  ``out`` may be x.
+
+    ``axes``: tokens have positions on up to four axes (time, height, width of a
+    patch), and each pair belongs to one: ``axes=(16, 24, 24)`` gives the first 16
+    pairs to axis 0, the next 24 to axis 1 and so on with axis_order "blocks", and
+    deals them out in turn with "cyclic" (0, 1, 2, 0, 1, 2, ..., an axis that has its
+    share drops out).  positions are then (axes, tokens) or (axes, batch, tokens), pair
+    j's root is row ``positions[axis(j)]``, column j of the table, and a position
+    outside the table makes the pairs of its axis NaN."""
     direction = _lib.TRANSFORM_DIRECTION_IDS.get(transform_direction)
     if direction is None:
         raise ValueError(f"transform_direction must be one of {sorted(_lib.TRANSFORM_DIRECTION_IDS)}, "
                          f"got {transform_direction!r}")
-    return (_native or _load()).rotate(x, positions, table, _layout(layout), direction, out)
+    return (_native or _load()).rotate(x, positions, table, _layout(layout), direction, out, _axes(axes, axis_order))
 
 
 # ------------------------------------------------------------------------------- cache
 
-def append_rotated(cache, k, v, block_table, held, starts, table=None, *, layout: str = "half", positions=None, q=None):
+def append_rotated(cache, k, v, block_table, held, starts, table=None, *, layout: str = "half", positions=None, axes=None,
+                   axis_order: str = "blocks", q=None):
     """Append each sequence's new rows behind the ``held[s]`` tokens it has.
 
     k, v: (tokens, kv_heads, dim), float32, float16 or bfloat16.  Keys are rotated
@@ -171,9 +236,13 @@ def append_rotated(cache, k, v, block_table, held, starts, table=None, *, layout
     Two sequences must not append to one page.  Rows whose page is not in the table
     are dropped.
 
+    ``axes`` and ``axis_order``: positions of several axes, as in ``rotate_positions``;
+    the table and ``positions``, (axes, tokens), have to be given.
+
     q: (tokens, q_heads, dim) of k's type; its rotated rows are returned (else None).
     ``cache_attention`` takes them in float16 or bfloat16."""
-    return (_native or _load()).append(cache, k, v, block_table, held, starts, table, _layout(layout), positions, q)
+    return (_native or _load()).append(cache, k, v, block_table, held, starts, table, _layout(layout), positions, q,
+                                       _axes(axes, axis_order))
 
 
 def read_cache(cache, block_table, first, starts, tokens: int, *, dtype=torch.bfloat16):

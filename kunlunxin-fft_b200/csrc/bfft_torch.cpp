@@ -37,6 +37,8 @@ struct Entries {
     decltype(&bfft_cache_attention_workspace) workspace;
     decltype(&bfft_cache_attention) attention;
     decltype(&bfft_last_error) last_error;
+    decltype(&bfft_rotate_axes) rotate_axes;
+    decltype(&bfft_cache_append_axes) append_axes;
 } g_entry{};
 
 std::string text(const char* s) { return s; }
@@ -198,6 +200,20 @@ int64_t table_rotated(const Tensor& t, int64_t most, int64_t device) {
     return rotated;
 }
 
+// The axes of a rotation's pairs as bfft/cache.py hands them over: their number, then the
+// axis of each pair; empty for positions of one axis.
+std::string axes_of(PyObject* o, int64_t rotated) {
+    if (o == Py_None) return {};
+    if (!PyBytes_Check(o) || PyBytes_GET_SIZE(o) < 2) value_error("bad axes");
+    std::string axes(PyBytes_AS_STRING(o), (size_t)PyBytes_GET_SIZE(o));
+    if (2 * ((int64_t)axes.size() - 1) != rotated)
+        value_error("axes have ", (int64_t)axes.size() - 1, " pairs, the table has ", rotated / 2);
+    return axes;
+}
+bfft_axes_desc axes_desc(const std::string& axes, const Tensor& positions) {
+    return {axes.data() + 1, axes[0], positions.stride(0)};
+}
+
 int64_t positions_64(const Tensor& t, int64_t device) {
     if (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong)
         type_error("positions must be int32 or int64, got ", at::toString(t.scalar_type()));
@@ -291,7 +307,7 @@ int64_t integer(PyObject* o, const char* name, int64_t least) {
 // ------------------------------------------------------------------ rotation
 
 Tensor launch_rotate(const Tensor& x, const Tensor& positions, const Tensor& table, int64_t layout, int64_t direction,
-                     const Tensor* out) {
+                     const std::string& axes, const Tensor* out) {
     bfft_rotate_desc d;
     const bool batched = x.dim() == 4;
     const int64_t at = batched ? 1 : 0;
@@ -308,7 +324,8 @@ Tensor launch_rotate(const Tensor& x, const Tensor& positions, const Tensor& tab
     d.y_batch = batched ? y.stride(0) : 0;
     d.y_token = y.stride(at);
     d.y_head = y.stride(at + 1);
-    d.pos_batch = positions.dim() == 2 ? positions.stride(0) : 0;
+    const int64_t lead = axes.empty() ? 0 : 1;  // positions: (axes,) before the tokens
+    d.pos_batch = positions.dim() == lead + 2 ? positions.stride(lead) : 0;
     d.pos_token = positions.stride(positions.dim() - 1);
     d.table_rows = table.size(0);
     d.type = x.scalar_type() == at::kFloat ? BFFT_F32 : x.scalar_type() == at::kHalf ? BFFT_F16 : BFFT_BF16;
@@ -317,8 +334,15 @@ Tensor launch_rotate(const Tensor& x, const Tensor& positions, const Tensor& tab
     d.pos64 = positions.scalar_type() == at::kLong;
     d.device = x.get_device();
     if (out) written(y);
-    check(g_entry.rotate(&d, x.data_ptr(), positions.data_ptr(), table.data_ptr(), y.data_ptr(), stream_of(d.device)),
-          "rotate_positions");
+    if (axes.empty()) {
+        check(g_entry.rotate(&d, x.data_ptr(), positions.data_ptr(), table.data_ptr(), y.data_ptr(), stream_of(d.device)),
+              "rotate_positions");
+    } else {
+        const bfft_axes_desc a = axes_desc(axes, positions);
+        check(g_entry.rotate_axes(&d, &a, x.data_ptr(), positions.data_ptr(), table.data_ptr(), y.data_ptr(),
+                                  stream_of(d.device)),
+              "rotate_positions");
+    }
     return y;
 }
 
@@ -326,31 +350,33 @@ Tensor launch_rotate(const Tensor& x, const Tensor& positions, const Tensor& tab
 // is the opposite direction's rotation, itself differentiable.
 struct Rotate : public torch::autograd::Function<Rotate> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& positions,
-                          const Tensor& table, int64_t layout, int64_t direction) {
+                          const Tensor& table, int64_t layout, int64_t direction, const std::string& axes) {
         ctx->save_for_backward({positions, table});
+        ctx->saved_data["axes"] = axes;
         ctx->saved_data["layout"] = layout;
         ctx->saved_data["direction"] = direction;
-        return launch_rotate(x, positions, table, layout, direction, nullptr);
+        return launch_rotate(x, positions, table, layout, direction, axes, nullptr);
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const int64_t layout = ctx->saved_data["layout"].toInt(), direction = ctx->saved_data["direction"].toInt();
+        const std::string& axes = ctx->saved_data["axes"].toStringRef();
         Tensor dy = grads[0];
         if (dy.stride(-1) != 1) dy = dy.contiguous();
         Tensor dx;
         if (at::GradMode::is_enabled() && dy.requires_grad())
-            dx = Rotate::apply(dy, saved[0], saved[1], layout, 1 - direction);
+            dx = Rotate::apply(dy, saved[0], saved[1], layout, 1 - direction, axes);
         else
-            dx = launch_rotate(dy, saved[0], saved[1], layout, 1 - direction, nullptr);
-        return {dx, Tensor(), Tensor(), Tensor(), Tensor()};
+            dx = launch_rotate(dy, saved[0], saved[1], layout, 1 - direction, axes, nullptr);
+        return {dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 
-// rotate(x, positions, table, layout, direction, out)
+// rotate(x, positions, table, layout, direction, out, axes)
 PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 6, "rotate takes 6 arguments");
+    TORCH_CHECK(n == 7, "rotate takes 7 arguments");
     const Tensor &x = tensor(args[0], "x"), &positions = tensor(args[1], "positions"), &table = tensor(args[2], "table");
     const int64_t layout = integer(args[3], "layout", 0), direction = integer(args[4], "direction", 0);
     type_id(x, "x");
@@ -359,14 +385,20 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t device = x.get_device();
     if (x.dim() != 3 && x.dim() != 4)
         value_error("x must be (tokens, heads, dim) or (batch, tokens, heads, dim), got ", shape_of(x));
-    table_rotated(table, x.size(-1), device);
+    const std::string axes = axes_of(args[6], table_rotated(table, x.size(-1), device));
     constant(table, "table");
     if (x.stride(-1) != 1) value_error("x must have adjacent elements in its last dimension");
     positions_64(positions, device);
     const int64_t tokens = x.size(-3);
-    const bool flat = positions.dim() == 1 && positions.size(0) == tokens;
-    if (!flat && !(x.dim() == 4 && positions.dim() == 2 && positions.size(0) == x.size(0) && positions.size(1) == tokens))
-        value_error("positions must be (tokens,) or (batch, tokens) of x ", shape_of(x), ", got ", shape_of(positions));
+    const int64_t lead = axes.empty() ? 0 : 1;
+    const bool all = !lead || (positions.dim() > 1 && positions.size(0) == axes[0]);
+    const bool flat = positions.dim() == lead + 1 && positions.size(lead) == tokens;
+    if (!all || (!flat && !(x.dim() == 4 && positions.dim() == lead + 2 && positions.size(lead) == x.size(0) &&
+                            positions.size(lead + 1) == tokens))) {
+        const std::string first = lead ? "(" + std::to_string((int)axes[0]) + " axes, " : "(";
+        value_error("positions must be ", first, "tokens) or ", first, "batch, tokens) of x ", shape_of(x), ", got ",
+                    shape_of(positions));
+    }
     const Tensor* out = nullptr;
     if (args[5] != Py_None) {
         out = &tensor(args[5], "out");
@@ -379,18 +411,18 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     if (x.requires_grad() && at::GradMode::is_enabled()) {
         if (out) value_error("out cannot be given where x requires a gradient");
-        return THPVariable_Wrap(Rotate::apply(x, positions, table, layout, direction));
+        return THPVariable_Wrap(Rotate::apply(x, positions, table, layout, direction, axes));
     }
-    return THPVariable_Wrap(launch_rotate(x, positions, table, layout, direction, out));
+    return THPVariable_Wrap(launch_rotate(x, positions, table, layout, direction, axes, out));
     END_HANDLE_TH_ERRORS
 }
 
 // ------------------------------------------------------------------ cache
 
-// append(cache, k, v, block_table, held, starts, table, layout, positions, q)
+// append(cache, k, v, block_table, held, starts, table, layout, positions, q, axes)
 PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 10, "append takes 10 arguments");
+    TORCH_CHECK(n == 11, "append takes 11 arguments");
     const Cache c = cache_of(args[0]);
     apart_whole(*c.parts[0], *c.parts[1], "cache k and v");
     apart_whole(*c.parts[2], *c.parts[3], "cache k_scale and v_scale");
@@ -415,10 +447,22 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
         d.table_rows = table.size(0);
     }
     d.layout = integer(args[7], "layout", 0);
+    std::string axes;
+    bfft_axes_desc by_axis{};
+    if (args[10] != Py_None) {
+        if (!d.table || args[8] == Py_None) value_error("axes need a table and positions");
+        axes = axes_of(args[10], d.rotated);
+    }
     if (args[8] != Py_None) {
         const Tensor& positions = tensor(args[8], "positions");
         d.pos64 = positions_64(positions, c.device);
-        if (positions.dim() != 1 || positions.size(0) != tokens || !positions.is_contiguous())
+        if (!axes.empty()) {
+            if (positions.dim() != 2 || positions.size(0) != axes[0] || positions.size(1) != tokens ||
+                (tokens > 1 && positions.stride(1) != 1))
+                value_error("positions must be (", (int64_t)axes[0], " axes, ", tokens, "), adjacent within an axis, got ",
+                            shape_of(positions));
+            by_axis = axes_desc(axes, positions);
+        } else if (positions.dim() != 1 || positions.size(0) != tokens || !positions.is_contiguous())
             value_error("positions must be contiguous (", tokens, ",), got ", shape_of(positions));
         d.positions = positions.data_ptr();
     }
@@ -447,7 +491,9 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     if (tokens) {
         for (const Tensor* t : c.parts) written(*t);
-        check(g_entry.append(&c.desc, &q, &d, stream_of(c.device)), "append_rotated");
+        check(axes.empty() ? g_entry.append(&c.desc, &q, &d, stream_of(c.device))
+                           : g_entry.append_axes(&c.desc, &q, &d, &by_axis, stream_of(c.device)),
+              "append_rotated");
     }
     if (!out.defined()) Py_RETURN_NONE;
     return THPVariable_Wrap(out);
@@ -540,12 +586,12 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// bind(addresses of rotate, append, read, workspace, attention, last_error)
+// bind(addresses of rotate, append, read, workspace, attention, last_error, rotate_axes, append_axes)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 6, "bind takes 6 addresses");
-    void* p[6];
-    for (int i = 0; i < 6; ++i) {
+    TORCH_CHECK(n == 8, "bind takes 8 addresses");
+    void* p[8];
+    for (int i = 0; i < 8; ++i) {
         p[i] = PyLong_AsVoidPtr(args[i]);
         if (!p[i]) value_error("null entry point");
     }
@@ -555,6 +601,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     g_entry.workspace = reinterpret_cast<decltype(g_entry.workspace)>(p[3]);
     g_entry.attention = reinterpret_cast<decltype(g_entry.attention)>(p[4]);
     g_entry.last_error = reinterpret_cast<decltype(g_entry.last_error)>(p[5]);
+    g_entry.rotate_axes = reinterpret_cast<decltype(g_entry.rotate_axes)>(p[6]);
+    g_entry.append_axes = reinterpret_cast<decltype(g_entry.append_axes)>(p[7]);
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
