@@ -409,6 +409,29 @@ BFFT_EXPORT bfft_status bfft_cache_attention_workspace(const bfft_cache_desc* ca
 BFFT_EXPORT bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
                                              const bfft_attention_desc* desc, void* stream);
 
+/* What rows see beside the mask and the window. */
+typedef struct bfft_span_desc {
+    int64_t sinks;           /* a window does not hide the first `sinks` tokens */
+    const void* groups;      /* [n_groups + 1] int32: sequences [groups[g], groups[g + 1]) are group g;
+                                null with n_groups = 1: all sequences           */
+    const void* shared;      /* [n_groups] int32: tokens that its sequences share */
+    int64_t n_groups;        /* 0: nothing is shared                            */
+} bfft_span_desc;
+
+/* bfft_cache_attention with first tokens that stay visible and with shared prefixes.  The
+ * sequences of a group name the same pages for their first shared[g] tokens; the whole
+ * pages of these are read from the row of the block table of the group's first sequence,
+ * once for the group's rows.  `groups` ascends; sequences outside it share nothing.  The
+ * results are those of rows that read their own pages.  Tables up to 2^30 tokens wide.
+ * The workspace with groups: each row tile's parts, those of some six waves of CTAs more
+ * and, for prefixes on the tensor cores, 256 rows for each CTA. */
+BFFT_EXPORT bfft_status bfft_cache_attention_span_workspace(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
+                                                            const bfft_attention_desc* desc, const bfft_span_desc* span,
+                                                            size_t* bytes);
+BFFT_EXPORT bfft_status bfft_cache_attention_span(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
+                                                  const bfft_attention_desc* desc, const bfft_span_desc* span,
+                                                  void* stream);
+
 /* Status bits the kernels set on `device` when a bounded wait expired
  * (bit 0: a TMA pass gave up waiting for a tile copy and returned early, so
  * its output is incomplete).  Synchronises the device; clear != 0 resets the

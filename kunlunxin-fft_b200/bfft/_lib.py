@@ -36,7 +36,8 @@ EXPORTS = ("bfft_api_version", "bfft_last_error", "bfft_plan_create", "bfft_plan
            "bfft_stream_plan_create", "bfft_stream_plan_info", "bfft_stream_execute", "bfft_stream_plan_destroy",
            "bfft_dist_p2p_prepare", "bfft_dist_p2p_attach", "bfft_dist_p2p_attach_pointers", "bfft_dist_p2p_phase",
            "bfft_rotate_positions", "bfft_cache_append", "bfft_cache_read", "bfft_cache_attention_workspace",
-           "bfft_cache_attention", "bfft_rotate_axes", "bfft_cache_append_axes")
+           "bfft_cache_attention", "bfft_rotate_axes", "bfft_cache_append_axes", "bfft_cache_attention_span_workspace",
+           "bfft_cache_attention_span")
 
 
 class PlanDesc(ctypes.Structure):
@@ -108,6 +109,8 @@ def load() -> ctypes.CDLL:
         desc = ctypes.c_char_p  # descriptors of the position and cache calls: packed bytes
         L.bfft_rotate_positions.argtypes = [desc, vp, vp, vp, vp, vp]
         L.bfft_cache_append.argtypes = [desc, desc, desc, vp]
+        L.bfft_cache_attention_span_workspace.argtypes = [desc, desc, desc, desc, ctypes.POINTER(sz)]
+        L.bfft_cache_attention_span.argtypes = [desc, desc, desc, desc, vp]
         L.bfft_rotate_axes.argtypes = [desc, desc, vp, vp, vp, vp, vp]
         L.bfft_cache_append_axes.argtypes = [desc, desc, desc, desc, vp]
         L.bfft_cache_read.argtypes = [desc, desc, i64, vp, vp, i64, vp]

@@ -72,7 +72,8 @@ def _load():
             module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
                           for name in ("bfft_rotate_positions", "bfft_cache_append", "bfft_cache_read",
                                        "bfft_cache_attention_workspace", "bfft_cache_attention", "bfft_last_error",
-                                       "bfft_rotate_axes", "bfft_cache_append_axes")))
+                                       "bfft_rotate_axes", "bfft_cache_append_axes", "bfft_cache_attention_span_workspace",
+                                       "bfft_cache_attention_span")))
             _native = module
     return _native
 
@@ -256,7 +257,7 @@ def read_cache(cache, block_table, first, starts, tokens: int, *, dtype=torch.bf
 
 
 def cache_attention(q, cache, block_table, lens, starts, *, softmax_scale: float | None = None, causal: bool = True,
-                    window: int = 0, return_lse: bool = False, out=None):
+                    window: int = 0, sinks: int = 0, shared=None, groups=None, return_lse: bool = False, out=None):
     """softmax(softmax_scale q k^T) v of ragged query rows over the cache.
 
     q: (tokens, q_heads, dim), float16 or bfloat16, q_heads a multiple of the
@@ -267,6 +268,17 @@ def cache_attention(q, cache, block_table, lens, starts, *, softmax_scale: float
     of those (rows that are not causal: from there to the sequence's end).  A row that
     sees no token gets zeros and a log-sum-exp of -inf.
 
+    ``sinks``: the window does not hide the first ``sinks`` tokens of a sequence.
+
+    ``shared``: sequences that begin with the same tokens and name the same pages for
+    them.  Sequences ``groups[g] .. groups[g + 1]`` (int32, (groups + 1,), ascending; None:
+    all are one group) share their first ``shared[g]`` tokens (int32, (groups,)): the whole
+    pages among these are read once for the group, from the block table's row of its first
+    sequence.  The results are those of a call without, but for roundings.  Sequences in
+    no group share nothing.  Worth it for few rows a sequence: from 256 rows a kv head on
+    (query tokens times heads) a sequence fills the kernel's row tiles by itself and the
+    call goes without.
+
     The weights, times their block's value scale, are rounded to float16 before they
     meet the codes, with a row's largest near float16's top: to 2^-11 down to 2^-24 of
     the largest (few rows: 2^-28), to nothing under 2^-34 (2^-38).
@@ -274,4 +286,4 @@ def cache_attention(q, cache, block_table, lens, starts, *, softmax_scale: float
     Returns out (tokens, q_heads, dim), with ``return_lse`` also the rows' log-sum-exp
     (tokens, q_heads) float32."""
     return (_native or _load()).attention(q, cache, block_table, lens, starts, softmax_scale, causal, window, return_lse,
-                                          out)
+                                          out, sinks, shared, groups)

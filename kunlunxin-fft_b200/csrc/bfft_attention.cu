@@ -1,39 +1,8 @@
-// bfft_attention.cu -- attention of ragged query rows over a paged 8-bit cache.
-//
-//     out_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(t q_i . k_j - m_i),
-// over the tokens j that row i sees, with the running maximum m_i and sum kept
-// in 32 bits while the tokens pass once.
-#include <cuda_runtime.h>
-
-#include <atomic>
-#include <cmath>
-
-#include "../../include/bfft.h"
-#include "bfft_async.cuh"
-#include "bfft_cache.cuh"
-#include "bfft_kernels.cuh"
+// bfft_attention.cu -- attention of ragged query rows over a paged 8-bit cache: entry
+// points and plans, and the kernels' plain form (see bfft_attention.cuh).
+#include "bfft_attention.cuh"
 
 using namespace bfft;
-
-namespace bfft {
-
-struct AttentionArgs {
-    CacheView cache;
-    SequenceView seq;  // lens: tokens of each sequence in the cache
-    const void* q;
-    void* out;
-    float* lse;
-    int64_t qt, qh, ot, oh;
-    int q_heads, group;  // group = q_heads / kv_heads
-    int causal, window;
-    float scale_log2;    // softmax_scale * log2(e)
-    int q_packs, o_packs;  // rows of q / out start on 16 bytes
-};
-
-}  // namespace bfft
-
-#include "bfft_attention_split.cuh"
-#include "bfft_attention_tiles.cuh"
 
 namespace {
 
@@ -67,6 +36,10 @@ EncodeTiledFn encoder() {
     return fn;
 }
 
+}  // namespace
+
+namespace bfft {
+
 // The codes as [pages][kv_heads * page * dim / 128][128 bytes], boxes of 16 tokens,
 // 128-byte swizzle (heads of 64, 128 or 256 elements: whole lines).
 bool encode_codes(CUtensorMap* m, const void* codes, const bfft_cache_desc* c) {
@@ -81,6 +54,10 @@ bool encode_codes(CUtensorMap* m, const void* codes, const bfft_cache_desc* c) {
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+
+}  // namespace bfft
+
+namespace {
 
 int sm_count(int64_t device) {
     static std::atomic<int> counts[64];
@@ -97,32 +74,19 @@ int sm_count(int64_t device) {
     return n;
 }
 
-// Tokens that a row tile of `tile` query tokens sees at most.
+// Tokens that a row tile of `tile` query tokens sees at most, `sinks` first ones among them.
 int64_t seen_cover(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d, int tile,
-                   int align) {
+                   int align, int64_t sinks) {
     int64_t cover = q->max_pages * c->page;
     if (d->causal && d->window > 0) {
-        const int64_t w = d->window + tile - 1 + align - 1;
+        const int64_t w = d->window + tile - 1 + align - 1 + (sinks + 15) / 16 * 16;
         if (w < cover) cover = w;
     }
     return cover;
 }
 
-// Chunks and slots of the kernel for many rows.
-struct TilePlan {
-    int tile_tokens, by_token, chunk, chunks;
-    int64_t slots, ctas;
-    size_t bytes;
-};
-
-// How a call is cut: row tiles and chunks of the token axis.
-struct SplitPlan {
-    int nt, tile_tokens, token_tiles, by_token, chunk, chunks, cluster, entries;
-    int64_t slots, ctas;
-    size_t bytes;
-};
-
-SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d, int sms) {
+SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d, int sms,
+                     int64_t sinks) {
     SplitPlan p;
     const int64_t group = d->q_heads / c->kv_heads;
     const int64_t each = q->tokens / q->seqs + (q->tokens % q->seqs != 0);  // rows of a sequence, about
@@ -133,7 +97,7 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
     const int64_t runs = q->tokens / p.tile_tokens + q->seqs;
     p.by_token = q->tokens <= runs;
     p.slots = p.by_token ? q->tokens : runs;
-    const int64_t cover = seen_cover(c, q, d, p.tile_tokens, 16);
+    const int64_t cover = seen_cover(c, q, d, p.tile_tokens, 16, sinks);
     const int64_t tiles = (q->tokens + p.tile_tokens - 1) / p.tile_tokens;
     const int64_t units = tiles * p.token_tiles * c->kv_heads, resident = 3 * (int64_t)sms;
     // Where rows are many, chunks of 2048 tokens (512..4096 measure alike for 64 ragged
@@ -176,7 +140,7 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
         chunk = ((cover + n - 1) / n + 31) / 32 * 32;
         if (chunk > most) chunk = most / 32 * 32;
     }
-    p.entries = (int)(chunk / c->page + 2);
+    p.entries = (int)(chunk / c->page + (sinks ? 5 : 2));
     p.chunk = (int)chunk;
     const int64_t n = (cover + chunk - 1) / chunk;
     p.chunks = (int)n;
@@ -196,21 +160,22 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
 // (apart 234 and 392), of 512 rows 661 (33 and 392).  Heads over 128 (S and O of two
 // halves are more than tensor memory) and groups over 128 stay with the split kernel:
 // 2 x 2048 rows of 16 heads of 256 over 8192 and 16384 tokens 10.6 ms, of 128 0.45.
-bool use_tiles(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d) {
+bool use_tiles(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d, int64_t sinks) {
     const int64_t group = d->q_heads / c->kv_heads, each = q->tokens / q->seqs;
     if (c->dim > 128 || group > 128 || each * group < 48) return false;
-    const double pairs = (double)q->tokens * (double)d->q_heads * (double)seen_cover(c, q, d, 1, 1);
+    const double pairs = (double)q->tokens * (double)d->q_heads * (double)seen_cover(c, q, d, 1, 1, sinks);
     return pairs * (double)c->dim >= 3.0e6 * 128;
 }
 
-TilePlan plan_tiles(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d, int sms) {
+TilePlan plan_tiles(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d, int sms,
+                    int64_t sinks) {
     TilePlan p;
     const int64_t group = d->q_heads / c->kv_heads;
     p.tile_tokens = (int)(256 / group);
     const int64_t runs = q->tokens / p.tile_tokens + q->seqs;
     p.by_token = q->tokens <= runs;
     p.slots = p.by_token ? q->tokens : runs;
-    const int64_t cover = seen_cover(c, q, d, p.tile_tokens, 128);
+    const int64_t cover = seen_cover(c, q, d, p.tile_tokens, sinks ? 16 : 128, sinks);
     const int64_t units = (q->tokens + p.tile_tokens - 1) / p.tile_tokens * c->kv_heads;
     int64_t chunks = units >= sms ? 1 : sms / units;
     int64_t chunk = (cover + chunks - 1) / chunks;
@@ -224,127 +189,161 @@ TilePlan plan_tiles(const bfft_cache_desc* c, const bfft_sequence_desc* q, const
     return p;
 }
 
-template <int DP, typename T, int CODE>
-cudaError_t launch_tiles(const TileArgs& a, const TilePlan& p, cudaStream_t s) {
-    static std::atomic<bool> ready[64];
-    using G = TileGeo<DP>;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    auto* kernel = k_attention_tiles<DP, T, CODE>;
-    if (!ready[dev].load(std::memory_order_acquire)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
-        if (e != cudaSuccess) return e;
-        ready[dev].store(true, std::memory_order_release);
+// A call with groups: which kernel takes the prefixes and which the sequences' own tokens,
+// and the items and the workspace of each.
+struct GroupPlan {
+    bool prefix_tiles, own_tiles;
+    SplitPlan split;   // nt, tile_tokens, token_tiles, entries, ctas
+    TilePlan tiles;    // tile_tokens, ctas
+    ItemArgs split_items, tile_items;
+    size_t places, split_parts, tile_parts, bytes;  // bytes of the parts of the workspace, in its order
+};
+
+// Sequences that have many rows each fill their row tiles by themselves: sharing saves them
+// nothing, and the prefix is a part of their own tokens like any other.
+bool worth_sharing(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d) {
+    return q->tokens / q->seqs * (d->q_heads / c->kv_heads) < 256;
+}
+
+GroupPlan plan_groups(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d,
+                      const bfft_span_desc* w, int sms) {
+    GroupPlan p{};
+    const int64_t group = d->q_heads / c->kv_heads, kv = c->kv_heads;
+    const int64_t each = q->tokens / q->seqs + (q->tokens % q->seqs != 0), shared = q->tokens / w->n_groups;
+    p.own_tiles = use_tiles(c, q, d, w->sinks);
+    // as use_tiles, for a group's rows
+    p.prefix_tiles = p.own_tiles;
+    if (!p.prefix_tiles && c->dim <= 128 && group <= 128 && shared * group >= 48)
+        p.prefix_tiles = (double)q->tokens * (double)d->q_heads * (double)seen_cover(c, q, d, 1, 1, w->sinks) *
+                             (double)c->dim >= 3.0e6 * 128;
+    SplitPlan& s = p.split;
+    s.nt = (p.prefix_tiles ? each : shared) * group > 8 && c->dim <= 128 ? 2 : 1;
+    const int64_t rows = 8 * s.nt;
+    s.tile_tokens = group <= rows ? (int)(rows / group) : 1;
+    s.token_tiles = group <= rows ? 1 : (int)((group + rows - 1) / rows);
+    s.entries = 384;
+    p.tiles.tile_tokens = (int)(256 / (group < 256 ? group : 256));
+    auto items = [&](bool prefixes, bool own, int64_t tile, int64_t parts, int64_t wanted, int least, int unit) {
+        ItemArgs x{};
+        x.prefixes = prefixes;
+        x.own = own;
+        x.target = (int)(wanted / kv > 0 ? wanted / kv : 1);
+        x.least = least;
+        x.unit = unit;
+        // every row tile may end with a piece that is not full
+        x.most = x.target + ((prefixes ? q->tokens / tile + w->n_groups : 0) + (own ? q->tokens / tile + q->seqs : 0)) * parts;
+        return x;
+    };
+    p.split_items = items(!p.prefix_tiles, !p.own_tiles, s.tile_tokens, s.token_tiles, 2 * 3 * (int64_t)sms, 256, 32);
+    p.tile_items = items(p.prefix_tiles, p.own_tiles, p.tiles.tile_tokens, 1, sms, 512, 128);
+    const bool split = !p.own_tiles, tiles = p.prefix_tiles;
+    s.ctas = split ? p.split_items.most * kv : 0;
+    p.tiles.ctas = tiles ? p.tile_items.most * kv : 0;
+    p.places = (size_t)q->tokens * 2 * sizeof(int4);
+    p.split_parts = (size_t)(s.ctas * rows) * (size_t)(c->dim + 2) * 4;
+    p.tile_parts = (size_t)(p.tiles.ctas * 256) * (size_t)(c->dim + 2) * 4;
+    p.bytes = p.places + p.split_parts + p.tile_parts;
+    return p;
+}
+
+template <typename T>
+cudaError_t run_groups(const AttentionArgs& a, const SpanArgs& w, const GroupPlan& p, const bfft_cache_desc* c, char* ws,
+                       unsigned int* status, cudaStream_t s) {
+    int4* own_of = reinterpret_cast<int4*>(ws);
+    int4* prefix_of = own_of + a.seq.tokens;
+    float* split_parts = reinterpret_cast<float*>(ws + p.places);
+    float* split_stats = split_parts + p.split.ctas * 8 * p.split.nt * c->dim;
+    float* tile_parts = reinterpret_cast<float*>(ws + p.places + p.split_parts);
+    float* tile_stats = tile_parts + p.tiles.ctas * 256 * c->dim;
+    cudaError_t e = cudaSuccess;
+    if (p.tiles.ctas) {
+        TileArgs t{};
+        t.a = a;
+        t.parts = tile_parts;
+        t.stats = tile_stats;
+        t.tile_tokens = p.tiles.tile_tokens;
+        t.status = status;
+        t.span = w;
+        t.items = p.tile_items;
+        t.items.own_of = own_of;
+        t.items.prefix_of = prefix_of;
+        e = run_tiles<T, kGroups>(t, p.tiles, c, s);
     }
-    return launch_dependent(kernel, (unsigned)p.ctas, G::THREADS, G::SMEM, s, a);
-}
-
-template <typename T>
-cudaError_t run_join(const SplitArgs& a, cudaStream_t s) {
-    const unsigned rows = (unsigned)(a.a.seq.tokens * a.a.q_heads);
-    return a.chunks > 16 ? launch_dependent(k_attention_join<T, 16>, rows, 512, 0, s, a)
-                         : launch_dependent(k_attention_join<T, 4>, rows, 128, 0, s, a);
-}
-
-template <typename T>
-cudaError_t run_tiles(const TileArgs& a, const TilePlan& p, const bfft_cache_desc* c, cudaStream_t s) {
-    cudaError_t e;
-    if (c->dim <= 64)
-        e = c->code == BFFT_CODE_INT8 ? launch_tiles<64, T, kCodeInt8>(a, p, s) : launch_tiles<64, T, kCodeE4m3>(a, p, s);
-    else
-        e = c->code == BFFT_CODE_INT8 ? launch_tiles<128, T, kCodeInt8>(a, p, s)
-                                      : launch_tiles<128, T, kCodeE4m3>(a, p, s);
-    if (e != cudaSuccess || p.chunks == 1) return e;
-    SplitArgs j{};
-    j.a = a.a;
-    j.parts = a.parts;
-    j.stats = a.stats;
-    j.chunks = a.chunks;
-    return run_join<T>(j, s);
-}
-
-template <int DP, bool EXACT, int NT, typename T, int CODE>
-cudaError_t launch_split(const SplitArgs& a, const SplitPlan& p, const CUtensorMap& km, const CUtensorMap& vm,
-                         cudaStream_t s) {
-    static std::atomic<bool> ready[64];
-    using G = SplitGeo<DP, EXACT, NT>;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    auto* kernel = k_attention_split<DP, EXACT, NT, T, CODE>;
-    if (!ready[dev].load(std::memory_order_acquire)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmemMost);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                     (int)cudaSharedmemCarveoutMaxShared);
-        if (e != cudaSuccess) return e;
-        ready[dev].store(true, std::memory_order_release);
+    if (e == cudaSuccess && p.split.ctas) {
+        SplitArgs t{};
+        t.a = a;
+        t.parts = split_parts;
+        t.stats = split_stats;
+        t.tile_tokens = p.split.tile_tokens;
+        t.token_tiles = p.split.token_tiles;
+        t.entries = p.split.entries;
+        t.status = status;
+        t.span = w;
+        t.items = p.split_items;
+        t.items.own_of = own_of;
+        t.items.prefix_of = prefix_of;
+        e = run_split<T, kGroups>(t, p.split, c, s);
     }
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[2];
-    cfg.gridDim = dim3((unsigned)p.ctas);
-    cfg.blockDim = dim3(kSplitThreads);
-    cfg.dynamicSmemBytes = split_smem(a.a.cache.dim, G::ROWS, a.entries);
-    cfg.stream = s;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // as launch_dependent
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)p.chunks;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = p.cluster ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a, km, vm);
+    if (e != cudaSuccess) return e;
+    const JoinSet split{split_parts, split_stats, nullptr, 8 * p.split.nt, p.split.ctas};
+    const JoinSet tiles{tile_parts, tile_stats, nullptr, 256, p.tiles.ctas};
+    JoinArgs j{a, {p.own_tiles ? tiles : split, p.prefix_tiles ? tiles : split}};
+    j.set[0].place = own_of;
+    j.set[1].place = prefix_of;
+    return run_join_items<T>(j, s);
 }
 
-template <typename T, int CODE>
-cudaError_t split_shape(const SplitArgs& a, const SplitPlan& p, const CUtensorMap& km, const CUtensorMap& vm,
-                        cudaStream_t s) {
-    const int dim = a.a.cache.dim;
-    if (dim == 64)
-        return p.nt == 1 ? launch_split<64, true, 1, T, CODE>(a, p, km, vm, s)
-                         : launch_split<64, true, 2, T, CODE>(a, p, km, vm, s);
-    if (dim == 128)
-        return p.nt == 1 ? launch_split<128, true, 1, T, CODE>(a, p, km, vm, s)
-                         : launch_split<128, true, 2, T, CODE>(a, p, km, vm, s);
-    if (dim == 256) return launch_split<256, true, 1, T, CODE>(a, p, km, vm, s);
-    if (dim < 128)
-        return p.nt == 1 ? launch_split<128, false, 1, T, CODE>(a, p, km, vm, s)
-                         : launch_split<128, false, 2, T, CODE>(a, p, km, vm, s);
-    return launch_split<256, false, 1, T, CODE>(a, p, km, vm, s);
-}
-
-template <typename T>
-cudaError_t run_split(const SplitArgs& a, const SplitPlan& p, const bfft_cache_desc* c, cudaStream_t s) {
-    CUtensorMap km{}, vm{};
-    if (c->dim == 64 || c->dim == 128 || c->dim == 256)
-        if (!encode_codes(&km, c->k, c) || !encode_codes(&vm, c->v, c)) return cudaErrorNotSupported;
-    cudaError_t e = c->code == BFFT_CODE_INT8 ? split_shape<T, kCodeInt8>(a, p, km, vm, s)
-                                              : split_shape<T, kCodeE4m3>(a, p, km, vm, s);
-    if (e != cudaSuccess || p.chunks == 1 || p.cluster) return e;
-    return run_join<T>(a, s);
-}
-
-}  // namespace
-
-extern "C" bfft_status bfft_cache_attention_workspace(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
-                                                      const bfft_attention_desc* d, size_t* bytes) {
-    if (!bytes) return fail(BFFT_ERR_VALUE, "null pointer");
-    const bfft_status st = check(cache, seqs, d);
-    if (st != BFFT_OK) return st;
-    if (!seqs->tokens)
-        *bytes = 0;
-    else
-        *bytes = use_tiles(cache, seqs, d) ? plan_tiles(cache, seqs, d, sm_count(d->device)).bytes
-                                           : plan_split(cache, seqs, d, sm_count(d->device)).bytes;
+// The form of a call: sinks matter beside a window only.
+bfft_status check_span(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs, const bfft_attention_desc* d,
+                       const bfft_span_desc* w, int* form) {
+    *form = kPlain;
+    if (w->sinks < 0 || w->sinks > 0x3fffffffLL) return fail(BFFT_ERR_VALUE, "bad count of first tokens %lld", (long long)w->sinks);
+    if (w->n_groups < 0 || w->n_groups > 0x7ffffffeLL) return fail(BFFT_ERR_SHAPE, "bad group count %lld", (long long)w->n_groups);
+    if (w->n_groups && (!w->shared || (!w->groups && w->n_groups > 1))) return fail(BFFT_ERR_VALUE, "null pointer");
+    if (!aligned(w->groups, 4) || !aligned(w->shared, 4)) return fail(BFFT_ERR_VALUE, "misaligned pointer");
+    if (!seqs->tokens) return BFFT_OK;
+    if (w->n_groups && worth_sharing(cache, seqs, d))
+        *form = kGroups;
+    else if (w->sinks && d->window > 0)
+        *form = kSinks;
+    if (*form != kPlain && seqs->max_pages > 0x3fffffffLL / cache->page)
+        return fail(BFFT_ERR_SHAPE, "tables of %lld pages of %lld tokens are too wide", (long long)seqs->max_pages,
+                    (long long)cache->page);
     return BFFT_OK;
 }
 
-extern "C" bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
-                                            const bfft_attention_desc* d, void* stream) {
-    const bfft_status st = check(cache, seqs, d);
+bfft_status workspace_call(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs, const bfft_attention_desc* d,
+                           const bfft_span_desc* w, size_t* bytes) {
+    if (!bytes) return fail(BFFT_ERR_VALUE, "null pointer");
+    bfft_status st = check(cache, seqs, d);
+    int form = kPlain;
+    if (st == BFFT_OK && w) st = check_span(cache, seqs, d, w, &form);
+    if (st != BFFT_OK) return st;
+    const int64_t sinks = form == kSinks ? w->sinks : 0;
+    const int sms = sm_count(d->device);
+    if (!seqs->tokens)
+        *bytes = 0;
+    else if (form == kGroups)
+        *bytes = plan_groups(cache, seqs, d, w, sms).bytes;
+    else
+        *bytes = use_tiles(cache, seqs, d, sinks) ? plan_tiles(cache, seqs, d, sms, sinks).bytes
+                                                  : plan_split(cache, seqs, d, sms, sinks).bytes;
+    return BFFT_OK;
+}
+
+template <int MODE>
+cudaError_t run_plan(bool tiles, const TileArgs& ta, const TilePlan& tp, const SplitArgs& sa, const SplitPlan& sp, int64_t type,
+                     const bfft_cache_desc* c, cudaStream_t s) {
+    if (tiles)
+        return type == BFFT_F16 ? run_tiles<__half, MODE>(ta, tp, c, s) : run_tiles<__nv_bfloat16, MODE>(ta, tp, c, s);
+    return type == BFFT_F16 ? run_split<__half, MODE>(sa, sp, c, s) : run_split<__nv_bfloat16, MODE>(sa, sp, c, s);
+}
+
+bfft_status attention_call(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs, const bfft_attention_desc* d,
+                           const bfft_span_desc* w, void* stream) {
+    bfft_status st = check(cache, seqs, d);
+    int form = kPlain;
+    if (st == BFFT_OK && w) st = check_span(cache, seqs, d, w, &form);
     if (st != BFFT_OK) return st;
     if (seqs->tokens == 0) return BFFT_OK;
     AttentionArgs a;
@@ -367,30 +366,74 @@ extern "C" bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const 
     unsigned int* status;
     cudaError_t e = device_status_word(&status);
     if (e != cudaSuccess) return launched(e, "cache_attention");
-    const bool tiles = use_tiles(cache, seqs, d);
+    const int sms = sm_count(d->device);
+    SpanArgs span{};
+    if (form != kPlain) span.sinks = d->window > 0 ? (int)w->sinks : 0;
+    auto room = [&](int64_t ctas, size_t bytes) {
+        if (ctas > 0x7fffffffLL || seqs->tokens * d->q_heads > 0x7fffffffLL)
+            return fail(BFFT_ERR_SHAPE, "too many rows: %lld", (long long)seqs->tokens);
+        if (bytes && (!d->workspace || d->workspace_bytes < (int64_t)bytes))
+            return fail(BFFT_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)d->workspace_bytes,
+                        (long long)bytes);
+        if (bytes && !aligned(d->workspace, 16)) return fail(BFFT_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+        return BFFT_OK;
+    };
+    if (form == kGroups) {
+        span.groups = static_cast<const int32_t*>(w->groups);
+        span.shared = static_cast<const int32_t*>(w->shared);
+        span.n_groups = (int)w->n_groups;
+        const GroupPlan p = plan_groups(cache, seqs, d, w, sms);
+        st = room(p.split.ctas > p.tiles.ctas ? p.split.ctas : p.tiles.ctas, p.bytes);
+        if (st != BFFT_OK) return st;
+        count_launches(1 + (p.split.ctas > 0) + (p.tiles.ctas > 0));
+        char* ws = static_cast<char*>(d->workspace);
+        return launched(d->type == BFFT_F16 ? run_groups<__half>(a, span, p, cache, ws, status, s)
+                                            : run_groups<__nv_bfloat16>(a, span, p, cache, ws, status, s),
+                        "cache_attention");
+    }
+    const bool tiles = use_tiles(cache, seqs, d, span.sinks);
     TilePlan tp{};
     SplitPlan sp{};
     if (tiles)
-        tp = plan_tiles(cache, seqs, d, sm_count(d->device));
+        tp = plan_tiles(cache, seqs, d, sms, span.sinks);
     else
-        sp = plan_split(cache, seqs, d, sm_count(d->device));
+        sp = plan_split(cache, seqs, d, sms, span.sinks);
     const int chunks = tiles ? tp.chunks : sp.chunks;
-    const size_t bytes = tiles ? tp.bytes : sp.bytes;
-    if ((tiles ? tp.ctas : sp.ctas) > 0x7fffffffLL || seqs->tokens * d->q_heads > 0x7fffffffLL)
-        return fail(BFFT_ERR_SHAPE, "too many rows: %lld", (long long)seqs->tokens);
-    if (bytes && (!d->workspace || d->workspace_bytes < (int64_t)bytes))
-        return fail(BFFT_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)d->workspace_bytes,
-                    (long long)bytes);
-    if (bytes && !aligned(d->workspace, 16)) return fail(BFFT_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+    st = room(tiles ? tp.ctas : sp.ctas, tiles ? tp.bytes : sp.bytes);
+    if (st != BFFT_OK) return st;
     float* parts = static_cast<float*>(d->workspace);
     float* stats = parts ? parts + seqs->tokens * d->q_heads * chunks * cache->dim : nullptr;
     count_launches(chunks > 1 && !sp.cluster ? 2 : 1);
-    if (tiles) {
-        TileArgs ta{a, parts, stats, tp.chunk, tp.chunks, tp.tile_tokens, tp.by_token, tp.slots, status};
-        e = d->type == BFFT_F16 ? run_tiles<__half>(ta, tp, cache, s) : run_tiles<__nv_bfloat16>(ta, tp, cache, s);
-    } else {
-        SplitArgs sa{a, parts, stats, sp.chunk, sp.chunks, sp.tile_tokens, sp.token_tiles, sp.by_token, sp.slots, sp.cluster, sp.entries, status};
-        e = d->type == BFFT_F16 ? run_split<__half>(sa, sp, cache, s) : run_split<__nv_bfloat16>(sa, sp, cache, s);
-    }
+    const TileArgs ta{a,           parts,    stats,  tp.chunk, tp.chunks, tp.tile_tokens,
+                      tp.by_token, tp.slots, status, span,     {}};
+    const SplitArgs sa{a,           parts,    stats,      sp.chunk,   sp.chunks, sp.tile_tokens, sp.token_tiles,
+                       sp.by_token, sp.slots, sp.cluster, sp.entries, status,    span,           {}};
+    e = form == kSinks ? run_plan<kSinks>(tiles, ta, tp, sa, sp, d->type, cache, s)
+                       : run_plan<kPlain>(tiles, ta, tp, sa, sp, d->type, cache, s);
     return launched(e, "cache_attention");
+}
+
+}  // namespace
+
+extern "C" bfft_status bfft_cache_attention_workspace(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
+                                                      const bfft_attention_desc* d, size_t* bytes) {
+    return workspace_call(cache, seqs, d, nullptr, bytes);
+}
+
+extern "C" bfft_status bfft_cache_attention_span_workspace(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
+                                                           const bfft_attention_desc* d, const bfft_span_desc* w,
+                                                           size_t* bytes) {
+    if (!w) return fail(BFFT_ERR_VALUE, "null pointer");
+    return workspace_call(cache, seqs, d, w, bytes);
+}
+
+extern "C" bfft_status bfft_cache_attention(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
+                                            const bfft_attention_desc* d, void* stream) {
+    return attention_call(cache, seqs, d, nullptr, stream);
+}
+
+extern "C" bfft_status bfft_cache_attention_span(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
+                                                 const bfft_attention_desc* d, const bfft_span_desc* w, void* stream) {
+    if (!w) return fail(BFFT_ERR_VALUE, "null pointer");
+    return attention_call(cache, seqs, d, w, stream);
 }

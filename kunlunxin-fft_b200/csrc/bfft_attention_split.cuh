@@ -1,5 +1,5 @@
 // bfft_attention_split.cuh -- attention of few query rows over a long axis of
-// 8-bit tokens (single tokens, drafted tokens).  Included by bfft_attention.cu.
+// 8-bit tokens (single tokens, drafted tokens).  Included by bfft_attention.cuh.
 //
 // Bound by the cache's bytes: with G query heads to a kv head a code (one byte)
 // meets G products, far under the tensor rate, so the design is about keeping
@@ -62,8 +62,10 @@ struct SplitArgs {
     int by_token;        // slots are tokens (else runs of tile_tokens, see slot_rows)
     int64_t slots;
     int cluster;         // the chunks of a row tile are one thread-block cluster, which joins them
-    int entries;         // pages that a chunk can touch
+    int entries;         // pages that a chunk can touch (kSinks, kGroups: that are held at a time)
     unsigned int* status;
+    SpanArgs span;
+    ItemArgs items;      // kGroups
 };
 
 constexpr int kSplitWarps = 4;
@@ -261,7 +263,7 @@ struct SplitGeo {
     __host__ __device__ static constexpr int half_bytes(int dim) { return split_half_bytes(dim); }
 };
 
-template <int DP, bool EXACT, int NT, typename T, int CODE>
+template <int DP, bool EXACT, int NT, typename T, int CODE, int MODE>
 __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     k_attention_split(SplitArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using G = SplitGeo<DP, EXACT, NT>;
@@ -277,31 +279,79 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
 
     // which rows and tokens
     int64_t i = blockIdx.x;
-    const int chunk = (int)(i % p.chunks);
-    i /= p.chunks;
-    const int kv = (int)(i % a.cache.kv_heads);
-    i /= a.cache.kv_heads;
-    const int part = (int)(i % p.token_tiles);
-    const int64_t slot = i / p.token_tiles;
+    int chunk = 0, kv, part;
+    SlotRows sr;
+    Item it{};
+    if constexpr (MODE == kGroups) {
+        __shared__ ItemScratch scratch;
+        kv = (int)(i % a.cache.kv_heads);
+        if (!find_item<kSplitThreads>(a, p.span, p.items, i / a.cache.kv_heads, p.tile_tokens, p.token_tiles, scratch, it))
+            return;
+        part = it.part;
+        chunk = it.chunk;
+        sr.s = it.table_row;
+        sr.first = it.token;
+        sr.n = it.n;
+    } else {
+        chunk = (int)(i % p.chunks);
+        i /= p.chunks;
+        kv = (int)(i % a.cache.kv_heads);
+        i /= a.cache.kv_heads;
+        part = (int)(i % p.token_tiles);
+    }
     if (tid == 0) {
         for (int b = 0; b < kSplitWarps * G::STAGES; ++b) mbar_init(&full[b], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    SlotRows sr;
-    if (!slot_rows(a.seq, slot, p.tile_tokens, p.by_token, sr)) return;
+    if constexpr (MODE != kGroups)
+        if (!slot_rows(a.seq, i / p.token_tiles, p.tile_tokens, p.by_token, sr)) return;
     const int head0 = part * G::ROWS;                       // of the group, where a token takes several tiles
     const int per_token = p.token_tiles > 1 ? min(a.group - head0, G::ROWS) : a.group;
     const int rows = sr.n * per_token;
-    int64_t len = a.seq.lens[sr.s];
-    const int64_t most = (int64_t)a.seq.max_pages << a.cache.page_log2;
-    if (len > most) len = most;
-    const int64_t pos0 = (int64_t)a.seq.lens[sr.s] - sr.rows + sr.place;
-    int64_t lo_min, hi_max, lo_max, hi_min;
-    seen_range(a, pos0, len, lo_min, hi_min);
-    seen_range(a, pos0 + sr.n - 1, len, lo_max, hi_max);
-    const int64_t base = (lo_min & ~(int64_t)15) + (int64_t)chunk * p.chunk;
-    int64_t end = base + p.chunk;
-    if (end > hi_max) end = hi_max;
+    // [base, end) of the axis: kPlain counts sequence tokens, the others places of `axis`
+    int64_t len = 0, pos0 = 0, base, end, lo_min = 0, hi_max, lo_max = 0, hi_min;
+    Axis axis{};
+    TokenSpan mine_span{0, 0, 0};  // kSinks, kGroups: of query token `lane` of the tile
+    if constexpr (MODE == kPlain) {
+        len = a.seq.lens[sr.s];
+        const int64_t most = (int64_t)a.seq.max_pages << a.cache.page_log2;
+        if (len > most) len = most;
+        pos0 = (int64_t)a.seq.lens[sr.s] - sr.rows + sr.place;
+        seen_range(a, pos0, len, lo_min, hi_min);
+        seen_range(a, pos0 + sr.n - 1, len, lo_max, hi_max);
+        base = (lo_min & ~(int64_t)15) + (int64_t)chunk * p.chunk;
+        end = base + p.chunk;
+        if (end > hi_max) end = hi_max;
+    } else {
+        int first = 0;
+        if (MODE == kGroups) first = it.from;
+        if (lane < sr.n) {
+            if constexpr (MODE == kGroups)
+                mine_span = item_span(a, p.span, it, sr.first + lane);
+            else
+                mine_span = token_span(a, p.span, (int64_t)a.seq.lens[sr.s] - sr.rows + sr.place + lane, a.seq.lens[sr.s],
+                                       0, 0x7fffffff);
+        } else {
+            mine_span.sinks = first;
+        }
+        const bool some = mine_span.lo < mine_span.hi;
+        axis = make_axis(first, __reduce_min_sync(0xffffffffu, some ? mine_span.lo : 0x7fffffff),
+                         __reduce_max_sync(0xffffffffu, some ? mine_span.hi : 0),
+                         __reduce_max_sync(0xffffffffu, mine_span.sinks));
+        const int pieces = MODE == kGroups ? it.chunks : p.chunks;
+        const int64_t each = ((axis.total + pieces - 1) / pieces + 31) & ~31;
+        base = chunk * each;
+        end = base + each;
+        if (end > axis.total) end = axis.total;
+    }
+    const bool direct = MODE == kGroups && !it.prefix && !it.shares && it.chunks == 1;
+    if constexpr (MODE == kGroups) {  // where the join finds the parts of the tile's tokens
+        if (kv == 0 && part == 0 && chunk == 0 && tid < sr.n) {
+            const int flags = (direct ? kPlaceDone : 0) | (!it.prefix && it.shares ? kPlacePrefix : 0);
+            (it.prefix ? p.items.prefix_of : p.items.own_of)[sr.first + tid] =
+                make_int4((int)(blockIdx.x / a.cache.kv_heads), it.chunks, p.token_tiles > 1 ? 0 : tid * a.group, flags);
+        }
+    }
     // row r of the tile: query token r / per_token, head r % per_token
     auto row_of = [&](int r, int64_t& token, int& head) {
         const int t = r / per_token;
@@ -320,15 +370,17 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
             if (p.cluster) {
                 cta_ml[tid * 2] = -INFINITY;
                 cta_ml[tid * 2 + 1] = 0.f;
-            } else if (p.chunks > 1) {
-                float* st = p.stats + ((token * a.q_heads + head) * p.chunks + chunk) * 2;
+            } else if (MODE == kGroups ? !direct : p.chunks > 1) {
+                const int64_t at = MODE == kGroups ? (int64_t)blockIdx.x * G::ROWS + tid
+                                                   : (token * a.q_heads + head) * p.chunks + chunk;
+                float* st = p.stats + at * 2;
                 st[0] = -INFINITY;
                 st[1] = 0.f;
             } else if (a.lse) {
                 a.lse[token * a.q_heads + head] = -INFINITY;
             }
         }
-        if (p.chunks == 1)
+        if (MODE == kGroups ? direct : p.chunks == 1)
             for (int e = tid; e < rows * dim; e += kSplitThreads) {
                 int64_t token;
                 int head;
@@ -337,34 +389,96 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
             }
         if (!p.cluster) return;
     } else {
-    // from here on tokens are counted from `base`, in 32 bits
-    const int lg = a.cache.page_log2;
-    const int64_t page0 = base >> lg;
-    const int off = (int)(base & (((int64_t)1 << lg) - 1)), span = (int)(end - base);
-    const int entries = ((off + span - 1) >> lg) + 1;
-    auto rel = [&](int64_t t) { return (int)(t < base ? 0 : t - base > span ? span : t - base); };
-    const int lo_all = rel(lo_max), hi_all = rel(hi_min), lo_any = rel(lo_min);
-    for (int e = tid; e < entries; e += kSplitThreads) {
-        const int64_t id = a.seq.block_table[sr.s * a.seq.table_stride + page0 + e];
-        page_ids[e] = id >= 0 && id < a.cache.pages ? (int)id : -1;
+    // From here on tokens are counted in 32 bits: kPlain from `base`, the others in places
+    // of the axis.  A segment is what the table of pages holds: kPlain's chunks are one.
+    const int lg = a.cache.page_log2, page_mask = (1 << lg) - 1;
+    int64_t page0 = 0;
+    int off = 0, span = 0, entries = 0;  // of kPlain: base's place in its page, tokens, pages
+    int seg = 0, stop = 0, heads = 0, head_off = 0, main_off = 0, head_page = 0, main_page = 0;  // of the others: the segment
+    // [seg, stop), its first tokens' pages, and the places of seg (of the window's first token) in theirs
+    if constexpr (MODE == kPlain) {
+        page0 = base >> lg;
+        off = (int)(base & page_mask);
+        span = (int)(end - base);
+        entries = ((off + span - 1) >> lg) + 1;
+        stop = span;
     }
+    auto open_segment = [&](int from) {
+        seg = from;
+        const int room = (p.entries - 4) << lg;
+        stop = (int)end - from > room ? from + room : (int)end;
+        const int turn = axis.head < from ? from : axis.head < stop ? axis.head : stop;  // first tokens before it
+        head_off = (axis.first + from) & page_mask;
+        head_page = (axis.first + from) >> lg;
+        heads = turn > from ? ((head_off + turn - from - 1) >> lg) + 1 : 0;
+        const int at = axis.main + (turn - axis.head);
+        main_off = (at & page_mask) - turn;
+        main_page = at >> lg;
+        entries = heads + (stop > turn ? ((main_off + stop - 1) >> lg) + 1 : 0);
+    };
+    // the table's entry of place t, and t's place in its page
+    auto entry_of = [&](int t) {
+        if constexpr (MODE == kPlain) return (off + t) >> lg;
+        return t < axis.head ? (head_off + t - seg) >> lg : heads + ((main_off + t) >> lg);
+    };
+    auto slot_of = [&](int t) {
+        if constexpr (MODE == kPlain) return (off + t) & page_mask;
+        return (t < axis.head ? head_off + t - seg : main_off + t) & page_mask;
+    };
+    auto load_pages = [&] {
+        for (int e = tid; e < entries; e += kSplitThreads) {
+            int64_t at = page0 + e;
+            if (MODE != kPlain) at = e < heads ? head_page + e : main_page + e - heads;
+            const int64_t id = a.seq.block_table[sr.s * a.seq.table_stride + at];
+            page_ids[e] = id >= 0 && id < a.cache.pages ? (int)id : -1;
+        }
+    };
+    auto load_scales = [&] {
+        bool small = false;
+        for (int e = tid; e < entries; e += kSplitThreads) {
+            const int id = page_ids[e];
+            if (id >= 0) {
+                const int64_t b = (int64_t)id * a.cache.kv_heads + kv;
+                scales[e] = block_scale(a.cache.k_scale[b], a.cache.v_scale[b]);
+                small |= small_scale(scales[e]);
+            } else {
+                scales[e].kind = kDeadBlock;
+            }
+        }
+        return small;
+    };
+    auto rel = [&](int64_t t) { return (int)(t < base ? 0 : t - base > span ? span : t - base); };
+    int lo_all, hi_all, lo_any, sinks_all = 0;
+    if constexpr (MODE == kPlain) {
+        lo_all = rel(lo_max);
+        hi_all = rel(hi_min);
+        lo_any = rel(lo_min);
+    } else {
+        open_segment((int)base);
+        lo_any = axis.lo_any;
+        const bool valid = lane < sr.n;
+        lo_all = __reduce_max_sync(0xffffffffu, valid ? axis.place(mine_span.lo) : -0x7fffffff);
+        hi_all = __reduce_min_sync(0xffffffffu, valid ? axis.place(mine_span.hi) : 0x7fffffff);
+        sinks_all = __reduce_min_sync(0xffffffffu, valid ? mine_span.sinks - axis.first : 0x7fffffff);
+    }
+    load_pages();
     __syncthreads();
 
-    // ring: tile t of this warp covers tokens [base + 32 (t kSplitWarps + warp), + 32)
-    const int tiles = (span + 31) >> 5;
+    // ring: tile t of this warp covers tokens [seg + 32 (t kSplitWarps + warp), + 32)
+    int tiles = (stop - seg + 31) >> 5;
     unsigned char* mine = ring + warp * (G::STAGES * 4 * G::half_bytes(dim));
     uint64_t* bars = full + warp * G::STAGES;
     const int lines = EXACT ? DP / 8 : 1;  // 128-byte lines of 16 tokens
     auto fetch = [&](int t, int stage) {   // lanes 0..3: keys of half 0, 1, values of half 0, 1
-        const int tok = t * 32 + (lane & 1) * 16;
+        const int tok = seg + t * 32 + (lane & 1) * 16;
         int id = -1;
-        if (lane < 4 && tok < span) id = page_ids[(off + tok) >> lg];
+        if (lane < 4 && tok < stop) id = page_ids[entry_of(tok)];
         const unsigned any = __ballot_sync(0xffffffffu, id >= 0);
         if (lane == 0) mbar_arrive_expect_tx(&bars[stage], (uint32_t)(__popc(any) * G::half_bytes(dim)));
         __syncwarp();
         if (id >= 0) {
             unsigned char* dst = mine + (stage * 4 + lane) * G::half_bytes(dim);
-            const int slot_in = (off + tok) & ((1 << lg) - 1);
+            const int slot_in = slot_of(tok);
             if constexpr (EXACT) {
                 tma_load_3d(dst, lane < 2 ? &kmap : &vmap, 0, ((kv << lg) + slot_in) / 16 * lines, id, &bars[stage]);
             } else {
@@ -374,24 +488,14 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
             }
         }
     };
-    int ahead = warp;  // next tile to fetch
-    for (int s = 0; s < G::STAGES && ahead < tiles; ++s, ahead += kSplitWarps) fetch(ahead, s);
-    bool any_small = false;
-    for (int e = tid; e < entries; e += kSplitThreads) {
-        const int id = page_ids[e];
-        if (id >= 0) {
-            const int64_t b = (int64_t)id * a.cache.kv_heads + kv;
-            scales[e] = block_scale(a.cache.k_scale[b], a.cache.v_scale[b]);
-            any_small |= small_scale(scales[e]);
-        } else {
-            scales[e].kind = kDeadBlock;
-        }
-    }
+    int ahead = warp, fetched = 0;  // next tile to fetch, and how many were
+    for (int s = 0; s < G::STAGES && ahead < tiles; ++s, ahead += kSplitWarps, ++fetched) fetch(ahead, s);
+    bool any_small = load_scales();
 
     // queries as B fragments: lane (g, q4) holds row g of each 8-row tile, dims 16 (4 i + q4) + 4 t ..
     uint32_t qf[NT][G::KS][2];
     float row_scale[NT][2];      // of rows 2 q4, 2 q4 + 1: softmax scale (log2) times the row's power
-    int row_lo[NT][2], row_hi[NT][2];
+    int row_lo[NT][2], row_hi[NT][2], row_sinks[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int r = nt * 8 + g;
@@ -425,13 +529,21 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
         for (int j = 0; j < 2; ++j) {
             row_scale[nt][j] = __shfl_sync(0xffffffffu, up, (2 * q4 + j) * 4) * a.scale_log2;
             const int rr = nt * 8 + 2 * q4 + j;
-            int64_t lo, hi;
-            seen_range(a, pos0 + (rr < rows ? rr / per_token : 0), len, lo, hi);
-            row_lo[nt][j] = rel(lo);
-            row_hi[nt][j] = rel(hi);
+            if constexpr (MODE == kPlain) {
+                int64_t lo, hi;
+                seen_range(a, pos0 + (rr < rows ? rr / per_token : 0), len, lo, hi);
+                row_lo[nt][j] = rel(lo);
+                row_hi[nt][j] = rel(hi);
+                row_sinks[nt][j] = 0;
+            } else {
+                const int of = rr < rows ? rr / per_token : 0;
+                row_lo[nt][j] = axis.place(__shfl_sync(0xffffffffu, mine_span.lo, of));
+                row_hi[nt][j] = axis.place(__shfl_sync(0xffffffffu, mine_span.hi, of));
+                row_sinks[nt][j] = __shfl_sync(0xffffffffu, mine_span.sinks, of) - axis.first;
+            }
         }
     }
-    const bool small = __syncthreads_or(any_small);  // a small value scale in the chunk
+    bool small = __syncthreads_or(any_small);  // a small value scale in the chunk (kPlain), or so far
     if (small) {
         for (int e = tid; e < entries; e += kSplitThreads) to_small(scales[e]);
         __syncthreads();
@@ -456,15 +568,16 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     const int tk = row_token(g);
 
     bool ok = true;
-    int it = 0;
-    for (int t = warp; t < tiles; t += kSplitWarps, ++it) {
-        const int stage = it % G::STAGES;
-        ok = mbar_wait_limited(&bars[stage], (uint32_t)((it / G::STAGES) & 1), p.status);
+    int used = 0;  // tiles that this warp has waited for
+    for (;;) {     // segments
+    for (int t = warp; t < tiles; t += kSplitWarps, ++used) {
+        const int stage = used % G::STAGES;
+        ok = mbar_wait_limited(&bars[stage], (uint32_t)((used / G::STAGES) & 1), p.status);
         if (__any_sync(0xffffffffu, !ok)) {
             ok = false;
             break;
         }
-        const int tok0 = t * 32;
+        const int tok0 = seg + t * 32;
         const unsigned char* buf = mine + stage * 4 * G::half_bytes(dim);
         float z[2][NT][4];
         BlockScale bs[2];
@@ -473,9 +586,9 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int tok = tok0 + 16 * h;
-            const int e = (off + tok) >> lg;
+            const int e = entry_of(tok);
             bs[h] = scales[e < entries ? e : entries - 1];
-            live[h] = tok < span && bs[h].kind != kDeadBlock;
+            live[h] = tok < stop && bs[h].kind != kDeadBlock;
             if (!live[h]) continue;
             const unsigned char* kb = buf + h * G::half_bytes(dim);
 #pragma unroll
@@ -499,7 +612,8 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
                         mma_f16(z[h][nt], a0, a1, a2, a3, qf[nt][c * 4 + s][0], qf[nt][c * 4 + s][1]);
                 }
             }
-            const bool inside = tok >= lo_all && tok + 16 <= hi_all;  // hi_all is at most span
+            bool inside = tok >= lo_all && tok + 16 <= hi_all;  // kPlain: hi_all is at most span
+            if (MODE != kPlain) inside = (inside && tok + 16 <= stop) || tok + 16 <= sinks_all;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -507,7 +621,9 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
                     float v = z[h][nt][c] * (bs[h].key * row_scale[nt][c & 1]) + bs[h].log2_value;
                     if (!inside) {
                         const int j = tok + tk + (c >> 1) * 8;
-                        if (j < row_lo[nt][c & 1] || j >= row_hi[nt][c & 1]) v = -INFINITY;
+                        bool hidden = j < row_lo[nt][c & 1] || j >= row_hi[nt][c & 1];
+                        if (MODE != kPlain) hidden = hidden && j >= row_sinks[nt][c & 1];
+                        if (hidden) v = -INFINITY;
                     }
                     z[h][nt][c] = v;
                     worst = fmaxf(worst, v == -INFINITY ? v : v - m[nt][c & 1]);
@@ -573,7 +689,8 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
             const int t0 = row_token(2 * q4), t1 = row_token(2 * q4 + 1);
             const int toks[4] = {t0, t1, t0 + 8, t1 + 8};
             uint32_t w[4][G::VW];
-            const bool whole = tok >= lo_any && tok + 16 <= span;
+            bool whole = tok >= lo_any && tok + 16 <= stop;
+            if (MODE != kPlain) whole = (whole && tok + 16 <= axis.hi_any) || tok + 16 <= axis.sinks_any;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 if constexpr (DP == 64) {
@@ -595,7 +712,9 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
                 }
                 if (!whole) {  // codes of slots that no row sees may be anything: 0 times NaN is NaN
                     const int j = tok + toks[k];
-                    if (j < lo_any || j >= span)
+                    bool drop = j < lo_any || j >= stop;
+                    if (MODE != kPlain) drop = (j < lo_any || j >= axis.hi_any) && j >= axis.sinks_any;
+                    if (drop)
 #pragma unroll
                         for (int c = 0; c < G::VW; ++c) w[k][c] = 0;
                 }
@@ -616,11 +735,37 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
         if (ahead < tiles) {
             fetch(ahead, stage);
             ahead += kSplitWarps;
+            ++fetched;
         }
     }
     if (!ok)  // status bit 0 is set; wait (bounded) for the copies that are still under way
-        for (int t = warp + kSplitWarps * it; t < ahead; t += kSplitWarps, ++it)
-            mbar_wait_limited(&bars[it % G::STAGES], (uint32_t)((it / G::STAGES) & 1), p.status);
+        for (int b = used; b < used + G::STAGES; ++b)
+            if (b < fetched) mbar_wait_limited(&bars[b % G::STAGES], (uint32_t)((b / G::STAGES) & 1), p.status);
+    if (MODE == kPlain || stop >= (int)end) break;
+    // the next pages, once every warp is done with these
+    __syncthreads();
+    open_segment(stop);
+    load_pages();
+    __syncthreads();
+    tiles = ok ? (stop - seg + 31) >> 5 : 0;  // a warp whose wait expired does no more
+    ahead = warp;
+    for (int s = 0; s < G::STAGES && ahead < tiles; ++s, ahead += kSplitWarps, ++fetched)
+        fetch(ahead, (used + s) % G::STAGES);
+    any_small = load_scales();
+    const bool now_small = __syncthreads_or(any_small) || small;
+    if (now_small) {
+        for (int e = tid; e < entries; e += kSplitThreads) to_small(scales[e]);
+        if (!small) {  // the sums so far in the smaller unit
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                l[nt][0] *= SmallScales::factor;
+                l[nt][1] *= SmallScales::factor;
+            }
+        }
+        __syncthreads();
+    }
+    small = now_small;
+    }
 
     griddep_launch_dependents();  // the joining kernel's CTAs may take their places and wait for this grid
     // join the warps: rows' m and l, then O, through the ring's memory
@@ -685,8 +830,9 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
                 cta_ml[r * 2] = top;
                 cta_ml[r * 2 + 1] = sum;
             }
-        } else if (p.chunks > 1) {
-            const int64_t at_part = (token * a.q_heads + head) * p.chunks + chunk;
+        } else if (MODE == kGroups ? !direct : p.chunks > 1) {
+            const int64_t at_part = MODE == kGroups ? (int64_t)blockIdx.x * G::ROWS + r
+                                                    : (token * a.q_heads + head) * p.chunks + chunk;
             *reinterpret_cast<float4*>(p.parts + at_part * dim + d) = v;
             if (d == 0) {
                 p.stats[at_part * 2] = top;
@@ -821,6 +967,108 @@ __global__ void __launch_bounds__(WARPS * 32) k_attention_join(SplitArgs p) {
     }
     if (a.lse && tid == 0)
         a.lse[i] = sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * 0.693147180559945309f;
+}
+
+// Joins the parts of a call with groups: a CTA a (token, kv head), a warp a head in turn,
+// lanes over the dimensions.  The parts of a token are those of its own row tile's items
+// and of its group's.  What the places say is checked against the parts that there are:
+// with tables that contradict themselves it may be anything.
+constexpr int kJoinWarps = 4;
+
+struct JoinSet {
+    const float *parts, *stats;
+    const int4* place;
+    int rows;        // of a tile
+    int64_t blocks;  // item * kv_heads + head at most
+};
+struct JoinArgs {
+    AttentionArgs a;
+    JoinSet set[2];  // own tokens, prefixes
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32) k_attention_join_items(JoinArgs p) {
+    const AttentionArgs& a = p.a;
+    griddep_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = a.cache.dim, kv_heads = a.cache.kv_heads;
+    const int64_t token = blockIdx.x / kv_heads;
+    const int kv = (int)(blockIdx.x - token * kv_heads);
+    if (token < a.seq.starts[0] || token >= a.seq.starts[a.seq.seqs]) return;  // no sequence's row
+    const int4 own = p.set[0].place[token];
+    if (own.w & kPlaceDone) return;
+    const int4 pre = own.w & kPlacePrefix ? p.set[1].place[token] : make_int4(0, 0, 0, 0);
+    for (int h = warp; h < a.group; h += kJoinWarps) {
+        int64_t first[2];  // part of the first piece, and pieces
+        int n[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const JoinSet& s = p.set[k];
+            const int4 at = k ? pre : own;
+            const int r = at.z + h, part = r / s.rows;
+            const int64_t item = (int64_t)at.x + (int64_t)part * at.y;
+            first[k] = item * kv_heads + kv;
+            n[k] = at.y;
+            if (at.x < 0 || at.y < 0 || at.z < 0 || at.z > 255 || (item + at.y) * kv_heads > s.blocks) n[k] = 0;
+            first[k] = first[k] * s.rows + r % s.rows;
+        }
+        const int all = n[0] + n[1];
+        auto stat = [&](int c) {
+            const int k = c >= n[0];
+            const JoinSet& s = p.set[k];
+            return reinterpret_cast<const float2*>(s.stats)[first[k] + (int64_t)(c - (k ? n[0] : 0)) * kv_heads * s.rows];
+        };
+        float top = -INFINITY;
+        for (int c = lane; c < all; c += 32) top = fmaxf(top, stat(c).x);
+#pragma unroll
+        for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+        float sum = 0.f;
+        for (int c0 = 0; c0 < all; c0 += 32) {
+            float f = 0.f;
+            if (c0 + lane < all) {
+                const float2 v = stat(c0 + lane);
+                // a NaN sum without a maximum keeps its weight: the row is NaN
+                f = v.y == 0.f ? 0.f : v.x == -INFINITY ? 1.f : exp2_approx(v.x - top);
+                sum += v.y * f;
+            }
+            const int m = min(32, all - c0);
+#pragma unroll 8
+            for (int j = 0; j < m; ++j) {
+                const float g = __shfl_sync(0xffffffffu, f, j);
+                const int c = c0 + j, k = c >= n[0];
+                const JoinSet& s = p.set[k];
+                const float4* o = reinterpret_cast<const float4*>(
+                    s.parts + (first[k] + (int64_t)(c - (k ? n[0] : 0)) * kv_heads * s.rows) * dim);
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    if (g != 0.f && (q * 32 + lane) * 4 < dim) {
+                        const float4 x = o[q * 32 + lane];
+                        acc[q].x += x.x * g;
+                        acc[q].y += x.y * g;
+                        acc[q].z += x.z * g;
+                        acc[q].w += x.w * g;
+                    }
+            }
+        }
+#pragma unroll
+        for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int head = kv * a.group + h;
+        T* y = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int d = (q * 32 + lane) * 4;
+            if (d < dim) {
+                y[d] = from_f32<T>(acc[q].x * inv);
+                y[d + 1] = from_f32<T>(acc[q].y * inv);
+                y[d + 2] = from_f32<T>(acc[q].z * inv);
+                y[d + 3] = from_f32<T>(acc[q].w * inv);
+            }
+        }
+        if (a.lse && lane == 0)
+            a.lse[token * a.q_heads + head] =
+                sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * 0.693147180559945309f;
+    }
 }
 
 }  // namespace bfft

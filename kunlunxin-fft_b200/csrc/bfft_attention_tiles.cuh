@@ -1,5 +1,5 @@
 // bfft_attention_tiles.cuh -- attention of many query rows (a prompt's chunk) over
-// 8-bit tokens on the tensor cores (tcgen05).  Included by bfft_attention.cu.
+// 8-bit tokens on the tensor cores (tcgen05).  Included by bfft_attention.cuh.
 //
 // A CTA takes up to 256 rows of one kv head (query tokens times the group's heads,
 // so all of them share the keys) and walks the tokens in tiles of 128:
@@ -49,6 +49,8 @@ struct TileArgs {
     int by_token;
     int64_t slots;
     unsigned int* status;
+    SpanArgs span;
+    ItemArgs items;    // kGroups
 };
 
 template <int DP>
@@ -183,7 +185,7 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&d)[16]) {
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <int DP, typename T, int CODE>
+template <int DP, typename T, int CODE, int MODE>
 __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(TileArgs p) {
     using G = TileGeo<DP>;
     extern __shared__ unsigned char smem_raw[];
@@ -193,23 +195,103 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
 
     // which rows and tokens
     int64_t i = blockIdx.x;
-    const int chunk = (int)(i % p.chunks);
-    i /= p.chunks;
-    const int kv = (int)(i % a.cache.kv_heads);
-    const int64_t slot = i / a.cache.kv_heads;
+    int chunk, kv;
     SlotRows sr;
-    if (!slot_rows(a.seq, slot, p.tile_tokens, p.by_token, sr)) return;
+    Item it{};
+    if constexpr (MODE == kGroups) {
+        __shared__ ItemScratch scratch;
+        kv = (int)(i % a.cache.kv_heads);
+        if (!find_item<G::THREADS>(a, p.span, p.items, i / a.cache.kv_heads, p.tile_tokens, 1, scratch, it)) return;
+        chunk = it.chunk;
+        sr.s = it.table_row;
+        sr.first = it.token;
+        sr.n = it.n;
+    } else {
+        chunk = (int)(i % p.chunks);
+        i /= p.chunks;
+        kv = (int)(i % a.cache.kv_heads);
+        if (!slot_rows(a.seq, i / a.cache.kv_heads, p.tile_tokens, p.by_token, sr)) return;
+    }
     const int rows = sr.n * a.group;
-    int64_t len = a.seq.lens[sr.s];
-    const int64_t most = (int64_t)a.seq.max_pages << lg;
-    if (len > most) len = most;
-    const int64_t pos0 = (int64_t)a.seq.lens[sr.s] - sr.rows + sr.place;
-    int64_t lo_min, hi_max, lo_max, hi_min;
-    seen_range(a, pos0, len, lo_min, hi_min);
-    seen_range(a, pos0 + sr.n - 1, len, lo_max, hi_max);
-    const int64_t base = (lo_min & ~(int64_t)127) + (int64_t)chunk * p.chunk;
-    int64_t end = base + p.chunk;
-    if (end > hi_max) end = hi_max;
+    // [base, end) of the axis and what its rows see: kPlain counts sequence tokens, the
+    // others places of `axis` (what some row sees there: axis.lo_any, hi_any, sinks_any)
+    int64_t len = 0, pos0 = 0, base, end, lo_min, hi_max, lo_max, hi_min;
+    Axis axis{};
+    TokenSpan row_span{0, 0, 0};  // of row tid
+    int sinks_all = 0;
+    if constexpr (MODE == kPlain) {
+        len = a.seq.lens[sr.s];
+        const int64_t most = (int64_t)a.seq.max_pages << lg;
+        if (len > most) len = most;
+        pos0 = (int64_t)a.seq.lens[sr.s] - sr.rows + sr.place;
+        seen_range(a, pos0, len, lo_min, hi_min);
+        seen_range(a, pos0 + sr.n - 1, len, lo_max, hi_max);
+        base = (lo_min & ~(int64_t)127) + (int64_t)chunk * p.chunk;
+        end = base + p.chunk;
+        if (end > hi_max) end = hi_max;
+    } else {
+        __shared__ int bound[6];  // least and largest lo, hi and sinks of the rows
+        int first = 0;
+        if (MODE == kGroups) first = it.from;
+        if (tid < 6) bound[tid] = tid == 0 || tid == 3 || tid == 5 ? 0x7fffffff : tid == 4 ? first : tid == 1 ? -0x7fffffff : 0;
+        __syncthreads();
+        if (tid < 256) {
+            const bool valid = tid < rows;
+            if (valid) {
+                const int of = tid / a.group;
+                if constexpr (MODE == kGroups)
+                    row_span = item_span(a, p.span, it, sr.first + of);
+                else
+                    row_span = token_span(a, p.span, (int64_t)a.seq.lens[sr.s] - sr.rows + sr.place + of,
+                                          a.seq.lens[sr.s], 0, 0x7fffffff);
+            } else {
+                row_span.sinks = first;
+            }
+            const bool some = row_span.lo < row_span.hi;
+            const int v[6] = {__reduce_min_sync(0xffffffffu, some ? row_span.lo : 0x7fffffff),
+                              __reduce_max_sync(0xffffffffu, valid ? row_span.lo : -0x7fffffff),
+                              __reduce_max_sync(0xffffffffu, some ? row_span.hi : 0),
+                              __reduce_min_sync(0xffffffffu, valid ? row_span.hi : 0x7fffffff),
+                              __reduce_max_sync(0xffffffffu, row_span.sinks),
+                              __reduce_min_sync(0xffffffffu, valid ? row_span.sinks : 0x7fffffff)};
+            if (lane == 0) {
+                atomicMin(&bound[0], v[0]);
+                atomicMax(&bound[1], v[1]);
+                atomicMax(&bound[2], v[2]);
+                atomicMin(&bound[3], v[3]);
+                atomicMax(&bound[4], v[4]);
+                atomicMin(&bound[5], v[5]);
+            }
+        }
+        __syncthreads();
+        axis = make_axis(first, bound[0], bound[2], bound[4]);
+        lo_min = axis.lo_any;
+        hi_max = axis.hi_any;
+        lo_max = axis.place(bound[1]);
+        hi_min = axis.place(bound[3]);
+        sinks_all = bound[5] - first;
+        const int pieces = MODE == kGroups ? it.chunks : p.chunks;
+        const int64_t each = ((axis.total + pieces - 1) / pieces + 127) & ~127;
+        base = chunk * each;
+        end = base + each;
+        if (end > axis.total) end = axis.total;
+    }
+    const bool direct = MODE == kGroups ? !it.prefix && !it.shares && it.chunks == 1 : p.chunks == 1;
+    if constexpr (MODE == kGroups) {  // where the join finds the parts of the tile's tokens
+        if (kv == 0 && chunk == 0 && tid < sr.n) {
+            const int flags = (direct ? kPlaceDone : 0) | (!it.prefix && it.shares ? kPlacePrefix : 0);
+            (it.prefix ? p.items.prefix_of : p.items.own_of)[sr.first + tid] =
+                make_int4((int)(blockIdx.x / a.cache.kv_heads), it.chunks, tid * a.group, flags);
+        }
+    }
+    auto part_of = [&](int64_t token, int head, int r) {
+        return MODE == kGroups ? (int64_t)blockIdx.x * 256 + r : (token * a.q_heads + head) * p.chunks + chunk;
+    };
+    // a sequence token at a place of the axis
+    auto token_at = [&](int64_t t) -> int64_t {
+        if constexpr (MODE == kPlain) return t;
+        return t < axis.head ? axis.first + t : axis.main + (t - axis.head);
+    };
     auto row_of = [&](int r, int64_t& token, int& head) {
         const int t = r / a.group;
         token = sr.first + t;
@@ -220,15 +302,15 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
             int64_t token;
             int head;
             row_of(r, token, head);
-            if (p.chunks > 1) {
-                float* st = p.stats + ((token * a.q_heads + head) * p.chunks + chunk) * 2;
+            if (!direct) {
+                float* st = p.stats + part_of(token, head, r) * 2;
                 st[0] = -INFINITY;
                 st[1] = 0.f;
             } else if (a.lse) {
                 a.lse[token * a.q_heads + head] = -INFINITY;
             }
         }
-        if (p.chunks == 1)
+        if (direct)
             for (int e = tid; e < rows * dim; e += G::THREADS) {
                 int64_t token;
                 int head;
@@ -328,8 +410,14 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
         }
         const float row_scale = up * a.scale_log2;
         const bool ordinary = a.scale_log2 >= 0.f;  // the largest product is the largest score
-        int64_t row_lo, row_hi;
-        seen_range(a, pos0 + (mine ? r / a.group : 0), len, row_lo, row_hi);
+        int64_t row_lo, row_hi, row_sinks = 0;
+        if constexpr (MODE == kPlain) {
+            seen_range(a, pos0 + (mine ? r / a.group : 0), len, row_lo, row_hi);
+        } else {
+            row_lo = axis.place(row_span.lo);
+            row_hi = axis.place(row_span.hi);
+            row_sinks = row_span.sinks - axis.first;
+        }
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_addr = tmem + G::S0 + h * 128 + lanes, o_addr = tmem + G::O0 + h * 128 + lanes;
         float m = -INFINITY, l = 0.f;
@@ -339,7 +427,8 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                 ok = wait(&scale_full[j % G::SLOTS], (uint32_t)((j / G::SLOTS) & 1));
                 // what the tile needs besides its scores, before they are there
                 const int64_t tok0 = base + (int64_t)j * G::N;
-                const bool inside = tok0 >= lo_max && tok0 + G::N <= hi_min;
+                bool inside = tok0 >= lo_max && tok0 + G::N <= hi_min;
+                if (MODE != kPlain) inside = inside || tok0 + G::N <= sinks_all;
                 const BlockScale* bs = scale_s + (j % G::SLOTS) * G::GROUPS;
                 const bool plain = inside && ordinary && tile_kind[j % G::SLOTS] == 0;
                 ok = ok && wait(&s_full[h], (uint32_t)(j & 1));
@@ -370,7 +459,7 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                     }
                 } else {
                     // exponents in the scores' place, -inf where the row does not see the token
-                    const int64_t lo = row_lo - tok0, hi = row_hi - tok0;
+                    const int64_t lo = row_lo - tok0, hi = row_hi - tok0, sinks = row_sinks - tok0;
 #pragma unroll
                     for (int g = 0; g < G::GROUPS; ++g) {
                         const BlockScale b = bs[g];
@@ -378,8 +467,9 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                         const float f = b.key * row_scale;
 #pragma unroll
                         for (int k = g * 16; k < g * 16 + 16; ++k) {
-                            const float z = !dead && k >= lo && k < hi ? fmaf(__uint_as_float(s[k]), f, b.log2_value)
-                                                                       : -INFINITY;
+                            bool seen = k >= lo && k < hi;
+                            if (MODE != kPlain) seen = seen || k < sinks;
+                            const float z = !dead && seen ? fmaf(__uint_as_float(s[k]), f, b.log2_value) : -INFINITY;
                             top = fmaxf(top, z);
                             s[k] = __float_as_uint(z);
                         }
@@ -470,7 +560,7 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 const bool small = *small_s;
                 if (small) m += SmallScales::shift;
-                const int64_t at = ((token * a.q_heads + head) * p.chunks + chunk);
+                const int64_t at = part_of(token, head, r);
                 T* y = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
 #pragma unroll
                 for (int c = 0; c < DP / 32; ++c) {
@@ -485,7 +575,7 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                     for (int k = 0; k < 32; k += 8) {
                         const int d = c * 32 + k;
                         if (d >= dim) continue;
-                        if (p.chunks > 1) {
+                        if (!direct) {
 #pragma unroll
                             for (int x = 0; x < 8; x += 4)
                                 *reinterpret_cast<uint4*>(p.parts + at * dim + d + x) =
@@ -504,7 +594,7 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                     }
                 }
                 if (mine) {
-                    if (p.chunks > 1) {
+                    if (!direct) {
                         p.stats[at * 2] = m;
                         p.stats[at * 2 + 1] = l;
                     } else if (a.lse) {
@@ -542,12 +632,15 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                 // codes that no row sees may be anything: as values they become zeros (0 times NaN is NaN)
                 const int64_t tok0 = base + (int64_t)j * G::N;
                 const BlockScale* bs = scale_s + (j % G::SLOTS) * G::GROUPS;
-                const bool whole = tok0 >= lo_min && tok0 + G::N <= hi_max;
+                bool whole = tok0 >= lo_min && tok0 + G::N <= hi_max;
+                if (MODE != kPlain) whole = whole || tok0 + G::N <= axis.sinks_any;
 #pragma unroll
                 for (int k = 0; k < PER; ++k) {
                     const int row = row0 + k * STEP;
                     bool keep = bs[row >> 4].kind != kDeadBlock;
-                    if (!whole) keep = keep && tok0 + row >= lo_min && tok0 + row < hi_max;
+                    bool seen = tok0 + row >= lo_min && tok0 + row < hi_max;
+                    if (MODE != kPlain) seen = seen || tok0 + row < axis.sinks_any;
+                    if (!whole) keep = keep && seen;
                     if (!keep) w[k] = make_uint4(0, 0, 0, 0);
                 }
             }
@@ -572,10 +665,11 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::OTHER_REGS));
         if (warp == 12) {
         // ------------------------------------------------------------ loads
-        const int unit = 1 << lg, blocks = G::N / unit, per = unit / 16;  // tokens of a copy, copies of a tile
+        // tokens of a copy, copies of a tile: the axis's tiles start anywhere in a page but in kPlain
+        const int unit = MODE == kPlain ? 1 << lg : 16, blocks = G::N / unit, per = unit / 16;
         auto page_at = [&](int64_t tok) -> int {
-            if (tok >= end || tok + 15 < lo_min) return -1;
-            const int64_t id = a.seq.block_table[sr.s * a.seq.table_stride + (tok >> lg)];
+            if (tok >= end || (MODE == kPlain && tok + 15 < lo_min)) return -1;
+            const int64_t id = a.seq.block_table[sr.s * a.seq.table_stride + (token_at(tok) >> lg)];
             return id >= 0 && id < a.cache.pages ? (int)id : -1;
         };
         // lanes 0..7: the 16-token groups of a tile; page numbers three tiles ahead of the copies, scales two
@@ -595,7 +689,7 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
             const unsigned mask = ((1u << per) - 1u) << ((lane * per) & 31);
             const bool copy = lane < blocks && (groups & mask);
             const int page = __shfl_sync(0xffffffffu, id, copy ? __ffs(groups & mask) - 1 : 0);
-            const int64_t tok = base + (int64_t)j * G::N + lane * unit;
+            const int64_t tok = token_at(base + (int64_t)j * G::N + lane * unit);
             src = ((((int64_t)page * a.cache.kv_heads + kv) << lg) + (tok & (((int64_t)1 << lg) - 1))) * dim;
             return __ballot_sync(0xffffffffu, copy);
         };
@@ -644,11 +738,19 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                 wait(&raw_full[b % G::RAW_RING], (uint32_t)((b / G::RAW_RING) & 1));
     } else if (warp >= 14) {
         // ------------------------------------------------------------ value scales of the blocks that are seen
-        const int64_t seen = base > lo_min ? base : lo_min;
         bool small = false;
-        for (int64_t b = (seen >> lg) + (tid - 448); b <= (end - 1) >> lg; b += 64) {
-            const int64_t id = a.seq.block_table[sr.s * a.seq.table_stride + b];
-            if (id >= 0 && id < a.cache.pages) small |= small_scale(block_scale(0.f, a.cache.v_scale[id * a.cache.kv_heads + kv]));
+        auto look = [&](int64_t from, int64_t to) {  // tokens [from, to)
+            for (int64_t b = (from >> lg) + (tid - 448); b <= (to - 1) >> lg; b += 64) {
+                const int64_t id = a.seq.block_table[sr.s * a.seq.table_stride + b];
+                if (id >= 0 && id < a.cache.pages)
+                    small |= small_scale(block_scale(0.f, a.cache.v_scale[id * a.cache.kv_heads + kv]));
+            }
+        };
+        if constexpr (MODE == kPlain) {
+            look(base > lo_min ? base : lo_min, end);
+        } else {
+            if (base < axis.head) look(axis.first + base, axis.first + (end < axis.head ? end : axis.head));
+            if (end > axis.head) look(token_at(base > axis.head ? base : axis.head), token_at(end - 1) + 1);
         }
         if (small) *small_s = 1;
         __threadfence_block();

@@ -39,6 +39,8 @@ struct Entries {
     decltype(&bfft_last_error) last_error;
     decltype(&bfft_rotate_axes) rotate_axes;
     decltype(&bfft_cache_append_axes) append_axes;
+    decltype(&bfft_cache_attention_span_workspace) span_workspace;
+    decltype(&bfft_cache_attention_span) span_attention;
 } g_entry{};
 
 std::string text(const char* s) { return s; }
@@ -526,10 +528,10 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// attention(q, cache, block_table, lens, starts, softmax_scale, causal, window, return_lse, out)
+// attention(q, cache, block_table, lens, starts, softmax_scale, causal, window, return_lse, out, sinks, shared, groups)
 PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 10, "attention takes 10 arguments");
+    TORCH_CHECK(n == 13, "attention takes 13 arguments");
     const Tensor& q = tensor(args[0], "q");
     const Cache c = cache_of(args[1]);
     bfft_attention_desc d{};
@@ -550,6 +552,30 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (causal < 0 || want_lse < 0) throw python_error();
     d.causal = causal;
     d.window = integer(args[7], "window", 0);
+    bfft_span_desc span{};
+    span.sinks = integer(args[10], "sinks", 0);
+    if (args[11] != Py_None) {
+        const Tensor& shared = tensor(args[11], "shared");
+        of_type(shared, "shared", at::kInt);
+        on_device(shared, "shared", c.device);
+        if (shared.dim() != 1 || !shared.is_contiguous())
+            value_error("shared must be contiguous (groups,), got ", shape_of(shared));
+        span.n_groups = shared.size(0);
+        span.shared = shared.data_ptr();
+        if (args[12] != Py_None) {
+            const Tensor& groups = tensor(args[12], "groups");
+            of_type(groups, "groups", at::kInt);
+            on_device(groups, "groups", c.device);
+            if (groups.dim() != 1 || groups.size(0) != span.n_groups + 1 || !groups.is_contiguous())
+                value_error("groups must be contiguous (", span.n_groups + 1, ",), got ", shape_of(groups));
+            span.groups = groups.data_ptr();
+        } else if (span.n_groups != 1) {
+            value_error("shared must be (1,) where no groups are given, got ", shape_of(shared));
+        }
+    } else if (args[12] != Py_None) {
+        value_error("groups without shared");
+    }
+    const bool spans = span.sinks || span.n_groups;
     Tensor out, lse, scratch;
     if (args[9] != Py_None) {
         out = tensor(args[9], "out");
@@ -572,26 +598,30 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         d.o_head = out.stride(1);
         d.device = c.device;
         size_t bytes = 0;
-        check(g_entry.workspace(&c.desc, &s, &d, &bytes), "cache_attention");
+        check(spans ? g_entry.span_workspace(&c.desc, &s, &d, &span, &bytes) : g_entry.workspace(&c.desc, &s, &d, &bytes),
+              "cache_attention");
         if (bytes) {
             scratch = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte).requires_grad(false));
             d.workspace = scratch.data_ptr();
             d.workspace_bytes = (int64_t)bytes;
         }
         if (args[9] != Py_None) written(out);
-        check(g_entry.attention(&c.desc, &s, &d, stream_of(c.device)), "cache_attention");
+        check(spans ? g_entry.span_attention(&c.desc, &s, &d, &span, stream_of(c.device))
+                    : g_entry.attention(&c.desc, &s, &d, stream_of(c.device)),
+              "cache_attention");
     }
     if (want_lse) return pair(out, lse);
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }
 
-// bind(addresses of rotate, append, read, workspace, attention, last_error, rotate_axes, append_axes)
+// bind(addresses of rotate, append, read, workspace, attention, last_error, rotate_axes, append_axes, span_workspace,
+// span_attention)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 8, "bind takes 8 addresses");
-    void* p[8];
-    for (int i = 0; i < 8; ++i) {
+    TORCH_CHECK(n == 10, "bind takes 10 addresses");
+    void* p[10];
+    for (int i = 0; i < 10; ++i) {
         p[i] = PyLong_AsVoidPtr(args[i]);
         if (!p[i]) value_error("null entry point");
     }
@@ -603,6 +633,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     g_entry.last_error = reinterpret_cast<decltype(g_entry.last_error)>(p[5]);
     g_entry.rotate_axes = reinterpret_cast<decltype(g_entry.rotate_axes)>(p[6]);
     g_entry.append_axes = reinterpret_cast<decltype(g_entry.append_axes)>(p[7]);
+    g_entry.span_workspace = reinterpret_cast<decltype(g_entry.span_workspace)>(p[8]);
+    g_entry.span_attention = reinterpret_cast<decltype(g_entry.span_attention)>(p[9]);
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
