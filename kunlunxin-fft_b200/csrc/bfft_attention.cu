@@ -231,7 +231,7 @@ GroupPlan plan_groups(const bfft_cache_desc* c, const bfft_sequence_desc* q, con
         x.least = least;
         x.unit = unit;
         // every row tile may end with a piece that is not full
-        x.most = x.target + ((prefixes ? q->tokens / tile + w->n_groups : 0) + (own ? q->tokens / tile + q->seqs : 0)) * parts;
+        x.most = x.target + 2 + ((prefixes ? q->tokens / tile + w->n_groups : 0) + (own ? q->tokens / tile + q->seqs : 0)) * parts;
         return x;
     };
     p.split_items = items(!p.prefix_tiles, !p.own_tiles, s.tile_tokens, s.token_tiles, 2 * 3 * (int64_t)sms, 256, 32);

@@ -121,164 +121,169 @@ __device__ __forceinline__ int sequence_shared(const AttentionArgs& a, const Spa
     }
     return p.groups[lo] <= s && s < p.groups[lo + 1] ? shared_tokens(a, p, lo) : 0;
 }
-// Rows of sequences [s0, s1).
-__device__ __forceinline__ void rows_of(const AttentionArgs& a, int s0, int s1, int64_t& t0, int64_t& t1) {
+// Rows [t0, t0 + n) of sequences [s0, s1).
+__device__ __forceinline__ int rows_of(const AttentionArgs& a, int s0, int s1, int& t0) {
     t0 = a.seq.starts[s0];
-    t1 = a.seq.starts[s1];
-    if (t1 > a.seq.tokens) t1 = a.seq.tokens;
-    if (t0 < 0 || t1 < t0) t1 = t0 = 0;
+    int t1 = a.seq.starts[s1];
+    if (t1 > a.seq.tokens) t1 = (int)a.seq.tokens;
+    if (t0 < 0) t0 = t1;
+    return t1 > t0 ? t1 - t0 : 0;
+}
+
+// A group's or a sequence's row tiles (times parts), and the tokens that each walks.
+struct Unit {
+    int s0, s1, t0, rows, len;
+    int shared;     // tokens that it is about (a group), or that come before them
+    int tiles, length;
+};
+__device__ __forceinline__ Unit unit_of(const AttentionArgs& a, const SpanArgs& p, const ItemArgs& x, int u, int tile,
+                                        int parts) {
+    Unit v;
+    const int groups = x.prefixes ? p.n_groups : 0;
+    const bool prefix = u < groups;
+    if (prefix) {
+        group_sequences(a, p, u, v.s0, v.s1);
+        v.len = 0;
+        v.shared = shared_tokens(a, p, u);
+    } else {
+        v.s0 = u - groups;
+        v.s1 = v.s0 + 1;
+        v.len = a.seq.lens[v.s0];
+        v.shared = sequence_shared(a, p, v.s0);
+    }
+    v.rows = rows_of(a, v.s0, v.s1, v.t0);
+    v.tiles = (int)((unsigned)(v.rows + tile - 1) / (unsigned)tile) * parts;
+    // tokens up to the end, from the first that the first row (causal: the last row tile's) sees
+    const int most = a.seq.max_pages << a.cache.page_log2;  // 2^30 at most
+    const int end = prefix ? v.shared : min(v.len, most), first = prefix ? 0 : v.shared;
+    int lo = first, sinks = 0;
+    if (a.window > 0) {
+        const int window = min(a.window, 1 << 30);
+        lo = max(first, prefix ? end - window : v.len - (a.causal ? min(v.rows, tile) : v.rows) - window + 1);
+        sinks = max(min(p.sinks, lo) - first, 0);
+    }
+    v.length = max(end - lo + sinks, 0);
+    if (prefix && !v.length) v.tiles = 0;
+    return v;
 }
 
 // A row tile's piece of the axis.
 struct Item {
     int table_row;          // of the block table
     int s0, s1;             // sequences that its rows are of
-    int64_t token;          // its first row
-    int n;                  // query tokens
+    int token, n;           // its first row, query tokens
     int part;               // of a token's heads
     int chunk, chunks;
     int from, to;           // tokens that it is about
-    bool prefix, shares;
+    int pos, len;           // of a sequence: its first row's place, its tokens
+    int prefix, shares;
 };
 
 struct ItemScratch {
-    long long sum[32];
-    int chunk, found, rest, chunks;
+    float weight[32];
+    int sum[2][32];
+    int found;
+    Item item;
 };
 
-// Row tiles (times parts) of unit u, groups before sequences, and tokens along the axis.
-__device__ __forceinline__ void unit_shape(const AttentionArgs& a, const SpanArgs& p, const ItemArgs& x, int u, int tile,
-                                           int parts, int64_t& tiles, int64_t& length) {
-    const int groups = x.prefixes ? p.n_groups : 0;
-    int64_t t0, t1;
-    if (u < groups) {
-        int s0, s1;
-        group_sequences(a, p, u, s0, s1);
-        rows_of(a, s0, s1, t0, t1);
-        length = shared_tokens(a, p, u);
-        if (a.window > 0 && length > (int64_t)a.window + p.sinks) length = (int64_t)a.window + p.sinks;
-        tiles = length ? (t1 - t0 + tile - 1) / tile * parts : 0;
-        return;
-    }
-    const int s = u - groups;
-    rows_of(a, s, s + 1, t0, t1);
-    const int64_t n = t1 - t0, len = a.seq.lens[s];
-    const int first = sequence_shared(a, p, s);
-    // the longest of the first and the last row tile
-    length = 0;
-    for (int k = 0; k < 2; ++k) {
-        const int64_t at = k ? (n > tile ? n - tile : 0) : 0, end = k ? n : (n < tile ? n : tile);
-        const TokenSpan lo = token_span(a, p, len - n + at, len, first, 0x7fffffff);
-        const TokenSpan hi = token_span(a, p, len - n + end - 1, len, first, 0x7fffffff);
-        const int64_t m = (int64_t)(hi.hi - lo.lo) + (hi.sinks < lo.lo ? hi.sinks - first : 0);
-        if (m > length) length = m;
-    }
-    tiles = (n + tile - 1) / tile * parts;
-}
-
-// Tokens of a piece for items of x.target: what the rows' tokens come to, shared out.
-__device__ __forceinline__ int64_t item_chunk(const ItemArgs& x, long long total) {
-    int64_t c = (total + x.target - 1) / x.target;
-    c = (c + x.unit - 1) / x.unit * x.unit;
-    return c > x.least ? c : x.least;
-}
-
-// Finds item i by itself, block-wide: every block makes the same sums over the sequences'
-// tables, so the items need no list in memory and no launch that makes one.
+// Finds item i, block-wide: every block makes the same sums over the sequences' tables, so
+// the items need no list in memory and no launch that makes one.  Tokens of an item: those
+// that all row tiles walk, shared out over x.target items.  A block runs this once, from a cold
+// instruction cache: short code and 32-bit divisions are what counts.
 template <int THREADS>
-__device__ __forceinline__ bool find_item(const AttentionArgs& a, const SpanArgs& p, const ItemArgs& x, int64_t i, int tile,
+__device__ __forceinline__ bool find_item(const AttentionArgs& a, const SpanArgs& p, const ItemArgs& x, int i, int tile,
                                           int parts, ItemScratch& sh, Item& it) {
     constexpr int WARPS = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int groups = x.prefixes ? p.n_groups : 0, units = groups + (x.own ? a.seq.seqs : 0);
-    int64_t tiles = 0, length = 0;
-    long long total = 0;
-    for (int u = tid; u < units; u += THREADS) {
-        unit_shape(a, p, x, u, tile, parts, tiles, length);
-        total += tiles * length;
-    }
+    // units in rounds of a block's threads: once to sum them up and, where they take more
+    // than one round, once more to look for the item
+    const int rounds = (units + THREADS - 1) / THREADS, last = rounds > 1 ? 2 * rounds : 1;
+    float total = 0.f;
+    unsigned chunk = 1;
+    int before = 0;  // items of the units before this round's
+    if (tid == 0) sh.found = 0;
+#pragma unroll 1
+    for (int round = 0; round < last; ++round) {
+        const int u = (round < rounds ? round : round - rounds) * THREADS + tid;
+        Unit v{};
+        if (u < units) v = unit_of(a, p, x, u, tile, parts);
+        if (round < rounds) {
+            total += (float)v.tiles * (float)v.length;
+            if (round < rounds - 1) continue;
 #pragma unroll
-    for (int w = 16; w; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
-    if (lane == 0) sh.sum[warp] = total;
-    if (tid == 0) sh.found = -1;
-    __syncthreads();
-    total = 0;
+            for (int w = 16; w; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
+            if (lane == 0) sh.weight[warp] = total;
+            __syncthreads();
+            total = 0.f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) total += sh.sum[w];
-    const int64_t chunk = item_chunk(x, total);
-    long long before = 0;  // items of the units before this round's
-    for (int u0 = 0; u0 < units; u0 += THREADS) {
-        const int u = u0 + tid;
-        if (units > THREADS && u < units) unit_shape(a, p, x, u, tile, parts, tiles, length);
-        const long long pieces = u < units ? (length > chunk ? (length + chunk - 1) / chunk : 1) : 0;
-        const long long mine = u < units ? tiles * pieces : 0;
-        long long upto = mine;
+            for (int w = 0; w < WARPS; ++w) total += sh.weight[w];
+            // (the sum's rounding is far under the one token that is added)
+            const int share = (int)fminf(total / (float)x.target, 1.0e9f) + 1;
+            chunk = max((unsigned)(share + x.unit - 1) / (unsigned)x.unit * x.unit, (unsigned)x.least);
+            if (rounds > 1) continue;
+        }
+        const int pieces = (unsigned)v.length > chunk ? (int)(((unsigned)v.length + chunk - 1) / chunk) : 1;
+        const int mine = v.tiles * pieces;
+        int upto = mine;
 #pragma unroll
         for (int w = 1; w < 32; w <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, upto, w);
-            if (lane >= w) upto += v;
+            const int y = __shfl_up_sync(0xffffffffu, upto, w);
+            if (lane >= w) upto += y;
         }
+        if (lane == 31) sh.sum[round & 1][warp] = upto;
         __syncthreads();
-        if (lane == 31) sh.sum[warp] = upto;
-        __syncthreads();
-        long long all = 0, under = before;
+        int all = 0, under = before;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) under += sh.sum[w];
-            all += sh.sum[w];
+            if (w < warp) under += sh.sum[round & 1][w];
+            all += sh.sum[round & 1][w];
         }
-        const long long from = under + upto - mine;
-        if (i >= from && i < from + mine) {
-            sh.found = u;
-            sh.rest = (int)(i - from);
-            sh.chunks = (int)pieces;
+        const int rest = i - (under + upto - mine);
+        if (rest >= 0 && rest < mine) {
+            Item& f = sh.item;
+            const unsigned at = (unsigned)rest / (unsigned)pieces, t = at / (unsigned)parts;
+            f.prefix = u < groups;
+            f.table_row = f.s0 = v.s0;
+            f.s1 = v.s1;
+            f.chunks = pieces;
+            f.chunk = rest - (int)at * pieces;
+            f.part = (int)at - (int)t * parts;
+            f.token = v.t0 + (int)t * tile;
+            f.n = min(v.rows - (int)t * tile, tile);
+            f.from = f.prefix ? 0 : v.shared;
+            f.to = f.prefix ? v.shared : 0x7fffffff;
+            f.shares = v.shared > 0;
+            f.pos = v.len - v.rows + (int)t * tile;
+            f.len = v.len;
+            sh.found = 1;
         }
         before += all;
         if (i < before) break;
     }
     __syncthreads();
-    const int u = sh.found;
-    if (u < 0) return false;
-    it.prefix = u < groups;
-    if (it.prefix) {
-        group_sequences(a, p, u, it.s0, it.s1);
-        it.from = 0;
-        it.to = shared_tokens(a, p, u);
-        it.shares = true;
-    } else {
-        it.s0 = u - groups;
-        it.s1 = it.s0 + 1;
-        it.from = sequence_shared(a, p, it.s0);
-        it.to = 0x7fffffff;
-        it.shares = it.from > 0;
-    }
-    it.table_row = it.s0;
-    it.chunks = sh.chunks;
-    it.chunk = sh.rest % it.chunks;
-    const int at = sh.rest / it.chunks;
-    it.part = at % parts;
-    int64_t t0, t1;
-    rows_of(a, it.s0, it.s1, t0, t1);
-    it.token = t0 + (int64_t)(at / parts) * tile;
-    it.n = (int)(t1 - it.token < tile ? t1 - it.token : tile);
+    if (!sh.found) return false;
+    it = sh.item;
     return true;
 }
 
-// What row `token` sees of the item's tokens.
-__device__ __forceinline__ TokenSpan item_span(const AttentionArgs& a, const SpanArgs& p, const Item& it, int64_t token) {
-    int lo = it.s0, n = it.s1 - it.s0;
-    while (n > 1) {  // the largest s with starts[s] <= token
-        const int half = n >> 1;
-        if (a.seq.starts[lo + half] <= token) {
-            lo += half;
-            n -= half;
-        } else {
-            n = half;
+// What the item's rows see of its tokens, a query token each, in shared memory; `spans` holds
+// empty ones before (no_spans).  A group's rows are found from its sequences, a thread each:
+// each row's own search of its sequence took 3900 clocks.
+template <int THREADS>
+__device__ __forceinline__ void item_spans(const AttentionArgs& a, const SpanArgs& p, const Item& it, TokenSpan* spans) {
+    if (!it.prefix) {
+        for (int t = threadIdx.x; t < it.n; t += THREADS)
+            spans[t] = token_span(a, p, (int64_t)it.pos + t, it.len, it.from, it.to);
+    } else {
+        for (int s = it.s0 + (int)threadIdx.x; s < it.s1; s += THREADS) {
+            int t0;
+            const int n = rows_of(a, s, s + 1, t0), len = a.seq.lens[s];
+            for (int t = max(t0, it.token); t < min(t0 + n, it.token + it.n); ++t)
+                spans[t - it.token] = token_span(a, p, (int64_t)len - n + (t - t0), len, it.from, it.to);
         }
     }
-    int64_t t0, t1;
-    rows_of(a, lo, lo + 1, t0, t1);
-    return token_span(a, p, (int64_t)a.seq.lens[lo] - (t1 - t0) + (token - t0), a.seq.lens[lo], it.from, it.to);
+    __syncthreads();
 }
 
 }  // namespace bfft

@@ -282,11 +282,16 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     int chunk = 0, kv, part;
     SlotRows sr;
     Item it{};
+    TokenSpan mine_span{0, 0, 0};  // kSinks, kGroups: of query token `lane` of the tile
     if constexpr (MODE == kGroups) {
         __shared__ ItemScratch scratch;
-        kv = (int)(i % a.cache.kv_heads);
-        if (!find_item<kSplitThreads>(a, p.span, p.items, i / a.cache.kv_heads, p.tile_tokens, p.token_tiles, scratch, it))
-            return;
+        __shared__ TokenSpan spans[16];
+        if (tid < 16) spans[tid] = TokenSpan{0, 0, 0};
+        const unsigned item = blockIdx.x / (unsigned)a.cache.kv_heads;
+        kv = (int)(blockIdx.x - item * a.cache.kv_heads);
+        if (!find_item<kSplitThreads>(a, p.span, p.items, (int)item, p.tile_tokens, p.token_tiles, scratch, it)) return;
+        item_spans<kSplitThreads>(a, p.span, it, spans);
+        if (lane < it.n) mine_span = spans[lane];
         part = it.part;
         chunk = it.chunk;
         sr.s = it.table_row;
@@ -311,7 +316,6 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     // [base, end) of the axis: kPlain counts sequence tokens, the others places of `axis`
     int64_t len = 0, pos0 = 0, base, end, lo_min = 0, hi_max, lo_max = 0, hi_min;
     Axis axis{};
-    TokenSpan mine_span{0, 0, 0};  // kSinks, kGroups: of query token `lane` of the tile
     if constexpr (MODE == kPlain) {
         len = a.seq.lens[sr.s];
         const int64_t most = (int64_t)a.seq.max_pages << a.cache.page_log2;
@@ -325,15 +329,10 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     } else {
         int first = 0;
         if (MODE == kGroups) first = it.from;
-        if (lane < sr.n) {
-            if constexpr (MODE == kGroups)
-                mine_span = item_span(a, p.span, it, sr.first + lane);
-            else
-                mine_span = token_span(a, p.span, (int64_t)a.seq.lens[sr.s] - sr.rows + sr.place + lane, a.seq.lens[sr.s],
-                                       0, 0x7fffffff);
-        } else {
-            mine_span.sinks = first;
-        }
+        if (MODE == kSinks && lane < sr.n)
+            mine_span = token_span(a, p.span, (int64_t)a.seq.lens[sr.s] - sr.rows + sr.place + lane, a.seq.lens[sr.s], 0,
+                                   0x7fffffff);
+        if (lane >= sr.n) mine_span.sinks = first;
         const bool some = mine_span.lo < mine_span.hi;
         axis = make_axis(first, __reduce_min_sync(0xffffffffu, some ? mine_span.lo : 0x7fffffff),
                          __reduce_max_sync(0xffffffffu, some ? mine_span.hi : 0),
@@ -442,7 +441,7 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
                 scales[e] = block_scale(a.cache.k_scale[b], a.cache.v_scale[b]);
                 small |= small_scale(scales[e]);
             } else {
-                scales[e].kind = kDeadBlock;
+                scales[e] = BlockScale{0.f, 0.f, 0.f, kDeadBlock};
             }
         }
         return small;
@@ -508,14 +507,34 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
             x = static_cast<const T*>(a.q) + token * a.qt + head * a.qh;
         }
         float e[G::KS][4];
+        if (a.q_packs) {  // 16 adjacent elements of this lane's columns, by two loads
+#pragma unroll
+            for (int c = 0; c < G::KS / 4; ++c) {
+                const int d = 16 * (4 * c + q4);
+                Pack<T, 8> w[2];
+                if (x && (EXACT || d < dim)) {
+                    w[0] = *reinterpret_cast<const Pack<T, 8>*>(x + d);
+                    w[1] = *reinterpret_cast<const Pack<T, 8>*>(x + d + 8);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[0].v[j] = w[1].v[j] = from_f32<T>(0.f);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) e[4 * c + j / 4][j & 3] = to_f32(w[j >> 3].v[j & 7]);
+            }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < G::KS; ++ks)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int d = 16 * (4 * (ks >> 2) + q4) + 4 * (ks & 3) + j;
+                    e[ks][j] = x && (EXACT || d < dim) ? to_f32(x[d]) : 0.f;
+                }
+        }
 #pragma unroll
         for (int ks = 0; ks < G::KS; ++ks)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int d = 16 * (4 * (ks >> 2) + q4) + 4 * (ks & 3) + j;
-                e[ks][j] = x && (EXACT || d < dim) ? to_f32(x[d]) : 0.f;
-                big = fmaxf(big, fabsf(e[ks][j]));
-            }
+            for (int j = 0; j < 4; ++j) big = fmaxf(big, fabsf(e[ks][j]));
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
         float down, up;
@@ -579,56 +598,84 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
         }
         const int tok0 = seg + t * 32;
         const unsigned char* buf = mine + stage * 4 * G::half_bytes(dim);
+        // Both halves' tokens go through each step side by side, dead ones too (their scores
+        // become -inf, their codes zeros): twice the products in flight, and no branches
+        // between them.
         float z[2][NT][4];
         BlockScale bs[2];
-        bool live[2];
-        float worst = -INFINITY;  // largest z - m of this lane
+        bool live[2], inside = true, whole = true;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int tok = tok0 + 16 * h;
             const int e = entry_of(tok);
             bs[h] = scales[e < entries ? e : entries - 1];
             live[h] = tok < stop && bs[h].kind != kDeadBlock;
-            if (!live[h]) continue;
-            const unsigned char* kb = buf + h * G::half_bytes(dim);
+            bool in = tok >= lo_all && tok + 16 <= hi_all;  // kPlain: hi_all is at most span
+            if (MODE != kPlain) in = (in && tok + 16 <= stop) || tok + 16 <= sinks_all;
+            inside = inside && in && live[h];
+            in = tok >= lo_any && tok + 16 <= stop;
+            if (MODE != kPlain) in = (in && tok + 16 <= axis.hi_any) || tok + 16 <= axis.sinks_any;
+            whole = whole && in && live[h];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) z[h][nt][0] = z[h][nt][1] = z[h][nt][2] = z[h][nt][3] = 0.f;
+        }
 #pragma unroll
-            for (int c = 0; c < (DP + 63) / 64; ++c) {
-                uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
-                const int col = 16 * (4 * c + q4);
+        for (int c = 0; c < (DP + 63) / 64; ++c) {
+            uint4 w[2][2];
+            const int col = 16 * (4 * c + q4);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const unsigned char* kb = buf + h * G::half_bytes(dim);
+                w[h][0] = w[h][1] = make_uint4(0, 0, 0, 0);
                 if (EXACT || col < dim) {
-                    w0 = *reinterpret_cast<const uint4*>(kb + at(tk * dim + col));
-                    w1 = *reinterpret_cast<const uint4*>(kb + at((tk + 8) * dim + col));
+                    w[h][0] = *reinterpret_cast<const uint4*>(kb + at(tk * dim + col));
+                    w[h][1] = *reinterpret_cast<const uint4*>(kb + at((tk + 8) * dim + col));
                 }
-                const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
+            }
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t u0 = s == 0 ? w[h][0].x : s == 1 ? w[h][0].y : s == 2 ? w[h][0].z : w[h][0].w;
+                    const uint32_t u1 = s == 0 ? w[h][1].x : s == 1 ? w[h][1].y : s == 2 ? w[h][1].z : w[h][1].w;
                     uint32_t a0, a1, a2, a3;
-                    widen<CODE>(u0[s], a0, a2);
-                    widen<CODE>(u1[s], a1, a3);
+                    widen<CODE>(u0, a0, a2);
+                    widen<CODE>(u1, a1, a3);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
                         mma_f16(z[h][nt], a0, a1, a2, a3, qf[nt][c * 4 + s][0], qf[nt][c * 4 + s][1]);
                 }
-            }
-            bool inside = tok >= lo_all && tok + 16 <= hi_all;  // kPlain: hi_all is at most span
-            if (MODE != kPlain) inside = (inside && tok + 16 <= stop) || tok + 16 <= sinks_all;
+        }
+        float worst = -INFINITY;  // largest z - m of this lane
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    z[h][nt][c] = z[h][nt][c] * (bs[h].key * row_scale[nt][c & 1]) + bs[h].log2_value;
+        if (!inside) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int j = tok0 + 16 * h + tk + (c >> 1) * 8;
+                        bool hidden = j < row_lo[nt][c & 1] || j >= row_hi[nt][c & 1];
+                        if (MODE != kPlain) hidden = hidden && j >= row_sinks[nt][c & 1];
+                        if (hidden || !live[h]) z[h][nt][c] = -INFINITY;
+                    }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    float v = z[h][nt][c] * (bs[h].key * row_scale[nt][c & 1]) + bs[h].log2_value;
-                    if (!inside) {
-                        const int j = tok + tk + (c >> 1) * 8;
-                        bool hidden = j < row_lo[nt][c & 1] || j >= row_hi[nt][c & 1];
-                        if (MODE != kPlain) hidden = hidden && j >= row_sinks[nt][c & 1];
-                        if (hidden) v = -INFINITY;
-                    }
-                    z[h][nt][c] = v;
+                    const float v = z[h][nt][c];
                     worst = fmaxf(worst, v == -INFINITY ? v : v - m[nt][c & 1]);
                 }
-        }
         if (__any_sync(0xffffffffu, worst > kRenew)) {  // a score far over a reference (or the first one): renew them
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -636,8 +683,7 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
                 for (int j = 0; j < 2; ++j) {
                     float top = -INFINITY;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        if (live[h]) top = fmaxf(top, fmaxf(z[h][nt][j], z[h][nt][2 + j]));
+                    for (int h = 0; h < 2; ++h) top = fmaxf(top, fmaxf(z[h][nt][j], z[h][nt][2 + j]));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -652,26 +698,72 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
                     }
                 }
         }
+        // values: tokens t0, t1, t0 + 8, t1 + 8 of this lane, dims 4 w .. 4 w + 3 of its columns
+        const int t0 = row_token(2 * q4), t1 = row_token(2 * q4 + 1);
+        const int toks[4] = {t0, t1, t0 + 8, t1 + 8};
+        uint32_t w[2][4][G::VW];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            if (!live[h]) continue;
-            const int tok = tok0 + 16 * h;
-            uint32_t pf[NT][2];
+            const unsigned char* vb = buf + (2 + h) * G::half_bytes(dim);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-                float e0 = exp2_approx(z[h][nt][0] - m0), e1 = exp2_approx(z[h][nt][1] - m1);
-                float e2 = exp2_approx(z[h][nt][2] - m0), e3 = exp2_approx(z[h][nt][3] - m1);
-                l[nt][0] += (e0 + e2) * bs[h].inv_value;
-                l[nt][1] += (e1 + e3) * bs[h].inv_value;
-                if (bs[h].kind) {
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (DP == 64) {
+                    uint2 x = make_uint2(0, 0);
+                    if (EXACT || 8 * g < dim) x = *reinterpret_cast<const uint2*>(vb + at(toks[k] * dim + 8 * g));
+                    w[h][k][0] = x.x;
+                    w[h][k][1] = x.y;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < DP / 128; ++c) {
+                        uint4 x = make_uint4(0, 0, 0, 0);
+                        const int col = 16 * g + 128 * c;
+                        if (EXACT || col < dim) x = *reinterpret_cast<const uint4*>(vb + at(toks[k] * dim + col));
+                        w[h][k][4 * c] = x.x;
+                        w[h][k][4 * c + 1] = x.y;
+                        w[h][k][4 * c + 2] = x.z;
+                        w[h][k][4 * c + 3] = x.w;
+                    }
+                }
+            }
+        }
+        if (!whole) {  // codes of slots that no row sees may be anything: 0 times NaN is NaN
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int j = tok0 + 16 * h + toks[k];
+                    bool drop = j < lo_any || j >= stop;
+                    if (MODE != kPlain) drop = (j < lo_any || j >= axis.hi_any) && j >= axis.sinks_any;
+                    if (drop || !live[h])
+#pragma unroll
+                        for (int c = 0; c < G::VW; ++c) w[h][k][c] = 0;
+                }
+        }
+        float e[2][NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) e[h][nt][c] = exp2_approx(z[h][nt][c] - (c & 1 ? m1 : m0));
+                l[nt][0] += (e[h][nt][0] + e[h][nt][2]) * bs[h].inv_value;
+                l[nt][1] += (e[h][nt][1] + e[h][nt][3]) * bs[h].inv_value;
+            }
+        }
+        if (bs[0].kind | bs[1].kind) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (!bs[h].kind) continue;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
                     if (bs[h].kind == 2) {  // values that are not finite spoil the rows that see one of them
                         int seen0 = z[h][nt][0] != -INFINITY || z[h][nt][2] != -INFINITY;
                         int seen1 = z[h][nt][1] != -INFINITY || z[h][nt][3] != -INFINITY;
 #pragma unroll
-                        for (int w = 4; w < 32; w <<= 1) {
-                            seen0 |= __shfl_xor_sync(0xffffffffu, seen0, w);
-                            seen1 |= __shfl_xor_sync(0xffffffffu, seen1, w);
+                        for (int d = 4; d < 32; d <<= 1) {
+                            seen0 |= __shfl_xor_sync(0xffffffffu, seen0, d);
+                            seen1 |= __shfl_xor_sync(0xffffffffu, seen1, d);
                         }
 #pragma unroll
                         for (int u = 0; u < 2 * G::VW; ++u) {
@@ -679,58 +771,31 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
                             if (seen1) o[nt][u][1] = o[nt][u][3] = __int_as_float(0x7fffffff);
                         }
                     }
-                    e0 = e1 = e2 = e3 = 0.f;
-                }
-                pf[nt][0] = movmatrix_trans(pack_f16(e0, e1));
-                pf[nt][1] = movmatrix_trans(pack_f16(e2, e3));
-            }
-            // values: tokens t0, t1, t0 + 8, t1 + 8 of this lane, dims 4 w .. 4 w + 3 of its columns
-            const unsigned char* vb = buf + (2 + h) * G::half_bytes(dim);
-            const int t0 = row_token(2 * q4), t1 = row_token(2 * q4 + 1);
-            const int toks[4] = {t0, t1, t0 + 8, t1 + 8};
-            uint32_t w[4][G::VW];
-            bool whole = tok >= lo_any && tok + 16 <= stop;
-            if (MODE != kPlain) whole = (whole && tok + 16 <= axis.hi_any) || tok + 16 <= axis.sinks_any;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if constexpr (DP == 64) {
-                    uint2 x = make_uint2(0, 0);
-                    if (EXACT || 8 * g < dim) x = *reinterpret_cast<const uint2*>(vb + at(toks[k] * dim + 8 * g));
-                    w[k][0] = x.x;
-                    w[k][1] = x.y;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < DP / 128; ++c) {
-                        uint4 x = make_uint4(0, 0, 0, 0);
-                        const int col = 16 * g + 128 * c;
-                        if (EXACT || col < dim) x = *reinterpret_cast<const uint4*>(vb + at(toks[k] * dim + col));
-                        w[k][4 * c] = x.x;
-                        w[k][4 * c + 1] = x.y;
-                        w[k][4 * c + 2] = x.z;
-                        w[k][4 * c + 3] = x.w;
-                    }
-                }
-                if (!whole) {  // codes of slots that no row sees may be anything: 0 times NaN is NaN
-                    const int j = tok + toks[k];
-                    bool drop = j < lo_any || j >= stop;
-                    if (MODE != kPlain) drop = (j < lo_any || j >= axis.hi_any) && j >= axis.sinks_any;
-                    if (drop)
-#pragma unroll
-                        for (int c = 0; c < G::VW; ++c) w[k][c] = 0;
+                    e[h][nt][0] = e[h][nt][1] = e[h][nt][2] = e[h][nt][3] = 0.f;
                 }
             }
+        }
+        uint32_t pf[2][NT][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                pf[h][nt][0] = movmatrix_trans(pack_f16(e[h][nt][0], e[h][nt][1]));
+                pf[h][nt][1] = movmatrix_trans(pack_f16(e[h][nt][2], e[h][nt][3]));
+            }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int c = 0; c < G::VW; ++c)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     const uint32_t sel = s ? 0x7362 : 0x5140;
                     uint32_t a0, a1, a2, a3;
-                    widen<CODE>(__byte_perm(w[0][c], w[1][c], sel), a0, a1);
-                    widen<CODE>(__byte_perm(w[2][c], w[3][c], sel), a2, a3);
+                    widen<CODE>(__byte_perm(w[h][0][c], w[h][1][c], sel), a0, a1);
+                    widen<CODE>(__byte_perm(w[h][2][c], w[h][3][c], sel), a2, a3);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * c + s], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * c + s], a0, a1, a2, a3, pf[h][nt][0], pf[h][nt][1]);
                 }
-        }
         __syncwarp();
         if (ahead < tiles) {
             fetch(ahead, stage);
@@ -991,34 +1056,35 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_attention_join_items(JoinAr
     const AttentionArgs& a = p.a;
     griddep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = a.cache.dim, kv_heads = a.cache.kv_heads;
-    const int64_t token = blockIdx.x / kv_heads;
-    const int kv = (int)(blockIdx.x - token * kv_heads);
-    if (token < a.seq.starts[0] || token >= a.seq.starts[a.seq.seqs]) return;  // no sequence's row
-    const int4 own = p.set[0].place[token];
-    if (own.w & kPlaceDone) return;
-    const int4 pre = own.w & kPlacePrefix ? p.set[1].place[token] : make_int4(0, 0, 0, 0);
+    const int token = (int)(blockIdx.x / (unsigned)kv_heads), kv = (int)blockIdx.x - token * kv_heads;
+    int4 at[2] = {p.set[0].place[token], p.set[1].place[token]};
+    const int rows_from = a.seq.starts[0], rows_to = a.seq.starts[a.seq.seqs];
+    if (token < rows_from || token >= rows_to || (at[0].w & kPlaceDone)) return;  // no sequence's row, or written
+    if (!(at[0].w & kPlacePrefix)) at[1].y = 0;
     for (int h = warp; h < a.group; h += kJoinWarps) {
-        int64_t first[2];  // part of the first piece, and pieces
+        int64_t first[2], step[2];  // row of the first piece's part, rows to the next
         int n[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const JoinSet& s = p.set[k];
-            const int4 at = k ? pre : own;
-            const int r = at.z + h, part = r / s.rows;
-            const int64_t item = (int64_t)at.x + (int64_t)part * at.y;
-            first[k] = item * kv_heads + kv;
-            n[k] = at.y;
-            if (at.x < 0 || at.y < 0 || at.z < 0 || at.z > 255 || (item + at.y) * kv_heads > s.blocks) n[k] = 0;
-            first[k] = first[k] * s.rows + r % s.rows;
+            const int r = at[k].z + h, part = r / s.rows;
+            const int64_t item = (int64_t)at[k].x + (int64_t)part * at[k].y;
+            const bool fits = at[k].x >= 0 && at[k].y >= 0 && at[k].z >= 0 && at[k].z <= 255 &&
+                              (item + at[k].y) * kv_heads <= s.blocks;
+            n[k] = fits ? at[k].y : 0;
+            first[k] = (item * kv_heads + kv) * s.rows + (r - part * s.rows);
+            step[k] = (int64_t)kv_heads * s.rows;
         }
         const int all = n[0] + n[1];
         auto stat = [&](int c) {
-            const int k = c >= n[0];
-            const JoinSet& s = p.set[k];
-            return reinterpret_cast<const float2*>(s.stats)[first[k] + (int64_t)(c - (k ? n[0] : 0)) * kv_heads * s.rows];
+            const bool own = c < n[0];
+            const float2* st = reinterpret_cast<const float2*>(own ? p.set[0].stats : p.set[1].stats);
+            return st[own ? first[0] + c * step[0] : first[1] + (c - n[0]) * step[1]];
         };
-        float top = -INFINITY;
-        for (int c = lane; c < all; c += 32) top = fmaxf(top, stat(c).x);
+        float2 v0 = make_float2(-INFINITY, 0.f);  // of piece `lane`
+        if (lane < all) v0 = stat(lane);
+        float top = v0.x;
+        for (int c = lane + 32; c < all; c += 32) top = fmaxf(top, stat(c).x);
 #pragma unroll
         for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
         float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
@@ -1026,29 +1092,32 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_attention_join_items(JoinAr
         for (int c0 = 0; c0 < all; c0 += 32) {
             float f = 0.f;
             if (c0 + lane < all) {
-                const float2 v = stat(c0 + lane);
+                const float2 v = c0 ? stat(c0 + lane) : v0;
                 // a NaN sum without a maximum keeps its weight: the row is NaN
                 f = v.y == 0.f ? 0.f : v.x == -INFINITY ? 1.f : exp2_approx(v.x - top);
                 sum += v.y * f;
             }
-            const int m = min(32, all - c0);
+            auto take = [&](int k, int from, int to) {  // pieces [from, to) of set k among these 32
+                const int before = k ? n[0] : 0;
+                const float* o = p.set[k].parts + (first[k] + (int64_t)(from - before) * step[k]) * dim + lane * 4;
+                const int64_t stride = step[k] * dim;
 #pragma unroll 8
-            for (int j = 0; j < m; ++j) {
-                const float g = __shfl_sync(0xffffffffu, f, j);
-                const int c = c0 + j, k = c >= n[0];
-                const JoinSet& s = p.set[k];
-                const float4* o = reinterpret_cast<const float4*>(
-                    s.parts + (first[k] + (int64_t)(c - (k ? n[0] : 0)) * kv_heads * s.rows) * dim);
+                for (int c = from; c < to; ++c, o += stride) {
+                    const float g = __shfl_sync(0xffffffffu, f, c - c0);
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
-                    if (g != 0.f && (q * 32 + lane) * 4 < dim) {
-                        const float4 x = o[q * 32 + lane];
-                        acc[q].x += x.x * g;
-                        acc[q].y += x.y * g;
-                        acc[q].z += x.z * g;
-                        acc[q].w += x.w * g;
-                    }
-            }
+                    for (int q = 0; q < 2; ++q)
+                        if (g != 0.f && (q * 32 + lane) * 4 < dim) {
+                            const float4 x = *reinterpret_cast<const float4*>(o + q * 128);
+                            acc[q].x += x.x * g;
+                            acc[q].y += x.y * g;
+                            acc[q].z += x.z * g;
+                            acc[q].w += x.w * g;
+                        }
+                }
+            };
+            const int end = min(c0 + 32, all), mid = min(max(n[0], c0), end);
+            take(0, c0, mid);
+            take(1, mid, end);
         }
 #pragma unroll
         for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
@@ -1059,14 +1128,21 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_attention_join_items(JoinAr
         for (int q = 0; q < 2; ++q) {
             const int d = (q * 32 + lane) * 4;
             if (d < dim) {
-                y[d] = from_f32<T>(acc[q].x * inv);
-                y[d + 1] = from_f32<T>(acc[q].y * inv);
-                y[d + 2] = from_f32<T>(acc[q].z * inv);
-                y[d + 3] = from_f32<T>(acc[q].w * inv);
+                Pack<T, 4> w;
+                w.v[0] = from_f32<T>(acc[q].x * inv);
+                w.v[1] = from_f32<T>(acc[q].y * inv);
+                w.v[2] = from_f32<T>(acc[q].z * inv);
+                w.v[3] = from_f32<T>(acc[q].w * inv);
+                if (a.o_packs) {
+                    *reinterpret_cast<Pack<T, 4>*>(y + d) = w;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[d + k] = w.v[k];
+                }
             }
         }
         if (a.lse && lane == 0)
-            a.lse[token * a.q_heads + head] =
+            a.lse[(int64_t)token * a.q_heads + head] =
                 sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * 0.693147180559945309f;
     }
 }

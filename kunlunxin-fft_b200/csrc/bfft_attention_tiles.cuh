@@ -70,7 +70,7 @@ struct TileGeo {
     static constexpr int SLOTS = 8;              // tiles whose block scales are held
     static constexpr int GROUPS = N / 16;         // of 16 tokens
     static constexpr int BODY = 2 * Q_HALF + T_RING * T_BUF + RAW_RING * RAW_BUF;
-    static constexpr int BARS = 2 * RAW_RING + 2 * T_RING + SLOTS + 2 + 2 * 2 + 1 + 2 + 1;
+    static constexpr int BARS = 2 * RAW_RING + 2 * T_RING + SLOTS + 2 + 2 * 2 + 2 + 2 + 1;
     // at least half of an SM's shared memory: a second CTA could not have its tensor memory
     static constexpr int SMEM_NEED = 1024 + BODY + SLOTS * GROUPS * 16 + BARS * 8 + 8 + SLOTS * 4 + 4;
     static constexpr int SMEM = SMEM_NEED > 118 * 1024 ? SMEM_NEED : 118 * 1024;
@@ -185,6 +185,47 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&d)[16]) {
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// The rows of a warp, one a lane in tensor memory, to rows of E in memory, by way of shared
+// memory so that whole lines are written (a lane a row took 11900 clocks of a CTA's end, 32
+// lines to an instruction).  2 DP bytes of each row at a time; `at` is the lane's own row.
+template <int DP>
+struct Stage {
+    static constexpr int ROW = 2 * DP, PITCH = ROW + 16, BYTES = 32 * PITCH;
+    static_assert(4 * BYTES <= 2 * TileGeo<DP>::Q_HALF && 4 * BYTES <= TileGeo<DP>::T_RING * TileGeo<DP>::T_BUF, "room");
+};
+template <int DP, typename E, typename Value>
+__device__ __forceinline__ void write_rows(unsigned char* stage, uint32_t o_addr, int dim, bool mine, E* to, int64_t at,
+                                           Value value) {
+    constexpr int COLS = Stage<DP>::ROW / (int)sizeof(E), PER = 16 / (int)sizeof(E);
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int c0 = 0; c0 < dim; c0 += COLS) {
+#pragma unroll 1
+        for (int c = 0; c < COLS; c += 32) {
+            uint32_t o[32];
+            tmem_load(o_addr + c0 + c, o);
+#pragma unroll
+            for (int k = 0; k < 32; k += PER) {
+                Pack<E, PER> w;
+#pragma unroll
+                for (int x = 0; x < PER; ++x) w.v[x] = value(__uint_as_float(o[k + x]));
+                *reinterpret_cast<Pack<E, PER>*>(stage + lane * Stage<DP>::PITCH + (c + k) * (int)sizeof(E)) = w;
+            }
+        }
+        __syncwarp();
+        const int pieces = (dim - c0 < COLS ? dim - c0 : COLS) / PER;  // of 16 bytes of a row
+#pragma unroll 4
+        for (int e = lane; e < 32 * pieces; e += 32) {
+            const int row = pieces == COLS / PER ? e / (COLS / PER) : e / pieces, piece = e - row * pieces;
+            const int64_t from = __shfl_sync(0xffffffffu, at, row);
+            const bool has = __shfl_sync(0xffffffffu, (int)mine, row);
+            const uint4 w = *reinterpret_cast<const uint4*>(stage + row * Stage<DP>::PITCH + piece * 16);
+            if (has) *reinterpret_cast<uint4*>(to + from + c0 + piece * PER) = w;
+        }
+        __syncwarp();
+    }
+}
+
 template <int DP, typename T, int CODE, int MODE>
 __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(TileArgs p) {
     using G = TileGeo<DP>;
@@ -198,10 +239,16 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
     int chunk, kv;
     SlotRows sr;
     Item it{};
+    TokenSpan row_span{0, 0, 0};  // kSinks, kGroups: of row tid
     if constexpr (MODE == kGroups) {
         __shared__ ItemScratch scratch;
-        kv = (int)(i % a.cache.kv_heads);
-        if (!find_item<G::THREADS>(a, p.span, p.items, i / a.cache.kv_heads, p.tile_tokens, 1, scratch, it)) return;
+        TokenSpan* spans = reinterpret_cast<TokenSpan*>(align_smem<1024>(smem_raw));  // what the queries take later
+        if (tid < 256) spans[tid] = TokenSpan{0, 0, 0};
+        const unsigned item = blockIdx.x / (unsigned)a.cache.kv_heads;
+        kv = (int)(blockIdx.x - item * a.cache.kv_heads);
+        if (!find_item<G::THREADS>(a, p.span, p.items, (int)item, p.tile_tokens, 1, scratch, it)) return;
+        item_spans<G::THREADS>(a, p.span, it, spans);
+        if (tid < it.n * a.group) row_span = spans[(unsigned)tid / (unsigned)a.group];
         chunk = it.chunk;
         sr.s = it.table_row;
         sr.first = it.token;
@@ -217,7 +264,6 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
     // others places of `axis` (what some row sees there: axis.lo_any, hi_any, sinks_any)
     int64_t len = 0, pos0 = 0, base, end, lo_min, hi_max, lo_max, hi_min;
     Axis axis{};
-    TokenSpan row_span{0, 0, 0};  // of row tid
     int sinks_all = 0;
     if constexpr (MODE == kPlain) {
         len = a.seq.lens[sr.s];
@@ -237,16 +283,10 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
         __syncthreads();
         if (tid < 256) {
             const bool valid = tid < rows;
-            if (valid) {
-                const int of = tid / a.group;
-                if constexpr (MODE == kGroups)
-                    row_span = item_span(a, p.span, it, sr.first + of);
-                else
-                    row_span = token_span(a, p.span, (int64_t)a.seq.lens[sr.s] - sr.rows + sr.place + of,
-                                          a.seq.lens[sr.s], 0, 0x7fffffff);
-            } else {
-                row_span.sinks = first;
-            }
+            if (MODE == kSinks && valid)
+                row_span = token_span(a, p.span, (int64_t)a.seq.lens[sr.s] - sr.rows + sr.place + tid / a.group,
+                                      a.seq.lens[sr.s], 0, 0x7fffffff);
+            if (!valid) row_span.sinks = first;
             const bool some = row_span.lo < row_span.hi;
             const int v[6] = {__reduce_min_sync(0xffffffffu, some ? row_span.lo : 0x7fffffff),
                               __reduce_max_sync(0xffffffffu, valid ? row_span.lo : -0x7fffffff),
@@ -329,7 +369,8 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
     uint64_t* bars = reinterpret_cast<uint64_t*>(scale_s + G::SLOTS * G::GROUPS);
     uint64_t *raw_full = bars, *raw_empty = raw_full + G::RAW_RING, *t_full = raw_empty + G::RAW_RING,
              *t_empty = t_full + G::T_RING, *scale_full = t_empty + G::T_RING, *s_full = scale_full + G::SLOTS,
-             *p_half = s_full + 2, *p_full = p_half + 2, *q_full = p_full + 2, *o_full = q_full + 1, *drained = o_full + 2;
+             *p_half = s_full + 2, *p_full = p_half + 2, *q_full = p_full + 2, *q_raw = q_full + 1, *o_full = q_raw + 1,
+             *drained = o_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + G::BARS);
     int* tile_kind = reinterpret_cast<int*>(bars + G::BARS + 1);  // of a tile: 0 where all its blocks are ordinary
     volatile int* small_s = tile_kind + G::SLOTS;                 // whether the chunk has a small value scale
@@ -356,9 +397,11 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
             mbar_init(&o_full[h], 1);
         }
         mbar_init(q_full, 256);
+        mbar_init(q_raw, 1);
         mbar_init(drained, 1);
         *small_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (a.q_packs) mbar_arrive_expect_tx(q_raw, (uint32_t)(rows * dim * 2));
     }
     tmem_fence_before();
     __syncthreads();
@@ -374,36 +417,67 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
         int64_t token = 0;
         int head = 0;
         if (mine) row_of(r, token, head);
+        // Each thread's row comes by the copy engine (64 dims of it to a panel), all rows in
+        // flight at once, and is brought to float16 and the swizzle in its place: DP / 8 lanes
+        // to a row, in a short loop, as this runs once and from a cold instruction cache.
+        // (Loads into registers took 9700 clocks with warm instructions, 18000 with cold ones.)
         float up = 1.f;
+        bool ok = true;
         {
+            constexpr int LANES = DP / 8, ROWS = 32 / LANES, AHEAD = 4;  // lanes of a row, rows at a time
+            const int c = lane % LANES, sub = lane / LANES;
             const T* x = static_cast<const T*>(a.q) + token * a.qt + head * a.qh;
-            float big = 0.f, down;
-            Pack<T, 8> w[DP / 8];  // the whole row in flight at once
-#pragma unroll
-            for (int c = 0; c < DP / 8; ++c) {
-                if (!mine || 8 * c >= dim) {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) w[c].v[k] = from_f32<T>(0.f);
-                } else if (a.q_packs) {
-                    w[c] = *reinterpret_cast<const Pack<T, 8>*>(x + 8 * c);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) w[c].v[k] = x[8 * c + k];
+            if (a.q_packs) {
+                if (mine) {
+                    unsigned char* to = q_s + h * G::Q_HALF + (r & 127) * 128;
+                    bulk_load(to, x, (uint32_t)(dim < 64 ? dim : 64) * 2, q_raw);
+                    if (dim > 64) bulk_load(to + G::Q_PANEL, x + 64, (uint32_t)(dim - 64) * 2, q_raw);
                 }
+                ok = wait(q_raw, 0);
             }
+            unsigned char* q_row = q_s + h * G::Q_HALF + (c >> 3) * G::Q_PANEL + ((warp & 3) << 5) * 128;
+#pragma unroll 1
+            for (int i = 0; i < LANES; i += AHEAD) {
+                Pack<T, 8> w[AHEAD];
 #pragma unroll
-            for (int c = 0; c < DP / 8; ++c)
+                for (int j = 0; j < AHEAD; ++j) {
+                    const int row = (i + j) * ROWS + sub;
+                    if ((warp << 5) + row >= rows || 8 * c >= dim)
+                        w[j] = Pack<T, 8>{};
+                    else
+                        w[j] = *reinterpret_cast<const Pack<T, 8>*>(q_row + row * 128 + ((c & 7) << 4));
+                }
+                if (!a.q_packs) {
+                    const int64_t own = reinterpret_cast<intptr_t>(x);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) big = fmaxf(big, fabsf(to_f32(w[c].v[k])));
-            row_power<T>(big, down, up);
-            unsigned char* q_row = q_s + h * G::Q_HALF + (r & 127) * 128;
+                    for (int j = 0; j < AHEAD; ++j) {
+                        const int row = (i + j) * ROWS + sub;
+                        const T* y = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, own, row)) + 8 * c;
+                        if ((warp << 5) + row < rows && 8 * c < dim) {
 #pragma unroll
-            for (int c = 0; c < DP / 8; ++c) {
-                uint32_t e[4];
+                            for (int k = 0; k < 8; ++k) w[j].v[k] = y[k];
+                        }
+                    }
+                }
+                __syncwarp();  // a line's lanes have read it
 #pragma unroll
-                for (int k = 0; k < 4; ++k) e[k] = pack_f16(to_f32(w[c].v[2 * k]) * down, to_f32(w[c].v[2 * k + 1]) * down);
-                *reinterpret_cast<uint4*>(q_row + (c >> 3) * G::Q_PANEL + (((c & 7) ^ (r & 7)) << 4)) =
-                    make_uint4(e[0], e[1], e[2], e[3]);
+                for (int j = 0; j < AHEAD; ++j) {
+                    const int row = (i + j) * ROWS + sub;
+                    float big = 0.f, down, power;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) big = fmaxf(big, fabsf(to_f32(w[j].v[k])));
+#pragma unroll
+                    for (int d = 1; d < LANES; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+                    row_power<T>(big, down, power);
+                    uint32_t e[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        e[k] = pack_f16(to_f32(w[j].v[2 * k]) * down, to_f32(w[j].v[2 * k + 1]) * down);
+                    *reinterpret_cast<uint4*>(q_row + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+                        make_uint4(e[0], e[1], e[2], e[3]);
+                    power = __shfl_sync(0xffffffffu, power, (lane % ROWS) * LANES);
+                    if (lane / ROWS == i + j) up = power;
+                }
             }
             fence_proxy_async_smem();
             mbar_arrive(q_full);
@@ -421,10 +495,9 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_addr = tmem + G::S0 + h * 128 + lanes, o_addr = tmem + G::O0 + h * 128 + lanes;
         float m = -INFINITY, l = 0.f;
-        bool ok = true;
         if (h < halves) {
             for (int j = 0; j < tiles; ++j) {
-                ok = wait(&scale_full[j % G::SLOTS], (uint32_t)((j / G::SLOTS) & 1));
+                ok = ok && wait(&scale_full[j % G::SLOTS], (uint32_t)((j / G::SLOTS) & 1));
                 // what the tile needs besides its scores, before they are there
                 const int64_t tok0 = base + (int64_t)j * G::N;
                 bool inside = tok0 >= lo_max && tok0 + G::N <= hi_min;
@@ -561,36 +634,24 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                 const bool small = *small_s;
                 if (small) m += SmallScales::shift;
                 const int64_t at = part_of(token, head, r);
-                T* y = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
+                const float unit = small ? SmallScales::factor : 1.f;
+                // Half 0 stages its rows where the queries were, half 1 where the widened codes
+                // were: nothing but half 1's last product over values can be under way here.
+                unsigned char* stage = (h ? t_s : q_s) + (warp & 3) * Stage<DP>::BYTES;
+                if (!direct) {
+                    write_rows<DP>(stage, o_addr, dim, mine, p.parts, at * dim, [&](float v) { return v * unit; });
+                } else if (a.o_packs) {
+                    write_rows<DP>(stage, o_addr, dim, mine, static_cast<T*>(a.out), token * a.ot + head * a.oh,
+                                   [&](float v) { return from_f32<T>(v * unit * inv); });
+                } else {
+                    T* y = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
 #pragma unroll
-                for (int c = 0; c < DP / 32; ++c) {
-                    uint32_t o[32];
-                    tmem_load(o_addr + c * 32, o);
-                    if (!mine) continue;
-                    if (small) {
+                    for (int c = 0; c < DP / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_load(o_addr + c * 32, o);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * SmallScales::factor);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        const int d = c * 32 + k;
-                        if (d >= dim) continue;
-                        if (!direct) {
-#pragma unroll
-                            for (int x = 0; x < 8; x += 4)
-                                *reinterpret_cast<uint4*>(p.parts + at * dim + d + x) =
-                                    make_uint4(o[k + x], o[k + x + 1], o[k + x + 2], o[k + x + 3]);
-                        } else {
-                            Pack<T, 8> w;
-#pragma unroll
-                            for (int x = 0; x < 8; ++x) w.v[x] = from_f32<T>(__uint_as_float(o[k + x]) * inv);
-                            if (a.o_packs) {
-                                *reinterpret_cast<Pack<T, 8>*>(y + d) = w;
-                            } else {
-#pragma unroll
-                                for (int x = 0; x < 8; ++x) y[d + x] = w.v[x];
-                            }
-                        }
+                        for (int k = 0; k < 32; ++k)
+                            if (mine && c * 32 + k < dim) y[c * 32 + k] = from_f32<T>(__uint_as_float(o[k]) * unit * inv);
                     }
                 }
                 if (mine) {
