@@ -196,7 +196,8 @@ struct GroupPlan {
     SplitPlan split;   // nt, tile_tokens, token_tiles, entries, ctas
     TilePlan tiles;    // tile_tokens, ctas
     ItemArgs split_items, tile_items;
-    size_t places, split_parts, tile_parts, bytes;  // bytes of the parts of the workspace, in its order
+    bool split_list, tile_list;  // items that are listed first
+    size_t places, split_items_at, tile_items_at, split_parts_at, tile_parts_at, bytes;  // of the workspace
 };
 
 // Sequences that have many rows each fill their row tiles by themselves: sharing saves them
@@ -239,10 +240,17 @@ GroupPlan plan_groups(const bfft_cache_desc* c, const bfft_sequence_desc* q, con
     const bool split = !p.own_tiles, tiles = p.prefix_tiles;
     s.ctas = split ? p.split_items.most * kv : 0;
     p.tiles.ctas = tiles ? p.tile_items.most * kv : 0;
+    SpanArgs counts{};
+    counts.n_groups = (int)w->n_groups;
+    p.split_list = split && unit_count(counts, p.split_items, (int)q->seqs) > kFewUnits;
+    p.tile_list = tiles && unit_count(counts, p.tile_items, (int)q->seqs) > kFewUnits;
+    // places, the items' lists (behind a count), the parts
     p.places = (size_t)q->tokens * 2 * sizeof(int4);
-    p.split_parts = (size_t)(s.ctas * rows) * (size_t)(c->dim + 2) * 4;
-    p.tile_parts = (size_t)(p.tiles.ctas * 256) * (size_t)(c->dim + 2) * 4;
-    p.bytes = p.places + p.split_parts + p.tile_parts;
+    p.split_items_at = (p.places + 63) / 64 * 64;
+    p.tile_items_at = p.split_items_at + (p.split_list ? (size_t)(p.split_items.most + 1) * sizeof(Item) : 0);
+    p.split_parts_at = p.tile_items_at + (p.tile_list ? (size_t)(p.tile_items.most + 1) * sizeof(Item) : 0);
+    p.tile_parts_at = p.split_parts_at + (size_t)(s.ctas * rows) * (size_t)(c->dim + 2) * 4;
+    p.bytes = p.tile_parts_at + (size_t)(p.tiles.ctas * 256) * (size_t)(c->dim + 2) * 4;
     return p;
 }
 
@@ -251,11 +259,25 @@ cudaError_t run_groups(const AttentionArgs& a, const SpanArgs& w, const GroupPla
                        unsigned int* status, cudaStream_t s) {
     int4* own_of = reinterpret_cast<int4*>(ws);
     int4* prefix_of = own_of + a.seq.tokens;
-    float* split_parts = reinterpret_cast<float*>(ws + p.places);
-    float* split_stats = split_parts + p.split.ctas * 8 * p.split.nt * c->dim;
-    float* tile_parts = reinterpret_cast<float*>(ws + p.places + p.split_parts);
+    float* split_parts = reinterpret_cast<float*>(ws + p.split_parts_at);
+    float* split_stats = split_parts + p.split.ctas * 8 * p.split.nt * c->dim;  // 16-byte aligned, as all parts are
+    float* tile_parts = reinterpret_cast<float*>(ws + p.tile_parts_at);
     float* tile_stats = tile_parts + p.tiles.ctas * 256 * c->dim;
     cudaError_t e = cudaSuccess;
+    auto listed = [&](ItemArgs x, bool list, size_t at, int tile, int parts) {
+        x.own_of = own_of;
+        x.prefix_of = prefix_of;
+        if (!list || e != cudaSuccess) return x;
+        int* count = reinterpret_cast<int*>(ws + at);
+        Item* items = reinterpret_cast<Item*>(ws + at) + 1;
+        e = list_items(a, w, x, tile, parts, items, count, s);
+        x.list = items;
+        x.count = count;
+        return x;
+    };
+    const ItemArgs tile_items = listed(p.tile_items, p.tile_list, p.tile_items_at, p.tiles.tile_tokens, 1);
+    const ItemArgs split_items = listed(p.split_items, p.split_list, p.split_items_at, p.split.tile_tokens, p.split.token_tiles);
+    if (e != cudaSuccess) return e;
     if (p.tiles.ctas) {
         TileArgs t{};
         t.a = a;
@@ -264,9 +286,7 @@ cudaError_t run_groups(const AttentionArgs& a, const SpanArgs& w, const GroupPla
         t.tile_tokens = p.tiles.tile_tokens;
         t.status = status;
         t.span = w;
-        t.items = p.tile_items;
-        t.items.own_of = own_of;
-        t.items.prefix_of = prefix_of;
+        t.items = tile_items;
         e = run_tiles<T, kGroups>(t, p.tiles, c, s);
     }
     if (e == cudaSuccess && p.split.ctas) {
@@ -279,9 +299,7 @@ cudaError_t run_groups(const AttentionArgs& a, const SpanArgs& w, const GroupPla
         t.entries = p.split.entries;
         t.status = status;
         t.span = w;
-        t.items = p.split_items;
-        t.items.own_of = own_of;
-        t.items.prefix_of = prefix_of;
+        t.items = split_items;
         e = run_split<T, kGroups>(t, p.split, c, s);
     }
     if (e != cudaSuccess) return e;
@@ -385,7 +403,7 @@ bfft_status attention_call(const bfft_cache_desc* cache, const bfft_sequence_des
         const GroupPlan p = plan_groups(cache, seqs, d, w, sms);
         st = room(p.split.ctas > p.tiles.ctas ? p.split.ctas : p.tiles.ctas, p.bytes);
         if (st != BFFT_OK) return st;
-        count_launches(1 + (p.split.ctas > 0) + (p.tiles.ctas > 0));
+        count_launches(1 + (p.split.ctas > 0) + (p.tiles.ctas > 0) + p.split_list + p.tile_list);
         char* ws = static_cast<char*>(d->workspace);
         return launched(d->type == BFFT_F16 ? run_groups<__half>(a, span, p, cache, ws, status, s)
                                             : run_groups<__nv_bfloat16>(a, span, p, cache, ws, status, s),

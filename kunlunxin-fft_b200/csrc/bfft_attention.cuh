@@ -162,9 +162,14 @@ cudaError_t run_split(const SplitArgs& a, const SplitPlan& p, const bfft_cache_d
 }
 
 
+// Compiled in bfft_attention_groups.cu.
+cudaError_t list_items(const AttentionArgs& a, const SpanArgs& p, const ItemArgs& x, int tile, int parts, Item* list,
+                       int* count, cudaStream_t s);
+
 template <typename T>
 cudaError_t run_join_items(const JoinArgs& a, cudaStream_t s) {
-    return launch_dependent(k_attention_join_items<T>, (unsigned)(a.a.seq.tokens * a.a.cache.kv_heads), kJoinWarps * 32, 0,
+    return launch_dependent(k_attention_join_items<T>, (unsigned)(a.a.seq.tokens * a.a.cache.kv_heads),
+                            (a.a.group > kJoinWarps ? 2 : 1) * kJoinWarps * 32, 0,
                             s, a);
 }
 

@@ -17,6 +17,20 @@ struct SpanArgs {
     const int32_t* shared;
 };
 
+// A row tile's piece of the axis.
+struct Item {
+    int table_row;          // of the block table
+    int s0, s1;             // sequences that its rows are of
+    int token, n;           // its first row, query tokens
+    int part;               // of a token's heads
+    int chunk, chunks;
+    int from, to;           // tokens that it is about
+    int pos, len;           // of a sequence: its first row's place, its tokens
+    int prefix, shares;
+    int spare[2];
+};
+static_assert(sizeof(Item) == 64, "four loads");
+
 // One call with groups: row tiles of groups over their prefixes, then row tiles of
 // sequences over their own tokens, each cut along the axis.  Item i and kv head h are
 // block i * kv_heads + h; its parts are rows [block * rows of a tile, ...) of `parts`.
@@ -26,6 +40,8 @@ struct ItemArgs {
     int least;              // tokens of an item at least
     int unit;               // and a multiple of this
     int64_t most;           // items a kv head at most (the grid)
+    const Item* list;       // where there are more than 32 units: the items, and how many
+    const int* count;
     int4* own_of;           // [tokens] where a token's parts are: see ItemPlace
     int4* prefix_of;
 };
@@ -89,13 +105,10 @@ __device__ __forceinline__ Axis make_axis(int first, int lo_min, int hi_max, int
     return x;
 }
 
-// Whole pages of the tokens that group g shares.
-__device__ __forceinline__ int shared_tokens(const AttentionArgs& a, const SpanArgs& p, int g) {
-    const int64_t most = (int64_t)a.seq.max_pages << a.cache.page_log2;
-    int64_t n = p.shared[g];
-    if (n > most) n = most;
-    if (n > 0x7fffffff) n = 0x7fffffff;
-    return n > 0 ? (int)(n >> a.cache.page_log2 << a.cache.page_log2) : 0;
+// Tokens of the whole pages among n.
+__device__ __forceinline__ int whole_pages(const AttentionArgs& a, int n) {
+    n = min(n, a.seq.max_pages << a.cache.page_log2);  // 2^30 at most
+    return n > 0 ? n >> a.cache.page_log2 << a.cache.page_log2 : 0;
 }
 // Sequences of group g.
 __device__ __forceinline__ void group_sequences(const AttentionArgs& a, const SpanArgs& p, int g, int& s0, int& s1) {
@@ -106,9 +119,9 @@ __device__ __forceinline__ void group_sequences(const AttentionArgs& a, const Sp
         s1 = min(max(p.groups[g + 1], s0), s1);
     }
 }
-// What sequence s shares: the largest g with groups[g] <= s.
-__device__ __forceinline__ int sequence_shared(const AttentionArgs& a, const SpanArgs& p, int s) {
-    if (!p.groups) return shared_tokens(a, p, 0);
+// The group of sequence s, or -1: the largest g with groups[g] <= s, if s lies before its end.
+__device__ __forceinline__ int group_of(const AttentionArgs& a, const SpanArgs& p, int s) {
+    if (!p.groups) return 0;
     int lo = 0, n = p.n_groups;
     while (n > 1) {
         const int half = n >> 1;
@@ -119,15 +132,14 @@ __device__ __forceinline__ int sequence_shared(const AttentionArgs& a, const Spa
             n = half;
         }
     }
-    return p.groups[lo] <= s && s < p.groups[lo + 1] ? shared_tokens(a, p, lo) : 0;
+    return p.groups[lo] <= s && s < p.groups[lo + 1] ? lo : -1;
 }
-// Rows [t0, t0 + n) of sequences [s0, s1).
-__device__ __forceinline__ int rows_of(const AttentionArgs& a, int s0, int s1, int& t0) {
-    t0 = a.seq.starts[s0];
-    int t1 = a.seq.starts[s1];
-    if (t1 > a.seq.tokens) t1 = (int)a.seq.tokens;
-    if (t0 < 0) t0 = t1;
-    return t1 > t0 ? t1 - t0 : 0;
+// The rows [t0, t0 + n) that lie from starts' entry `from` to entry `to`.
+__device__ __forceinline__ int rows_between(const AttentionArgs& a, int from, int to, int& t0) {
+    t0 = from;
+    if (to > a.seq.tokens) to = (int)a.seq.tokens;
+    if (t0 < 0) t0 = to;
+    return to > t0 ? to - t0 : 0;
 }
 
 // A group's or a sequence's row tiles (times parts), and the tokens that each walks.
@@ -141,17 +153,16 @@ __device__ __forceinline__ Unit unit_of(const AttentionArgs& a, const SpanArgs& 
     Unit v;
     const int groups = x.prefixes ? p.n_groups : 0;
     const bool prefix = u < groups;
-    if (prefix) {
-        group_sequences(a, p, u, v.s0, v.s1);
-        v.len = 0;
-        v.shared = shared_tokens(a, p, u);
-    } else {
-        v.s0 = u - groups;
-        v.s1 = v.s0 + 1;
-        v.len = a.seq.lens[v.s0];
-        v.shared = sequence_shared(a, p, v.s0);
-    }
-    v.rows = rows_of(a, v.s0, v.s1, v.t0);
+    v.s0 = u - groups;
+    v.s1 = v.s0 + 1;
+    if (prefix) group_sequences(a, p, u, v.s0, v.s1);
+    // the loads of what follows side by side: each waits for memory once
+    const int t0 = a.seq.starts[v.s0], t1 = a.seq.starts[v.s1], len = a.seq.lens[v.s0 < a.seq.seqs ? v.s0 : 0];
+    const int g = prefix ? u : group_of(a, p, v.s0);
+    const int shared = g >= 0 ? p.shared[g] : 0;
+    v.rows = rows_between(a, t0, t1, v.t0);
+    v.shared = whole_pages(a, shared);
+    v.len = prefix ? 0 : len;
     v.tiles = (int)((unsigned)(v.rows + tile - 1) / (unsigned)tile) * parts;
     // tokens up to the end, from the first that the first row (causal: the last row tile's) sees
     const int most = a.seq.max_pages << a.cache.page_log2;  // 2^30 at most
@@ -167,108 +178,81 @@ __device__ __forceinline__ Unit unit_of(const AttentionArgs& a, const SpanArgs& 
     return v;
 }
 
-// A row tile's piece of the axis.
-struct Item {
-    int table_row;          // of the block table
-    int s0, s1;             // sequences that its rows are of
-    int token, n;           // its first row, query tokens
-    int part;               // of a token's heads
-    int chunk, chunks;
-    int from, to;           // tokens that it is about
-    int pos, len;           // of a sequence: its first row's place, its tokens
-    int prefix, shares;
-};
+// Tokens of an item: those that all row tiles walk, `total`, shared out over x.target items.
+// (The sum's rounding is far under the one token that is added.)
+__device__ __forceinline__ unsigned item_tokens(const ItemArgs& x, float total) {
+    const int share = (int)fminf(total / (float)x.target, 1.0e9f) + 1;
+    return max((unsigned)(share + x.unit - 1) / (unsigned)x.unit * x.unit, (unsigned)x.least);
+}
+__device__ __forceinline__ int pieces_of(const Unit& v, unsigned chunk) {
+    return (unsigned)v.length > chunk ? (int)(((unsigned)v.length + chunk - 1) / chunk) : 1;
+}
+// Item `rest` of unit u.
+__device__ __forceinline__ void fill_item(Item& f, const Unit& v, bool prefix, int rest, int pieces, int tile, int parts) {
+    const unsigned at = (unsigned)rest / (unsigned)pieces, t = at / (unsigned)parts;
+    f.prefix = prefix;
+    f.table_row = f.s0 = v.s0;
+    f.s1 = v.s1;
+    f.chunks = pieces;
+    f.chunk = rest - (int)at * pieces;
+    f.part = (int)at - (int)t * parts;
+    f.token = v.t0 + (int)t * tile;
+    f.n = min(v.rows - (int)t * tile, tile);
+    f.from = prefix ? 0 : v.shared;
+    f.to = prefix ? v.shared : 0x7fffffff;
+    f.shares = v.shared > 0;
+    f.pos = v.len - v.rows + (int)t * tile;
+    f.len = v.len;
+}
 
-struct ItemScratch {
-    float weight[32];
-    int sum[2][32];
-    int found;
-    Item item;
-};
+// Units that a call's warps look at by themselves; more have their items listed first.
+constexpr int kFewUnits = 32;
+__host__ __device__ inline int unit_count(const SpanArgs& p, const ItemArgs& x, int seqs) {
+    return (x.prefixes ? p.n_groups : 0) + (x.own ? seqs : 0);
+}
 
-// Finds item i, block-wide: every block makes the same sums over the sequences' tables, so
-// the items need no list in memory and no launch that makes one.  Tokens of an item: those
-// that all row tiles walk, shared out over x.target items.  A block runs this once, from a cold
-// instruction cache: short code and 32-bit divisions are what counts.
-template <int THREADS>
+// Finds item i, each warp for itself.  With few units every warp makes the same sums over
+// the sequences' tables, so that no launch has to come before (a block does this once, from
+// a cold instruction cache: short code and few waits for memory are what counts).
 __device__ __forceinline__ bool find_item(const AttentionArgs& a, const SpanArgs& p, const ItemArgs& x, int i, int tile,
-                                          int parts, ItemScratch& sh, Item& it) {
-    constexpr int WARPS = THREADS / 32;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int groups = x.prefixes ? p.n_groups : 0, units = groups + (x.own ? a.seq.seqs : 0);
-    // units in rounds of a block's threads: once to sum them up and, where they take more
-    // than one round, once more to look for the item
-    const int rounds = (units + THREADS - 1) / THREADS, last = rounds > 1 ? 2 * rounds : 1;
-    float total = 0.f;
-    unsigned chunk = 1;
-    int before = 0;  // items of the units before this round's
-    if (tid == 0) sh.found = 0;
-#pragma unroll 1
-    for (int round = 0; round < last; ++round) {
-        const int u = (round < rounds ? round : round - rounds) * THREADS + tid;
-        Unit v{};
-        if (u < units) v = unit_of(a, p, x, u, tile, parts);
-        if (round < rounds) {
-            total += (float)v.tiles * (float)v.length;
-            if (round < rounds - 1) continue;
+                                          int parts, Item& it) {
+    const int lane = threadIdx.x & 31;
+    if (x.list) {
+        const int count = *x.count;
+        const int4* from = reinterpret_cast<const int4*>(x.list + i);
+        int4* to = reinterpret_cast<int4*>(&it);
 #pragma unroll
-            for (int w = 16; w; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
-            if (lane == 0) sh.weight[warp] = total;
-            __syncthreads();
-            total = 0.f;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) total += sh.weight[w];
-            // (the sum's rounding is far under the one token that is added)
-            const int share = (int)fminf(total / (float)x.target, 1.0e9f) + 1;
-            chunk = max((unsigned)(share + x.unit - 1) / (unsigned)x.unit * x.unit, (unsigned)x.least);
-            if (rounds > 1) continue;
-        }
-        const int pieces = (unsigned)v.length > chunk ? (int)(((unsigned)v.length + chunk - 1) / chunk) : 1;
-        const int mine = v.tiles * pieces;
-        int upto = mine;
-#pragma unroll
-        for (int w = 1; w < 32; w <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, upto, w);
-            if (lane >= w) upto += y;
-        }
-        if (lane == 31) sh.sum[round & 1][warp] = upto;
-        __syncthreads();
-        int all = 0, under = before;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) under += sh.sum[round & 1][w];
-            all += sh.sum[round & 1][w];
-        }
-        const int rest = i - (under + upto - mine);
-        if (rest >= 0 && rest < mine) {
-            Item& f = sh.item;
-            const unsigned at = (unsigned)rest / (unsigned)pieces, t = at / (unsigned)parts;
-            f.prefix = u < groups;
-            f.table_row = f.s0 = v.s0;
-            f.s1 = v.s1;
-            f.chunks = pieces;
-            f.chunk = rest - (int)at * pieces;
-            f.part = (int)at - (int)t * parts;
-            f.token = v.t0 + (int)t * tile;
-            f.n = min(v.rows - (int)t * tile, tile);
-            f.from = f.prefix ? 0 : v.shared;
-            f.to = f.prefix ? v.shared : 0x7fffffff;
-            f.shares = v.shared > 0;
-            f.pos = v.len - v.rows + (int)t * tile;
-            f.len = v.len;
-            sh.found = 1;
-        }
-        before += all;
-        if (i < before) break;
+        for (int k = 0; k < 4; ++k) to[k] = from[k];
+        return i < count;
     }
-    __syncthreads();
-    if (!sh.found) return false;
-    it = sh.item;
+    const int groups = x.prefixes ? p.n_groups : 0, units = unit_count(p, x, a.seq.seqs);
+    Unit v{};
+    if (lane < units) v = unit_of(a, p, x, lane, tile, parts);
+    float total = (float)v.tiles * (float)v.length;
+#pragma unroll
+    for (int w = 16; w; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
+    const int pieces = pieces_of(v, item_tokens(x, total));
+    const int mine = v.tiles * pieces;
+    int upto = mine;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, w);
+        if (lane >= w) upto += y;
+    }
+    const int rest = i - (upto - mine);
+    const unsigned who = __ballot_sync(0xffffffffu, rest >= 0 && rest < mine);
+    if (!who) return false;
+    Item f{};
+    fill_item(f, v, lane < groups, rest, pieces, tile, parts);
+    const int* fields = reinterpret_cast<const int*>(&f);
+    int* out = reinterpret_cast<int*>(&it);
+#pragma unroll
+    for (int k = 0; k < (int)(sizeof(Item) / 4); ++k) out[k] = __shfl_sync(0xffffffffu, fields[k], __ffs(who) - 1);
     return true;
 }
 
-// What the item's rows see of its tokens, a query token each, in shared memory; `spans` holds
-// empty ones before (no_spans).  A group's rows are found from its sequences, a thread each:
+// What the item's rows see of its tokens, a query token each, in shared memory, after a
+// barrier behind which `spans` holds empty ones.  A group's rows are found from its sequences, a thread each:
 // each row's own search of its sequence took 3900 clocks.
 template <int THREADS>
 __device__ __forceinline__ void item_spans(const AttentionArgs& a, const SpanArgs& p, const Item& it, TokenSpan* spans) {
@@ -278,7 +262,8 @@ __device__ __forceinline__ void item_spans(const AttentionArgs& a, const SpanArg
     } else {
         for (int s = it.s0 + (int)threadIdx.x; s < it.s1; s += THREADS) {
             int t0;
-            const int n = rows_of(a, s, s + 1, t0), len = a.seq.lens[s];
+            const int from = a.seq.starts[s], to = a.seq.starts[s + 1], len = a.seq.lens[s];
+            const int n = rows_between(a, from, to, t0);
             for (int t = max(t0, it.token); t < min(t0 + n, it.token + it.n); ++t)
                 spans[t - it.token] = token_span(a, p, (int64_t)len - n + (t - t0), len, it.from, it.to);
         }

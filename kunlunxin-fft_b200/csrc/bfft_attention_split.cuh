@@ -280,16 +280,16 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     // which rows and tokens
     int64_t i = blockIdx.x;
     int chunk = 0, kv, part;
-    SlotRows sr;
+    SlotRows sr{};
     Item it{};
     TokenSpan mine_span{0, 0, 0};  // kSinks, kGroups: of query token `lane` of the tile
     if constexpr (MODE == kGroups) {
-        __shared__ ItemScratch scratch;
         __shared__ TokenSpan spans[16];
         if (tid < 16) spans[tid] = TokenSpan{0, 0, 0};
         const unsigned item = blockIdx.x / (unsigned)a.cache.kv_heads;
         kv = (int)(blockIdx.x - item * a.cache.kv_heads);
-        if (!find_item<kSplitThreads>(a, p.span, p.items, (int)item, p.tile_tokens, p.token_tiles, scratch, it)) return;
+        if (!find_item(a, p.span, p.items, (int)item, p.tile_tokens, p.token_tiles, it)) return;
+        __syncthreads();
         item_spans<kSplitThreads>(a, p.span, it, spans);
         if (lane < it.n) mine_span = spans[lane];
         part = it.part;
@@ -388,6 +388,30 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
             }
         if (!p.cluster) return;
     } else {
+    // The queries of this lane's rows, 16 adjacent elements by two loads, on their way while
+    // the pages are looked up.
+    auto query_of = [&](int r) -> const T* {
+        if (r >= rows) return nullptr;
+        int64_t token;
+        int head;
+        row_of(r, token, head);
+        return static_cast<const T*>(a.q) + token * a.qt + head * a.qh;
+    };
+    Pack<T, 8> q_raw[NT][G::KS / 4][2];
+    if (a.q_packs) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const T* x = query_of(nt * 8 + g);
+#pragma unroll
+            for (int c = 0; c < G::KS / 4; ++c) {
+                const int d = 16 * (4 * c + q4);
+                const bool has = x && (EXACT || d < dim);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    q_raw[nt][c][j] = has ? *reinterpret_cast<const Pack<T, 8>*>(x + d + 8 * j) : Pack<T, 8>{};
+            }
+        }
+    }
     // From here on tokens are counted in 32 bits: kPlain from `base`, the others in places
     // of the axis.  A segment is what the table of pages holds: kPlain's chunks are one.
     const int lg = a.cache.page_log2, page_mask = (1 << lg) - 1;
@@ -432,13 +456,20 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
             page_ids[e] = id >= 0 && id < a.cache.pages ? (int)id : -1;
         }
     };
-    auto load_scales = [&] {
+    float2 scale_raw = make_float2(0.f, 0.f);  // of this thread's first entry
+    auto fetch_scale = [&](int e) {
+        const int id = page_ids[e];
+        if (id < 0) return make_float2(0.f, 0.f);
+        const int64_t b = (int64_t)id * a.cache.kv_heads + kv;
+        return make_float2(a.cache.k_scale[b], a.cache.v_scale[b]);
+    };
+    auto load_scales = [&] {  // those behind scale_raw follow
         bool small = false;
+#pragma unroll 1
         for (int e = tid; e < entries; e += kSplitThreads) {
-            const int id = page_ids[e];
-            if (id >= 0) {
-                const int64_t b = (int64_t)id * a.cache.kv_heads + kv;
-                scales[e] = block_scale(a.cache.k_scale[b], a.cache.v_scale[b]);
+            if (e != tid) scale_raw = fetch_scale(e);
+            if (page_ids[e] >= 0) {
+                scales[e] = block_scale(scale_raw.x, scale_raw.y);
                 small |= small_scale(scales[e]);
             } else {
                 scales[e] = BlockScale{0.f, 0.f, 0.f, kDeadBlock};
@@ -489,7 +520,7 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     };
     int ahead = warp, fetched = 0;  // next tile to fetch, and how many were
     for (int s = 0; s < G::STAGES && ahead < tiles; ++s, ahead += kSplitWarps, ++fetched) fetch(ahead, s);
-    bool any_small = load_scales();
+    if (tid < entries) scale_raw = fetch_scale(tid);
 
     // queries as B fragments: lane (g, q4) holds row g of each 8-row tile, dims 16 (4 i + q4) + 4 t ..
     uint32_t qf[NT][G::KS][2];
@@ -499,29 +530,13 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     for (int nt = 0; nt < NT; ++nt) {
         const int r = nt * 8 + g;
         float big = 0.f;
-        const T* x = nullptr;
-        if (r < rows) {
-            int64_t token;
-            int head;
-            row_of(r, token, head);
-            x = static_cast<const T*>(a.q) + token * a.qt + head * a.qh;
-        }
+        const T* x = query_of(r);
         float e[G::KS][4];
-        if (a.q_packs) {  // 16 adjacent elements of this lane's columns, by two loads
+        if (a.q_packs) {
 #pragma unroll
-            for (int c = 0; c < G::KS / 4; ++c) {
-                const int d = 16 * (4 * c + q4);
-                Pack<T, 8> w[2];
-                if (x && (EXACT || d < dim)) {
-                    w[0] = *reinterpret_cast<const Pack<T, 8>*>(x + d);
-                    w[1] = *reinterpret_cast<const Pack<T, 8>*>(x + d + 8);
-                } else {
+            for (int c = 0; c < G::KS / 4; ++c)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) w[0].v[j] = w[1].v[j] = from_f32<T>(0.f);
-                }
-#pragma unroll
-                for (int j = 0; j < 16; ++j) e[4 * c + j / 4][j & 3] = to_f32(w[j >> 3].v[j & 7]);
-            }
+                for (int j = 0; j < 16; ++j) e[4 * c + j / 4][j & 3] = to_f32(q_raw[nt][c][j >> 3].v[j & 7]);
         } else {
 #pragma unroll
             for (int ks = 0; ks < G::KS; ++ks)
@@ -562,6 +577,7 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
             }
         }
     }
+    bool any_small = load_scales();
     bool small = __syncthreads_or(any_small);  // a small value scale in the chunk (kPlain), or so far
     if (small) {
         for (int e = tid; e < entries; e += kSplitThreads) to_small(scales[e]);
@@ -816,6 +832,7 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
     ahead = warp;
     for (int s = 0; s < G::STAGES && ahead < tiles; ++s, ahead += kSplitWarps, ++fetched)
         fetch(ahead, (used + s) % G::STAGES);
+    if (tid < entries) scale_raw = fetch_scale(tid);
     any_small = load_scales();
     const bool now_small = __syncthreads_or(any_small) || small;
     if (now_small) {
@@ -1038,7 +1055,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_attention_join(SplitArgs p) {
 // lanes over the dimensions.  The parts of a token are those of its own row tile's items
 // and of its group's.  What the places say is checked against the parts that there are:
 // with tables that contradict themselves it may be anything.
-constexpr int kJoinWarps = 4;
+constexpr int kJoinWarps = 4;  // (8 where a kv head has more than 4 heads)
 
 struct JoinSet {
     const float *parts, *stats;
@@ -1052,16 +1069,17 @@ struct JoinArgs {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) k_attention_join_items(JoinArgs p) {
+__global__ void __launch_bounds__(2 * kJoinWarps * 32) k_attention_join_items(JoinArgs p) {
     const AttentionArgs& a = p.a;
     griddep_wait();
+    constexpr int BATCH = 8;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = a.cache.dim, kv_heads = a.cache.kv_heads;
     const int token = (int)(blockIdx.x / (unsigned)kv_heads), kv = (int)blockIdx.x - token * kv_heads;
     int4 at[2] = {p.set[0].place[token], p.set[1].place[token]};
     const int rows_from = a.seq.starts[0], rows_to = a.seq.starts[a.seq.seqs];
     if (token < rows_from || token >= rows_to || (at[0].w & kPlaceDone)) return;  // no sequence's row, or written
     if (!(at[0].w & kPlacePrefix)) at[1].y = 0;
-    for (int h = warp; h < a.group; h += kJoinWarps) {
+    for (int h = warp; h < a.group; h += (int)(blockDim.x >> 5)) {
         int64_t first[2], step[2];  // row of the first piece's part, rows to the next
         int n[2];
 #pragma unroll
@@ -1076,48 +1094,57 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_attention_join_items(JoinAr
             step[k] = (int64_t)kv_heads * s.rows;
         }
         const int all = n[0] + n[1];
-        auto stat = [&](int c) {
-            const bool own = c < n[0];
-            const float2* st = reinterpret_cast<const float2*>(own ? p.set[0].stats : p.set[1].stats);
-            return st[own ? first[0] + c * step[0] : first[1] + (c - n[0]) * step[1]];
+        auto row_of = [&](int c) { return c < n[0] ? first[0] + c * step[0] : first[1] + (c - n[0]) * step[1]; };
+        auto stat = [&](int c, int64_t row) {
+            return reinterpret_cast<const float2*>(c < n[0] ? p.set[0].stats : p.set[1].stats)[row];
         };
-        float2 v0 = make_float2(-INFINITY, 0.f);  // of piece `lane`
-        if (lane < all) v0 = stat(lane);
-        float top = v0.x;
-        for (int c = lane + 32; c < all; c += 32) top = fmaxf(top, stat(c).x);
+        int64_t row = lane < all ? row_of(lane) : 0;  // of piece `lane`, then of those 32 behind
+        float2 v = lane < all ? stat(lane, row) : make_float2(-INFINITY, 0.f);
+        float top = v.x;
+        for (int c = lane + 32; c < all; c += 32) top = fmaxf(top, stat(c, row_of(c)).x);
 #pragma unroll
         for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
         float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
         float sum = 0.f;
+#pragma unroll 1
         for (int c0 = 0; c0 < all; c0 += 32) {
-            float f = 0.f;
-            if (c0 + lane < all) {
-                const float2 v = c0 ? stat(c0 + lane) : v0;
-                // a NaN sum without a maximum keeps its weight: the row is NaN
-                f = v.y == 0.f ? 0.f : v.x == -INFINITY ? 1.f : exp2_approx(v.x - top);
-                sum += v.y * f;
+            const int c = c0 + lane;
+            if (c0 && c < all) {
+                row = row_of(c);
+                v = stat(c, row);
             }
-            auto take = [&](int k, int from, int to) {  // pieces [from, to) of set k among these 32
-                const int before = k ? n[0] : 0;
-                const float* o = p.set[k].parts + (first[k] + (int64_t)(from - before) * step[k]) * dim + lane * 4;
-                const int64_t stride = step[k] * dim;
-#pragma unroll 8
-                for (int c = from; c < to; ++c, o += stride) {
-                    const float g = __shfl_sync(0xffffffffu, f, c - c0);
+            // a NaN sum without a maximum keeps its weight: the row is NaN
+            const float f = c >= all || v.y == 0.f ? 0.f : v.x == -INFINITY ? 1.f : exp2_approx(v.x - top);
+            if (c < all) sum += v.y * f;
+            const float* part = (c < n[0] ? p.set[0].parts : p.set[1].parts) + row * dim;
+            const int m = min(32, all - c0);
+#pragma unroll 1
+            for (int j0 = 0; j0 < m; j0 += BATCH) {  // parts in flight together
+                float4 x[BATCH][2];
+                float g[BATCH];
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) {
+                    const int from = j0 + j < m ? j0 + j : 0;
+                    g[j] = j0 + j < m ? __shfl_sync(0xffffffffu, f, from) : 0.f;
+                    const float4* o = reinterpret_cast<const float4*>(
+                        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(part), from));
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        x[j][q] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (g[j] != 0.f && (q * 32 + lane) * 4 < dim) x[j][q] = o[q * 32 + lane];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j)
 #pragma unroll
                     for (int q = 0; q < 2; ++q)
-                        if (g != 0.f && (q * 32 + lane) * 4 < dim) {
-                            const float4 x = *reinterpret_cast<const float4*>(o + q * 128);
-                            acc[q].x += x.x * g;
-                            acc[q].y += x.y * g;
-                            acc[q].z += x.z * g;
-                            acc[q].w += x.w * g;
+                        if (g[j] != 0.f) {  // 0 times what is not there may be NaN
+                            acc[q].x += x[j][q].x * g[j];
+                            acc[q].y += x[j][q].y * g[j];
+                            acc[q].z += x[j][q].z * g[j];
+                            acc[q].w += x[j][q].w * g[j];
                         }
-                }
-            };
-            const int end = min(c0 + 32, all), mid = min(max(n[0], c0), end);
-            take(0, c0, mid);
-            take(1, mid, end);
+            }
         }
 #pragma unroll
         for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);

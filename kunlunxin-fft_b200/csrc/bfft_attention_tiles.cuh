@@ -234,25 +234,71 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
     griddep_wait();
     const int dim = a.cache.dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lg = a.cache.page_log2;
 
+    unsigned char* q_s = align_smem<1024>(smem_raw);
+    unsigned char* t_s = q_s + 2 * G::Q_HALF;
+    unsigned char* raw_s = t_s + G::T_RING * G::T_BUF;
+    BlockScale* scale_s = reinterpret_cast<BlockScale*>(raw_s + G::RAW_RING * G::RAW_BUF);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(scale_s + G::SLOTS * G::GROUPS);
+    uint64_t *raw_full = bars, *raw_empty = raw_full + G::RAW_RING, *t_full = raw_empty + G::RAW_RING,
+             *t_empty = t_full + G::T_RING, *scale_full = t_empty + G::T_RING, *s_full = scale_full + G::SLOTS,
+             *p_half = s_full + 2, *p_full = p_half + 2, *q_full = p_full + 2, *q_raw = q_full + 1, *o_full = q_raw + 1,
+             *drained = o_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + G::BARS);
+    int* tile_kind = reinterpret_cast<int*>(bars + G::BARS + 1);  // of a tile: 0 where all its blocks are ordinary
+    volatile int* small_s = tile_kind + G::SLOTS;                 // whether the chunk has a small value scale
+    if (tid == 0) {
+        for (int b = 0; b < G::RAW_RING; ++b) {
+            mbar_init(&raw_full[b], 1);
+            mbar_init(&raw_empty[b], 128);
+        }
+        for (int b = 0; b < G::T_RING; ++b) {
+            mbar_init(&t_full[b], 128);
+            mbar_init(&t_empty[b], 1);
+        }
+        for (int b = 0; b < G::SLOTS; ++b) mbar_init(&scale_full[b], 1);
+        for (int h = 0; h < 2; ++h) {
+            mbar_init(&s_full[h], 1);
+            mbar_init(&p_half[h], 128);
+            mbar_init(&p_full[h], 128);
+            mbar_init(&o_full[h], 1);
+        }
+        mbar_init(q_full, 256);
+        mbar_init(q_raw, 1);
+        mbar_init(drained, 1);
+        *small_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     // which rows and tokens
     int64_t i = blockIdx.x;
     int chunk, kv;
-    SlotRows sr;
+    SlotRows sr{};
     Item it{};
     TokenSpan row_span{0, 0, 0};  // kSinks, kGroups: of row tid
+    // Each row comes by the copy engine (64 dims of it to a panel), all rows in flight at once.
+    auto fetch_queries = [&] {
+        if (!a.q_packs || tid >= sr.n * a.group) return;
+        if (tid == 0) mbar_arrive_expect_tx(q_raw, (uint32_t)(sr.n * a.group * dim * 2));
+        const int t = (unsigned)tid / (unsigned)a.group;
+        const T* x = static_cast<const T*>(a.q) + (sr.first + t) * a.qt + (kv * a.group + tid - t * a.group) * a.qh;
+        unsigned char* to = q_s + (tid >> 7) * G::Q_HALF + (tid & 127) * 128;
+        bulk_load(to, x, (uint32_t)(dim < 64 ? dim : 64) * 2, q_raw);
+        if (dim > 64) bulk_load(to + G::Q_PANEL, x + 64, (uint32_t)(dim - 64) * 2, q_raw);
+    };
+    auto wait = [&](uint64_t* b, uint32_t parity) { return mbar_wait_limited(b, parity, p.status); };
     if constexpr (MODE == kGroups) {
-        __shared__ ItemScratch scratch;
-        TokenSpan* spans = reinterpret_cast<TokenSpan*>(align_smem<1024>(smem_raw));  // what the queries take later
+        TokenSpan* spans = reinterpret_cast<TokenSpan*>(t_s);  // what the widened codes take later
         if (tid < 256) spans[tid] = TokenSpan{0, 0, 0};
         const unsigned item = blockIdx.x / (unsigned)a.cache.kv_heads;
         kv = (int)(blockIdx.x - item * a.cache.kv_heads);
-        if (!find_item<G::THREADS>(a, p.span, p.items, (int)item, p.tile_tokens, 1, scratch, it)) return;
-        item_spans<G::THREADS>(a, p.span, it, spans);
-        if (tid < it.n * a.group) row_span = spans[(unsigned)tid / (unsigned)a.group];
+        if (!find_item(a, p.span, p.items, (int)item, p.tile_tokens, 1, it)) return;
         chunk = it.chunk;
         sr.s = it.table_row;
         sr.first = it.token;
         sr.n = it.n;
+        __syncthreads();
+        fetch_queries();
+        item_spans<G::THREADS>(a, p.span, it, spans);
+        if (tid < it.n * a.group) row_span = spans[(unsigned)tid / (unsigned)a.group];
     } else {
         chunk = (int)(i % p.chunks);
         i /= p.chunks;
@@ -338,6 +384,7 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
         head = kv * a.group + (r - t * a.group);
     };
     if (base >= end) {  // nothing of the axis in this chunk
+        if (MODE == kGroups && a.q_packs) wait(q_raw, 0);  // the queries are under way
         for (int r = tid; r < rows; r += G::THREADS) {
             int64_t token;
             int head;
@@ -362,53 +409,16 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
     const int tiles = (int)((end - base + G::N - 1) / G::N);
     const int halves = rows > 128 ? 2 : 1;
 
-    unsigned char* q_s = align_smem<1024>(smem_raw);
-    unsigned char* t_s = q_s + 2 * G::Q_HALF;
-    unsigned char* raw_s = t_s + G::T_RING * G::T_BUF;
-    BlockScale* scale_s = reinterpret_cast<BlockScale*>(raw_s + G::RAW_RING * G::RAW_BUF);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(scale_s + G::SLOTS * G::GROUPS);
-    uint64_t *raw_full = bars, *raw_empty = raw_full + G::RAW_RING, *t_full = raw_empty + G::RAW_RING,
-             *t_empty = t_full + G::T_RING, *scale_full = t_empty + G::T_RING, *s_full = scale_full + G::SLOTS,
-             *p_half = s_full + 2, *p_full = p_half + 2, *q_full = p_full + 2, *q_raw = q_full + 1, *o_full = q_raw + 1,
-             *drained = o_full + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + G::BARS);
-    int* tile_kind = reinterpret_cast<int*>(bars + G::BARS + 1);  // of a tile: 0 where all its blocks are ordinary
-    volatile int* small_s = tile_kind + G::SLOTS;                 // whether the chunk has a small value scale
     if (warp == 13) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                      "r"(G::TMEM)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (tid == 0) {
-        for (int b = 0; b < G::RAW_RING; ++b) {
-            mbar_init(&raw_full[b], 1);
-            mbar_init(&raw_empty[b], 128);
-        }
-        for (int b = 0; b < G::T_RING; ++b) {
-            mbar_init(&t_full[b], 128);
-            mbar_init(&t_empty[b], 1);
-        }
-        for (int b = 0; b < G::SLOTS; ++b) mbar_init(&scale_full[b], 1);
-        for (int h = 0; h < 2; ++h) {
-            mbar_init(&s_full[h], 1);
-            mbar_init(&p_half[h], 128);
-            mbar_init(&p_full[h], 128);
-            mbar_init(&o_full[h], 1);
-        }
-        mbar_init(q_full, 256);
-        mbar_init(q_raw, 1);
-        mbar_init(drained, 1);
-        *small_s = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (a.q_packs) mbar_arrive_expect_tx(q_raw, (uint32_t)(rows * dim * 2));
-    }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = *tmem_slot;
-    auto wait = [&](uint64_t* b, uint32_t parity) { return mbar_wait_limited(b, parity, p.status); };
-
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::ROW_REGS));
         // ------------------------------------------------------------ rows
@@ -417,24 +427,17 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
         int64_t token = 0;
         int head = 0;
         if (mine) row_of(r, token, head);
-        // Each thread's row comes by the copy engine (64 dims of it to a panel), all rows in
-        // flight at once, and is brought to float16 and the swizzle in its place: DP / 8 lanes
-        // to a row, in a short loop, as this runs once and from a cold instruction cache.
-        // (Loads into registers took 9700 clocks with warm instructions, 18000 with cold ones.)
+        // The queries, brought to float16 and the swizzle in their place: DP / 8 lanes to a
+        // row, in a short loop, as this runs once and from a cold instruction cache.  (Loads
+        // into registers took 9700 clocks with warm instructions, 18000 with cold ones.)
         float up = 1.f;
         bool ok = true;
         {
             constexpr int LANES = DP / 8, ROWS = 32 / LANES, AHEAD = 4;  // lanes of a row, rows at a time
             const int c = lane % LANES, sub = lane / LANES;
             const T* x = static_cast<const T*>(a.q) + token * a.qt + head * a.qh;
-            if (a.q_packs) {
-                if (mine) {
-                    unsigned char* to = q_s + h * G::Q_HALF + (r & 127) * 128;
-                    bulk_load(to, x, (uint32_t)(dim < 64 ? dim : 64) * 2, q_raw);
-                    if (dim > 64) bulk_load(to + G::Q_PANEL, x + 64, (uint32_t)(dim - 64) * 2, q_raw);
-                }
-                ok = wait(q_raw, 0);
-            }
+            if (MODE != kGroups) fetch_queries();
+            if (a.q_packs) ok = wait(q_raw, 0);
             unsigned char* q_row = q_s + h * G::Q_HALF + (c >> 3) * G::Q_PANEL + ((warp & 3) << 5) * 128;
 #pragma unroll 1
             for (int i = 0; i < LANES; i += AHEAD) {
@@ -627,6 +630,7 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                 }
                 written(&p_full[h]);
             }
+            griddep_launch_dependents();  // the next kernel's CTAs may be placed as these end
             if (ok) ok = !__any_sync(0xffffffffu, !wait(&o_full[h], 0));
             if (ok) {
                 tmem_fence_after();
@@ -689,12 +693,12 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
 #pragma unroll
             for (int k = 0; k < PER; ++k)
                 w[k] = inside_head ? *reinterpret_cast<const uint4*>(src + k * STEP * dim) : make_uint4(0, 0, 0, 0);
-            if (value) {
+            const int64_t tok0 = base + (int64_t)j * G::N;
+            bool whole = tok0 >= lo_min && tok0 + G::N <= hi_max;
+            if (MODE != kPlain) whole = whole || tok0 + G::N <= axis.sinks_any;
+            if (value && !(whole && tile_kind[j % G::SLOTS] == 0)) {
                 // codes that no row sees may be anything: as values they become zeros (0 times NaN is NaN)
-                const int64_t tok0 = base + (int64_t)j * G::N;
                 const BlockScale* bs = scale_s + (j % G::SLOTS) * G::GROUPS;
-                bool whole = tok0 >= lo_min && tok0 + G::N <= hi_max;
-                if (MODE != kPlain) whole = whole || tok0 + G::N <= axis.sinks_any;
 #pragma unroll
                 for (int k = 0; k < PER; ++k) {
                     const int row = row0 + k * STEP;
