@@ -235,7 +235,14 @@ GroupPlan plan_groups(const bfft_cache_desc* c, const bfft_sequence_desc* q, con
         x.most = x.target + 2 + ((prefixes ? q->tokens / tile + w->n_groups : 0) + (own ? q->tokens / tile + q->seqs : 0)) * parts;
         return x;
     };
-    p.split_items = items(!p.prefix_tiles, !p.own_tiles, s.tile_tokens, s.token_tiles, 2 * 3 * (int64_t)sms, 256, 32);
+    // Two waves of CTAs' worth of items of the few-row kernel, one of the row tiles: 200
+    // sequences of 16..2048 own tokens take 445 us (four waves: 466), 64 of 16..1024 over a
+    // prefix of 16384 77 us (prefix in two waves: 98).  A piece costs a CTA's start, so none
+    // is short where there are row tiles for every CTA's place (the 64: pieces of 256 on 77
+    // us, of 512 74, of 1024 75); where there are few, 256 (5 sequences 15.1 us, of 512 15.4).
+    const int64_t own_units = (q->tokens / s.tile_tokens + q->seqs) * s.token_tiles * kv;
+    const int least = own_units >= 3 * (int64_t)sms ? 512 : 256;
+    p.split_items = items(!p.prefix_tiles, !p.own_tiles, s.tile_tokens, s.token_tiles, 2 * 3 * (int64_t)sms, least, 32);
     p.tile_items = items(p.prefix_tiles, p.own_tiles, p.tiles.tile_tokens, 1, sms, 512, 128);
     const bool split = !p.own_tiles, tiles = p.prefix_tiles;
     s.ctas = split ? p.split_items.most * kv : 0;
@@ -264,19 +271,22 @@ cudaError_t run_groups(const AttentionArgs& a, const SpanArgs& w, const GroupPla
     float* tile_parts = reinterpret_cast<float*>(ws + p.tile_parts_at);
     float* tile_stats = tile_parts + p.tiles.ctas * 256 * c->dim;
     cudaError_t e = cudaSuccess;
-    auto listed = [&](ItemArgs x, bool list, size_t at, int tile, int parts) {
+    auto list_of = [&](ItemArgs& x, bool list, size_t at, int tile, int parts) {
+        ListArgs l{};
         x.own_of = own_of;
         x.prefix_of = prefix_of;
-        if (!list || e != cudaSuccess) return x;
-        int* count = reinterpret_cast<int*>(ws + at);
-        Item* items = reinterpret_cast<Item*>(ws + at) + 1;
-        e = list_items(a, w, x, tile, parts, items, count, s);
-        x.list = items;
-        x.count = count;
-        return x;
+        if (!list) return l;
+        l = ListArgs{x, tile, parts, reinterpret_cast<Item*>(ws + at) + 1, reinterpret_cast<int*>(ws + at)};
+        x.list = l.list;
+        x.count = l.count;
+        return l;
     };
-    const ItemArgs tile_items = listed(p.tile_items, p.tile_list, p.tile_items_at, p.tiles.tile_tokens, 1);
-    const ItemArgs split_items = listed(p.split_items, p.split_list, p.split_items_at, p.split.tile_tokens, p.split.token_tiles);
+    ItemArgs tile_items = p.tile_items, split_items = p.split_items;
+    const ListArgs tile_list = list_of(tile_items, p.tile_list, p.tile_items_at, p.tiles.tile_tokens, 1);
+    const ListArgs split_list = list_of(split_items, p.split_list, p.split_items_at, p.split.tile_tokens, p.split.token_tiles);
+    if (tile_list.list) e = run_list(a, w, tile_list, s);
+    // where row tiles run too, one of their blocks does it on the way
+    if (split_list.list && !p.tiles.ctas) e = run_list(a, w, split_list, s);
     if (e != cudaSuccess) return e;
     if (p.tiles.ctas) {
         TileArgs t{};
@@ -287,6 +297,7 @@ cudaError_t run_groups(const AttentionArgs& a, const SpanArgs& w, const GroupPla
         t.status = status;
         t.span = w;
         t.items = tile_items;
+        t.others = split_list;
         e = run_tiles<T, kGroups>(t, p.tiles, c, s);
     }
     if (e == cudaSuccess && p.split.ctas) {
@@ -403,7 +414,7 @@ bfft_status attention_call(const bfft_cache_desc* cache, const bfft_sequence_des
         const GroupPlan p = plan_groups(cache, seqs, d, w, sms);
         st = room(p.split.ctas > p.tiles.ctas ? p.split.ctas : p.tiles.ctas, p.bytes);
         if (st != BFFT_OK) return st;
-        count_launches(1 + (p.split.ctas > 0) + (p.tiles.ctas > 0) + p.split_list + p.tile_list);
+        count_launches(1 + (p.split.ctas > 0) + (p.tiles.ctas > 0) + (p.split_list && !p.tiles.ctas) + p.tile_list);
         char* ws = static_cast<char*>(d->workspace);
         return launched(d->type == BFFT_F16 ? run_groups<__half>(a, span, p, cache, ws, status, s)
                                             : run_groups<__nv_bfloat16>(a, span, p, cache, ws, status, s),

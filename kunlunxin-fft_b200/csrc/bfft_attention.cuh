@@ -71,7 +71,7 @@ cudaError_t launch_tiles(const TileArgs& a, const TilePlan& p, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         ready[dev].store(true, std::memory_order_release);
     }
-    return launch_dependent(kernel, (unsigned)p.ctas, G::THREADS, G::SMEM, s, a);
+    return launch_dependent(kernel, (unsigned)p.ctas + (MODE == kGroups && a.others.list != nullptr), G::THREADS, G::SMEM, s, a);
 }
 
 template <typename T>
@@ -163,14 +163,15 @@ cudaError_t run_split(const SplitArgs& a, const SplitPlan& p, const bfft_cache_d
 
 
 // Compiled in bfft_attention_groups.cu.
-cudaError_t list_items(const AttentionArgs& a, const SpanArgs& p, const ItemArgs& x, int tile, int parts, Item* list,
-                       int* count, cudaStream_t s);
+cudaError_t run_list(const AttentionArgs& a, const SpanArgs& p, const ListArgs& l, cudaStream_t s);
 
 template <typename T>
 cudaError_t run_join_items(const JoinArgs& a, cudaStream_t s) {
-    return launch_dependent(k_attention_join_items<T>, (unsigned)(a.a.seq.tokens * a.a.cache.kv_heads),
-                            (a.a.group > kJoinWarps ? 2 : 1) * kJoinWarps * 32, 0,
-                            s, a);
+    const unsigned blocks = (unsigned)(a.a.seq.tokens * a.a.cache.kv_heads);
+    const unsigned threads = (a.a.group > kJoinWarps ? 2 : 1) * kJoinWarps * 32;
+    if (a.a.cache.dim > 128) return launch_dependent(k_attention_join_items<T, 2, 4>, blocks, threads, 0, s, a);
+    return blocks <= 1024 ? launch_dependent(k_attention_join_items<T, 1, 8>, blocks, threads, 0, s, a)
+                          : launch_dependent(k_attention_join_items<T, 1, 4>, blocks, threads, 0, s, a);
 }
 
 // Compiled in bfft_attention_sinks.cu and bfft_attention_groups.cu.

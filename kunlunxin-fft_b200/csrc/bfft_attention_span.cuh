@@ -251,6 +251,70 @@ __device__ __forceinline__ bool find_item(const AttentionArgs& a, const SpanArgs
     return true;
 }
 
+// Lists the items of more units, by one block: long pieces before short ones (in sixteen
+// classes), as blocks start in the order of their items.  The order within a class is that
+// of the atomics; a token's parts are joined in the order of its axis wherever they lie.
+constexpr int kListThreads = 512;
+struct ListArgs {
+    ItemArgs items;
+    int tile, parts;  // query tokens of a row tile, tiles of a token
+    Item* list;       // null: nothing to list
+    int* count;
+};
+__device__ __forceinline__ void list_items(const AttentionArgs& a, const SpanArgs& p, const ListArgs& l) {
+    constexpr int WARPS = kListThreads / 32, CLASSES = 16;
+    __shared__ float sums[WARPS];
+    __shared__ int first[CLASSES];
+    const ItemArgs& x = l.items;
+    const int tile = l.tile, parts = l.parts;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int groups = x.prefixes ? p.n_groups : 0, units = unit_count(p, x, a.seq.seqs);
+    if (tid < CLASSES) first[tid] = 0;
+    float total = 0.f;
+    unsigned chunk = 1;
+    // three looks at every unit: the sum, the classes' counts, the items
+#pragma unroll 1
+    for (int look = 0; look < 3; ++look) {
+#pragma unroll 1
+        for (int u = tid; u < units; u += kListThreads) {
+            const Unit v = unit_of(a, p, x, u, tile, parts);
+            if (look == 0) {
+                total += (float)v.tiles * (float)v.length;
+                continue;
+            }
+            const int pieces = pieces_of(v, chunk), mine = v.tiles * pieces;
+            const unsigned each = ((unsigned)v.length + pieces - 1) / pieces;
+            const int of = CLASSES - 1 - (int)min(each * (float)CLASSES / (float)chunk, CLASSES - 1.f);
+            const int at = mine ? atomicAdd(&first[of], mine) : 0;
+            if (look == 2)
+                for (int k = 0; k < mine && at + k < x.most; ++k)
+                    fill_item(l.list[at + k], v, u < groups, k, pieces, tile, parts);
+        }
+        if (look == 0) {
+#pragma unroll
+            for (int w = 16; w; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
+            if (lane == 0) sums[warp] = total;
+            __syncthreads();
+            total = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) total += sums[w];
+            chunk = item_tokens(x, total);
+        } else if (look == 1) {
+            __syncthreads();
+            if (tid == 0) {
+                int sum = 0;
+                for (int c = 0; c < CLASSES; ++c) {
+                    const int n = first[c];
+                    first[c] = sum;
+                    sum += n;
+                }
+                *l.count = sum < x.most ? sum : (int)x.most;
+            }
+            __syncthreads();
+        }
+    }
+}
+
 // What the item's rows see of its tokens, a query token each, in shared memory, after a
 // barrier behind which `spans` holds empty ones.  A group's rows are found from its sequences, a thread each:
 // each row's own search of its sequence took 3900 clocks.

@@ -1068,11 +1068,13 @@ struct JoinArgs {
     JoinSet set[2];  // own tokens, prefixes
 };
 
-template <typename T>
-__global__ void __launch_bounds__(2 * kJoinWarps * 32) k_attention_join_items(JoinArgs p) {
+// Q: float4 of a row in a lane.  BATCH: parts in flight together, eight where there are few
+// rows, as each waits for memory a few times over; four where there are many, for more CTAs
+// on an SM (3696 CTAs of 8 warps: 42 us with 97 registers a thread).
+template <typename T, int Q, int BATCH>
+__global__ void __launch_bounds__(2 * kJoinWarps * 32, BATCH == 8 ? 2 : 5) k_attention_join_items(JoinArgs p) {
     const AttentionArgs& a = p.a;
     griddep_wait();
-    constexpr int BATCH = 8;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = a.cache.dim, kv_heads = a.cache.kv_heads;
     const int token = (int)(blockIdx.x / (unsigned)kv_heads), kv = (int)blockIdx.x - token * kv_heads;
     int4 at[2] = {p.set[0].place[token], p.set[1].place[token]};
@@ -1104,7 +1106,9 @@ __global__ void __launch_bounds__(2 * kJoinWarps * 32) k_attention_join_items(Jo
         for (int c = lane + 32; c < all; c += 32) top = fmaxf(top, stat(c, row_of(c)).x);
 #pragma unroll
         for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-        float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+        float4 acc[Q];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
         float sum = 0.f;
 #pragma unroll 1
         for (int c0 = 0; c0 < all; c0 += 32) {
@@ -1117,28 +1121,30 @@ __global__ void __launch_bounds__(2 * kJoinWarps * 32) k_attention_join_items(Jo
             const float f = c >= all || v.y == 0.f ? 0.f : v.x == -INFINITY ? 1.f : exp2_approx(v.x - top);
             if (c < all) sum += v.y * f;
             const float* part = (c < n[0] ? p.set[0].parts : p.set[1].parts) + row * dim;
-            const int m = min(32, all - c0);
-#pragma unroll 1
-            for (int j0 = 0; j0 < m; j0 += BATCH) {  // parts in flight together
-                float4 x[BATCH][2];
+            // those that count, a batch in flight together (0 times what was not written may be NaN)
+            unsigned left = __ballot_sync(0xffffffffu, f != 0.f);
+            while (left) {
+                float4 x[BATCH][Q];
                 float g[BATCH];
 #pragma unroll
                 for (int j = 0; j < BATCH; ++j) {
-                    const int from = j0 + j < m ? j0 + j : 0;
-                    g[j] = j0 + j < m ? __shfl_sync(0xffffffffu, f, from) : 0.f;
-                    const float4* o = reinterpret_cast<const float4*>(
-                        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(part), from));
+                    g[j] = 0.f;
+                    if (left) {
+                        const int from = __ffs(left) - 1;
+                        left &= left - 1;
+                        g[j] = __shfl_sync(0xffffffffu, f, from);
+                        const float4* o = reinterpret_cast<const float4*>(
+                            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(part), from));
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        x[j][q] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (g[j] != 0.f && (q * 32 + lane) * 4 < dim) x[j][q] = o[q * 32 + lane];
+                        for (int q = 0; q < Q; ++q)
+                            if ((q * 32 + lane) * 4 < dim) x[j][q] = o[q * 32 + lane];
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < BATCH; ++j)
+                    if (g[j] != 0.f)
 #pragma unroll
-                    for (int q = 0; q < 2; ++q)
-                        if (g[j] != 0.f) {  // 0 times what is not there may be NaN
+                        for (int q = 0; q < Q; ++q) {
                             acc[q].x += x[j][q].x * g[j];
                             acc[q].y += x[j][q].y * g[j];
                             acc[q].z += x[j][q].z * g[j];
@@ -1152,7 +1158,7 @@ __global__ void __launch_bounds__(2 * kJoinWarps * 32) k_attention_join_items(Jo
         const int head = kv * a.group + h;
         T* y = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q < Q; ++q) {
             const int d = (q * 32 + lane) * 4;
             if (d < dim) {
                 Pack<T, 4> w;

@@ -51,6 +51,7 @@ struct TileArgs {
     unsigned int* status;
     SpanArgs span;
     ItemArgs items;    // kGroups
+    ListArgs others;   // kGroups: the few-row kernel's items, which block 0 lists
 };
 
 template <int DP>
@@ -233,6 +234,15 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
     const AttentionArgs& a = p.a;
     griddep_wait();
     const int dim = a.cache.dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lg = a.cache.page_log2;
+    unsigned block = blockIdx.x;
+    if (MODE == kGroups && p.others.list) {
+        static_assert(kListThreads == G::THREADS, "a block lists");
+        if (block == 0) {
+            list_items(a, p.span, p.others);
+            return;
+        }
+        --block;
+    }
 
     unsigned char* q_s = align_smem<1024>(smem_raw);
     unsigned char* t_s = q_s + 2 * G::Q_HALF;
@@ -288,8 +298,8 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
     if constexpr (MODE == kGroups) {
         TokenSpan* spans = reinterpret_cast<TokenSpan*>(t_s);  // what the widened codes take later
         if (tid < 256) spans[tid] = TokenSpan{0, 0, 0};
-        const unsigned item = blockIdx.x / (unsigned)a.cache.kv_heads;
-        kv = (int)(blockIdx.x - item * a.cache.kv_heads);
+        const unsigned item = block / (unsigned)a.cache.kv_heads;
+        kv = (int)(block - item * a.cache.kv_heads);
         if (!find_item(a, p.span, p.items, (int)item, p.tile_tokens, 1, it)) return;
         chunk = it.chunk;
         sr.s = it.table_row;
@@ -367,11 +377,11 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
         if (kv == 0 && chunk == 0 && tid < sr.n) {
             const int flags = (direct ? kPlaceDone : 0) | (!it.prefix && it.shares ? kPlacePrefix : 0);
             (it.prefix ? p.items.prefix_of : p.items.own_of)[sr.first + tid] =
-                make_int4((int)(blockIdx.x / a.cache.kv_heads), it.chunks, tid * a.group, flags);
+                make_int4((int)(block / (unsigned)a.cache.kv_heads), it.chunks, tid * a.group, flags);
         }
     }
     auto part_of = [&](int64_t token, int head, int r) {
-        return MODE == kGroups ? (int64_t)blockIdx.x * 256 + r : (token * a.q_heads + head) * p.chunks + chunk;
+        return MODE == kGroups ? (int64_t)block * 256 + r : (token * a.q_heads + head) * p.chunks + chunk;
     };
     // a sequence token at a place of the axis
     auto token_at = [&](int64_t t) -> int64_t {
