@@ -121,14 +121,19 @@ struct AxisMap {
 };
 
 // Roots of unit u for the token whose first position is element `at`; NaN for the pairs of
-// an axis whose row the table lacks.  The positions of all axes load side by side.  A unit
-// within one axis (runs of pairs) loads its roots as packs, another (pairs dealt in turn)
-// eight bytes a pair: both from a row or two of a table that stays in L2, once for a
-// token's heads.
+// an axis whose row the table lacks.  A unit within one axis (runs of pairs) needs that
+// axis's position and loads its roots as packs, as with one axis; another (pairs dealt in
+// turn) loads the positions of all axes side by side and eight bytes a pair.
 template <int P>
 __device__ __forceinline__ void load_axis_roots(const float2* __restrict__ table, int64_t rows, int pairs, const AxisMap& m,
                                                 const void* positions, int pos64, int64_t at, int u, float (&c)[P],
                                                 float (&s)[P]) {
+    constexpr uint32_t UNIT = (1u << 2 * P) - 1;
+    const uint32_t which = (m.of[(u * P) >> 4] >> (2 * ((u * P) & 15))) & UNIT;
+    if (which == ((which & 3) * 0x55555555u & UNIT)) {
+        load_roots<P>(table, rows, pairs, position_at(positions, pos64, at + (which & 3) * m.stride), u, c, s);
+        return;
+    }
     int row[4];
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
@@ -138,15 +143,10 @@ __device__ __forceinline__ void load_axis_roots(const float2* __restrict__ table
             if (p >= 0 && p < rows) row[a] = (int)p;
         }
     }
-    auto pick = [&](uint32_t a) { return a < 2 ? (a ? row[1] : row[0]) : (a == 2 ? row[2] : row[3]); };
-    const uint32_t which = (m.of[(u * P) >> 4] >> (2 * ((u * P) & 15))) & ((1u << 2 * P) - 1);
-    if (which == ((which & 3) * 0x55555555u & ((1u << 2 * P) - 1))) {
-        load_roots<P>(table, rows, pairs, pick(which & 3), u, c, s);
-        return;
-    }
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const int r = pick((which >> (2 * i)) & 3);
+        const uint32_t a = (which >> (2 * i)) & 3;
+        const int r = a < 2 ? (a ? row[1] : row[0]) : (a == 2 ? row[2] : row[3]);
         float2 w = make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
         if (r >= 0) w = table[(int64_t)r * pairs + u * P + i];
         c[i] = w.x;
@@ -227,28 +227,61 @@ __device__ __forceinline__ void rotate_heads(const T* x, T* y, int64_t xh, int64
     }
 }
 
+// Root of pair j for the token whose first position is element `at`.
+__device__ __forceinline__ float2 axis_root(const float2* __restrict__ table, int64_t rows, int pairs, const AxisMap& m,
+                                            const void* positions, int pos64, int64_t at, int j) {
+    const int64_t p = position_at(positions, pos64, at + ((m.of[j >> 4] >> (2 * (j & 15))) & 3) * m.stride);
+    return p >= 0 && p < rows ? table[p * pairs + j] : make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
+}
+// The roots of the tokens that a block rotates, in shared memory: neighbouring threads load
+// neighbouring pairs, each once (16384 tokens of 32 heads, axes dealt in turn: 53 us where
+// each thread loaded its own eight bytes at a time).
+
 template <typename T, int P, int LAYOUT, typename Axes>
 __global__ void __launch_bounds__(256, 3) k_rotate(RotateArgs a, const __grid_constant__ Axes axes) {
     griddep_wait();
     griddep_launch_dependents();
+    constexpr bool AXES = std::is_same_v<Axes, AxisMap>;
     const int u = threadIdx.x;
     const int64_t slot = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const int64_t row = slot / a.groups;
-    if (row >= a.rows) return;
     const int g = (int)(slot - row * a.groups);
     const int64_t b = row / a.tokens, t = row - b * a.tokens;
+    const float2* mine = nullptr;  // this token's roots
+    if constexpr (AXES) {
+        extern __shared__ float2 roots[];
+        const int pairs = a.shape.rotated / 2;
+        const int64_t row0 = (int64_t)blockIdx.x * blockDim.y / a.groups;
+        int64_t rows = ((int64_t)(blockIdx.x + 1) * blockDim.y - 1) / a.groups + 1;
+        if (rows > a.rows) rows = a.rows;
+        const int count = (int)(rows - row0) * pairs;
+        for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < count; i += blockDim.x * blockDim.y) {
+            const int r = i / pairs;
+            const int64_t rb = (row0 + r) / a.tokens, rt = row0 + r - rb * a.tokens;
+            const int j = i - r * pairs;  // pair j is the unit j / P's pair j % P: a unit's pairs lie rot_units apart
+            roots[r * pairs + j % P * a.shape.rot_units + j / P] =
+                axis_root(a.table, a.table_rows, pairs, axes, a.positions, a.pos64, rb * a.pb + rt * a.pt, j);
+        }
+        __syncthreads();
+        mine = roots + (row - row0) * pairs + u;
+    }
+    if (row >= a.rows) return;
     int o0, o1;
     unit_offsets<P, LAYOUT>(a.shape, u, o0, o1);
     rotate_heads<T, P, LAYOUT>(static_cast<const T*>(a.x) + b * a.xb + t * a.xt, static_cast<T*>(a.y) + b * a.yb + t * a.yt,
                                a.xh, a.yh, a.heads, g, a.groups, o0, o1, u < a.shape.rot_units, a.sign,
                                [&](float (&c)[P], float (&s)[P]) {
-                                   const int64_t at = b * a.pb + t * a.pt;
-                                   if constexpr (std::is_same_v<Axes, AxisMap>)
-                                       load_axis_roots<P>(a.table, a.table_rows, a.shape.rotated / 2, axes, a.positions,
-                                                          a.pos64, at, u, c, s);
-                                   else
+                                   if constexpr (AXES) {
+#pragma unroll
+                                       for (int i = 0; i < P; ++i) {
+                                           const float2 w = mine[i * a.shape.rot_units];
+                                           c[i] = w.x;
+                                           s[i] = w.y;
+                                       }
+                                   } else {
                                        load_roots<P>(a.table, a.table_rows, a.shape.rotated / 2,
-                                                     position_at(a.positions, a.pos64, at), u, c, s);
+                                                     position_at(a.positions, a.pos64, b * a.pb + t * a.pt), u, c, s);
+                                   }
                                });
 }
 
@@ -629,8 +662,10 @@ __global__ void __launch_bounds__(256, 3) k_rotate_new(AppendArgs a, const __gri
 // ---------------------------------------------------------------- launches
 template <typename T, int P, typename Axes>
 cudaError_t rotate_layout(int layout, const RotateArgs& a, const Axes& x, dim3 grid, dim3 block, cudaStream_t s) {
-    if (layout == BFFT_PAIRS_HALF) return launch_dependent(k_rotate<T, P, BFFT_PAIRS_HALF, Axes>, grid.x, block, 0, s, a, x);
-    return launch_dependent(k_rotate<T, P, BFFT_PAIRS_INTERLEAVED, Axes>, grid.x, block, 0, s, a, x);
+    // the roots of a block's tokens (see k_rotate)
+    const size_t smem = std::is_same_v<Axes, AxisMap> ? ((block.y - 1) / a.groups + 2) * (size_t)(a.shape.rotated / 2) * 8 : 0;
+    if (layout == BFFT_PAIRS_HALF) return launch_dependent(k_rotate<T, P, BFFT_PAIRS_HALF, Axes>, grid.x, block, smem, s, a, x);
+    return launch_dependent(k_rotate<T, P, BFFT_PAIRS_INTERLEAVED, Axes>, grid.x, block, smem, s, a, x);
 }
 template <typename T, typename Axes>
 cudaError_t rotate_pack(int p, int layout, const RotateArgs& a, const Axes& x, dim3 grid, dim3 block, cudaStream_t s) {
