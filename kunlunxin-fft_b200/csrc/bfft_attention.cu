@@ -55,6 +55,21 @@ bool encode_codes(CUtensorMap* m, const void* codes, const bfft_cache_desc* c) {
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_queries(CUtensorMap* m, const AttentionArgs& a, bool half, int tile_tokens) {
+    EncodeTiledFn enc = encoder();
+    const int64_t heads = a.q_heads, dim = a.cache.dim;
+    // (the stride of a dimension of one is not used, and a map takes no zero)
+    const int64_t head = heads > 1 ? a.qh : dim, token = a.seq.tokens > 1 ? a.qt : heads * dim;
+    if (!enc || !a.q_packs || head <= 0 || token <= 0 || token >= (int64_t)1 << 38 || head >= (int64_t)1 << 38) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)a.seq.tokens};
+    cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)token * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)tile_tokens};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return enc(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), dims,
+               strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace bfft
 
 namespace {
@@ -434,7 +449,8 @@ bfft_status attention_call(const bfft_cache_desc* cache, const bfft_sequence_des
     float* stats = parts ? parts + seqs->tokens * d->q_heads * chunks * cache->dim : nullptr;
     count_launches(chunks > 1 && !sp.cluster ? 2 : 1);
     const TileArgs ta{a,           parts,    stats,  tp.chunk, tp.chunks, tp.tile_tokens,
-                      tp.by_token, tp.slots, status, span,     {}};
+                      tp.by_token, tp.slots, status, 0,        span,      {},
+                      {}};
     const SplitArgs sa{a,           parts,    stats,      sp.chunk,   sp.chunks, sp.tile_tokens, sp.token_tiles,
                        sp.by_token, sp.slots, sp.cluster, sp.entries, status,    span,           {}};
     e = form == kSinks ? run_plan<kSinks>(tiles, ta, tp, sa, sp, d->type, cache, s)

@@ -11,6 +11,7 @@
 
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/bfft.h"
 #include "bfft_async.cuh"
@@ -56,9 +57,12 @@ struct SplitPlan {
 
 // Defined in bfft_attention.cu: a map of the codes for boxes of 16 tokens.
 bool encode_codes(CUtensorMap* m, const void* codes, const bfft_cache_desc* c);
+// A map of the queries for boxes of 64 dims, a kv head's heads and a row tile's tokens; false
+// where rows and strides do not start on 16 bytes.
+bool encode_queries(CUtensorMap* m, const AttentionArgs& a, bool half, int tile_tokens);
 
 template <int DP, typename T, int CODE, int MODE>
-cudaError_t launch_tiles(const TileArgs& a, const TilePlan& p, cudaStream_t s) {
+cudaError_t launch_tiles(TileArgs a, const TilePlan& p, cudaStream_t s) {
     static std::atomic<bool> ready[64];
     using G = TileGeo<DP>;
     int dev = 0;
@@ -71,7 +75,9 @@ cudaError_t launch_tiles(const TileArgs& a, const TilePlan& p, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         ready[dev].store(true, std::memory_order_release);
     }
-    return launch_dependent(kernel, (unsigned)p.ctas + (MODE == kGroups && a.others.list != nullptr), G::THREADS, G::SMEM, s, a);
+    CUtensorMap queries{};
+    a.q_tma = encode_queries(&queries, a.a, std::is_same_v<T, __half>, a.tile_tokens);
+    return launch_dependent(kernel, (unsigned)p.ctas + (MODE == kGroups && a.others.list != nullptr), G::THREADS, G::SMEM, s, a, queries);
 }
 
 template <typename T>

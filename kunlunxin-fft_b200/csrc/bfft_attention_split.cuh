@@ -1072,7 +1072,7 @@ struct JoinArgs {
 // rows, as each waits for memory a few times over; four where there are many, for more CTAs
 // on an SM (3696 CTAs of 8 warps: 42 us with 97 registers a thread).
 template <typename T, int Q, int BATCH>
-__global__ void __launch_bounds__(2 * kJoinWarps * 32, BATCH == 8 ? 2 : 5) k_attention_join_items(JoinArgs p) {
+__global__ void __launch_bounds__(2 * kJoinWarps * 32, BATCH == 8 || Q == 2 ? 2 : 5) k_attention_join_items(JoinArgs p) {
     const AttentionArgs& a = p.a;
     griddep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = a.cache.dim, kv_heads = a.cache.kv_heads;

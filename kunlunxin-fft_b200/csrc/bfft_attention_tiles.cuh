@@ -49,6 +49,7 @@ struct TileArgs {
     int by_token;
     int64_t slots;
     unsigned int* status;
+    int q_tma;         // the queries come by the map (else they are loaded element by element)
     SpanArgs span;
     ItemArgs items;    // kGroups
     ListArgs others;   // kGroups: the few-row kernel's items, which block 0 lists
@@ -228,7 +229,7 @@ __device__ __forceinline__ void write_rows(unsigned char* stage, uint32_t o_addr
 }
 
 template <int DP, typename T, int CODE, int MODE>
-__global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(TileArgs p) {
+__global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(TileArgs p, const __grid_constant__ CUtensorMap qmap) {
     using G = TileGeo<DP>;
     extern __shared__ unsigned char smem_raw[];
     const AttentionArgs& a = p.a;
@@ -284,15 +285,15 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
     SlotRows sr{};
     Item it{};
     TokenSpan row_span{0, 0, 0};  // kSinks, kGroups: of row tid
-    // Each row comes by the copy engine (64 dims of it to a panel), all rows in flight at once.
+    // The tile's rows by one box a panel, in the swizzle that the products read: tokens that
+    // are not the tile's come along and are no one's rows.  (A copy a row and panel took 7000
+    // clocks, 13 a copy.)
     auto fetch_queries = [&] {
-        if (!a.q_packs || tid >= sr.n * a.group) return;
-        if (tid == 0) mbar_arrive_expect_tx(q_raw, (uint32_t)(sr.n * a.group * dim * 2));
-        const int t = (unsigned)tid / (unsigned)a.group;
-        const T* x = static_cast<const T*>(a.q) + (sr.first + t) * a.qt + (kv * a.group + tid - t * a.group) * a.qh;
-        unsigned char* to = q_s + (tid >> 7) * G::Q_HALF + (tid & 127) * 128;
-        bulk_load(to, x, (uint32_t)(dim < 64 ? dim : 64) * 2, q_raw);
-        if (dim > 64) bulk_load(to + G::Q_PANEL, x + 64, (uint32_t)(dim - 64) * 2, q_raw);
+        if (!p.q_tma || tid != 0) return;
+        mbar_arrive_expect_tx(q_raw, (uint32_t)(G::PANELS * p.tile_tokens * a.group * 128));
+#pragma unroll
+        for (int panel = 0; panel < G::PANELS; ++panel)
+            tma_load_3d(q_s + panel * 2 * G::Q_PANEL, &qmap, panel * 64, kv * a.group, (int)sr.first, q_raw);
     };
     auto wait = [&](uint64_t* b, uint32_t parity) { return mbar_wait_limited(b, parity, p.status); };
     if constexpr (MODE == kGroups) {
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
         head = kv * a.group + (r - t * a.group);
     };
     if (base >= end) {  // nothing of the axis in this chunk
-        if (MODE == kGroups && a.q_packs) wait(q_raw, 0);  // the queries are under way
+        if (MODE == kGroups && p.q_tma) wait(q_raw, 0);  // the queries are under way
         for (int r = tid; r < rows; r += G::THREADS) {
             int64_t token;
             int head;
@@ -437,42 +438,37 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
         int64_t token = 0;
         int head = 0;
         if (mine) row_of(r, token, head);
-        // The queries, brought to float16 and the swizzle in their place: DP / 8 lanes to a
-        // row, in a short loop, as this runs once and from a cold instruction cache.  (Loads
-        // into registers took 9700 clocks with warm instructions, 18000 with cold ones.)
+        // The queries, brought to float16 in their place, DP / 8 lanes to a row, in a short
+        // loop: it runs once, from a cold instruction cache.  (Loads into registers took 9700
+        // clocks with warm instructions, 18000 with cold ones.)
         float up = 1.f;
         bool ok = true;
         {
             constexpr int LANES = DP / 8, ROWS = 32 / LANES, AHEAD = 4;  // lanes of a row, rows at a time
             const int c = lane % LANES, sub = lane / LANES;
-            const T* x = static_cast<const T*>(a.q) + token * a.qt + head * a.qh;
             if (MODE != kGroups) fetch_queries();
-            if (a.q_packs) ok = wait(q_raw, 0);
-            unsigned char* q_row = q_s + h * G::Q_HALF + (c >> 3) * G::Q_PANEL + ((warp & 3) << 5) * 128;
+            if (p.q_tma) ok = wait(q_raw, 0);
+            const int64_t at = token * a.qt + head * a.qh;
+            unsigned char* q_row = q_s + (c >> 3) * 2 * G::Q_PANEL + (warp << 5) * 128;
+            const bool as_they_are = p.q_tma && std::is_same_v<T, __half>;
 #pragma unroll 1
-            for (int i = 0; i < LANES; i += AHEAD) {
+            for (int i = 0; i < (as_they_are ? 0 : LANES); i += AHEAD) {
                 Pack<T, 8> w[AHEAD];
 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j) {
                     const int row = (i + j) * ROWS + sub;
-                    if ((warp << 5) + row >= rows || 8 * c >= dim)
-                        w[j] = Pack<T, 8>{};
-                    else
-                        w[j] = *reinterpret_cast<const Pack<T, 8>*>(q_row + row * 128 + ((c & 7) << 4));
+                    w[j] = *reinterpret_cast<const Pack<T, 8>*>(q_row + row * 128 + (((c & 7) ^ (row & 7)) << 4));
                 }
-                if (!a.q_packs) {
-                    const int64_t own = reinterpret_cast<intptr_t>(x);
+                if (!p.q_tma) {
 #pragma unroll
                     for (int j = 0; j < AHEAD; ++j) {
                         const int row = (i + j) * ROWS + sub;
-                        const T* y = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, own, row)) + 8 * c;
-                        if ((warp << 5) + row < rows && 8 * c < dim) {
+                        const T* y = static_cast<const T*>(a.q) + __shfl_sync(0xffffffffu, at, row) + 8 * c;
+                        const bool has = (warp << 5) + row < rows && 8 * c < dim;
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) w[j].v[k] = y[k];
-                        }
+                        for (int k = 0; k < 8; ++k) w[j].v[k] = has ? y[k] : from_f32<T>(0.f);
                     }
                 }
-                __syncwarp();  // a line's lanes have read it
 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j) {
                     const int row = (i + j) * ROWS + sub;
@@ -837,11 +833,11 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                        v_low = desc_low(smem_u32(t_s), G::PANEL);
         auto scores = [&](int h, int j) {
             const int buf = 2 * j % G::T_RING;
-            const uint32_t qa = q_low + (h ? G::Q_HALF >> 4 : 0), ka = k_low + buf * (G::T_BUF >> 4);
+            const uint32_t qa = q_low + (h ? G::Q_PANEL >> 4 : 0), ka = k_low + buf * (G::T_BUF >> 4);
             const uint32_t d = tmem + G::S0 + h * 128;
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
-                mma_ss(d, qa + (((k >> 2) * G::Q_PANEL + (k & 3) * 32) >> 4),
+                mma_ss(d, qa + (((k >> 2) * 2 * G::Q_PANEL + (k & 3) * 32) >> 4),
                        ka + (((k >> 2) * G::PANEL + (k & 3) * 32) >> 4), qk, k > 0);
             mma_commit(&s_full[h]);
             if (h == halves - 1) mma_commit(&t_empty[buf]);
