@@ -422,9 +422,10 @@ typedef struct bfft_span_desc {
  * sequences of a group name the same pages for their first shared[g] tokens; the whole
  * pages of these are read from the row of the block table of the group's first sequence,
  * once for the group's rows.  `groups` ascends; sequences outside it share nothing.  The
- * results are those of rows that read their own pages.  Tables up to 2^30 tokens wide.
- * The workspace with groups: each row tile's parts, those of some six waves of CTAs more
- * and, for prefixes on the tensor cores, 256 rows for each CTA. */
+ * results are those of rows that read their own pages, but for roundings.  Tables up to
+ * 2^30 tokens wide.  The workspace with groups holds the row tiles' parts and those of some
+ * waves of CTAs more, 512 MB at most: calls that would need more, and calls with 256 rows
+ * or more to a sequence and kv head, are made as without groups. */
 BFFT_EXPORT bfft_status bfft_cache_attention_span_workspace(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
                                                             const bfft_attention_desc* desc, const bfft_span_desc* span,
                                                             size_t* bytes);

@@ -277,7 +277,7 @@ def cache_attention(q, cache, block_table, lens, starts, *, softmax_scale: float
     sequence.  The results are those of a call without, but for roundings.  Sequences in
     no group share nothing.  Worth it for few rows a sequence: from 256 rows a kv head on
     (query tokens times heads) a sequence fills the kernel's row tiles by itself and the
-    call goes without.
+    call goes without, as it does where its workspace would pass 512 MB.
 
     The weights, times their block's value scale, are rounded to float16 before they
     meet the codes, with a row's largest near float16's top: to 2^-11 down to 2^-24 of

@@ -215,12 +215,6 @@ struct GroupPlan {
     size_t places, split_items_at, tile_items_at, split_parts_at, tile_parts_at, bytes;  // of the workspace
 };
 
-// Sequences that have many rows each fill their row tiles by themselves: sharing saves them
-// nothing, and the prefix is a part of their own tokens like any other.
-bool worth_sharing(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d) {
-    return q->tokens / q->seqs * (d->q_heads / c->kv_heads) < 256;
-}
-
 GroupPlan plan_groups(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d,
                       const bfft_span_desc* w, int sms) {
     GroupPlan p{};
@@ -274,6 +268,15 @@ GroupPlan plan_groups(const bfft_cache_desc* c, const bfft_sequence_desc* q, con
     p.tile_parts_at = p.split_parts_at + (size_t)(s.ctas * rows) * (size_t)(c->dim + 2) * 4;
     p.bytes = p.tile_parts_at + (size_t)(p.tiles.ctas * 256) * (size_t)(c->dim + 2) * 4;
     return p;
+}
+
+// Sequences that have many rows each fill their row tiles by themselves: sharing saves them
+// nothing, and the prefix is a part of their own tokens like any other.  So it is where the
+// parts, two or more of each row, would take more than 512 MB.
+bool worth_sharing(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d,
+                   const bfft_span_desc* w) {
+    return q->tokens / q->seqs * (d->q_heads / c->kv_heads) < 256 &&
+           plan_groups(c, q, d, w, sm_count(d->device)).bytes <= (size_t)512 << 20;
 }
 
 template <typename T>
@@ -346,7 +349,7 @@ bfft_status check_span(const bfft_cache_desc* cache, const bfft_sequence_desc* s
     if (w->n_groups && (!w->shared || (!w->groups && w->n_groups > 1))) return fail(BFFT_ERR_VALUE, "null pointer");
     if (!aligned(w->groups, 4) || !aligned(w->shared, 4)) return fail(BFFT_ERR_VALUE, "misaligned pointer");
     if (!seqs->tokens) return BFFT_OK;
-    if (w->n_groups && worth_sharing(cache, seqs, d))
+    if (w->n_groups && worth_sharing(cache, seqs, d, w))
         *form = kGroups;
     else if (w->sinks && d->window > 0)
         *form = kSinks;

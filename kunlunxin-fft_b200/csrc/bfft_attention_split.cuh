@@ -992,6 +992,8 @@ __global__ void __launch_bounds__(WARPS * 32) k_attention_join(SplitArgs p) {
     const int64_t i = blockIdx.x;
     const int64_t token = i / a.q_heads;
     const int head = (int)(i - token * a.q_heads);
+    const int rows_from = a.seq.starts[0], rows_to = a.seq.starts[a.seq.seqs];
+    if (token < rows_from || token >= rows_to) return;  // no sequence's row: it stays as it is
     const float2* st = reinterpret_cast<const float2*>(p.stats) + i * p.chunks;
     const float* parts = p.parts + i * p.chunks * dim;
     float top = -INFINITY;

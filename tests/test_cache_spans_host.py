@@ -73,3 +73,17 @@ def test_workspaces(lib):
         assert workspace(lib, same, seqs=3, tokens=300, heads=32, dim=128, width=4096, window=window) == plain.value
     narrow, wide = (workspace(lib, span_desc(), seqs=64, tokens=64, heads=32, dim=128, width=w) for w in (4096, 1 << 20))
     assert narrow == wide < 128 << 20
+
+
+def test_workspace_with_groups_is_bounded(lib):
+    """Where the parts would pass 512 MB the call is made, and its workspace counted, as without groups."""
+    for seqs, each, heads in ((64, 1, 32), (4096, 1, 32), (4096, 1, 64), (4096, 31, 64), (20000, 7, 128), (512, 4, 64)):
+        n, plain = ctypes.c_size_t(), ctypes.c_size_t()
+        q = pack_attention(A, A, 0, heads * 128, 128, heads * 128, 128, heads, 2, 1, 0, 1.0, 0, 0, 0)
+        s = pack_sequences(A, 512, A, A, seqs, 512, seqs * each)
+        c = cache_desc(pages=100000, heads=8, page=64, dim=128)
+        assert lib.bfft_cache_attention_span_workspace(c, s, q, span_desc(), ctypes.byref(n)) == _lib.OK
+        assert lib.bfft_cache_attention_workspace(c, s, q, ctypes.byref(plain)) == _lib.OK
+        assert n.value <= 512 << 20 or n.value == plain.value
+        if seqs * each <= 4096:
+            assert n.value <= 512 << 20

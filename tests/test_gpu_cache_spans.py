@@ -289,9 +289,10 @@ def test_shared_many_rows(code, dtype, page, heads, group, dim, each, causal, wi
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("page, dim", [(64, 128), (16, 64), (128, 80)])
 @pytest.mark.parametrize("causal, window, sinks", [(True, 0, 0), (True, 3100, 9), (False, 0, 0)])
-def test_shared_prompts(code, page, dim, causal, window, sinks):
+@pytest.mark.parametrize("groups", [None, [1, 7]])
+def test_shared_prompts(code, page, dim, causal, window, sinks, groups):
     """Questions of some tens of rows behind one text: prefixes and own tokens both on the tensor-core tiles."""
-    prefix, groups = [3500], None
+    prefix = [3500]
     new = [31, 40, 17, 60, 50, 21, 44, 33]
     lens = [3500 + n + 150 * (i % 3) for i, n in enumerate(new)]
     lens[2] = 11                                             # six of whose rows see nothing
@@ -300,6 +301,42 @@ def test_shared_prompts(code, page, dim, causal, window, sinks):
     q = normal(p.g, sum(new), 8, dim, dtype=BF16) * 1.5
     assert 48 <= sum(new) // 8 * 4 < 256 and takes_tiles(p, q, sum(new) // 8, causal=causal, window=window, sinks=sinks)
     check_spans(p, q, lens, new, causal=causal, window=window, sinks=sinks, shared=prefix, groups=groups)
+
+
+@pytest.mark.parametrize("form", ["plain", "sinks", "shared"])
+@pytest.mark.parametrize("dim", [64, 112])
+def test_row_tiles_of_odd_queries(form, dim):
+    """Queries that the copy engine cannot take: rows on odd elements, and one row that stands for many."""
+    seqs, each = 210, 2
+    kw = {"plain": {}, "sinks": {"window": 1900, "sinks": 3}, "shared": {"shared": [1984]}}[form]
+    lens = [2000 + i % 50 for i in range(seqs)] if form == "shared" else [4100, 3000]
+    new = [each] * seqs if form == "shared" else [200, 220]
+    p = Pages(dim, lens, [0] * len(lens), code="int8", page=64, heads=2, dim=dim)
+    if form == "shared":
+        share(p, [1984], [0, seqs])
+    q = normal(p.g, 420, 8, dim + 1, dtype=BF16)[..., 1:]
+    assert takes_tiles(p, q, 420 if form == "shared" else 210, **({} if form == "shared" else kw))
+    check_spans(p, q, lens, new, **kw)
+    same = normal(p.g, 1, 8, dim, dtype=BF16)
+    want = check_spans(p, same.expand(420, 8, dim).contiguous(), lens, new, **kw)
+    got = check_spans(p, same.expand(420, 8, dim), lens, new, **kw)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    head = normal(p.g, 420, 1, dim, dtype=F16)
+    assert torch.equal(check_spans(p, head.expand(420, 8, dim), lens, new, **kw)[0],
+                       check_spans(p, head.expand(420, 8, dim).contiguous(), lens, new, **kw)[0])
+
+
+@pytest.mark.parametrize("new, lens, window", [
+    ([1], [30000], 9000), ([1, 1], [700, 90], 500), ([40], [9000], 5000), ([600, 70], [4100, 800], 2000),
+])
+def test_rows_behind_the_last_sequence_stay(new, lens, window):
+    """Direct, by a cluster, by chunks that a second kernel joins, and by row tiles."""
+    p = Pages(9, lens, [0] * len(lens), code="int8", page=64, heads=2, dim=128)
+    q = normal(p.g, sum(new) + 3, 8, 128, dtype=BF16)
+    for kw in ({"window": window, "sinks": 4}, {"window": window}, {}):
+        left = torch.full_like(q, 7.0)
+        bfft.cache_attention(q, p.cache, p.table, ints(lens), ints(cumulative(new)), out=left, **kw)
+        assert (left[sum(new):] == 7.0).all() and left[:sum(new)].isfinite().all()
 
 
 def test_sharing_is_left_out_where_sequences_have_many_rows():

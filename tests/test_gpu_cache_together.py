@@ -1,0 +1,140 @@
+"""The position and cache calls as a model with images uses them: one text and image that several users ask about.
+
+A prefix of text, image patches and text (positions of three axes) is appended once; each user's block table names
+its pages; the users' questions are appended behind it and answered token by token, once with the whole context and
+once with a window and first tokens that stay visible.  The result is compared with float64 attention over the rows
+before they were coded; the answering step is also captured and replayed.
+"""
+import pytest
+import torch
+
+import bfft
+from test_gpu_cache import BF16, F32, cumulative, generator, ints, normal
+from test_gpu_cache_axes import token_table
+
+pytestmark = pytest.mark.gpu
+
+AXES, ORDER = (16, 24, 24), "cyclic"
+
+
+def positions_of(prefix, tokens):
+    """Text, a 20 x 28 image, text behind it: positions (3, tokens) that the image's larger side advances."""
+    at = torch.arange(tokens)
+    image = prefix // 4
+    patch = (at - image).clamp(0, 559)
+    inside = (at >= image) & (at < image + 560)
+    text = torch.where(at < image, at, at - 560 + 28)
+    return torch.stack([torch.where(inside, image + x, text) for x in (torch.zeros_like(patch), patch // 28, patch % 28)])
+
+
+def exact(q, k, v, roots, new, window, sinks, group):
+    """Attention of a sequence's last `new` rows in float64: rows (tokens, heads, dim), roots (tokens, pairs, 2)."""
+    c, s = roots.double()[:, None].unbind(-1)
+
+    def turn(x, c, s):
+        a, b = x.double().chunk(2, -1)
+        return torch.cat((a * c - b * s, a * s + b * c), -1)
+
+    n = k.shape[0]
+    z = torch.einsum("qhd,khd->hqk", turn(q, c[n - new:], s[n - new:]), turn(k, c, s).repeat_interleave(group, 1))
+    key, pos = torch.arange(n, device="cuda"), torch.arange(n - new, n, device="cuda")[:, None]
+    hidden = key > pos
+    if window:
+        hidden |= (key <= pos - window) & (key >= sinks)
+    z = (z * q.shape[-1] ** -0.5).masked_fill(hidden, float("-inf"))
+    return torch.einsum("hqk,khd->qhd", torch.softmax(z, -1), v.double().repeat_interleave(group, 1))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("users, window, sinks", [(3, 0, 0), (3, 500, 4), (40, 0, 0), (40, 700, 20)])
+def test_users_of_one_image(code, users, window, sinks):
+    g = generator(users)
+    heads, kv, dim, page, prefix, steps = 8, 2, 128, 32, 1600, 3
+    asked = [5 + 13 * s % 60 for s in range(users)]
+    total = [prefix + n + steps for n in asked]
+    longest = max(total)
+    positions = positions_of(prefix, longest).to(torch.int32).cuda()
+    table = bfft.rotary_table(longest, dim, axes=AXES, axis_order=ORDER)
+    roots = token_table(table, positions, AXES, ORDER)
+    common, own = prefix // page, -(-(longest - prefix) // page)
+    cache = bfft.paged_cache(common + users * own, kv, page, dim, code=code)
+    ids = torch.randperm(common + users * own, device="cuda", generator=g).int()
+    pages = torch.cat((ids[:common].expand(users, common), ids[common:].view(users, own)), 1).contiguous()
+    rows = [normal(g, prefix, n, dim, dtype=BF16) for n in (heads, kv, kv)]                       # of the prefix
+    mine = [[normal(g, total[s] - prefix, n, dim, dtype=BF16) for n in (heads, kv, kv)] for s in range(users)]
+    how = {"axes": AXES, "axis_order": ORDER}
+
+    # the prefix, once
+    bfft.append_rotated(cache, rows[1], rows[2], pages[:1], ints([0]), ints([0, prefix]), table,
+                        positions=positions[:, :prefix], **how)
+
+    def step(held, new):
+        q, k, v = (torch.cat([mine[s][i][held[s] - prefix:held[s] - prefix + new[s]] for s in range(users)])
+                   for i in range(3))
+        where = torch.cat([positions[:, held[s]:held[s] + new[s]] for s in range(users)], 1).contiguous()
+        starts = ints(cumulative(new))
+        q = bfft.append_rotated(cache, k, v, pages, ints(held), starts, table, positions=where, q=q, **how)
+        lens = ints([h + n for h, n in zip(held, new)])
+        return bfft.cache_attention(q, cache, pages, lens, starts, window=window, sinks=sinks, shared=ints([prefix])).split(new)
+
+    held = [prefix] * users
+    out = [[y] for y in step(held, asked)]
+    held = [prefix + n for n in asked]
+    for _ in range(steps):
+        for s, y in enumerate(step(held, [1] * users)):
+            out[s].append(y)
+        held = [h + 1 for h in held]
+    for s in range(users):
+        q, k, v = (torch.cat((rows[i], mine[s][i])) for i in range(3))
+        want = exact(mine[s][0], k, v, roots[:total[s]], total[s] - prefix, window, sinks, heads // kv)
+        # a code is off by up to scale / 2 (2^-7.6 of the block's largest, some 3.5 deviations) or 2^-4 of itself, in
+        # the mean 1 / sqrt 3 of it, keys the same; the bounds of the example that decodes without images
+        error = (torch.cat(out[s]).double() - want).norm() / want.norm()
+        assert error < (0.03 if code == "int8" else 0.06)
+
+    # the answering step captured: tables on the device say where the users are
+    q, k, v = (normal(g, users, n, dim, dtype=BF16) for n in (heads, kv, kv))
+    at, lens, starts = ints([h - 1 for h in held]), ints(held), ints(list(range(users + 1)))
+    where, shared = positions[:, [h - 1 for h in held]].contiguous(), ints([prefix])
+
+    def answer():
+        r = bfft.append_rotated(cache, k, v, pages, at, starts, table, positions=where, q=q, **how)
+        return bfft.cache_attention(r, cache, pages, lens, starts, window=window, sinks=sinks, shared=shared)
+
+    want = answer()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = answer()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_training_of_queries_and_keys_with_axes():
+    """Gradients through the rotation of queries and keys into plain attention, against float64 autograd."""
+    g = generator(1)
+    tokens, heads, dim = 120, 3, 32
+    axes = (4, 6, 6)
+    table = bfft.rotary_table(64, dim, axes=axes, spectrum="axial")
+    positions = torch.randint(0, 64, (3, tokens), device="cuda", generator=g)
+    q, k, v, w = (normal(g, tokens, heads, dim, dtype=F32) for _ in range(4))
+
+    def attend(q, k, v):
+        z = torch.einsum("qhd,khd->hqk", q, k) * dim ** -0.5
+        return torch.einsum("hqk,khd->qhd", torch.softmax(z, -1), v)
+
+    x = [t.clone().requires_grad_(True) for t in (q, k)]
+    y = attend(*(bfft.rotate_positions(t, positions, table, axes=axes) for t in x), v)
+    got = torch.autograd.grad(y, x, w)
+    c, s = token_table(table, positions, axes, "blocks").double()[:, None].unbind(-1)
+
+    def turn(t):
+        a, b = t.chunk(2, -1)
+        return torch.cat((a * c - b * s, a * s + b * c), -1)
+
+    x = [t.double().requires_grad_(True) for t in (q, k)]
+    want = torch.autograd.grad(attend(turn(x[0]), turn(x[1]), v.double()), x, w.double())
+    for a, b in zip(got, want):
+        # sums of 120 products of values around 1 in 32 bits, three deep
+        assert (a.double() - b).abs().max() <= 2.0 ** -24 * 1000 * b.abs().max()
