@@ -275,9 +275,10 @@ def cache_attention(q, cache, block_table, lens, starts, *, softmax_scale: float
     all are one group) share their first ``shared[g]`` tokens (int32, (groups,)): the whole
     pages among these are read once for the group, from the block table's row of its first
     sequence.  The results are those of a call without, but for roundings.  Sequences in
-    no group share nothing.  Worth it for few rows a sequence: from 256 rows a kv head on
-    (query tokens times heads) a sequence fills the kernel's row tiles by itself and the
-    call goes without, as it does where its workspace would pass 512 MB.
+    no group share nothing.  The call goes without where that is as fast: over 128 rows a
+    kv head (query tokens times heads) of a sequence, where the prefixes would be under 24
+    MB to read again, were they as long as the table is wide, and where the workspace
+    would pass 512 MB.
 
     The weights, times their block's value scale, are rounded to float16 before they
     meet the codes, with a row's largest near float16's top: to 2^-11 down to 2^-24 of

@@ -204,140 +204,163 @@ TilePlan plan_tiles(const bfft_cache_desc* c, const bfft_sequence_desc* q, const
     return p;
 }
 
-// A call with groups: which kernel takes the prefixes and which the sequences' own tokens,
-// and the items and the workspace of each.
+// A call with groups: one launch for the prefixes and the sequences' own tokens where both
+// go to one kernel, else two.
+struct GroupLaunch {
+    bool prefixes, own, tiles;
+    SplitPlan split;      // nt, tile_tokens, token_tiles, entries, ctas
+    TilePlan row_tiles;   // tile_tokens, ctas
+    ItemArgs items;
+    bool list;            // the items are listed first
+    size_t list_at, parts_at;  // of the workspace
+    int tile_tokens() const { return tiles ? row_tiles.tile_tokens : split.tile_tokens; }
+    int token_tiles() const { return tiles ? 1 : split.token_tiles; }
+    int rows() const { return tiles ? 256 : 8 * split.nt; }
+    int64_t ctas() const { return tiles ? row_tiles.ctas : split.ctas; }
+};
 struct GroupPlan {
-    bool prefix_tiles, own_tiles;
-    SplitPlan split;   // nt, tile_tokens, token_tiles, entries, ctas
-    TilePlan tiles;    // tile_tokens, ctas
-    ItemArgs split_items, tile_items;
-    bool split_list, tile_list;  // items that are listed first
-    size_t places, split_items_at, tile_items_at, split_parts_at, tile_parts_at, bytes;  // of the workspace
+    GroupLaunch launch[2];
+    int launches;
+    size_t bytes;  // of the workspace: places of the tokens' parts, then per launch its list and parts
 };
 
 GroupPlan plan_groups(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d,
                       const bfft_span_desc* w, int sms) {
-    GroupPlan p{};
     const int64_t group = d->q_heads / c->kv_heads, kv = c->kv_heads;
     const int64_t each = q->tokens / q->seqs + (q->tokens % q->seqs != 0), shared = q->tokens / w->n_groups;
-    p.own_tiles = use_tiles(c, q, d, w->sinks);
+    const bool own_tiles = use_tiles(c, q, d, w->sinks);
     // as use_tiles, for a group's rows
-    p.prefix_tiles = p.own_tiles;
-    if (!p.prefix_tiles && c->dim <= 128 && group <= 128 && shared * group >= 48)
-        p.prefix_tiles = (double)q->tokens * (double)d->q_heads * (double)seen_cover(c, q, d, 1, 1, w->sinks) *
-                             (double)c->dim >= 3.0e6 * 128;
-    SplitPlan& s = p.split;
-    s.nt = (p.prefix_tiles ? each : shared) * group > 8 && c->dim <= 128 ? 2 : 1;
-    const int64_t rows = 8 * s.nt;
-    s.tile_tokens = group <= rows ? (int)(rows / group) : 1;
-    s.token_tiles = group <= rows ? 1 : (int)((group + rows - 1) / rows);
-    s.entries = 384;
-    p.tiles.tile_tokens = (int)(256 / (group < 256 ? group : 256));
-    auto items = [&](bool prefixes, bool own, int64_t tile, int64_t parts, int64_t wanted, int least, int unit) {
-        ItemArgs x{};
-        x.prefixes = prefixes;
-        x.own = own;
-        x.target = (int)(wanted / kv > 0 ? wanted / kv : 1);
-        x.least = least;
-        x.unit = unit;
-        // every row tile may end with a piece that is not full
-        x.most = x.target + 2 + ((prefixes ? q->tokens / tile + w->n_groups : 0) + (own ? q->tokens / tile + q->seqs : 0)) * parts;
-        return x;
-    };
-    // Two waves of CTAs' worth of items of the few-row kernel, one of the row tiles: 200
-    // sequences of 16..2048 own tokens take 445 us (four waves: 466), 64 of 16..1024 over a
-    // prefix of 16384 77 us (prefix in two waves: 98).  A piece costs a CTA's start, so none
-    // is short where there are row tiles for every CTA's place (the 64: pieces of 256 on 77
-    // us, of 512 74, of 1024 75); where there are few, 256 (5 sequences 15.1 us, of 512 15.4).
-    const int64_t own_units = (q->tokens / s.tile_tokens + q->seqs) * s.token_tiles * kv;
-    const int least = own_units >= 3 * (int64_t)sms ? 512 : 256;
-    p.split_items = items(!p.prefix_tiles, !p.own_tiles, s.tile_tokens, s.token_tiles, 2 * 3 * (int64_t)sms, least, 32);
-    p.tile_items = items(p.prefix_tiles, p.own_tiles, p.tiles.tile_tokens, 1, sms, 512, 128);
-    const bool split = !p.own_tiles, tiles = p.prefix_tiles;
-    s.ctas = split ? p.split_items.most * kv : 0;
-    p.tiles.ctas = tiles ? p.tile_items.most * kv : 0;
-    SpanArgs counts{};
-    counts.n_groups = (int)w->n_groups;
-    p.split_list = split && unit_count(counts, p.split_items, (int)q->seqs) > kFewUnits;
-    p.tile_list = tiles && unit_count(counts, p.tile_items, (int)q->seqs) > kFewUnits;
-    // places, the items' lists (behind a count), the parts
-    p.places = (size_t)q->tokens * 2 * sizeof(int4);
-    p.split_items_at = (p.places + 63) / 64 * 64;
-    p.tile_items_at = p.split_items_at + (p.split_list ? (size_t)(p.split_items.most + 1) * sizeof(Item) : 0);
-    p.split_parts_at = p.tile_items_at + (p.tile_list ? (size_t)(p.tile_items.most + 1) * sizeof(Item) : 0);
-    p.tile_parts_at = p.split_parts_at + (size_t)(s.ctas * rows) * (size_t)(c->dim + 2) * 4;
-    p.bytes = p.tile_parts_at + (size_t)(p.tiles.ctas * 256) * (size_t)(c->dim + 2) * 4;
+    const bool prefix_tiles =
+        own_tiles || (c->dim <= 128 && group <= 128 && shared * group >= 48 &&
+                      (double)q->tokens * (double)d->q_heads * (double)seen_cover(c, q, d, 1, 1, w->sinks) * (double)c->dim >=
+                          3.0e6 * 128);
+    // The few-row kernel's row tiles have 16 rows where a group's rows (a sequence's, where the
+    // prefixes go to the row tiles) fill more than 8.  One launch takes prefixes and own tokens
+    // then: two, with tiles of 8 rows for the sequences, are slower (8 sequences over 2048 + 200
+    // tokens 16.4 us by one, 24.9 by two; 64 in 8 groups over 4096 + 300 82 and 92).
+    auto tiles_of = [&](int64_t rows) { return rows * group > 8 && c->dim <= 128 ? 2 : 1; };
+    const int prefix_nt = prefix_tiles ? 0 : tiles_of(shared);
+    const int own_nt = own_tiles ? 0 : prefix_tiles ? tiles_of(each) : prefix_nt;
+    GroupPlan p{};
+    p.launches = prefix_nt == own_nt ? 1 : 2;
+    size_t at = ((size_t)q->tokens * 2 * sizeof(int4) + 63) / 64 * 64;
+    for (int k = 0; k < p.launches; ++k) {
+        GroupLaunch& l = p.launch[k];
+        l.prefixes = k == 0;
+        l.own = k == p.launches - 1;
+        const int nt = l.own ? own_nt : prefix_nt;
+        l.tiles = nt == 0;
+        if (l.tiles) {
+            l.row_tiles.tile_tokens = (int)(256 / group);
+        } else {
+            l.split.nt = nt;
+            const int64_t rows = 8 * nt;
+            l.split.tile_tokens = group <= rows ? (int)(rows / group) : 1;
+            l.split.token_tiles = group <= rows ? 1 : (int)((group + rows - 1) / rows);
+            l.split.entries = 384;
+        }
+        // Items: of the row tiles one wave of CTAs' worth (64 sequences over a prefix of 16384 77
+        // us, in two waves 98), of the few-row kernel two, one where there are few sequences, as
+        // in plan_split (200 sequences of 16..2048 own tokens 445 us, in four waves 466).  A
+        // piece costs a CTA's start, so none is short where there are row tiles for every
+        // CTA's place (the 64 with 16..1024 tokens of their own: pieces of 256 on 77 us, of 512
+        // 74, of 1024 75).
+        const int64_t units = ((l.prefixes ? q->tokens / l.tile_tokens() + w->n_groups : 0) +
+                               (l.own ? q->tokens / l.tile_tokens() + q->seqs : 0)) * l.token_tiles();
+        const int64_t places = (int64_t)sms * (l.tiles ? 1 : nt == 1 && c->dim <= 128 ? 3 : 2);
+        const int64_t wanted = places * (!l.tiles && l.own && q->seqs > 8 ? 2 : 1) / kv;
+        l.items.prefixes = l.prefixes;
+        l.items.own = l.own;
+        l.items.target = (int)(wanted > 0 ? wanted : 1);
+        l.items.least = l.tiles || units * kv >= places ? 512 : 256;
+        l.items.unit = l.tiles ? 128 : 32;
+        l.items.most = l.items.target + 2 + units;  // every row tile may end with a piece that is not full
+        (l.tiles ? l.row_tiles.ctas : l.split.ctas) = l.items.most * kv;
+        SpanArgs counts{};
+        counts.n_groups = (int)w->n_groups;
+        l.list = unit_count(counts, l.items, (int)q->seqs) > kFewUnits;
+        l.list_at = at;
+        at += l.list ? (size_t)(l.items.most + 1) * sizeof(Item) : 0;  // behind a count
+        l.parts_at = at;
+        at += ((size_t)l.ctas() * l.rows() * (size_t)(c->dim + 2) * 4 + 63) / 64 * 64;
+    }
+    p.bytes = at;
     return p;
 }
 
-// Sequences that have many rows each fill their row tiles by themselves: sharing saves them
-// nothing, and the prefix is a part of their own tokens like any other.  So it is where the
-// parts, two or more of each row, would take more than 512 MB.
+// Sharing saves the bytes of a prefix for each sequence but the first of a group, and costs
+// a second and a third launch.  The host knows the table's width, which is the prefix and
+// what follows, and so the most that can be saved: under 24 MB (4 sequences over 2048 tokens
+// of 8 kv heads of 128: 12.1 us alone, 14.6 shared; 8: 18.8 and 16.4) the call goes without.
+// So it does where a sequence's rows fill the 128 of half a row tile by themselves (16
+// sequences of 240 rows over 8192 tokens: 154 and 211), and where the parts, two or more of
+// each row, would take more than 512 MB.
 bool worth_sharing(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d,
                    const bfft_span_desc* w) {
-    return q->tokens / q->seqs * (d->q_heads / c->kv_heads) < 256 &&
-           plan_groups(c, q, d, w, sm_count(d->device)).bytes <= (size_t)512 << 20;
+    if (q->tokens / q->seqs * (d->q_heads / c->kv_heads) > 128) return false;
+    const double saved = (double)(q->seqs - w->n_groups) * (double)seen_cover(c, q, d, 1, 1, w->sinks) *
+                         (double)(c->kv_heads * c->dim * 2);
+    return saved >= 24.0e6 && plan_groups(c, q, d, w, sm_count(d->device)).bytes <= (size_t)512 << 20;
 }
 
 template <typename T>
 cudaError_t run_groups(const AttentionArgs& a, const SpanArgs& w, const GroupPlan& p, const bfft_cache_desc* c, char* ws,
                        unsigned int* status, cudaStream_t s) {
-    int4* own_of = reinterpret_cast<int4*>(ws);
-    int4* prefix_of = own_of + a.seq.tokens;
-    float* split_parts = reinterpret_cast<float*>(ws + p.split_parts_at);
-    float* split_stats = split_parts + p.split.ctas * 8 * p.split.nt * c->dim;  // 16-byte aligned, as all parts are
-    float* tile_parts = reinterpret_cast<float*>(ws + p.tile_parts_at);
-    float* tile_stats = tile_parts + p.tiles.ctas * 256 * c->dim;
+    int4* places[2] = {reinterpret_cast<int4*>(ws), reinterpret_cast<int4*>(ws) + a.seq.tokens};  // own, prefixes
+    JoinArgs join{a, {}};
+    ListArgs lists[2]{};
+    for (int k = 0; k < p.launches; ++k) {
+        const GroupLaunch& l = p.launch[k];
+        ItemArgs x = l.items;
+        x.own_of = places[0];
+        x.prefix_of = places[1];
+        if (l.list) {
+            x.count = reinterpret_cast<int*>(ws + l.list_at);
+            x.list = reinterpret_cast<Item*>(ws + l.list_at) + 1;
+        }
+        lists[k] = ListArgs{x, l.tile_tokens(), l.token_tiles(), const_cast<Item*>(x.list), const_cast<int*>(x.count)};
+    }
     cudaError_t e = cudaSuccess;
-    auto list_of = [&](ItemArgs& x, bool list, size_t at, int tile, int parts) {
-        ListArgs l{};
-        x.own_of = own_of;
-        x.prefix_of = prefix_of;
-        if (!list) return l;
-        l = ListArgs{x, tile, parts, reinterpret_cast<Item*>(ws + at) + 1, reinterpret_cast<int*>(ws + at)};
-        x.list = l.list;
-        x.count = l.count;
-        return l;
-    };
-    ItemArgs tile_items = p.tile_items, split_items = p.split_items;
-    const ListArgs tile_list = list_of(tile_items, p.tile_list, p.tile_items_at, p.tiles.tile_tokens, 1);
-    const ListArgs split_list = list_of(split_items, p.split_list, p.split_items_at, p.split.tile_tokens, p.split.token_tiles);
-    if (tile_list.list) e = run_list(a, w, tile_list, s);
-    // where row tiles run too, one of their blocks does it on the way
-    if (split_list.list && !p.tiles.ctas) e = run_list(a, w, split_list, s);
-    if (e != cudaSuccess) return e;
-    if (p.tiles.ctas) {
-        TileArgs t{};
-        t.a = a;
-        t.parts = tile_parts;
-        t.stats = tile_stats;
-        t.tile_tokens = p.tiles.tile_tokens;
-        t.status = status;
-        t.span = w;
-        t.items = tile_items;
-        t.others = split_list;
-        e = run_tiles<T, kGroups>(t, p.tiles, c, s);
+    const bool on_the_way = p.launches == 2 && p.launch[0].tiles && lists[1].list;  // a block of the row tiles lists
+    for (int k = 0; k < p.launches && e == cudaSuccess; ++k)
+        if (lists[k].list && !(k == 1 && on_the_way)) e = run_list(a, w, lists[k], s);
+    for (int k = 0; k < p.launches && e == cudaSuccess; ++k) {
+        const GroupLaunch& l = p.launch[k];
+        float* parts = reinterpret_cast<float*>(ws + l.parts_at);
+        float* stats = parts + l.ctas() * l.rows() * c->dim;
+        for (int set = 0; set < 2; ++set)
+            if (set ? l.prefixes : l.own) join.set[set] = JoinSet{parts, stats, places[set], l.rows(), l.ctas()};
+        if (l.tiles) {
+            TileArgs t{};
+            t.a = a;
+            t.parts = parts;
+            t.stats = stats;
+            t.tile_tokens = l.row_tiles.tile_tokens;
+            t.status = status;
+            t.span = w;
+            t.items = lists[k].items;
+            if (k == 0 && on_the_way) t.others = lists[1];
+            e = run_tiles<T, kGroups>(t, l.row_tiles, c, s);
+        } else {
+            SplitArgs t{};
+            t.a = a;
+            t.parts = parts;
+            t.stats = stats;
+            t.tile_tokens = l.split.tile_tokens;
+            t.token_tiles = l.split.token_tiles;
+            t.entries = l.split.entries;
+            t.status = status;
+            t.span = w;
+            t.items = lists[k].items;
+            e = run_split<T, kGroups>(t, l.split, c, s);
+        }
     }
-    if (e == cudaSuccess && p.split.ctas) {
-        SplitArgs t{};
-        t.a = a;
-        t.parts = split_parts;
-        t.stats = split_stats;
-        t.tile_tokens = p.split.tile_tokens;
-        t.token_tiles = p.split.token_tiles;
-        t.entries = p.split.entries;
-        t.status = status;
-        t.span = w;
-        t.items = split_items;
-        e = run_split<T, kGroups>(t, p.split, c, s);
-    }
-    if (e != cudaSuccess) return e;
-    const JoinSet split{split_parts, split_stats, nullptr, 8 * p.split.nt, p.split.ctas};
-    const JoinSet tiles{tile_parts, tile_stats, nullptr, 256, p.tiles.ctas};
-    JoinArgs j{a, {p.own_tiles ? tiles : split, p.prefix_tiles ? tiles : split}};
-    j.set[0].place = own_of;
-    j.set[1].place = prefix_of;
-    return run_join_items<T>(j, s);
+    return e == cudaSuccess ? run_join_items<T>(join, s) : e;
+}
+int group_launches(const GroupPlan& p) {
+    int n = p.launches + 1;
+    for (int k = 0; k < p.launches; ++k) n += p.launch[k].list && !(k == 1 && p.launch[0].tiles);
+    return n;
 }
 
 // The form of a call: sinks matter beside a window only.
@@ -430,9 +453,10 @@ bfft_status attention_call(const bfft_cache_desc* cache, const bfft_sequence_des
         span.shared = static_cast<const int32_t*>(w->shared);
         span.n_groups = (int)w->n_groups;
         const GroupPlan p = plan_groups(cache, seqs, d, w, sms);
-        st = room(p.split.ctas > p.tiles.ctas ? p.split.ctas : p.tiles.ctas, p.bytes);
+        st = room(p.launch[p.launches - 1].ctas() > p.launch[0].ctas() ? p.launch[p.launches - 1].ctas() : p.launch[0].ctas(),
+                  p.bytes);
         if (st != BFFT_OK) return st;
-        count_launches(1 + (p.split.ctas > 0) + (p.tiles.ctas > 0) + (p.split_list && !p.tiles.ctas) + p.tile_list);
+        count_launches(group_launches(p));
         char* ws = static_cast<char*>(d->workspace);
         return launched(d->type == BFFT_F16 ? run_groups<__half>(a, span, p, cache, ws, status, s)
                                             : run_groups<__nv_bfloat16>(a, span, p, cache, ws, status, s),

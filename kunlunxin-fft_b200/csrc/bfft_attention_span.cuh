@@ -286,9 +286,21 @@ __device__ __forceinline__ void list_items(const AttentionArgs& a, const SpanArg
             const unsigned each = ((unsigned)v.length + pieces - 1) / pieces;
             const int of = CLASSES - 1 - (int)min(each * (float)CLASSES / (float)chunk, CLASSES - 1.f);
             const int at = mine ? atomicAdd(&first[of], mine) : 0;
-            if (look == 2)
-                for (int k = 0; k < mine && at + k < x.most; ++k)
-                    fill_item(l.list[at + k], v, u < groups, k, pieces, tile, parts);
+            if (look == 1) continue;
+            // a warp writes the items of its lanes' units, the many of a group side by side
+            const unsigned active = __activemask();
+            for (unsigned left = active; left; left &= left - 1) {
+                const int from = __ffs(left) - 1;
+                Unit w;
+                const int* fields = reinterpret_cast<const int*>(&v);
+                int* out = reinterpret_cast<int*>(&w);
+#pragma unroll
+                for (int k = 0; k < (int)(sizeof(Unit) / 4); ++k) out[k] = __shfl_sync(active, fields[k], from);
+                const int n = __shfl_sync(active, mine, from), to = __shfl_sync(active, at, from),
+                          each_of = __shfl_sync(active, pieces, from), prefix = __shfl_sync(active, (int)(u < groups), from);
+                for (int k = __popc(active & ((1u << lane) - 1)); k < n && to + k < x.most; k += __popc(active))
+                    fill_item(l.list[to + k], w, prefix, k, each_of, tile, parts);
+            }
         }
         if (look == 0) {
 #pragma unroll

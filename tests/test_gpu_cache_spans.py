@@ -77,6 +77,21 @@ def takes_tiles(p, q, rows, *, causal=True, window=0, sinks=0, table=None):
             and q.shape[0] * q.shape[1] * cover(p, table, causal, window, sinks) * p.dim >= 3e6 * 128)
 
 
+def shares(p, q, seqs, groups, *, causal=True, window=0, sinks=0):
+    """Groups are told apart from 24 MB of re-read prefix (of the table's width) on, up to 128 rows a kv head."""
+    saved = (seqs - groups) * cover(p, None, causal, window, sinks) * p.heads * p.dim * 2
+    return q.shape[0] // seqs * (q.shape[1] // p.heads) <= 128 and saved >= 24e6
+
+
+def widen(p, seqs, groups):
+    """Entries behind the sequences' pages, as of tables made for longer ones, so that sharing is worth it."""
+    pages = -(-int(24e6) // ((seqs - groups) * p.heads * p.dim * 2 * p.page)) + 1
+    if pages > p.table.shape[1]:
+        table = torch.full((seqs, pages), -1, dtype=torch.int32, device="cuda")
+        table[:, :p.table.shape[1]] = p.table
+        p.table = table
+
+
 def share(p, shared, groups):
     """Makes the sequences of each group name the pages of its first for the whole pages among the shared tokens."""
     for g, n in enumerate(shared):
@@ -233,7 +248,9 @@ def grouped(seed, *, code, page, heads, dim, group, dtype=BF16, new=None):
     new = new or [1] * 10
     p = Pages(seed, lens, [max(0, 620 + page - n) for n in lens], code=code, page=page, heads=heads, dim=dim)
     share(p, shared, groups)
+    widen(p, 10, 3)
     q = normal(p.g, sum(new), heads * group, dim, dtype=dtype) * 1.5
+    assert shares(p, q, 10, 3)
     return p, q, lens, new, shared, groups
 
 
@@ -246,18 +263,36 @@ def test_shared_single_tokens(code, dtype, page, heads, group, dim):
     first = check_spans(p, q, lens, new, shared=shared, groups=groups)
     again = check_spans(p, q, lens, new, shared=shared, groups=groups)
     assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
-    check_spans(p, q, lens, new, shared=shared, groups=groups, window=250)
-    check_spans(p, q, lens, new, shared=shared, groups=groups, window=40, sinks=620)
 
 
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("page, heads, group, dim", SHAPES)
-@pytest.mark.parametrize("causal, window, sinks", [(True, 0, 0), (True, 70, 3), (False, 0, 0), (False, 433, 17)])
+@pytest.mark.parametrize("causal, window, sinks", [(True, 0, 0), (False, 0, 0), (False, 433, 17)])
 def test_shared_ragged_rows(code, page, heads, group, dim, causal, window, sinks):
     new = [3, 5, 1, 2, 7, 0, 4, 9, 2, 4]
     p, q, lens, new, shared, groups = grouped(dim * 3 + group, code=code, page=page, heads=heads, dim=dim, group=group,
                                               new=new)
     check_spans(p, q, lens, new, causal=causal, window=window, sinks=sinks, shared=shared, groups=groups)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("page, heads, group, dim", [(64, 2, 4, 128), (16, 4, 1, 80), (32, 2, 12, 256), (128, 3, 2, 64)])
+@pytest.mark.parametrize("window, sinks", [(250, 0), (40, 620), (333, 5), (70, 100)])
+@pytest.mark.parametrize("new", [[1], [1, 3, 1, 2, 4, 0, 2]])
+def test_shared_windows(code, page, heads, group, dim, window, sinks, new):
+    """Windows that end within the prefix, reach into it or leave only its first tokens: 450 sequences in 75 groups, by
+    the kernel of few rows."""
+    seqs, groups = 450, list(range(0, 451, 6))
+    shared = [620 if g % 3 else 160 for g in range(75)]
+    lens = [max(0, shared[s // 6] + (37 * s % 400 if s % 5 else -40)) + 4 for s in range(seqs)]
+    new = (new * seqs)[:seqs]
+    p = Pages(dim, lens, [max(0, 640 - n) for n in lens], code=code, page=page, heads=heads, dim=dim)
+    share(p, shared, groups)
+    q = normal(p.g, sum(new), heads * group, dim, dtype=BF16) * 1.5
+    how = {"window": window, "sinks": sinks}
+    assert shares(p, q, seqs, 75, **how) == (375 * (window + -(-sinks // 16) * 16) * heads * dim * 2 >= 24e6)
+    assert not takes_tiles(p, q, sum(new) // 75, **how)
+    check_spans(p, q, lens, new, shared=shared, groups=groups, **how)
 
 
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
@@ -279,6 +314,7 @@ def test_shared_many_rows(code, dtype, page, heads, group, dim, each, causal, wi
     share(p, prefix, groups)
     q = normal(p.g, sum(new), heads * group, dim, dtype=dtype) * 1.5
     rows = sum(new) // 2
+    assert shares(p, q, seqs, 2, causal=causal, window=window, sinks=sinks)
     assert takes_tiles(p, q, rows, causal=causal, window=window, sinks=sinks)
     assert not takes_tiles(p, q, sum(new) // seqs, causal=causal, window=window, sinks=sinks)
     first = check_spans(p, q, lens, new, causal=causal, window=window, sinks=sinks, shared=prefix, groups=groups)
@@ -292,14 +328,16 @@ def test_shared_many_rows(code, dtype, page, heads, group, dim, each, causal, wi
 @pytest.mark.parametrize("groups", [None, [1, 7]])
 def test_shared_prompts(code, page, dim, causal, window, sinks, groups):
     """Questions of some tens of rows behind one text: prefixes and own tokens both on the tensor-core tiles."""
-    prefix = [3500]
-    new = [31, 40, 17, 60, 50, 21, 44, 33]
+    prefix, seqs = [3500], 24
+    groups = groups and [1, seqs - 1]
+    new = [31, 40, 17, 28, 50, 21, 24, 33] * 3
     lens = [3500 + n + 150 * (i % 3) for i, n in enumerate(new)]
     lens[2] = 11                                             # six of whose rows see nothing
-    p = Pages(dim + page, lens, [max(0, 3520 - n) for n in lens], code=code, page=page, heads=2, dim=dim)
-    share(p, prefix, [0, 8])
-    q = normal(p.g, sum(new), 8, dim, dtype=BF16) * 1.5
-    assert 48 <= sum(new) // 8 * 4 < 256 and takes_tiles(p, q, sum(new) // 8, causal=causal, window=window, sinks=sinks)
+    p = Pages(dim + page, lens, [max(0, 3520 - n) for n in lens], code=code, page=page, heads=4, dim=dim)
+    share(p, prefix, [0, seqs])
+    q = normal(p.g, sum(new), 16, dim, dtype=BF16) * 1.5
+    assert shares(p, q, seqs, 1, causal=causal, window=window, sinks=sinks)
+    assert takes_tiles(p, q, sum(new) // seqs, causal=causal, window=window, sinks=sinks)
     check_spans(p, q, lens, new, causal=causal, window=window, sinks=sinks, shared=prefix, groups=groups)
 
 
@@ -314,6 +352,7 @@ def test_row_tiles_of_odd_queries(form, dim):
     p = Pages(dim, lens, [0] * len(lens), code="int8", page=64, heads=2, dim=dim)
     if form == "shared":
         share(p, [1984], [0, seqs])
+        assert shares(p, torch.empty(420, 8, dim), seqs, 1)
     q = normal(p.g, 420, 8, dim + 1, dtype=BF16)[..., 1:]
     assert takes_tiles(p, q, 420 if form == "shared" else 210, **({} if form == "shared" else kw))
     check_spans(p, q, lens, new, **kw)
@@ -346,7 +385,9 @@ def test_sharing_is_left_out_where_sequences_have_many_rows():
     q = normal(p.g, 500, 8, 128, dtype=BF16)
     got = check_spans(p, q, lens, new, shared=[1024])
     plain = bfft.cache_attention(q, p.cache, p.table, ints(lens), ints([0, 300, 500]))
-    assert torch.equal(got[0], plain)
+    assert torch.equal(got[0], plain) and not shares(p, q, 2, 1)
+    few = check_spans(p, q[:2], lens, [1, 1], shared=[1024])              # and where it saves a few bytes only
+    assert torch.equal(few[0], bfft.cache_attention(q[:2], p.cache, p.table, ints(lens), ints([0, 1, 2])))
 
 
 @pytest.mark.parametrize("dim, heads", [(16, 64), (32, 64)])
@@ -358,6 +399,7 @@ def test_pieces_longer_than_the_table_of_pages(dim, heads):
     shared = [0, 8000]
     groups = [0, 3, 9]
     share(p, shared, groups)
+    assert shares(p, q, 9, 2) and shares(p, q, 9, 2, window=8500, sinks=100)
     total = sum(lens[:3]) + sum(n - 8000 for n in lens[3:]) + 8000
     assert total / (2 * 3 * 148 // heads) > 380 * 16
     check_spans(p, q, lens, [1] * 9, shared=shared, groups=groups)
@@ -390,8 +432,9 @@ def test_shared_over_tiny_values(each, tiles):
     lens = [2000 + each + i % 90 for i in range(seqs)]
     p = Pages(each, lens, [0] * seqs, code="int8", page=32, heads=2, dim=128)
     share(p, [2000], [0, seqs])
+    widen(p, seqs, 1)
     q = normal(p.g, seqs * each, 8, 128, dtype=BF16)
-    assert takes_tiles(p, q, seqs * each) == tiles
+    assert shares(p, q, seqs, 1) and takes_tiles(p, q, seqs * each) == tiles
     for where in ([3], range(62)):                           # one page of the prefix, then all of it
         p.cache.v_scale[[p.ids[0][i] for i in where]] = 1e-36
         check_relative(p, q, lens, [each] * seqs, [2000])
@@ -405,9 +448,11 @@ def test_shared_over_tiny_values(each, tiles):
 def test_shared_ignores_what_no_row_sees(each):
     seqs = 60
     lens = [1024 + each + i % 50 for i in range(seqs)]
-    p = Pages(17, lens, [0] * seqs, code="e4m3", page=64, heads=2, dim=64)
+    p = Pages(17, lens, [0] * seqs, code="e4m3", page=64, heads=8, dim=64)
     share(p, [1024], [0, seqs])
-    q = normal(p.g, seqs * each, 8, 64, dtype=F16)
+    q = normal(p.g, seqs * each, 16, 64, dtype=F16)
+    assert shares(p, q, seqs, 1, window=500, sinks=3)
+    assert takes_tiles(p, q, seqs * each, window=500, sinks=3) == (each > 1)
     want = check_spans(p, q, lens, [each] * seqs, shared=[1030], window=500, sinks=3)
     low = 1024 + 1 + min(i % 50 for i in range(seqs)) - 500
     for w in (0, 1):
@@ -430,7 +475,9 @@ def test_nan_and_missing_pages_of_a_prefix(each):
     lens = [1200 + each] * 25 + [640] + [1200 + each] * 24
     p = Pages(23, lens, [600] * seqs, code="int8", page=64, heads=2, dim=64)
     share(p, [1152], [0, seqs])
+    widen(p, seqs, 1)
     q = normal(p.g, seqs * each, 4, 64, dtype=BF16)
+    assert shares(p, q, seqs, 1)
     args = (ints(lens), ints(cumulative([each] * seqs)))
     p.cache.v_scale[p.ids[0][12], 0] = math.nan              # tokens 768..: the sequence of 640 does not see them
     out = bfft.cache_attention(q, p.cache, p.table, *args, shared=ints([1152]))
@@ -454,8 +501,10 @@ def test_shared_strides_streams_graphs_and_out(each, seqs):
     lens = [900 + each + i % 70 for i in range(seqs)]
     p = Pages(41, lens, [100] * seqs, code="int8", page=16, heads=2, dim=64)
     share(p, [896], [0, seqs])
+    widen(p, seqs, 1)
     wide = normal(p.g, seqs * each, 12, 80, dtype=F16)
     q = wide[:, 2:10, 8:72]
+    assert shares(p, q, seqs, 1)
     new, starts = [each] * seqs, ints(cumulative([each] * seqs))
     want, want_lse = check_spans(p, q, lens, new, shared=[896])
     side = torch.cuda.Stream()
@@ -503,7 +552,7 @@ def test_two_graphs_and_two_streams_at_once():
         p = Pages(seed, lens, [0] * seqs, code="int8", page=64, heads=2, dim=128)
         share(p, [1472], [0, seqs])
         q = normal(p.g, seqs, 8, 128, dtype=BF16)
-        assert takes_tiles(p, q, seqs)
+        assert takes_tiles(p, q, seqs) and shares(p, q, seqs, 1)
         args = (q, p.cache, p.table, ints(lens), ints(list(range(seqs + 1))))
         want = bfft.cache_attention(*args, shared=ints([1472]))
         shared = ints([1472])
@@ -530,7 +579,9 @@ def test_many_sequences_and_groups():
     lens = [shared[s // 3] + 1 + s % 40 for s in range(seqs)]
     p = Pages(8, lens, [0] * seqs, code="int8", page=16, heads=1, dim=64)
     share(p, shared, groups)
+    widen(p, seqs, 500)
     q = normal(p.g, seqs, 4, 64, dtype=BF16)
+    assert shares(p, q, seqs, 500)
     check_spans(p, q, lens, [1] * seqs, shared=shared, groups=groups)
     check_spans(p, q, lens, [1] * seqs, shared=[shared[0]] + [0] * 4, groups=[0, 3, 3, 9, 1500, 1500])
 
@@ -542,7 +593,9 @@ def test_counts_of_shared_tokens_out_of_range(tokens):
     p = Pages(6, lens, [8, 0, 58], code="int8", page=16, heads=2, dim=64)
     if tokens > 0:
         share(p, [min(tokens, 208)], [0, 3])
+    widen(p, 3, 1)
     q = normal(p.g, 3, 8, 64, dtype=BF16)
+    assert shares(p, q, 3, 1)
     check_spans(p, q, lens, [1] * 3, shared=[tokens])
 
 

@@ -46,7 +46,7 @@ def exact(q, k, v, roots, new, window, sinks, group):
 
 
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
-@pytest.mark.parametrize("users, window, sinks", [(3, 0, 0), (3, 500, 4), (40, 0, 0), (40, 700, 20)])
+@pytest.mark.parametrize("users, window, sinks", [(3, 0, 0), (3, 500, 4), (40, 0, 0), (40, 1500, 20)])
 def test_users_of_one_image(code, users, window, sinks):
     g = generator(users)
     heads, kv, dim, page, prefix, steps = 8, 2, 128, 32, 1600, 3
