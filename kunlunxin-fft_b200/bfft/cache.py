@@ -6,12 +6,14 @@ queries and keys are rotated by unit roots of their positions, the keys and valu
 past tokens are kept in 8 bits, and new tokens attend to them.
 
 * ``rotary_table`` / ``rotate_positions``: the rotation, forward and inverse;
-  differentiable (the gradient is rotated by the conjugate roots).
+  differentiable (the gradient is rotated by the conjugate roots).  Positions of
+  several axes (time, height, width) turn each pair by its axis's.
 * ``paged_cache`` / ``append_rotated``: pages of 16..128 tokens hold int8 or e4m3
   codes with one scale per page and kv head; new tokens are rotated, quantised
   and written by one launch (two where few sequences append long runs).
 * ``cache_attention``: causal, windowed or full attention of ragged rows (one
-  token, a few drafted ones, or a prompt's chunk per sequence) over the cache.
+  token, a few drafted ones, or a prompt's chunk per sequence) over the cache;
+  first tokens that a window does not hide, prefixes that sequences share.
 * ``read_cache``: the values that the cache stands for.
 
 Ragged rows: sequence ``s`` owns rows ``starts[s] .. starts[s + 1]`` of a call's

@@ -166,10 +166,11 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
 }
 
 // Whether a call is one for the tensor-core tiles: with 48 rows or more to a kv
-// head (16 rows of 32 heads over 16384 tokens: 44 us, split kernel 73; 8 rows: 58
+// head (16 rows of 32 heads over 16384 tokens: 33 us, split kernel 49; 8 rows: 33
 // by either) and enough work to pay for a CTA's start and its 128-row halves, some
 // 3 million (query head, token) pairs of 128 dimensions: 40 rows of 32 heads over
-// 900 tokens 30 us by the split kernel and 42 by this, 128 rows 58 and 48.  The rows
+// 900 tokens 21 us by the split kernel and 29 by this; 128 rows, which the rule gives to
+// this, 21 and 33 since the split kernel takes a tile's halves side by side.  The rows
 // are the mean of the call's sequences, so one kernel takes a prompt and single tokens
 // together: a prompt of 4096 rows with 255 single tokens of 4096, 32 heads, 1139 us
 // (apart 234 and 392), of 512 rows 661 (33 and 392).  Heads over 128 (S and O of two

@@ -25,11 +25,15 @@
 //   passes 2^15.5 (a vote instead of a reduction on most tiles).  A CTA that meets
 //   a value scale under 2^-48 keeps its sum 2^36 times smaller (see SmallScales).
 //
+// * A tile's two 16-token halves go side by side through every step, dead ones masked
+//   instead of skipped: with 8 or 12 warps to an SM the chain of a tile's products,
+//   scores and exponentials is what a warp waits for (64 ragged sequences 399 us with the
+//   halves one after the other and a branch between them, 357 so on that GPU).
+//
 // 64 sequences of 1024..32768 tokens, one row of 32 heads each (8 kv heads, 128
-// dimensions): int8 417 us, 5440 GB/s, 0.83 of the measured HBM rate (417 to 455, 0.76,
-// on the GPUs that it was measured on; a GPU repeats itself within 1 %); e4m3, whose
-// codes take 2 instructions for 4 to widen instead of 5, 386 us and 0.90.  One
-// sequence of 131001 e4m3 tokens, 64 heads: 55 us, the joining kernel's among them.
+// dimensions): int8 357 to 362 us, 0.97 to 0.96 of the measured HBM rate; e4m3, whose
+// codes take 2 instructions for 4 to widen instead of 5, 356.  One sequence of 131001 e4m3
+// tokens, 64 heads: 55 us, the joining kernel's among them.
 #pragma once
 
 namespace bfft {

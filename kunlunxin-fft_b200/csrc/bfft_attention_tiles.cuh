@@ -25,7 +25,7 @@
 // 2 % of the two-prompt case).
 //
 // 2 x 2048 prompt rows of 32 heads (8 kv heads, 128 dimensions) over 8192 and 16384
-// int8 tokens: 860 us (854 to 882 by the GPU), 880 TFLOP/s, 0.54 of the measured bf16
+// int8 tokens: 840 us (826 to 862 by the GPU), 900 TFLOP/s, 0.54 of the measured bf16
 // rate.  Bound by the chain of a half's tile, not by one pipe: 4900 clocks a tile for
 // 2048 of tensor work; and by the schedule: 512 CTAs of 65 to 113 tiles in the order
 // of their slots end at 372 tile times where an even spread would be 318 (counted).
@@ -35,6 +35,12 @@
 // 64 tokens with two score buffers a half were slower (an M128 N64 product takes as
 // long as N128 when the widening shares its shared memory); waits that poll without
 // reading the clock, 975 us.
+//
+// A CTA's start and end count where its axis is short: 30k of the 178k clocks of a windowed
+// prompt's tile (2 x 2048 rows, window 4096 + 4: 382 us), 45k of 75k where 64 sequences share
+// 16384 tokens (42 us), some 10k of these instructions that the SM has not run yet (a second
+// launch of the same kernel starts so much earlier).  Hence the short loops there, and
+// copies and looks at tables as early as their addresses are known.
 #pragma once
 
 namespace bfft {
