@@ -124,7 +124,11 @@ def _axes_bytes(axes, axis_order) -> bytes:
 def _axes(axes, axis_order):
     if axes is None:
         return None
-    return _axes_bytes(axes if type(axes) is tuple else tuple(axes), axis_order)
+    axes = axes if type(axes) is tuple else tuple(axes)
+    for n in axes:  # (4.0, 6) and (True, 6) would be found as (4, 6) and (1, 6)
+        if type(n) is not int:
+            raise ValueError(f"axes must be integers, got {axes}")
+    return _axes_bytes(axes, axis_order)
 
 
 def _frequencies(rotated, base, scaling, factor, original, low_turns, high_turns, device):

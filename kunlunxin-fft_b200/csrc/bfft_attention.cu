@@ -298,7 +298,7 @@ GroupPlan plan_groups(const bfft_cache_desc* c, const bfft_sequence_desc* q, con
 // each row, would take more than 512 MB.
 bool worth_sharing(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d,
                    const bfft_span_desc* w) {
-    if (q->tokens / q->seqs * (d->q_heads / c->kv_heads) > 128) return false;
+    if (q->tokens / q->seqs * (d->q_heads / c->kv_heads) > 128 || q->seqs > 0x3fffffffLL) return false;
     const double saved = (double)(q->seqs - w->n_groups) * (double)seen_cover(c, q, d, 1, 1, w->sinks) *
                          (double)(c->kv_heads * c->dim * 2);
     return saved >= 24.0e6 && plan_groups(c, q, d, w, sm_count(d->device)).bytes <= (size_t)512 << 20;
@@ -369,7 +369,7 @@ bfft_status check_span(const bfft_cache_desc* cache, const bfft_sequence_desc* s
                        const bfft_span_desc* w, int* form) {
     *form = kPlain;
     if (w->sinks < 0 || w->sinks > 0x3fffffffLL) return fail(BFFT_ERR_VALUE, "bad count of first tokens %lld", (long long)w->sinks);
-    if (w->n_groups < 0 || w->n_groups > 0x7ffffffeLL) return fail(BFFT_ERR_SHAPE, "bad group count %lld", (long long)w->n_groups);
+    if (w->n_groups < 0 || w->n_groups > 0x3fffffffLL) return fail(BFFT_ERR_SHAPE, "bad group count %lld", (long long)w->n_groups);
     if (w->n_groups && (!w->shared || (!w->groups && w->n_groups > 1))) return fail(BFFT_ERR_VALUE, "null pointer");
     if (!aligned(w->groups, 4) || !aligned(w->shared, 4)) return fail(BFFT_ERR_VALUE, "misaligned pointer");
     if (!seqs->tokens) return BFFT_OK;

@@ -30,6 +30,13 @@ def test_bad_axes(axes):
         cache._axes_map(axes, "blocks")
 
 
+def test_numbers_that_compare_equal_are_not_taken_for_each_other():
+    assert cache._axes((1, 6), "blocks") == bytes((2, 0, 1, 1, 1, 1, 1, 1)) == cache._axes([1, 6], "blocks")
+    for axes in ((True, 6), (1.0, 6)):
+        with pytest.raises(ValueError, match="axes"):
+            cache._axes(axes, "blocks")
+
+
 def test_bad_orders_and_spectra():
     for kw in ({"axis_order": "rows", "axes": (4,)}, {"spectrum": "own", "axes": (4,)}, {"spectrum": "axial"},
                {"axes": (3,)}):
