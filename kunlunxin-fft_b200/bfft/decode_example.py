@@ -7,11 +7,15 @@ one paged 8-bit cache, and per step
     y = cache_attention(q, cache, pages, lens, starts)
 
 for two sequences of different lengths, first with their whole prompts as rows,
-then with one row each.  The result is compared with float64 attention over the
-unquantised rows; the gradient of the rotation is compared with its adjoint.
+then with one row each.  ``window`` and ``sinks`` make it a stream that sees its last
+tokens and its first ones; with ``common`` tokens the prompts begin alike, and the
+second user's block table names the first one's pages for them.  The result is compared
+with float64 attention over the unquantised rows; the gradient of the rotation is
+compared with its adjoint.
 
-Run: ``python -m bfft.decode_example [--prompt N] [--steps N] [--code int8|e4m3]``
-with the package directory on PYTHONPATH; prints one JSON object.
+Run: ``python -m bfft.decode_example [--prompt N] [--steps N] [--code int8|e4m3]
+[--window N] [--sinks N] [--common N]`` with the package directory on PYTHONPATH; prints
+one JSON object.
 """
 from __future__ import annotations
 
@@ -23,7 +27,7 @@ import torch
 from .cache import append_rotated, cache_attention, paged_cache, read_cache, rotary_table, rotate_positions
 
 
-def _exact(q, k, v, table, group: int):
+def _exact(q, k, v, table, group: int, window: int, sinks: int):
     """Causal attention of one sequence's rows in float64: rows (tokens, heads, dim)."""
     where = torch.arange(q.shape[0], device=q.device)
     c, s = table[where].double().unsqueeze(1).unbind(-1)
@@ -33,15 +37,21 @@ def _exact(q, k, v, table, group: int):
         return torch.cat((a * c - b * s, a * s + b * c), -1)
 
     z = torch.einsum("qhd,khd->hqk", turn(q), turn(k).repeat_interleave(group, 1)) * q.shape[-1] ** -0.5
-    z = z.masked_fill(where > where[:, None], float("-inf"))
+    hidden = where > where[:, None]
+    if window:
+        hidden |= (where <= where[:, None] - window) & (where >= sinks)
+    z = z.masked_fill(hidden, float("-inf"))
     return torch.einsum("hqk,khd->qhd", torch.softmax(z, -1), v.double().repeat_interleave(group, 1))
 
 
 def run(prompt: int = 300, steps: int = 20, code: str = "int8", q_heads: int = 16, kv_heads: int = 4, dim: int = 128,
-        page: int = 32, seed: int = 0, device="cuda") -> dict:
+        page: int = 32, seed: int = 0, device="cuda", window: int = 0, sinks: int = 0, common: int = 0) -> dict:
     g = torch.Generator(device=device)
     g.manual_seed(seed)
     prompts = [prompt, max(1, prompt // 3)]  # two users
+    common = common // page * page  # whole pages are shared
+    if not 0 <= common < min(prompts):
+        raise ValueError(f"the common tokens must be fewer than the shorter prompt's {min(prompts)}, got {common}")
     total = [n + steps for n in prompts]
     table = rotary_table(max(total), dim, device=device)
     per = -(-max(total) // page)
@@ -49,6 +59,9 @@ def run(prompt: int = 300, steps: int = 20, code: str = "int8", q_heads: int = 1
     pages = torch.randperm(2 * per, device=device, generator=g).to(torch.int32).view(2, per)
     rows = [[torch.randn(n, h, dim, device=device, generator=g).bfloat16() for h in (q_heads, kv_heads, kv_heads)]
             for n in total]
+    for i in (0, 1, 2):
+        rows[1][i][:common] = rows[0][i][:common]
+    pages[1, :common // page] = pages[0, :common // page]
 
     def ints(values):
         return torch.tensor(values, dtype=torch.int32, device=device)
@@ -58,10 +71,12 @@ def run(prompt: int = 300, steps: int = 20, code: str = "int8", q_heads: int = 1
         q, k, v = (torch.cat([rows[s][i][held[s]:held[s] + new[s]] for s in (0, 1)]) for i in (0, 1, 2))
         starts = ints([0, new[0], new[0] + new[1]])
         q = append_rotated(cache, k, v, pages, ints(held), starts, table, q=q)
-        y = cache_attention(q, cache, pages, ints([held[s] + new[s] for s in (0, 1)]), starts)
+        y = cache_attention(q, cache, pages, ints([held[s] + new[s] for s in (0, 1)]), starts, window=window, sinks=sinks,
+                            shared=ints([common]) if common else None)
         return y.split(new)
 
-    out = [[y] for y in step([0, 0], prompts)]
+    first = [0, common]  # what the second user finds in the cache
+    out = [[y] for y in step(first, [n - f for n, f in zip(prompts, first)])]
     held = list(prompts)
     for _ in range(steps):
         for s, y in enumerate(step(held, [1, 1])):
@@ -69,7 +84,7 @@ def run(prompt: int = 300, steps: int = 20, code: str = "int8", q_heads: int = 1
         held = [h + 1 for h in held]
     error = 0.0
     for s in (0, 1):
-        want = _exact(*rows[s], table, q_heads // kv_heads)
+        want = _exact(*rows[s], table, q_heads // kv_heads, window, sinks)[first[s]:]
         error = max(error, float((torch.cat(out[s]).double() - want).norm() / want.norm()))
 
     # what the cache stands for, and the rotation's gradient
@@ -89,8 +104,10 @@ def main() -> None:
     p.add_argument("--prompt", type=int, default=300)
     p.add_argument("--steps", type=int, default=20)
     p.add_argument("--code", choices=("int8", "e4m3"), default="int8")
+    for name in ("window", "sinks", "common"):
+        p.add_argument(f"--{name}", type=int, default=0)
     a = p.parse_args()
-    print(json.dumps(run(a.prompt, a.steps, a.code)))
+    print(json.dumps(run(a.prompt, a.steps, a.code, window=a.window, sinks=a.sinks, common=a.common)))
 
 
 if __name__ == "__main__":

@@ -111,6 +111,18 @@ def test_users_of_one_image(code, users, window, sinks):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("kw", [{"window": 40, "sinks": 4}, {"common": 64}, {"window": 100, "sinks": 33, "common": 32}])
+def test_decode_example_with_windows_and_common_prompts(code, kw):
+    from bfft import decode_example
+
+    got = decode_example.run(prompt=300, steps=5, code=code, **kw)
+    # as without: codes off by half a unit of the block's scale or 2^-4 of the value, keys the same
+    assert got["attention_rel_error"] < (0.03 if code == "int8" else 0.06) and got["gradient_is_adjoint"]
+    with pytest.raises(ValueError, match="common"):
+        decode_example.run(prompt=30, steps=1, code=code, common=32)
+
+
 def test_training_of_queries_and_keys_with_axes():
     """Gradients through the rotation of queries and keys into plain attention, against float64 autograd."""
     g = generator(1)
