@@ -279,7 +279,7 @@ GroupPlan plan_groups(const bfft_cache_desc* c, const bfft_sequence_desc* q, con
         (l.tiles ? l.row_tiles.ctas : l.split.ctas) = l.items.most * kv;
         SpanArgs counts{};
         counts.n_groups = (int)w->n_groups;
-        l.list = unit_count(counts, l.items, (int)q->seqs) > kFewUnits;
+        l.list = unit_count(counts, l.items, (int)q->seqs) > (k == 1 && p.launch[0].tiles ? kFewBesideTiles : kFewUnits);
         l.list_at = at;
         at += l.list ? (size_t)(l.items.most + 1) * sizeof(Item) : 0;  // behind a count
         l.parts_at = at;

@@ -205,8 +205,10 @@ __device__ __forceinline__ void fill_item(Item& f, const Unit& v, bool prefix, i
     f.len = v.len;
 }
 
-// Units that a call's warps look at by themselves; more have their items listed first.
-constexpr int kFewUnits = 32;
+// Units that a call's warps look at by themselves; more have their items listed first.  The
+// list is a launch of its own (32 sequences over 2048 + 200 tokens 42 us with it, 32
+// without), or free where a block of the row tiles makes it.
+constexpr int kFewUnits = 128, kFewBesideTiles = 32;
 __host__ __device__ inline int unit_count(const SpanArgs& p, const ItemArgs& x, int seqs) {
     return (x.prefixes ? p.n_groups : 0) + (x.own ? seqs : 0);
 }
@@ -227,28 +229,42 @@ __device__ __forceinline__ bool find_item(const AttentionArgs& a, const SpanArgs
     }
     const int groups = x.prefixes ? p.n_groups : 0, units = unit_count(p, x, a.seq.seqs);
     Unit v{};
-    if (lane < units) v = unit_of(a, p, x, lane, tile, parts);
-    float total = (float)v.tiles * (float)v.length;
+    float total = 0.f;
+#pragma unroll 1
+    for (int u = lane; u < units; u += 32) {
+        v = unit_of(a, p, x, u, tile, parts);
+        total += (float)v.tiles * (float)v.length;
+    }
 #pragma unroll
     for (int w = 16; w; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
-    const int pieces = pieces_of(v, item_tokens(x, total));
-    const int mine = v.tiles * pieces;
-    int upto = mine;
+    const unsigned chunk = item_tokens(x, total);
+    int before = 0;  // items of the units before these 32
+#pragma unroll 1
+    for (int u0 = 0; u0 < units; u0 += 32) {
+        const int u = u0 + lane;
+        if (units > 32) v = u < units ? unit_of(a, p, x, u, tile, parts) : Unit{};
+        const int pieces = pieces_of(v, chunk);
+        const int mine = v.tiles * pieces;
+        int upto = mine;
 #pragma unroll
-    for (int w = 1; w < 32; w <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, upto, w);
-        if (lane >= w) upto += y;
+        for (int w = 1; w < 32; w <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, w);
+            if (lane >= w) upto += y;
+        }
+        const int rest = i - before - (upto - mine);
+        const unsigned who = __ballot_sync(0xffffffffu, rest >= 0 && rest < mine);
+        if (who) {
+            Item f{};
+            fill_item(f, v, u < groups, rest, pieces, tile, parts);
+            const int* fields = reinterpret_cast<const int*>(&f);
+            int* out = reinterpret_cast<int*>(&it);
+#pragma unroll
+            for (int k = 0; k < (int)(sizeof(Item) / 4); ++k) out[k] = __shfl_sync(0xffffffffu, fields[k], __ffs(who) - 1);
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    const int rest = i - (upto - mine);
-    const unsigned who = __ballot_sync(0xffffffffu, rest >= 0 && rest < mine);
-    if (!who) return false;
-    Item f{};
-    fill_item(f, v, lane < groups, rest, pieces, tile, parts);
-    const int* fields = reinterpret_cast<const int*>(&f);
-    int* out = reinterpret_cast<int*>(&it);
-#pragma unroll
-    for (int k = 0; k < (int)(sizeof(Item) / 4); ++k) out[k] = __shfl_sync(0xffffffffu, fields[k], __ffs(who) - 1);
-    return true;
+    return false;
 }
 
 // Lists the items of more units, by one block: long pieces before short ones (in sixteen
