@@ -147,15 +147,18 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
     // lengths) are kept to 256 MB by longer chunks, as far as shared memory holds their
     // pages' scales (4.4 GB without: 512 sequences of 4 rows of 64 heads, 131072 tokens wide)
     const int64_t part = q->tokens * d->q_heads * (c->dim + 2) * 4, budget = (int64_t)256 << 20;
+    // entries of a chunk beside its whole pages: its two ends; with first tokens the ends of
+    // both of its pieces, and one where it is no whole pages (see open_segment)
+    const int64_t ends = sinks ? 5 : 2;
     if (!brief && (cover + chunk - 1) / chunk * part > budget) {
         const int64_t n = part < budget ? budget / part : 1;
         const int64_t room = (kSplitSmemMost - split_smem((int)c->dim, 8 * p.nt, 0)) / (int64_t)(sizeof(BlockScale) + 4);
-        int64_t most = (room - 2) * c->page;
+        int64_t most = (room - ends) * c->page;
         if (most > 1 << 20) most = 1 << 20;
         chunk = ((cover + n - 1) / n + 31) / 32 * 32;
         if (chunk > most) chunk = most / 32 * 32;
     }
-    p.entries = (int)(chunk / c->page + (sinks ? 5 : 2));
+    p.entries = (int)(chunk / c->page + ends);
     p.chunk = (int)chunk;
     const int64_t n = (cover + chunk - 1) / chunk;
     p.chunks = (int)n;
