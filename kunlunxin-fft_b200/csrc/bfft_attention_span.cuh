@@ -179,12 +179,13 @@ __device__ __forceinline__ Unit unit_of(const AttentionArgs& a, const SpanArgs& 
 }
 
 // Tokens of an item: those that all row tiles walk, `total`, shared out over x.target items.
-// (The sum's rounding is far under the one token that is added.)
-__device__ __forceinline__ unsigned item_tokens(const ItemArgs& x, float total) {
-    const int share = (int)fminf(total / (float)x.target, 1.0e9f) + 1;
+// The grid has room for target + 2 items more than there are row tiles: a share goes up to
+// the widest table (2^30 tokens), and what the sum rounds off is far under two shares.
+__host__ __device__ __forceinline__ unsigned item_tokens(const ItemArgs& x, float total) {
+    const int share = (int)fminf(total / (float)x.target, 1073741824.f) + 1;
     return max((unsigned)(share + x.unit - 1) / (unsigned)x.unit * x.unit, (unsigned)x.least);
 }
-__device__ __forceinline__ int pieces_of(const Unit& v, unsigned chunk) {
+__host__ __device__ __forceinline__ int pieces_of(const Unit& v, unsigned chunk) {
     return (unsigned)v.length > chunk ? (int)(((unsigned)v.length + chunk - 1) / chunk) : 1;
 }
 // Item `rest` of unit u.
