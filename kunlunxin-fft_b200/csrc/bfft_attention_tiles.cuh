@@ -234,6 +234,28 @@ __device__ __forceinline__ void write_rows(unsigned char* stage, uint32_t o_addr
     }
 }
 
+// The same by the rows' own lanes, 16 bytes at a time, where a CTA has one half only: the few
+// lines of a row are soon written, and the way through shared memory is a longer chain (4
+// sequences of 16 rows of 32 heads over 8192 tokens 71 us for 80, 16 rows over 16384 31 for 34,
+// 64 prompts of 20 rows over 2000 162 for 171).  With two halves whole lines win (2 prompts of
+// 100 rows with a window of 1000 tokens 41 us by own lanes, 39 so).
+template <int DP, typename E, typename Value>
+__device__ __forceinline__ void write_own_rows(uint32_t o_addr, int dim, bool mine, E* to, Value value) {
+    constexpr int PER = 16 / (int)sizeof(E);
+#pragma unroll 1
+    for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        tmem_load(o_addr + c, o);
+#pragma unroll
+        for (int k = 0; k < 32; k += PER) {
+            Pack<E, PER> w;
+#pragma unroll
+            for (int x = 0; x < PER; ++x) w.v[x] = value(__uint_as_float(o[k + x]));
+            if (mine && c + k < dim) *reinterpret_cast<Pack<E, PER>*>(to + c + k) = w;
+        }
+    }
+}
+
 template <int DP, typename T, int CODE, int MODE>
 __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(TileArgs p, const __grid_constant__ CUtensorMap qmap) {
     using G = TileGeo<DP>;
@@ -654,7 +676,15 @@ __global__ void __launch_bounds__(TileGeo<DP>::THREADS, 1) k_attention_tiles(Til
                 // Half 0 stages its rows where the queries were, half 1 where the widened codes
                 // were: nothing but half 1's last product over values can be under way here.
                 unsigned char* stage = (h ? t_s : q_s) + (warp & 3) * Stage<DP>::BYTES;
-                if (!direct) {
+                // (told apart as the rare case: otherwise the rows' loop is compiled to something
+                // slower, two prompts of 2048 rows 858 us instead of 845)
+                if (__builtin_expect(halves == 1 && (!direct || a.o_packs), 0)) {
+                    if (direct)
+                        write_own_rows<DP>(o_addr, dim, mine, static_cast<T*>(a.out) + token * a.ot + head * a.oh,
+                                           [&](float v) { return from_f32<T>(v * unit * inv); });
+                    else
+                        write_own_rows<DP>(o_addr, dim, mine, p.parts + at * dim, [&](float v) { return v * unit; });
+                } else if (!direct) {
                     write_rows<DP>(stage, o_addr, dim, mine, p.parts, at * dim, [&](float v) { return v * unit; });
                 } else if (a.o_packs) {
                     write_rows<DP>(stage, o_addr, dim, mine, static_cast<T*>(a.out), token * a.ot + head * a.oh,
