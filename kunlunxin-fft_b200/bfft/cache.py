@@ -122,8 +122,6 @@ def _axes_bytes(axes, axis_order) -> bytes:
 
 
 def _axes(axes, axis_order):
-    if axes is None:
-        return None
     axes = axes if type(axes) is tuple else tuple(axes)
     for n in axes:  # (4.0, 6) and (True, 6) would be found as (4, 6) and (1, 6)
         if type(n) is not int:
@@ -225,7 +223,8 @@ def rotate_positions(x, positions, table, *, layout: str = "half", transform_dir
     if direction is None:
         raise ValueError(f"transform_direction must be one of {sorted(_lib.TRANSFORM_DIRECTION_IDS)}, "
                          f"got {transform_direction!r}")
-    return (_native or _load()).rotate(x, positions, table, _layout(layout), direction, out, _axes(axes, axis_order))
+    return (_native or _load()).rotate(x, positions, table, _layout(layout), direction, out,
+                                       None if axes is None else _axes(axes, axis_order))
 
 
 # ------------------------------------------------------------------------------- cache
@@ -249,7 +248,7 @@ def append_rotated(cache, k, v, block_table, held, starts, table=None, *, layout
     q: (tokens, q_heads, dim) of k's type; its rotated rows are returned (else None).
     ``cache_attention`` takes them in float16 or bfloat16."""
     return (_native or _load()).append(cache, k, v, block_table, held, starts, table, _layout(layout), positions, q,
-                                       _axes(axes, axis_order))
+                                       None if axes is None else _axes(axes, axis_order))
 
 
 def read_cache(cache, block_table, first, starts, tokens: int, *, dtype=torch.bfloat16):
