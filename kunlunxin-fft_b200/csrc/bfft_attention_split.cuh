@@ -267,8 +267,12 @@ struct SplitGeo {
     __host__ __device__ static constexpr int half_bytes(int dim) { return split_half_bytes(dim); }
 };
 
+// Three CTAs an SM by their registers where that costs no spills: up to 168 for 8-row tiles and
+// for 64-wide heads (with 176 to 204, two CTAs, 16-row tiles of these were slower: 64 sequences
+// of 4 rows over 1000..9000 tokens 142 us for 129, 8 prompts of 100 rows with a window of 31
+// tokens 39 for 30).
 template <int DP, bool EXACT, int NT, typename T, int CODE, int MODE>
-__global__ void __launch_bounds__(kSplitThreads, NT == 1 && DP <= 128 ? 3 : 2)
+__global__ void __launch_bounds__(kSplitThreads, DP == 64 || (NT == 1 && DP == 128) ? 3 : 2)
     k_attention_split(SplitArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using G = SplitGeo<DP, EXACT, NT>;
     extern __shared__ unsigned char smem_raw[];
