@@ -426,7 +426,7 @@ typedef struct bfft_span_desc {
  * 2^30 tokens wide.  The workspace with groups holds the row tiles' parts and those of some
  * waves of CTAs more, 512 MB at most: calls that would need more, calls with more than 128
  * rows to a sequence and kv head, and calls whose prefixes, were they as long as the table
- * is wide, would be 24 MB or less to read again, are made as without groups. */
+ * is wide, would be under 24 MB to read again, are made as without groups. */
 BFFT_EXPORT bfft_status bfft_cache_attention_span_workspace(const bfft_cache_desc* cache, const bfft_sequence_desc* seqs,
                                                             const bfft_attention_desc* desc, const bfft_span_desc* span,
                                                             size_t* bytes);

@@ -280,10 +280,14 @@ def cache_attention(q, cache, block_table, lens, starts, *, softmax_scale: float
     all are one group) share their first ``shared[g]`` tokens (int32, (groups,)): the whole
     pages among these are read once for the group, from the block table's row of its first
     sequence.  The results are those of a call without, but for roundings.  Sequences in
-    no group share nothing.  The call goes without where that is as fast: over 128 rows a
-    kv head (query tokens times heads) of a sequence, where the prefixes would be under 24
-    MB to read again, were they as long as the table is wide, and where the workspace
-    would pass 512 MB.
+    no group share nothing.  The call goes without over 128 rows a kv head (query tokens
+    times heads) of a sequence, where the prefixes would be under 24 MB to read again, were
+    they as long as the table is wide, and where the workspace would pass 512 MB.  It knows
+    the table's width only: where most tokens are the sequences' own, or with one or two kv
+    heads and short prefixes, it can be slower than without (32 sequences over 2048 + 2000
+    tokens 71 us for 60, 128 of one kv head over 1024 + 100 37 for 21): leave `shared` out there.
+
+    With ``shared``, and with ``sinks`` beside a window, tables are up to 2^30 tokens wide.
 
     The weights, times their block's value scale, are rounded to float16 before they
     meet the codes, with a row's largest near float16's top: to 2^-11 down to 2^-24 of

@@ -118,14 +118,14 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
     // Where rows are many, chunks of 2048 tokens (512..4096 measure alike for 64 ragged
     // sequences).  Where they are few the table's width is shared out over a number of
     // CTAs that is counted as if three were resident on an SM (two are with 16 rows a
-    // tile, one with heads over 128) and as if row tiles were full (those of sequences of
+    // tile of heads over 64, one with heads over 128) and as if row tiles were full (those of sequences of
     // few rows are not: a tile's rows are one sequence's): "waves" times that many.  One
     // sequence of 131001 tokens, whose tiles are full: 71.6 us with 1, 75.8 with 2, 84.0
     // with 3, so 1, as a further wave's start costs more than it hides; 16 of 2000..8000
     // tokens, whose 4-row tiles are half full: 63.5, 59.4 and 69.6, so 2 for many
     // sequences.  The table's width is all that the host knows of the lengths: with a
-    // table of 131072 tokens one row over 700 takes 21.5 us (14.3 with a table of 700,
-    // timed with a cold L2), 8 over 4000 74.8 (37.9).
+    // table of 131072 tokens one row over 700 takes 18.4 us (12.3 with a table of 700,
+    // timed with a cold L2), 8 over 4000 61.4 (32.8).
     const int64_t waves = q->seqs > 8 ? 2 : 1;
     int64_t chunks = units >= 2 * resident ? (cover + 2047) / 2048 : waves * resident / units;
     if (chunks < 1) chunks = 1;
@@ -169,16 +169,16 @@ SplitPlan plan_split(const bfft_cache_desc* c, const bfft_sequence_desc* q, cons
 }
 
 // Whether a call is one for the tensor-core tiles: with 48 rows or more to a kv
-// head (16 rows of 32 heads over 16384 tokens: 33 us, split kernel 49; 8 rows: 33
+// head (16 rows of 32 heads over 16384 tokens: 31 us, split kernel 49; 8 rows: 33
 // by either) and enough work to pay for a CTA's start and its 128-row halves, some
 // 3 million (query head, token) pairs of 128 dimensions: 40 rows of 32 heads over
 // 900 tokens 21 us by the split kernel and 29 by this; 128 rows, which the rule gives to
 // this, 21 and 33 since the split kernel takes a tile's halves side by side.  The rows
 // are the mean of the call's sequences, so one kernel takes a prompt and single tokens
-// together: a prompt of 4096 rows with 255 single tokens of 4096, 32 heads, 1139 us
-// (apart 234 and 392), of 512 rows 661 (33 and 392).  Heads over 128 (S and O of two
+// together: a prompt of 4096 rows with 255 single tokens of 4096, 32 heads, 1124 us
+// (apart 205 and 337), of 512 rows over 512 520 (21 and 337).  Heads over 128 (S and O of two
 // halves are more than tensor memory) and groups over 128 stay with the split kernel:
-// 2 x 2048 rows of 16 heads of 256 over 8192 and 16384 tokens 10.6 ms, of 128 0.45.
+// 2 x 2048 rows of 16 heads of 256 over 8192 and 16384 tokens 8.6 ms, of 128 0.43.
 bool use_tiles(const bfft_cache_desc* c, const bfft_sequence_desc* q, const bfft_attention_desc* d, int64_t sinks) {
     const int64_t group = d->q_heads / c->kv_heads, each = q->tokens / q->seqs;
     if (c->dim > 128 || group > 128 || each * group < 48) return false;
@@ -268,7 +268,10 @@ GroupPlan plan_groups(const bfft_cache_desc* c, const bfft_sequence_desc* q, con
         // in plan_split (200 sequences of 16..2048 own tokens 445 us, in four waves 466).  A
         // piece costs a CTA's start, so none is short where there are row tiles for every
         // CTA's place (the 64 with 16..1024 tokens of their own: pieces of 256 on 77 us, of 512
-        // 74, of 1024 75).
+        // 74, of 1024 75).  An SM holds three CTAs of 8-row tiles, two of 16-row ones (of 64-wide
+        // heads three, counted as two); heads over 128 are counted as two too, though their rings leave room for one.  Counted as
+        // one: 64 sequences over 8192 + 200 tokens, 8 kv heads of 256, 260 us for 277, 8 over
+        // 32768 + 200 189 for 155, 32 of 2 kv heads over 2048 + 500 46 for 56.
         const int64_t units = ((l.prefixes ? q->tokens / l.tile_tokens() + w->n_groups : 0) +
                                (l.own ? q->tokens / l.tile_tokens() + q->seqs : 0)) * l.token_tiles();
         const int64_t places = (int64_t)sms * (l.tiles ? 1 : nt == 1 && c->dim <= 128 ? 3 : 2);

@@ -40,7 +40,7 @@ struct ItemArgs {
     int least;              // tokens of an item at least
     int unit;               // and a multiple of this
     int64_t most;           // items a kv head at most (the grid)
-    const Item* list;       // where there are more than 32 units: the items, and how many
+    const Item* list;       // where there are many units (see kFewUnits): the items, and how many
     const int* count;
     int4* own_of;           // [tokens] where a token's parts are: see ItemPlace
     int4* prefix_of;

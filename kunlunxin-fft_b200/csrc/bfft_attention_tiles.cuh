@@ -37,7 +37,7 @@
 // reading the clock, 975 us.
 //
 // A CTA's start and end count where its axis is short: 30k of the 178k clocks of a windowed
-// prompt's tile (2 x 2048 rows, window 4096 + 4: 382 us), 45k of 75k where 64 sequences share
+// prompt's tile (2 x 2048 rows, window 4096 + 4: 377 us), 45k of 75k where 64 sequences share
 // 16384 tokens (42 us), some 10k of these instructions that the SM has not run yet (a second
 // launch of the same kernel starts so much earlier).  Hence the short loops there, and
 // copies and looks at tables as early as their addresses are known.
